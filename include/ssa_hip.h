@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define SSA_ABI_VERSION 7
+#define SSA_ABI_VERSION 8
 
 typedef void* ssa_stream_t; /* hipStream_t */
 
@@ -471,6 +471,55 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
                         int64_t block, const int64_t* strides, const int32_t* kv_num,
                         const int32_t* kv_idx, int64_t W, float scale, void* workspace,
                         size_t workspace_bytes, ssa_stream_t stream);
+
+/*
+ * A paged key-value cache for requests of different lengths: no counterpart in the reference, the
+ * dense companion of the routed decode for serving. A pool (pages, Hkv, page, d) of a dtype is
+ * described by its (page, head, slot) element strides; page: a multiple of 16 up to 65536, d: a
+ * multiple of 8 up to 512. Token j of request b lies in page table[b][j / page] (table (B, W) int32,
+ * table_stride elements a row, W * page <= 2^31 - 1) at offset j % page; its slot number is
+ * page id * page + offset. Lengths are device data, so what does not fit them is found there: no
+ * entry point reads or writes through a bad length, slot or page id.
+ *
+ * ssa_paged_resize: brings the requests from lens to new_lens (B) int32. free_pages (pages) int32 is
+ *   a stack of which the first *nfree entries are free page ids. With have = ceil(lens / page) and
+ *   need = ceil(new_lens / page): the o-th page taken (requests in order, table entries ascending)
+ *   is free_pages[nfree - 1 - o]; then the o-th page given back goes to free_pages[left - 1 - o],
+ *   left the new count (*nfree = nfree - taken + given), and its table entry becomes -1. lens
+ *   becomes new_lens. The new tokens, request by request: cu (B + 1) int32 their offsets, slots (T)
+ *   int64 and pos (T, may be NULL) int32 each one's slot number and position, -1 and 0 past the
+ *   last. *status: 0; or nothing was changed (cu all 0, slots all -1): the number of pages lacking,
+ *   -1 (a length outside [0, W * page], or counts that do not fit the pool), -2 (more than T new
+ *   tokens). Pages given back in a call can be taken from the next call on. The table's entries of
+ *   different requests must not overlap in memory; new_lens may be lens itself.
+ * ssa_paged_append: keys and values k, v (T, Hkv, d) of new tokens into the pools at slots (T) int64
+ *   (distinct; rows whose slot lies outside the pool are skipped). strides[10] = k(t,h), v(t,h),
+ *   kpool(page,head,slot), vpool(page,head,slot).
+ * ssa_paged_attend: one query row per head and request, q, out (B, Hq, d), over keys j of
+ *   [max(0, len - window), len) (window 0: all), len = lens[b] (B) int32: softmax(scale * q.k) in
+ *   fp32, query head h reading key head h / (Hq / Hkv). lse (B, Hq) fp32, may be NULL: natural log
+ *   of the row's sum of exponentials. A row of length 0: out 0, lse -inf. A length outside
+ *   [0, W * page] or an attended page id outside [0, pages): out and lse NaN. k_new, v_new (B, Hkv,
+ *   d), both or none: the key and value at position len - 1, which the call stores into the pools
+ *   and attends (that page must be one request's alone; earlier pages may be shared). strides[14] =
+ *   q(b,h), kpool(page,head,slot), vpool(page,head,slot), out(b,h), k_new(b,h), v_new(b,h).
+ *   Workspace: ssa_paged_attend_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
+ * Rows start at multiples of 16 bytes (bases and strides).
+ */
+int ssa_paged_resize(int32_t* lens, const int32_t* new_lens, int32_t* table, int64_t table_stride,
+                     int64_t B, int64_t W, int64_t page, int32_t* free_pages, int64_t pages,
+                     int32_t* nfree, int64_t* slots, int32_t* pos, int64_t T, int32_t* cu,
+                     int32_t* status, ssa_stream_t stream);
+int ssa_paged_append(const void* k, const void* v, void* kpool, void* vpool, int dtype, int64_t T,
+                     int64_t Hkv, int64_t d, int64_t pages, int64_t page, const int64_t* strides,
+                     const int64_t* slots, ssa_stream_t stream);
+size_t ssa_paged_attend_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+                                       int64_t page, int64_t window);
+int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* lse, int dtype,
+                     int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t pages, int64_t page,
+                     const int32_t* table, int64_t table_stride, int64_t W, const int32_t* lens,
+                     const void* k_new, const void* v_new, const int64_t* strides, float scale,
+                     int64_t window, void* workspace, size_t workspace_bytes, ssa_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libssa_hip.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 SSA_OK, SSA_ERR_INVALID, SSA_ERR_UNSUPPORTED, SSA_ERR_HIP, SSA_ERR_WORKSPACE = 0, -1, -2, -3, -4
 F32, F16, BF16 = 0, 1, 2
@@ -96,6 +96,12 @@ _SIGNATURES = {
                                         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                         _c_p, _c_i64, _c_f, _c_i64, _c_f, _c_f, _c_p, _c_p, _c_i64,
                                         _c_p]),
+    "ssa_paged_resize": (_c_int, [_c_p] * 3 + [_c_i64] * 4 + [_c_p, _c_i64, _c_p, _c_p, _c_p,
+                                                              _c_i64, _c_p, _c_p, _c_p]),
+    "ssa_paged_append": (_c_int, [_c_p] * 4 + [_c_int] + [_c_i64] * 5 + [_c_p] * 3),
+    "ssa_paged_attend_workspace_size": (_c_sz, [_c_i64] * 7),
+    "ssa_paged_attend": (_c_int, [_c_p] * 5 + [_c_int] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] +
+                         [_c_p] * 4 + [_c_f, _c_i64, _c_p, _c_sz, _c_p]),
 }
 
 _lock = threading.Lock()

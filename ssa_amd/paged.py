@@ -1,0 +1,311 @@
+"""A paged key-value cache: many requests of different lengths in one pool of pages.
+
+    resize_pages(lens, new_lens, table, free, nfree, page, tokens)   pages taken and given back
+    append_pages(k, v, kpool, vpool, slots)                          new tokens into their slots
+    attend_pages(q, kpool, vpool, table, lens, ...)                  one new token per request
+    PagedCache                                                       the state these work on
+
+A pool is a (pages, Hkv, page, d) tensor (any strides with a contiguous last dimension, so a
+token-major (pages, page, Hkv, d) pool is passed transposed); token j of request b lies in page
+table[b, j // page] at slot j % page, and its slot number is table[b, j // page] * page + j % page.
+The lengths live on the device: every call is asynchronous on the current stream of the tensors'
+device, works under graph capture and synchronises with nothing. What a call can only find out on
+the device (a length beyond the table, too few free pages, a page id outside the pool) is answered
+there: resize_pages changes nothing and writes a status, append_pages skips the row, attend_pages
+returns NaN for the row; no call follows a bad length or page id.
+
+attend_pages is the dense counterpart of attend_rows and dense_decode (ivf_decode) for batches of
+requests: the decode of the layers that a routed model leaves dense or sliding. It is not
+differentiable. The reference has no paged cache.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .ssa_kernel import _aligned
+
+RESIZE_ERRORS = {-1: "a length, the free count or the pool does not fit the table",
+                 -2: "more new tokens than slots"}
+
+
+class Resized(NamedTuple):
+    """What resize_pages returns: of every new token (request by request, in order) its slot and
+    position, the first token of each request (B + 1 offsets), and the status (1,)."""
+    slots: torch.Tensor   # (tokens,) int64, -1 past the last new token
+    pos: torch.Tensor     # (tokens,) int32, 0 past the last new token
+    cu: torch.Tensor      # (B + 1,) int32
+    status: torch.Tensor  # (1,) int32: 0, the number of pages lacking, or a key of RESIZE_ERRORS
+
+
+def _launch(name, t, *args):
+    """Calls an entry point on the current stream of t's device."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_of(t))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _lib.stream_of(t))
+
+
+def _one_device(first, *others):
+    _lib.require_device(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def _int32(name, t, shape):
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} is {t.dtype}, expected torch.int32")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor, "
+                         f"got {tuple(t.shape)}")
+
+
+def _table(table):
+    if table.dtype != torch.int32:
+        raise TypeError(f"table is {table.dtype}, expected torch.int32")
+    if table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError("table must be (B, W) with a contiguous last dimension")
+    B, W = table.shape
+    return B, W, table.stride(0) if B > 1 else W
+
+
+def _pools(kpool, vpool):
+    if kpool.dim() != 4 or kpool.shape != vpool.shape:
+        raise ValueError(f"kpool and vpool must share a (pages, Hkv, page, d) shape, got "
+                         f"{tuple(kpool.shape)} and {tuple(vpool.shape)}")
+    if kpool.dtype != vpool.dtype:
+        raise TypeError("kpool and vpool must share a dtype")
+    if kpool.stride(3) != 1 or vpool.stride(3) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    return kpool.shape
+
+
+def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor,
+                 free: torch.Tensor, nfree: torch.Tensor, page: int, tokens: int,
+                 out: Resized | None = None) -> Resized:
+    """Brings the requests to new lengths, on the device.
+
+    lens, new_lens (B,) int32; table (B, W) int32; free (pages,) int32, a stack of the free page
+    ids of which the first nfree (1,) int32 are valid. lens, table, free and nfree are updated: a
+    request that grows takes pages from the top of the stack (requests in order), one that shrinks
+    gives its last pages back (their table entries become -1), lens becomes new_lens. Pages given
+    back in a call can be taken from the next call on. Growing and then shrinking back restores
+    table and free exactly.
+
+    tokens: room for the new tokens (at least the sum of the growths; more is padding). Returns a
+    Resized; `out` takes an earlier one of the same sizes to write into. All or nothing: if the
+    growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
+    slots are -1 and status says why."""
+    _one_device(lens, new_lens, table, free, nfree)
+    B, W, row = _table(table)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"tokens={tokens}")
+    _int32("lens", lens, (B,))
+    _int32("new_lens", new_lens, (B,))
+    _int32("nfree", nfree, (1,))
+    _int32("free", free, (free.numel(),))
+    if torch.compiler.is_compiling() and out is None:
+        from . import torch_ops as T
+        return Resized(*T.paged_resize(lens, new_lens, table, free, nfree, int(page), tokens))
+    if out is None:
+        dev = lens.device
+        out = Resized(torch.empty(tokens, device=dev, dtype=torch.int64),
+                      torch.empty(tokens, device=dev, dtype=torch.int32),
+                      torch.empty(B + 1, device=dev, dtype=torch.int32),
+                      torch.empty(1, device=dev, dtype=torch.int32))
+    else:
+        _one_device(lens, *out)
+        if out.slots.dtype != torch.int64 or out.slots.shape != (tokens,) \
+                or not out.slots.is_contiguous():
+            raise ValueError(f"out.slots must be a contiguous ({tokens},) int64 tensor")
+        _int32("out.pos", out.pos, (tokens,))
+        _int32("out.cu", out.cu, (B + 1,))
+        _int32("out.status", out.status, (1,))
+    _launch("ssa_paged_resize", lens, lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(),
+            row, B, W, int(page), free.data_ptr(), free.numel(), nfree.data_ptr(),
+            out.slots.data_ptr() if tokens else None, out.pos.data_ptr() if tokens else None,
+            tokens, out.cu.data_ptr(), out.status.data_ptr())
+    return out
+
+
+def append_pages(k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor,
+                 slots: torch.Tensor) -> None:
+    """Stores the tokens' keys and values k, v (T, Hkv, d) into the pools at slots (T,) int64
+    (slot = page id * page + offset; rows whose slot lies outside the pool, as -1, are skipped).
+    The slots of a call must be distinct."""
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        return T.paged_append(k, v, kpool, vpool, slots)
+    return _append_pages_impl(k, v, kpool, vpool, slots)
+
+
+def _append_pages_impl(k, v, kpool, vpool, slots):
+    _one_device(kpool, vpool, k, v, slots)
+    pages, hkv, page, d = _pools(kpool, vpool)
+    if k.dtype != kpool.dtype or v.dtype != kpool.dtype:
+        raise TypeError(f"k is {k.dtype} and v {v.dtype}, the cache holds {kpool.dtype}")
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous (T,) int64 tensor")
+    T = slots.shape[0]
+    if k.shape != (T, hkv, d) or v.shape != (T, hkv, d):
+        raise ValueError(f"k and v must be ({T}, {hkv}, {d}), got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if T == 0:
+        return
+    k, v = _aligned(k), _aligned(v)
+    strides = _lib.i64_array((*k.stride()[:2], *v.stride()[:2], *kpool.stride()[:3],
+                              *vpool.stride()[:3]))
+    _launch("ssa_paged_append", kpool, k.data_ptr(), v.data_ptr(), kpool.data_ptr(),
+            vpool.data_ptr(), _lib.dtype_code(kpool.dtype), T, hkv, d, pages, page, strides,
+            slots.data_ptr())
+
+
+def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor, k_new: torch.Tensor | None = None,
+                 v_new: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
+                 return_lse: bool = False, out: torch.Tensor | None = None):
+    """Attention of one token per request over its cached keys: q (B, Hq, d), out (B, Hq, d) in
+    q's dtype; request b attends its keys j < lens[b] (with a window, the last `window` of them),
+    softmax(scale * q.k) in fp32, query head h reading key head h // (Hq / Hkv). A request of
+    length 0 (an idle row of the batch) gets zeros and a log-sum of -inf.
+
+    k_new, v_new (B, Hkv, d): the token at position lens[b] - 1, stored into the cache by this
+    call and attended with the rest (the page that holds that position must be the request's own;
+    earlier pages may be shared between requests). return_lse: also the natural log of each row's
+    sum of exponentials (B, Hq) fp32, with which partial results can be joined."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        if k_new is None:
+            o, lse = T.paged_attend(q, kpool, vpool, table, lens, float(scale), int(window))
+        else:
+            o, lse = T.paged_step(q, kpool, vpool, table, lens, k_new, v_new, float(scale),
+                                  int(window))
+        if out is not None:
+            out.copy_(o)
+            o = out
+        return (o, lse) if return_lse else o
+    return _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window,
+                              return_lse, out)
+
+
+def _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, return_lse,
+                       out=None):
+    _one_device(q, kpool, vpool, table, lens, k_new, v_new, out)
+    pages, hkv, page, d = _pools(kpool, vpool)
+    dtype = kpool.dtype
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"q must be (B, Hq, {d}), got {tuple(q.shape)}")
+    B, hq, _ = q.shape
+    if q.dtype != dtype:
+        raise TypeError(f"q is {q.dtype}, the cache holds {dtype}")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
+    if k_new is not None:
+        if k_new.dtype != dtype or v_new.dtype != dtype:
+            raise TypeError(f"k_new is {k_new.dtype} and v_new {v_new.dtype}, the cache holds "
+                            f"{dtype}")
+        if k_new.shape != (B, hkv, d) or v_new.shape != (B, hkv, d):
+            raise ValueError(f"k_new and v_new must be ({B}, {hkv}, {d})")
+        k_new, v_new = _aligned(k_new), _aligned(v_new)
+    rows, W, row = _table(table)
+    if rows != B:
+        raise ValueError(f"table has {rows} rows for {B} requests")
+    _int32("lens", lens, (B,))
+    if out is None:
+        out = torch.empty(B, hq, d, device=q.device, dtype=dtype)
+    elif out.dtype != dtype or out.shape != (B, hq, d) or _aligned(out) is not out:
+        raise ValueError(f"out must be a ({B}, {hq}, {d}) {dtype} tensor with rows of 16-byte "
+                         "pieces")
+    lse = torch.empty(B, hq, device=q.device, dtype=torch.float32) if return_lse else None
+    if B == 0:
+        return (out, lse) if return_lse else out
+    q = _aligned(q)
+    new = (0, 0, 0, 0) if k_new is None else (*k_new.stride()[:2], *v_new.stride()[:2])
+    strides = _lib.i64_array((*q.stride()[:2], *kpool.stride()[:3], *vpool.stride()[:3],
+                              *out.stride()[:2], *new))
+    window = int(window)
+    ws_bytes = _lib.query("ssa_paged_attend_workspace_size", B, hq, hkv, d, W, page, window)
+    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
+    _launch("ssa_paged_attend", q, q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
+            out.data_ptr(), _lib.ptr(lse), _lib.dtype_code(dtype), B, hq, hkv, d, pages, page,
+            table.data_ptr(), row, W, lens.data_ptr(), _lib.ptr(k_new),
+            _lib.ptr(v_new), strides, float(scale), window, _lib.ptr(ws), ws_bytes)
+    return (out, lse) if return_lse else out
+
+
+class PagedCache:
+    """The keys and values of up to `requests` requests in `pages` pages per layer.
+
+    Every layer has a pool of its own; the table and the lengths are shared by the layers, so a
+    step resizes once and then appends and attends layer by layer:
+
+        r = cache.resize(cache.lens + grow, tokens)       # grow (requests,) int32 on the device
+        cache.append(layer, k, v, r.slots)                # a prompt's tokens, or
+        o = cache.step(layer, q, k_new, v_new)            # one token of every request
+
+    A request ends by a resize to length 0. `check` raises if the last resize did not fit (it
+    synchronises; a caller that keeps count of the pages need not call it)."""
+
+    def __init__(self, requests, max_len, pages, hkv, d, page=64, layers=1, dtype=torch.bfloat16,
+                 device="cuda", token_major=False):
+        if min(requests, max_len, pages, hkv, d, page, layers) < 1:
+            raise ValueError("PagedCache: sizes must be positive")
+        if page % 16 or d % 8 or d > 512:
+            raise ValueError(f"PagedCache: pages of a multiple of 16 tokens and head dims of a "
+                             f"multiple of 8 up to 512, got page={page}, d={d}")
+        _lib.dtype_code(dtype)
+        dev = torch.device(device)
+        i32 = dict(device=dev, dtype=torch.int32)
+        self.page = int(page)
+        shape = (layers, pages, page, hkv, d) if token_major else (layers, pages, hkv, page, d)
+        pool = torch.zeros(2, *shape, device=dev, dtype=dtype)
+        if token_major:
+            pool = pool.transpose(3, 4)
+        self.k, self.v = pool[0], pool[1]
+        self.table = torch.full((requests, -(-max_len // page)), -1, **i32)
+        self.lens = torch.zeros(requests, **i32)
+        self.free = torch.arange(pages, **i32).flip(0).contiguous()  # page 0 on top
+        self.nfree = torch.full((1,), pages, **i32)
+        self.status = torch.zeros(1, **i32)
+
+    @torch.no_grad()
+    def resize(self, new_lens: torch.Tensor, tokens: int, out: Resized | None = None) -> Resized:
+        """resize_pages on this cache's state."""
+        r = resize_pages(self.lens, new_lens, self.table, self.free, self.nfree, self.page,
+                         tokens, out)
+        self.status = r.status
+        return r
+
+    def check(self) -> None:
+        """Raises if the last resize changed nothing because it did not fit. Synchronises."""
+        status = int(self.status)
+        if status:
+            raise RuntimeError("resize: " + RESIZE_ERRORS.get(status, f"{status} pages lacking"))
+
+    @torch.no_grad()
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """append_pages into a layer's pools."""
+        append_pages(k, v, self.k[layer], self.v[layer], slots)
+
+    @torch.no_grad()
+    def attend(self, layer: int, q: torch.Tensor, **kwargs):
+        """attend_pages over a layer's pools (scale, window, return_lse, out as there)."""
+        return attend_pages(q, self.k[layer], self.v[layer], self.table, self.lens, **kwargs)
+
+    @torch.no_grad()
+    def step(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+             **kwargs):
+        """attend with the newest token of every request stored first."""
+        return self.attend(layer, q, k_new=k_new, v_new=v_new, **kwargs)
+
+
+__all__ = ["resize_pages", "append_pages", "attend_pages", "PagedCache", "Resized"]

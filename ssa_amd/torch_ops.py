@@ -19,7 +19,13 @@ dtypes. Run eagerly, the public functions call the library directly and skip the
     ssa_amd::decode_step(q, k_new, v_new, kcache!, vcache!, mu!, var!, kv_num!, kv_idx!,
                          workspace!, pos, block, top_c, budget_frac, local, coef2, scale) -> out
                                                                   ssa/ivf_decode.py:128-136
-    (! = written in place; workspace None runs the allocation-free ssa_decode_step_static)
+    ssa_amd::paged_resize(lens!, new_lens, table!, free!, nfree!, page, tokens)
+        -> (slots, pos, cu, status)
+    ssa_amd::paged_append(k, v, kpool!, vpool!, slots)
+    ssa_amd::paged_attend(q, kpool, vpool, table, lens, scale, window) -> (out, lse)
+    ssa_amd::paged_step(q, kpool!, vpool!, table, lens, k_new, v_new, scale, window) -> (out, lse)
+    (! = written in place; workspace None runs the allocation-free ssa_decode_step_static; the
+    reference has no paged cache)
 """
 from __future__ import annotations
 
@@ -151,3 +157,54 @@ def _(q, k_new, v_new, kcache, vcache, mu, var, kv_num, kv_idx, workspace, pos, 
       budget_frac, local, coef2, scale):
     B, Hq, d = q.shape
     return q.new_empty(B, Hq, d, dtype=kcache.dtype)
+
+
+@torch.library.custom_op("ssa_amd::paged_resize", mutates_args=("lens", "table", "free", "nfree"))
+def paged_resize(lens: Tensor, new_lens: Tensor, table: Tensor, free: Tensor, nfree: Tensor,
+                 page: int, tokens: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    from .paged import resize_pages
+    return tuple(resize_pages(lens, new_lens, table, free, nfree, page, tokens))
+
+
+@paged_resize.register_fake
+def _(lens, new_lens, table, free, nfree, page, tokens):
+    return (lens.new_empty(tokens, dtype=torch.int64), lens.new_empty(tokens),
+            lens.new_empty(lens.shape[0] + 1), lens.new_empty(1))
+
+
+@torch.library.custom_op("ssa_amd::paged_append", mutates_args=("kpool", "vpool"))
+def paged_append(k: Tensor, v: Tensor, kpool: Tensor, vpool: Tensor, slots: Tensor) -> None:
+    from .paged import _append_pages_impl
+    _append_pages_impl(k, v, kpool, vpool, slots)
+
+
+@paged_append.register_fake
+def _(k, v, kpool, vpool, slots):
+    return None
+
+
+@torch.library.custom_op("ssa_amd::paged_attend", mutates_args=())
+def paged_attend(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
+                 scale: float, window: int) -> tuple[Tensor, Tensor]:
+    from .paged import _attend_pages_impl
+    return _attend_pages_impl(q, kpool, vpool, table, lens, None, None, scale, window, True)
+
+
+@paged_attend.register_fake
+def _(q, kpool, vpool, table, lens, scale, window):
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            q.new_empty(q.shape[:2], dtype=_F32))
+
+
+@torch.library.custom_op("ssa_amd::paged_step", mutates_args=("kpool", "vpool"))
+def paged_step(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
+               k_new: Tensor, v_new: Tensor, scale: float,
+               window: int) -> tuple[Tensor, Tensor]:
+    from .paged import _attend_pages_impl
+    return _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, True)
+
+
+@paged_step.register_fake
+def _(q, kpool, vpool, table, lens, k_new, v_new, scale, window):
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            q.new_empty(q.shape[:2], dtype=_F32))

@@ -1,0 +1,147 @@
+"""The paged cache without a GPU: arguments refused at the C ABI, shapes of the registered operators,
+and the plain restatement that the GPU tests compare with."""
+import ctypes
+
+import pytest
+import torch
+
+from ssa_amd import _lib
+from ssa_amd import paged as P
+from tests import paged_util as U
+
+FAKE = ctypes.c_void_p(1 << 20)  # never dereferenced: validation fails first
+NULL = None
+
+
+def status(name, *args):
+    return getattr(_lib.lib(), name)(*args)
+
+
+def attend(**kw):
+    """ssa_paged_attend with one argument changed."""
+    a = dict(q=FAKE, kpool=FAKE, vpool=FAKE, out=FAKE, lse=NULL, dtype=_lib.BF16, B=2, Hq=4, Hkv=2,
+             d=64, pages=10, page=16, table=FAKE, table_stride=8, W=8, lens=FAKE, k_new=NULL,
+             v_new=NULL, strides=_lib.i64_array([256, 64, 2048, 1024, 64, 2048, 1024, 64, 256, 64,
+                                                 128, 64, 128, 64]),
+             scale=0.125, window=0, ws=FAKE, ws_bytes=1 << 30)
+    a.update(kw)
+    return status("ssa_paged_attend", *a.values(), None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(q=NULL), _lib.SSA_ERR_INVALID), (dict(lens=NULL), _lib.SSA_ERR_INVALID),
+    (dict(table=NULL), _lib.SSA_ERR_INVALID), (dict(k_new=FAKE), _lib.SSA_ERR_INVALID),
+    (dict(dtype=7), _lib.SSA_ERR_UNSUPPORTED), (dict(d=60), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(d=520), _lib.SSA_ERR_UNSUPPORTED), (dict(page=24), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(page=8), _lib.SSA_ERR_UNSUPPORTED), (dict(page=65552), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(Hq=3), _lib.SSA_ERR_INVALID), (dict(B=0), _lib.SSA_ERR_INVALID),
+    (dict(pages=0), _lib.SSA_ERR_INVALID), (dict(pages=2 ** 31), _lib.SSA_ERR_INVALID),
+    (dict(W=0), _lib.SSA_ERR_INVALID), (dict(W=9), _lib.SSA_ERR_INVALID),
+    (dict(W=2 ** 27, table_stride=2 ** 27), _lib.SSA_ERR_INVALID),
+    (dict(window=-1), _lib.SSA_ERR_INVALID), (dict(window=2 ** 31), _lib.SSA_ERR_INVALID),
+    (dict(q=ctypes.c_void_p((1 << 20) + 8)), _lib.SSA_ERR_INVALID),
+    (dict(strides=_lib.i64_array([256, 64, 2048, 1024, 60] + [64] * 9)), _lib.SSA_ERR_INVALID),
+])
+def test_attend_refuses(change, code):
+    assert attend(**change) == code
+    assert b"ssa_paged_attend" in _lib.lib().ssa_last_error()
+
+
+def test_append_and_resize_refuse():
+    st = _lib.i64_array([128, 64, 128, 64, 2048, 1024, 64, 2048, 1024, 64])
+    ap = lambda k, dt, T, d, page, s=st: status(  # noqa: E731
+        "ssa_paged_append", k, FAKE, FAKE, FAKE, dt, T, 2, d, 10, page, s, FAKE, None)
+    assert ap(NULL, _lib.F16, 4, 64, 16) == _lib.SSA_ERR_INVALID
+    assert ap(FAKE, 9, 4, 64, 16) == _lib.SSA_ERR_UNSUPPORTED
+    assert ap(FAKE, _lib.F16, 4, 20, 16) == _lib.SSA_ERR_UNSUPPORTED
+    assert ap(FAKE, _lib.F16, 4, 64, 20) == _lib.SSA_ERR_UNSUPPORTED
+    assert ap(FAKE, _lib.F16, -1, 64, 16) == _lib.SSA_ERR_INVALID
+    assert ap(FAKE, _lib.F16, 4, 64, 16, _lib.i64_array([65] + [64] * 9)) == _lib.SSA_ERR_INVALID
+    assert ap(FAKE, _lib.F16, 0, 64, 16) == _lib.SSA_OK  # nothing to store, nothing launched
+
+    def rs(lens=FAKE, stride=8, B=2, W=8, page=16, pages=10, slots=FAKE, T=4):
+        return status("ssa_paged_resize", lens, FAKE, FAKE, stride, B, W, page, FAKE, pages, FAKE,
+                      slots, NULL, T, FAKE, FAKE, None)
+    assert rs(lens=NULL) == _lib.SSA_ERR_INVALID
+    assert rs(B=0) == _lib.SSA_ERR_INVALID
+    assert rs(stride=7) == _lib.SSA_ERR_INVALID
+    assert rs(pages=0) == _lib.SSA_ERR_INVALID
+    assert rs(page=17) == _lib.SSA_ERR_UNSUPPORTED
+    assert rs(W=2 ** 27, stride=2 ** 27) == _lib.SSA_ERR_UNSUPPORTED
+    assert rs(T=-1) == _lib.SSA_ERR_INVALID
+    assert rs(slots=NULL) == _lib.SSA_ERR_INVALID
+
+
+def test_cpu_tensors_raise():
+    x = torch.zeros(1, 2, 64)
+    pool = torch.zeros(2, 2, 16, 64)
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.attend_pages(x, pool, pool, i.view(1, 1), i)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.append_pages(x, x, pool, pool, i.long())
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.resize_pages(i, i, i.view(1, 1), i, i, 16, 1)
+    for kw in (dict(page=24), dict(d=60), dict(d=520), dict(pages=0), dict(dtype=torch.int8)):
+        with pytest.raises((ValueError, TypeError)):
+            P.PagedCache(**{**dict(requests=1, max_len=10, pages=2, hkv=1, d=64, device="cpu"),
+                            **kw})
+
+
+def test_another_device_is_made_current(monkeypatch):
+    """A call for tensors of a device that is not the current one runs with that device current."""
+    from types import SimpleNamespace as NS
+    seen = []
+
+    class Device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            seen.append(("in", self.i))
+
+        def __exit__(self, *a):
+            seen.append(("out", self.i))
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 40 + t.device.index)
+    monkeypatch.setattr(_lib, "call", lambda *a: seen.append(a))
+    P._launch("x", NS(device=NS(index=0)), 1)
+    P._launch("y", NS(device=NS(index=1)), 2)
+    assert seen == [("x", 1, 40), ("in", 1), ("y", 2, 41), ("out", 1)]
+    a, b = (NS(device=NS(index=i), is_cuda=True) for i in (0, 1))
+    with pytest.raises(ValueError, match="tensors on"):
+        P._one_device(a, None, b)
+
+
+def test_registered_operators_give_shapes():
+    import ssa_amd  # noqa: F401  (registers the ops)
+    ops = torch.ops.ssa_amd
+    m = dict(device="meta")
+    q = torch.empty(3, 8, 64, dtype=torch.float16, **m)
+    pool = torch.empty(9, 2, 16, 64, dtype=torch.float16, **m)
+    new = torch.empty(3, 2, 64, dtype=torch.float16, **m)
+    lens = torch.empty(3, dtype=torch.int32, **m)
+    table = torch.empty(3, 4, dtype=torch.int32, **m)
+    for out, lse in (ops.paged_attend(q, pool, pool, table, lens, 0.1, 0),
+                     ops.paged_step(q, pool, pool.clone(), table, lens, new, new, 0.1, 5)):
+        assert out.shape == q.shape and out.dtype == q.dtype
+        assert lse.shape == (3, 8) and lse.dtype == torch.float32
+    free, nfree = torch.empty(9, dtype=torch.int32, **m), torch.empty(1, dtype=torch.int32, **m)
+    slots, pos, cu, st = ops.paged_resize(lens, lens.clone(), table, free, nfree, 16, 7)
+    assert slots.shape == pos.shape == (7,) and cu.shape == (4,) and st.shape == (1,)
+    assert slots.dtype == torch.int64 and pos.dtype == cu.dtype == st.dtype == torch.int32
+    assert ops.paged_append(new, new, pool, pool.clone(), slots[:3]) is None
+
+
+def test_plain_state_keeps_every_page_once():
+    import random
+    rng = random.Random(0)
+    s = U.PageState(6, 10, 40, 16)
+    for _ in range(200):
+        new = [rng.randrange(161) if rng.random() < 0.5 else n for n in s.lens]
+        s.resize(new, 2000)
+        used = [x for row, n in zip(s.table, s.lens) for x in row[:-(-n // 16)]]
+        assert sorted(used + s.free) == list(range(40))
+        assert all(x == -1 for row, n in zip(s.table, s.lens) for x in row[-(-n // 16):])
