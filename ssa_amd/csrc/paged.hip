@@ -5,6 +5,8 @@
 // Request b's token j lies in page table[b][j / page] at slot j % page.
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "paged_index.h"
 
@@ -230,14 +232,11 @@ struct AttendParams {
   int64_t qb, qh, ob, oh;                 // elements
   int64_t kpp, kph, kps, vpp, vph, vps;   // elements
   int64_t knb, knh, vnb, vnh;             // elements
+  int RT, items, units;  // row tiles of 16 heads; items aimed at (0: one per request); grid units
+  float* part;           // (item, key head, row tile): accumulators by lane
+  float* part_ml;        // their m and l, 16 each
+  int32_t* info;         // per request: its first item and their number
 };
-
-template <int DT>
-__device__ inline float load_elem(const char* base, int64_t i) {
-  if constexpr (DT == SSA_F32) return ((const float*)base)[i];
-  else if constexpr (DT == SSA_F16) return (float)((const _Float16*)base)[i];
-  else return (float)((const __bf16*)base)[i];
-}
 
 template <int DT>
 __device__ inline void store_elem(char* base, int64_t i, float x) {
@@ -246,82 +245,559 @@ __device__ inline void store_elem(char* base, int64_t i, float x) {
   else ((__bf16*)base)[i] = (__bf16)x;
 }
 
-// The new token's key and value into the slot of position len - 1, an element per thread.
-template <int DT>
-__global__ __launch_bounds__(256) void paged_store_new_kernel(AttendParams p) {
-  const int b = blockIdx.y, h = blockIdx.x;
-  const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
-  if (s.len == 0) return;
-  const int e = (s.len - 1) / p.page, off = (s.len - 1) - e * p.page;
-  const int64_t pg = p.table[b * p.table_stride + e];
-  if (pg < 0 || pg >= p.pages) return;
-  for (int c = threadIdx.x; c < p.d; c += 256) {
-    store_elem<DT>(p.kpool, pg * p.kpp + h * p.kph + off * p.kps + c,
-                   load_elem<DT>(p.k_new, b * p.knb + h * p.knh + c));
-    store_elem<DT>(p.vpool, pg * p.vpp + h * p.vph + off * p.vps + c,
-                   load_elem<DT>(p.v_new, b * p.vnb + h * p.vnh + c));
+// How a call is laid out, by type and padded head dim DP. The 16-bit products take 32 keys at once
+// (two subtiles), the fp32 ones 4, so their tile is one subtile where registers are short.
+template <int DT, int DP>
+struct Tile {
+  static constexpr int ES = DT == SSA_F32 ? 4 : 2;
+  static constexpr int NT = DT == SSA_F32 && DP > 64 ? 1 : 2;  // subtiles of 16 keys
+  static constexpr int NC = DP * ES / 64;                      // 64-byte chunks of a key row
+  static constexpr int CB = DT == SSA_F32 ? 64 : DP < 128 ? DP : 128;  // columns of a value block
+  static constexpr int LC = CB / 16;                           // of them a lane's
+  static constexpr int LW = LC * ES / 4;                       // in words
+  static constexpr int VB = DP / CB;
+  static constexpr int NA = DP / 16;  // accumulators of 16 columns x 16 heads
+  static constexpr bool kQInLds = NC >= 8;  // queries: registers are short
+  // fp16 weights are taken up to 2^14 so that the small ones keep their bits
+  static constexpr float kShift = DT == SSA_F16 ? 14.0f : 0.0f;
+};
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// One item of a call: the subtiles [begin, end) of request b, item j of n; `first_item` is the index
+// of the request's item 0 among all.
+struct Item {
+  int b, j, n, begin, end, first_item;
+  PagedSpan span;
+};
+
+// Finds item `index` from the lengths alone, each wave for itself: every lane sums a run of
+// requests, the wave adds the runs up. False past the last item.
+__device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
+  const int lane = threadIdx.x & 63;
+  if (p.items == 0) {  // an item per request
+    it.b = index;
+    it.span = paged_span(p.lens[index], p.window, p.cap);
+    it.j = 0;
+    it.n = 1;
+    it.first_item = index;
+    const int units = paged_units(it.span);
+    const PagedRange r = paged_item_range(it.span, units, 0, 1);
+    it.begin = r.begin;
+    it.end = units ? r.end : r.begin;
+    return true;
+  }
+  const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
+  int64_t units = 0;
+  for (int b = b0; b < b1; ++b) units += paged_units(paged_span(p.lens[b], p.window, p.cap));
+  for (int off = 32; off >= 1; off >>= 1) units += __shfl_xor(units, off);
+  const int chunk = paged_chunk(units, p.items);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += paged_items(paged_units(paged_span(p.lens[b], p.window, p.cap)), chunk);
+  int upto = mine;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(upto, off);
+    if (lane >= off) upto += y;
+  }
+  const unsigned long long past = __ballot(upto > index);
+  if (past == 0) return false;
+  const int owner = __builtin_ctzll(past);
+  int at = uniform(__builtin_amdgcn_readlane(upto - mine, owner));
+  for (int b = uniform(owner * run);; ++b) {
+    const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
+    const int u = paged_units(s), n = paged_items(u, chunk);
+    if (index < at + n) {
+      it.b = b;
+      it.j = index - at;
+      it.n = n;
+      it.first_item = at;
+      it.span = s;
+      const PagedRange r = paged_item_range(s, u, it.j, n);
+      it.begin = r.begin;
+      it.end = r.end;
+      return true;
+    }
+    at += n;
   }
 }
 
-// One wave per (request, query head): 64 keys at a time, a key's score per lane, the running maximum
-// and sum in fp32, the values added up with a lane's columns in registers.
+__device__ inline Item uniform(const Item& x) {
+  return Item{uniform(x.b),     uniform(x.j),   uniform(x.n),
+              uniform(x.begin), uniform(x.end), uniform(x.first_item),
+              PagedSpan{uniform(x.span.first), uniform(x.span.len), uniform((int)x.span.ok) != 0}};
+}
+
+// A wave's running softmax over its keys for 16 query heads: lane l holds head l % 16, accumulator
+// (vb, e) the columns vb CB + LC (4 (l / 16) + r) + e, r = 0..3. m: the largest score (log2 units),
+// l: sum of 2^(score - m + kShift) over the lane's own keys until they are added up.
+template <int NA>
+struct Softmax {
+  float m, l;
+  f32x4 acc[NA];
+};
+
+// Scales (m, l, acc) of two disjoint key sets to their common maximum and adds them.
+template <int NA>
+__device__ inline void join(Softmax<NA>& a, float m, float l, const f32x4* acc, int stride) {
+  const float mx = fmaxf(a.m, m), base = mx == -INFINITY ? 0.0f : mx;
+  const float x = __builtin_amdgcn_exp2f(a.m - base), y = __builtin_amdgcn_exp2f(m - base);
+  a.m = mx;
+  a.l = a.l * x + l * y;
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    const f32x4 o = acc[i * stride];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a.acc[i][r] = a.acc[i][r] * x + o[r] * y;
+  }
+}
+
+__device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c, bool bf16) {
+  if (bf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// A weight as the sum of two 16-bit parts, both positive where it is: the first takes the leading
+// bits of a little less than the weight, the second the rest. With one 16-bit weight the output
+// would be off by as much again as its own rounding; a second part of the other sign, or zero, would
+// turn an infinite value into NaN.
 template <int DT>
-__global__ __launch_bounds__(64) void paged_attend_rows_kernel(AttendParams p) {
-  __shared__ float qs[512], ps[64];
-  __shared__ int64_t vs[64];
-  const int lane = threadIdx.x, b = blockIdx.y, h = blockIdx.x, g = h / p.G;
-  const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
-  for (int c = lane; c < p.d; c += 64) qs[c] = load_elem<DT>(p.q, b * p.qb + h * p.qh + c);
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, acc[8] = {};
-  bool bad = !s.ok;
-  for (int j0 = s.first; j0 < s.len; j0 += 64) {
-    const int j = j0 + lane, n = min(64, s.len - j0);
-    float x = -INFINITY;
-    int64_t vrow = 0;
-    if (j < s.len) {
-      const int e = j / p.page, off = j - e * p.page;
-      int64_t pg = p.table[b * p.table_stride + e];
-      if (pg < 0 || pg >= p.pages) {
-        bad = true;
-        pg = 0;
+__device__ inline void split2(float p0, float p1, unsigned int& hi, unsigned int& lo) {
+  if constexpr (DT == SSA_BF16) {
+    const float less = 1.0f - 0x1p-8f;
+    const unsigned int a = __float_as_uint(p0 * less) & 0xffff0000u;
+    const unsigned int b = __float_as_uint(p1 * less) & 0xffff0000u;
+    hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 r = {(__bf16)(p0 - __uint_as_float(a)), (__bf16)(p1 - __uint_as_float(b))};
+    lo = __builtin_bit_cast(unsigned int, r);
+  } else {
+    const float less = 1.0f - 0x1p-11f;
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 * less, p1 * less));
+    hi = __builtin_bit_cast(unsigned int, h);
+    lo = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0],
+                                                                     p1 - (float)h[1]));
+  }
+}
+
+template <int W>
+struct Words {
+  unsigned int w[W];
+};
+
+// Loads through a buffer descriptor: a uniform base, a lane's 32-bit offset; an offset past the
+// descriptor's size reads as zero and touches no memory.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr int kSpan = 0x7fffffff, kOutside = -0x7fffffff - 1;
+
+__device__ inline Buffer buffer_at(const char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, kSpan, 0x00027000);
+}
+
+__device__ inline u32x4 load16(Buffer b, int off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+
+template <int W>
+__device__ inline Words<W> load_words(Buffer b, int off) {
+  if constexpr (W == 4)
+    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+  else
+    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
+}
+
+template <int W>
+__device__ inline void store_words(char* p, const Words<W>& r) {
+  if constexpr (W == 4) *(u32x4*)p = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+  else *(uint2*)p = uint2{r.w[0], r.w[1]};
+}
+
+// The rows of a lane's keys and values as they come from the cache, in the layouts of the products'
+// operands: keys lane l: row l % 16 of the subtile, 16 bytes at 64 c + 16 (l / 16) (the columns'
+// order within a product does not matter: queries lie alike); values: rows 4 (l / 16) + r, the
+// columns of Softmax.
+template <int DT, int DP>
+struct Rows {
+  using T = Tile<DT, DP>;
+  u32x4 k[T::NT][T::NC];
+  Words<T::LW> v[T::NT][4][T::VB];
+};
+
+// One wave stores the new token's key and value into the slot of position j. Its own later loads see
+// them; the row tiles of a key head each store the same bytes rather than wait for one another.
+template <int ES>
+__device__ inline void store_new(const AttendParams& p, int b, int g, int j) {
+  const int e = j / p.page, lane = threadIdx.x & 63;
+  const int64_t pg = p.table[b * p.table_stride + e], off = j - e * p.page;
+  if (pg >= 0 && pg < p.pages) {
+    for (int c = lane * 16; c < p.d * ES; c += 64 * 16) {
+      const u32x4 k = *(const u32x4*)(p.k_new + (b * p.knb + g * p.knh) * ES + c);
+      const u32x4 v = *(const u32x4*)(p.v_new + (b * p.vnb + g * p.vnh) * ES + c);
+      *(u32x4*)(p.kpool + (pg * p.kpp + g * p.kph + off * p.kps) * ES + c) = k;
+      *(u32x4*)(p.vpool + (pg * p.vpp + g * p.vph + off * p.vps) * ES + c) = v;
+    }
+  }
+  wave_lds_sync();
+}
+
+// Attention over one item by NW waves. Scores are K Q^T: a product's result then has a head per lane
+// column and the keys in the very order that the second product, V^T P^T, takes its weights in, so
+// weights never move between lanes and a head's statistics belong to its lanes. Bound by the reading of K
+// and V: a wave's next keys are in flight while it weighs the current values and the other way round.
+template <int DT, int DP, int NW, int WPE>
+__global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams p) {
+  using T = Tile<DT, DP>;
+  constexpr int NT = T::NT, NC = T::NC, VB = T::VB, LC = T::LC, LW = T::LW, NA = T::NA;
+  __shared__ f32x4 red[NW / 2][NA][64];
+  __shared__ float red_m[NW / 2][64], red_l[NW / 2][64];
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  // row tiles of one (item, key head) are 8 workgroups apart: on one XCD, whose L2 they share
+  const int id = blockIdx.x, rt = (id >> 3) % p.RT, unit = (id >> 3) / p.RT * 8 + (id & 7);
+  const int g = unit % p.Hkv;
+  Item found;
+  if (unit >= p.units || !find_item(p, unit / p.Hkv, found)) return;
+  const Item it = uniform(found);
+  const int first = it.span.first, len = it.span.len;
+  const int head = rt * 16 + col;
+  const bool live = head < p.G;
+  const int tiles = (it.end - it.begin + NT - 1) / NT;
+  const int i0 = uniform((int)((int64_t)tiles * wv / NW));
+  const int i1 = uniform((int)((int64_t)tiles * (wv + 1) / NW));
+
+  __shared__ u32x4 q_lds[T::kQInLds ? NC : 1][64];
+  u32x4 q[T::kQInLds ? 1 : NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (T::kQInLds && c % NW != wv) continue;
+    const int at = c * 64 + grp * 16;
+    u32x4 x = {0, 0, 0, 0};
+    if (live && at < p.d * T::ES)
+      x = *(const u32x4*)(p.q + (it.b * p.qb + (int64_t)(g * p.G + head) * p.qh) * T::ES + at);
+    if constexpr (T::kQInLds) q_lds[c][lane] = x;
+    else q[c] = x;
+  }
+  if constexpr (T::kQInLds) __syncthreads();
+
+  const char* const kbase = p.kpool + g * p.kph * T::ES;
+  const char* const vbase = p.vpool + g * p.vph * T::ES;
+  const int64_t kpp = p.kpp * T::ES, vpp = p.vpp * T::ES;
+  const int kps = (int)p.kps * T::ES, vps = (int)p.vps * T::ES, row_bytes = p.d * T::ES;
+  const int32_t* const row = p.table + it.b * p.table_stride;
+
+  // page and offset of 64 subtiles at a time, one per lane; the next 64 are on their way
+  int pid = 0, poff = 0, pid_next = 0, batch = it.begin + i0 * NT;
+  unsigned long long bad = 0;
+  const int sub_end = min(it.begin + i1 * NT, it.end);
+  auto pages_at = [&](int s) {
+    s += lane;
+    return s < sub_end ? row[s * 16 / p.page] : 0;
+  };
+  auto take_pages = [&](int x) {
+    bad |= __ballot(x < 0 || x >= p.pages);
+    pid = x < 0 || x >= p.pages ? 0 : x;
+    const int j = (batch + lane) * 16;
+    poff = j - j / p.page * p.page;
+  };
+  if (i0 < i1) {
+    const int x = pages_at(batch);
+    pid_next = pages_at(batch + 64);
+    if (p.k_new && sub_end * 16 >= len) store_new<T::ES>(p, it.b, g, len - 1);
+    take_pages(x);
+  }
+
+  Rows<DT, DP> rows;
+  Softmax<NA> st;
+  st.m = -INFINITY;
+  st.l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NA; ++i) st.acc[i] = f32x4{0, 0, 0, 0};
+
+  // pages of tile i's subtiles (the last one again past the wave's end)
+  int64_t pg[NT];
+  int off[NT];
+  auto locate = [&](int i) {
+    const int s = it.begin + i * NT;
+    if (s >= batch + 64) {
+      batch += 64;
+      take_pages(pid_next);
+      pid_next = pages_at(batch + 64);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int x = min(s + t, sub_end - 1) - batch;
+      pg[t] = __builtin_amdgcn_readlane(pid, x);
+      off[t] = __builtin_amdgcn_readlane(poff, x);
+    }
+  };
+  const int koff = col * kps + grp * 16;
+  int vcol[VB];
+#pragma unroll
+  for (int vb = 0; vb < VB; ++vb) {
+    const int c = vb * T::CB * T::ES + col * LW * 4;
+    vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
+  }
+  auto load_k = [&](int i) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Buffer src = buffer_at(kbase + (pg[t] * kpp + (int64_t)off[t] * kps));
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        rows.k[t][c] = load16(src, c * 64 + grp * 16 < row_bytes ? koff + c * 64 : kOutside);
+    }
+  };
+  auto load_v = [&](int i) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Buffer src = buffer_at(vbase + (pg[t] * vpp + (int64_t)off[t] * vps));
+      // rows that do not count may hold anything: read as zero
+      const int lo = max(first - (it.begin + i * NT + t) * 16, 0);
+      const int count = min(len - (it.begin + i * NT + t) * 16, 16) - lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = grp * 4 + r, at = (unsigned)(n - lo) < (unsigned)max(count, 0) ? n * vps
+                                                                                    : kOutside;
+#pragma unroll
+        for (int vb = 0; vb < VB; ++vb) rows.v[t][r][vb] = load_words<LW>(src, at + vcol[vb]);
       }
-      const int64_t krow = pg * p.kpp + g * p.kph + off * p.kps;
-      vrow = pg * p.vpp + g * p.vph + off * p.vps;
-      x = 0.0f;
-      for (int c = 0; c < p.d; ++c) x += qs[c] * load_elem<DT>(p.kpool, krow + c);
-      x *= p.scale_log2;
     }
-    float mx = x;
-    for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, lane_xor(mx, off));
-    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.0f : mn;
-    const float w = exp2f(x - base), a = exp2f(m - base);
-    float sum = w;
-    for (int off = 32; off >= 1; off >>= 1) sum += lane_xor(sum, off);
-    l = l * a + sum;
-    m = mn;
-    ps[lane] = w;
-    vs[lane] = vrow;
-    __syncthreads();
+  };
+
+  if (i0 < i1) {
+    locate(i0);
+    load_k(i0);
+    load_v(i0);
+  }
+  for (int i = i0; i < i1; ++i) {
+    const int j0 = (it.begin + i * NT) * 16;
+    const bool edge = j0 < first || j0 + NT * 16 > len;
+    if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
+    // scores: lane column a head, rows the keys 4 grp + r of each subtile
+    f32x4 s[NT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = lane + 64 * i;
-      if (c >= p.d) break;
-      float y = acc[i] * a;
-      for (int t = 0; t < n; ++t) y += ps[t] * load_elem<DT>(p.vpool, vs[t] + c);
-      acc[i] = y;
+    for (int t = 0; t < NT; ++t) s[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      u32x4 qc;
+      if constexpr (T::kQInLds) qc = q_lds[c][lane];
+      else qc = q[c];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (DT == SSA_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned int a = rows.k[t][c][e], b = qc[e];
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b),
+                                                        s[t], 0, 0, 0);
+          }
+        } else {
+          s[t] = mfma16(rows.k[t][c], qc, s[t], DT == SSA_BF16);
+        }
+      }
     }
+    const bool more = i + 1 < i1;
+    if (more) {
+      locate(i + 1);
+      load_k(i + 1);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = s[t][r] * p.scale_log2;
+        if (edge) {
+          const int j = j0 + t * 16 + grp * 4 + r;
+          if (j < first || j >= len) x = -INFINITY;
+        }
+        s[t][r] = x;
+        mx = fmaxf(mx, x);
+      }
+    mx = fmaxf(mx, lane_xor(mx, 16));
+    mx = fmaxf(mx, lane_xor(mx, 32));
+    if (__any(mx > st.m)) {
+      const float m = fmaxf(st.m, mx), a = __builtin_amdgcn_exp2f(st.m - m);
+      st.m = m;
+      st.l *= a;
+#pragma unroll
+      for (int n = 0; n < NA; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.acc[n][r] *= a;
+    }
+    const float base = (st.m == -INFINITY ? 0.0f : st.m) - T::kShift;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
+        sum += s[t][r];
+      }
+    st.l += sum;
+    if constexpr (DT == SSA_F32) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+            for (int e = 0; e < LC; ++e)
+              st.acc[vb * LC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __uint_as_float(rows.v[t][r][vb].w[e]), s[t][r], st.acc[vb * LC + e], 0, 0, 0);
+    } else {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          unsigned int a, b;
+          split2<DT>(s[t][2 * h], s[t][2 * h + 1], a, b);
+          hi[2 * t + h] = a;
+          lo[2 * t + h] = b;
+        }
+#pragma unroll
+      for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+        for (int e = 0; e < LC; ++e) {
+          // column e of the lane's values, key after key
+          u32x4 vt;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              vt[2 * t + h] = __builtin_amdgcn_perm(
+                  rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
+                  e % 2 ? 0x07060302u : 0x05040100u);
+          f32x4& acc = st.acc[vb * LC + e];
+          acc = mfma16(vt, hi, acc, DT == SSA_BF16);
+          acc = mfma16(vt, lo, acc, DT == SSA_BF16);
+        }
+    }
+    if (more) load_v(i + 1);
+  }
+  st.l += lane_xor(st.l, 16);
+  st.l += lane_xor(st.l, 32);
+  if (bad != 0 || !it.span.ok) st.l = NAN;
+
+  // the waves' results, half of them into the other half at a time
+#pragma unroll
+  for (int half = NW / 2; half >= 1; half >>= 1) {
+    if (wv >= half && wv < 2 * half) {
+      red_m[wv - half][lane] = st.m;
+      red_l[wv - half][lane] = st.l;
+#pragma unroll
+      for (int n = 0; n < NA; ++n) red[wv - half][n][lane] = st.acc[n];
+    }
+    __syncthreads();
+    if (wv < half) join(st, red_m[wv][lane], red_l[wv][lane], &red[wv][0][lane], 64);
     __syncthreads();
   }
-  bad = __any(bad);
-  const float inv = s.len == 0 ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = lane + 64 * i;
-    if (c < p.d) store_elem<DT>(p.out, b * p.ob + h * p.oh + c, bad ? NAN : acc[i] * inv);
+  if (wv != 0) return;
+
+  if (p.items != 0 && it.j == 0 && g == 0 && rt == 0 && lane == 0) {
+    p.info[2 * it.b] = it.first_item;
+    p.info[2 * it.b + 1] = it.n;
   }
-  if (p.lse && lane == 0)
-    p.lse[(int64_t)b * p.Hq + h] = bad ? NAN : s.len == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (it.n > 1) {
+    const int64_t part = (int64_t)(unit / p.Hkv * p.Hkv + g) * p.RT + rt;
+    if (live) {
+#pragma unroll
+      for (int n = 0; n < NA; ++n) ((f32x4*)p.part)[(part * NA + n) * 64 + lane] = st.acc[n];
+      if (grp == 0) {
+        p.part_ml[part * 32 + col] = st.m;
+        p.part_ml[part * 32 + 16 + col] = st.l;
+      }
+    }
+    return;
+  }
+  if (!live) return;
+  const float inv = len == 0 && it.span.ok ? 0.0f : 1.0f / st.l;
+  const int64_t h = g * p.G + head;
+  char* const to = p.out + (it.b * p.ob + h * p.oh) * T::ES;
+#pragma unroll
+  for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = vb * T::CB + LC * (grp * 4 + r);
+      if (c >= p.d) continue;
+      Words<LW> w;
+      if constexpr (DT == SSA_F32) {
+#pragma unroll
+        for (int e = 0; e < LC; ++e) {
+          const float x = st.acc[vb * LC + e][r] * inv;
+          w.w[e] = __float_as_uint(x);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < LC; e += 2) {
+          const float x = st.acc[vb * LC + e][r] * inv, y = st.acc[vb * LC + e + 1][r] * inv;
+          unsigned short a, b;
+          if constexpr (DT == SSA_BF16) {
+            a = __builtin_bit_cast(unsigned short, (__bf16)x);
+            b = __builtin_bit_cast(unsigned short, (__bf16)y);
+          } else {
+            a = __builtin_bit_cast(unsigned short, (_Float16)x);
+            b = __builtin_bit_cast(unsigned short, (_Float16)y);
+          }
+          w.w[e / 2] = a | (unsigned int)b << 16;
+        }
+      }
+      store_words<LW>(to + c * T::ES, w);
+    }
+  if (p.lse && grp == 0)
+    p.lse[(int64_t)it.b * p.Hq + h] = len == 0 && it.span.ok ? -INFINITY
+        : (st.m - T::kShift + __builtin_amdgcn_logf(st.l)) * kLn2;
+}
+
+// Joins a request's parts: a workgroup per accumulator of a (request, key head, row tile), its waves
+// taking every NW-th part. Rows without keys, and of lengths that do not fit, are answered here.
+template <int DT, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_join_kernel(AttendParams p) {
+  using T = Tile<DT, DP>;
+  constexpr int NA = T::NA, LC = T::LC;
+  __shared__ f32x4 red[NW][64];
+  __shared__ float red_m[NW][64], red_l[NW][64];
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int b = blockIdx.y, n = blockIdx.x % NA, g = blockIdx.x / NA / p.RT;
+  const int rt = blockIdx.x / NA % p.RT, head = rt * 16 + col;
+  const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
+  Softmax<1> st;
+  st.m = -INFINITY;
+  st.l = s.ok ? 0.0f : NAN;
+  st.acc[0] = f32x4{0, 0, 0, 0};
+  if (s.len > 0) {
+    const int first = p.info[2 * b], parts = p.info[2 * b + 1];
+    if (parts <= 1) return;  // written by its one item
+    for (int i = wv; i < parts; i += NW) {
+      const int64_t part = ((int64_t)(first + i) * p.Hkv + g) * p.RT + rt;
+      if (head < p.G)
+        join(st, p.part_ml[part * 32 + col], p.part_ml[part * 32 + 16 + col],
+             (const f32x4*)p.part + (part * NA + n) * 64 + lane, 0);
+    }
+    red_m[wv][lane] = st.m;
+    red_l[wv][lane] = st.l;
+    red[wv][lane] = st.acc[0];
+    __syncthreads();
+    if (wv != 0) return;
+    for (int w = 1; w < NW; ++w) join(st, red_m[w][lane], red_l[w][lane], &red[w][lane], 0);
+  }
+  if (wv != 0 || head >= p.G) return;
+  const float inv = s.len == 0 && s.ok ? 0.0f : 1.0f / st.l;
+  const int64_t h = g * p.G + head;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int c = n / LC * T::CB + LC * (grp * 4 + r) + n % LC;
+    if (c < p.d) store_elem<DT>(p.out, b * p.ob + h * p.oh + c, st.acc[0][r] * inv);
+  }
+  if (p.lse && grp == 0 && n == 0)
+    p.lse[(int64_t)b * p.Hq + h] = s.len == 0 && s.ok ? -INFINITY
+        : (st.m - T::kShift + __builtin_amdgcn_logf(st.l)) * kLn2;
 }
 
 bool fits_int(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
@@ -344,6 +820,52 @@ int check_pool(const char* who, int dtype, int64_t Hkv, int64_t d, int64_t pages
   SSA_REQUIRE(page > 0 && page % 16 == 0 && page <= 65536, SSA_ERR_UNSUPPORTED,
               "%s: page of %lld tokens (a multiple of 16 up to 65536)", who, (long long)page);
   return SSA_OK;
+}
+
+// How a call of these sizes is cut: known on the host without the lengths.
+struct Layout {
+  int64_t RT, items, max_items;  // items: 0 when every request is one item
+  int dp;
+  size_t part, part_ml, info, bytes;  // offsets into the workspace
+};
+
+Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
+              int64_t window) {
+  Layout y{};
+  y.RT = (Hq / Hkv + 15) / 16;
+  y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
+  const int64_t units = paged_most_units(W * page, (int)window);
+  const int64_t target = y.dp <= 128 ? 1024 : y.dp <= 256 ? 512 : 256;
+  y.items = units <= 1 ? 0 : std::max<int64_t>(1, target / (Hkv * y.RT));
+  y.max_items = y.items == 0 ? B : paged_most_items(B, y.items, units);
+  if (y.items == 0) return y;
+  const size_t parts = (size_t)y.max_items * Hkv * y.RT;
+  y.part_ml = parts * 16 * y.dp * 4;
+  y.info = y.part_ml + parts * 32 * 4;
+  y.bytes = (y.info + (size_t)B * 8 + 15) / 16 * 16;
+  return y;
+}
+
+template <int DT, int DP, int WPE>
+int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
+  constexpr int NW = 4;
+  paged_attend_kernel<DT, DP, NW, WPE><<<(unsigned)blocks, NW * 64, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_attend_kernel"));
+  if (p.items == 0) return SSA_OK;
+  const dim3 grid((unsigned)(DP / 16 * p.RT * p.Hkv), (unsigned)p.B);
+  if (p.items > 32) paged_join_kernel<DT, DP, 16><<<grid, 1024, 0, st>>>(p);
+  else paged_join_kernel<DT, DP, 4><<<grid, 256, 0, st>>>(p);
+  return launch_status("paged_join_kernel");
+}
+
+template <int DT>
+int run_attend_dim(const AttendParams& p, int dp, int64_t blocks, hipStream_t st) {
+  switch (dp) {
+    case 64: return run_attend<DT, 64, DT == SSA_F32 ? 3 : 4>(p, blocks, st);
+    case 128: return run_attend<DT, 128, 3>(p, blocks, st);
+    case 256: return run_attend<DT, 256, 2>(p, blocks, st);
+    default: return run_attend<DT, 512, 1>(p, blocks, st);
+  }
 }
 
 }  // namespace
@@ -408,7 +930,10 @@ extern "C" int ssa_paged_append(const void* k, const void* v, void* kpool, void*
 
 extern "C" size_t ssa_paged_attend_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t d,
                                                   int64_t W, int64_t page, int64_t window) {
-  return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 || W <= 0 || page <= 0 ||
+      !fits_int(window) || W > 0x7fffffff / page)
+    return 0;
+  return layout(B, Hq, Hkv, d, W, page, window).bytes;
 }
 
 extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* lse,
@@ -438,26 +963,46 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
                   (!k_new || (rows16(k_new, strides + 10, 2, es) &&
                               rows16(v_new, strides + 12, 2, es))),
               SSA_ERR_INVALID, "ssa_paged_attend: rows must start at multiples of 16 bytes");
-  AttendParams p{(const char*)q, (char*)kpool, (char*)vpool, (char*)out, lse, (const char*)k_new,
-                 (const char*)v_new, table, lens, table_stride, W * page, pages, (int)B, (int)Hq,
-                 (int)Hkv, (int)(Hq / Hkv), (int)d, (int)page, (int)window, scale * kLog2e,
-                 strides[0], strides[1], strides[8], strides[9], strides[2], strides[3],
-                 strides[4], strides[5], strides[6], strides[7],
-                 k_new ? strides[10] : 0, k_new ? strides[11] : 0, k_new ? strides[12] : 0,
-                 k_new ? strides[13] : 0};
-  hipStream_t st = (hipStream_t)stream;
-  const dim3 new_grid((unsigned)Hkv, (unsigned)B), grid((unsigned)Hq, (unsigned)B);
-#define SSA_PAGED_RUN(DT)                                             \
-  do {                                                                \
-    if (k_new) {                                                      \
-      paged_store_new_kernel<DT><<<new_grid, 256, 0, st>>>(p);        \
-      SSA_TRY(launch_status("paged_store_new_kernel"));               \
-    }                                                                 \
-    paged_attend_rows_kernel<DT><<<grid, 64, 0, st>>>(p);             \
-  } while (0)
-  if (dtype == SSA_F32) SSA_PAGED_RUN(SSA_F32);
-  else if (dtype == SSA_F16) SSA_PAGED_RUN(SSA_F16);
-  else SSA_PAGED_RUN(SSA_BF16);
-#undef SSA_PAGED_RUN
-  return launch_status("paged_attend_rows_kernel");
+  SSA_REQUIRE(strides[4] < (1 << 24) && strides[7] < (1 << 24), SSA_ERR_UNSUPPORTED,
+              "ssa_paged_attend: slots 2^24 elements apart or more");
+  const Layout y = layout(B, Hq, Hkv, d, W, page, window);
+  SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
+              SSA_ERR_WORKSPACE, "ssa_paged_attend: needs a 16-byte aligned workspace of %zu bytes, "
+              "got %zu", y.bytes, workspace_bytes);
+  AttendParams p{};
+  p.q = (const char*)q;
+  p.kpool = (char*)kpool;
+  p.vpool = (char*)vpool;
+  p.out = (char*)out;
+  p.lse = lse;
+  p.k_new = (const char*)k_new;
+  p.v_new = (const char*)v_new;
+  p.table = table;
+  p.lens = lens;
+  p.table_stride = table_stride;
+  p.cap = W * page;
+  p.pages = pages;
+  p.B = (int)B;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.G = (int)(Hq / Hkv);
+  p.d = (int)d;
+  p.page = (int)page;
+  p.window = (int)window;
+  p.scale_log2 = scale * kLog2e;
+  int64_t* const st[14] = {&p.qb, &p.qh, &p.kpp, &p.kph, &p.kps, &p.vpp, &p.vph,
+                           &p.vps, &p.ob, &p.oh, &p.knb, &p.knh, &p.vnb, &p.vnh};
+  for (int i = 0; i < (k_new ? 14 : 10); ++i) *st[i] = strides[i];
+  p.RT = (int)y.RT;
+  p.items = (int)y.items;
+  p.part = (float*)workspace;
+  p.part_ml = (float*)((char*)workspace + y.part_ml);
+  p.info = (int32_t*)((char*)workspace + y.info);
+  const int64_t units = y.max_items * Hkv, blocks = (units + 7) / 8 * 8 * y.RT;
+  SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_attend: too many rows in one call");
+  p.units = (int)units;
+  hipStream_t stream_ = (hipStream_t)stream;
+  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, blocks, stream_);
+  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, blocks, stream_);
+  return run_attend_dim<SSA_BF16>(p, y.dp, blocks, stream_);
 }

@@ -30,4 +30,47 @@ SSA_HD PagedSpan paged_span(int len, int window, int64_t cap) {
 
 SSA_HD int paged_pages(int len, int page) { return (int)(((int64_t)len + page - 1) / page); }
 
+// A request's keys are cut at multiples of 16 (a subtile, never across pages: pages hold a multiple
+// of 16 tokens) and dealt out in units of kPagedUnit subtiles.
+constexpr int kPagedUnit = 8;
+
+SSA_HD int paged_units(const PagedSpan& s) {
+  if (s.len == 0) return 0;
+  const int subtiles = (s.len - 1) / 16 + 1 - s.first / 16;
+  return (subtiles + kPagedUnit - 1) / kPagedUnit;
+}
+
+// The most units a request can have: its table row's keys, or its window's from any offset.
+SSA_HD int64_t paged_most_units(int64_t cap, int window) {
+  const int64_t keys = window > 0 && (int64_t)window + 15 < cap ? (int64_t)window + 15 : cap;
+  return (keys + 16 * kPagedUnit - 1) / (16 * kPagedUnit);
+}
+
+// The most items that B requests make when a call aims at `items`.
+SSA_HD int64_t paged_most_items(int64_t B, int64_t items, int64_t most_units) {
+  const int64_t cut = items + B, all = B * most_units;
+  return cut < all ? cut : all;
+}
+
+// Units per item so that a call's `units` make at most `items` items besides one more per request.
+SSA_HD int paged_chunk(int64_t units, int64_t items) {
+  return units <= items ? 1 : (int)((units + items - 1) / items);
+}
+
+SSA_HD int paged_items(int units, int chunk) { return (units + chunk - 1) / chunk; }
+
+// Subtiles [begin, end) of item j of n: the request's units spread evenly over its items.
+struct PagedRange {
+  int begin, end;
+};
+
+SSA_HD PagedRange paged_item_range(const PagedSpan& s, int units, int j, int n) {
+  const int a = s.first / 16, last = (s.len - 1) / 16 + 1;
+  PagedRange r;
+  r.begin = a + (int)((int64_t)units * j / n) * kPagedUnit;
+  r.end = a + (int)((int64_t)units * (j + 1) / n) * kPagedUnit;
+  if (r.end > last) r.end = last;
+  return r;
+}
+
 }  // namespace ssa

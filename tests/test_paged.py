@@ -145,3 +145,20 @@ def test_plain_state_keeps_every_page_once():
         used = [x for row, n in zip(s.table, s.lens) for x in row[:-(-n // 16)]]
         assert sorted(used + s.free) == list(range(40))
         assert all(x == -1 for row, n in zip(s.table, s.lens) for x in row[-(-n // 16):])
+
+
+def test_items_cover_every_key_once(tmp_path):
+    """csrc/paged_index.h compiled for the host: lengths and page tables that do not fit are answered
+    there, items cover the attended keys exactly and fit the workspace."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if cxx is None:
+        pytest.skip("no host compiler")
+    exe = tmp_path / "check"
+    subprocess.run([cxx, "-std=c++17", "-O1", f"-I{root / 'ssa_amd' / 'csrc'}", str(root / "tests/paged_index_check.cpp"),
+                    "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
