@@ -232,18 +232,31 @@ struct AttendParams {
   int64_t qb, qh, ob, oh;                 // elements
   int64_t kpp, kph, kps, vpp, vph, vps;   // elements
   int64_t knb, knh, vnb, vnh;             // elements
+  PageDiv div;           // by the subtiles of a page
   int RT, items, units;  // row tiles of 16 heads; items aimed at (0: one per request); grid units
-  float* part;           // (item, key head, row tile): accumulators by lane
-  float* part_ml;        // their m and l, 16 each
+  float* part;           // (item, query head, DP): parts of rows that several items share
+  float* part_ml;        // (item, query head, 2): their m and l
   int32_t* info;         // per request: its first item and their number
 };
 
+// Four values at element i (a multiple of 4) of a row, rounded to the type.
 template <int DT>
-__device__ inline void store_elem(char* base, int64_t i, float x) {
-  if constexpr (DT == SSA_F32) ((float*)base)[i] = x;
-  else if constexpr (DT == SSA_F16) ((_Float16*)base)[i] = (_Float16)x;
-  else ((__bf16*)base)[i] = (__bf16)x;
+__device__ inline void store_row4(char* base, int64_t i, const f32x4& x) {
+  if constexpr (DT == SSA_F32) {
+    *(f32x4*)(base + i * 4) = x;
+  } else {
+    unsigned int w[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float y = x[r];
+      if constexpr (DT == SSA_BF16) w[r] = __builtin_bit_cast(unsigned short, (__bf16)y);
+      else w[r] = __builtin_bit_cast(unsigned short, (_Float16)y);
+    }
+    *(uint2*)(base + i * 2) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+  }
 }
+
+constexpr float kF16Shift = 14.0f;
 
 // How a call is laid out, by type and padded head dim DP. The 16-bit products take 32 keys at once
 // (two subtiles), the fp32 ones 4, so their tile is one subtile where registers are short.
@@ -257,9 +270,10 @@ struct Tile {
   static constexpr int LW = LC * ES / 4;                       // in words
   static constexpr int VB = DP / CB;
   static constexpr int NA = DP / 16;  // accumulators of 16 columns x 16 heads
-  static constexpr bool kQInLds = NC >= 8;  // queries: registers are short
+  static constexpr bool kQInLds = NC >= 8;         // queries: registers are short
+  static constexpr int KP = NC >= 32 ? 4 : NC >= 16 ? 2 : 1;  // pieces that a tile's keys are taken in
   // fp16 weights are taken up to 2^14 so that the small ones keep their bits
-  static constexpr float kShift = DT == SSA_F16 ? 14.0f : 0.0f;
+  static constexpr float kShift = DT == SSA_F16 ? kF16Shift : 0.0f;
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -270,6 +284,28 @@ struct Item {
   int b, j, n, begin, end, first_item;
   PagedSpan span;
 };
+
+// Sums over the wave and up to (and with) each lane: a block of lanes takes the sum of the block
+// beside it, and its upper lanes add it to their prefix.
+struct LaneSums {
+  int all, upto;
+};
+
+__device__ inline LaneSums lane_sums(int x) {
+  const int lane = threadIdx.x & 63;
+  LaneSums s{x, x};
+  auto step = [&](int y, int off) {
+    s.upto += lane & off ? y : 0;
+    s.all += y;
+  };
+  step(lane_xor(s.all, 1), 1);
+  step(lane_xor(s.all, 2), 2);
+  step(lane_xor(s.all, 4), 4);
+  step(lane_xor(s.all, 8), 8);
+  step(lane_xor(s.all, 16), 16);
+  step(lane_xor(s.all, 32), 32);
+  return s;
+}
 
 // Finds item `index` from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. False past the last item.
@@ -285,6 +321,25 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
     const PagedRange r = paged_item_range(it.span, units, 0, 1);
     it.begin = r.begin;
     it.end = units ? r.end : r.begin;
+    return true;
+  }
+  if (p.B <= 64) {  // a request per lane
+    const int len = lane < p.B ? p.lens[lane] : 0;
+    const int units = paged_units(paged_span(len, p.window, p.cap));
+    // 64 of at most 2^24 units fit 32 bits
+    const int n = paged_items(units, paged_chunk(lane_sums(units).all, p.items));
+    const int upto = lane_sums(n).upto;
+    const unsigned long long past = __ballot(upto > index);
+    if (past == 0) return false;
+    it.b = __builtin_ctzll(past);
+    it.span = paged_span(__builtin_amdgcn_readlane(len, it.b), p.window, p.cap);
+    it.n = __builtin_amdgcn_readlane(n, it.b);
+    it.first_item = __builtin_amdgcn_readlane(upto - n, it.b);
+    it.j = index - it.first_item;
+    const PagedRange r = paged_item_range(
+        it.span, __builtin_amdgcn_readlane(units, it.b), it.j, it.n);
+    it.begin = r.begin;
+    it.end = r.end;
     return true;
   }
   const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
@@ -410,12 +465,6 @@ __device__ inline Words<W> load_words(Buffer b, int off) {
     return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
 }
 
-template <int W>
-__device__ inline void store_words(char* p, const Words<W>& r) {
-  if constexpr (W == 4) *(u32x4*)p = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
-  else *(uint2*)p = uint2{r.w[0], r.w[1]};
-}
-
 // The rows of a lane's keys and values as they come from the cache, in the layouts of the products'
 // operands: keys lane l: row l % 16 of the subtile, 16 bytes at 64 c + 16 (l / 16) (the columns'
 // order within a product does not matter: queries lie alike); values: rows 4 (l / 16) + r, the
@@ -423,22 +472,26 @@ __device__ inline void store_words(char* p, const Words<W>& r) {
 template <int DT, int DP>
 struct Rows {
   using T = Tile<DT, DP>;
-  u32x4 k[T::NT][T::NC];
+  u32x4 k[T::NT][T::NC / T::KP];
   Words<T::LW> v[T::NT][4][T::VB];
 };
 
-// One wave stores the new token's key and value into the slot of position j. Its own later loads see
-// them; the row tiles of a key head each store the same bytes rather than wait for one another.
+// The wave of a request's last keys stores the new token's key and value into the slot of position j
+// at its start: its own later loads see them, and the row tiles of a key head each store the same
+// bytes rather than wait for one another. (Kept in LDS until the last tile instead, a short request
+// takes 0.2 us longer.)
 template <int ES>
 __device__ inline void store_new(const AttendParams& p, int b, int g, int j) {
-  const int e = j / p.page, lane = threadIdx.x & 63;
+  const int e = page_of(j / 16, p.div), per = p.d * ES / 16;
   const int64_t pg = p.table[b * p.table_stride + e], off = j - e * p.page;
   if (pg >= 0 && pg < p.pages) {
-    for (int c = lane * 16; c < p.d * ES; c += 64 * 16) {
-      const u32x4 k = *(const u32x4*)(p.k_new + (b * p.knb + g * p.knh) * ES + c);
-      const u32x4 v = *(const u32x4*)(p.v_new + (b * p.vnb + g * p.vnh) * ES + c);
-      *(u32x4*)(p.kpool + (pg * p.kpp + g * p.kph + off * p.kps) * ES + c) = k;
-      *(u32x4*)(p.vpool + (pg * p.vpp + g * p.vph + off * p.vps) * ES + c) = v;
+    const char* k = p.k_new + (b * p.knb + g * p.knh) * ES;
+    const char* v = p.v_new + (b * p.vnb + g * p.vnh) * ES;
+    char* kto = p.kpool + (pg * p.kpp + g * p.kph + off * p.kps) * ES;
+    char* vto = p.vpool + (pg * p.vpp + g * p.vph + off * p.vps) * ES;
+    for (int i = threadIdx.x & 63; i < 2 * per; i += 64) {
+      const int c = (i < per ? i : i - per) * 16;
+      *(u32x4*)((i < per ? kto : vto) + c) = *(const u32x4*)((i < per ? k : v) + c);
     }
   }
   wave_lds_sync();
@@ -495,13 +548,12 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
   const int sub_end = min(it.begin + i1 * NT, it.end);
   auto pages_at = [&](int s) {
     s += lane;
-    return s < sub_end ? row[s * 16 / p.page] : 0;
+    return s < sub_end ? row[page_of(s, p.div)] : 0;
   };
   auto take_pages = [&](int x) {
     bad |= __ballot(x < 0 || x >= p.pages);
     pid = x < 0 || x >= p.pages ? 0 : x;
-    const int j = (batch + lane) * 16;
-    poff = j - j / p.page * p.page;
+    poff = (batch + lane) * 16 - page_of(batch + lane, p.div) * p.page;
   };
   if (i0 < i1) {
     const int x = pages_at(batch);
@@ -541,13 +593,15 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
     const int c = vb * T::CB * T::ES + col * LW * 4;
     vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
   }
-  auto load_k = [&](int i) {
+  auto load_k = [&](int i, int piece) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const Buffer src = buffer_at(kbase + (pg[t] * kpp + (int64_t)off[t] * kps));
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        rows.k[t][c] = load16(src, c * 64 + grp * 16 < row_bytes ? koff + c * 64 : kOutside);
+      for (int c = 0; c < NC / T::KP; ++c) {
+        const int at = (piece * (NC / T::KP) + c) * 64;
+        rows.k[t][c] = load16(src, at + grp * 16 < row_bytes ? koff + at : kOutside);
+      }
     }
   };
   auto load_v = [&](int i) {
@@ -569,7 +623,7 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
 
   if (i0 < i1) {
     locate(i0);
-    load_k(i0);
+    load_k(i0, 0);
     load_v(i0);
   }
   for (int i = i0; i < i1; ++i) {
@@ -582,6 +636,8 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
     for (int t = 0; t < NT; ++t) s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
+      constexpr int per = NC / T::KP;
+      if (c > 0 && c % per == 0) load_k(i, c / per);
       u32x4 qc;
       if constexpr (T::kQInLds) qc = q_lds[c][lane];
       else qc = q[c];
@@ -590,19 +646,19 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
         if constexpr (DT == SSA_F32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const unsigned int a = rows.k[t][c][e], b = qc[e];
+            const unsigned int a = rows.k[t][c % per][e], b = qc[e];
             s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b),
                                                         s[t], 0, 0, 0);
           }
         } else {
-          s[t] = mfma16(rows.k[t][c], qc, s[t], DT == SSA_BF16);
+          s[t] = mfma16(rows.k[t][c % per], qc, s[t], DT == SSA_BF16);
         }
       }
     }
     const bool more = i + 1 < i1;
     if (more) {
       locate(i + 1);
-      load_k(i + 1);
+      load_k(i + 1, 0);
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -703,101 +759,115 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
     p.info[2 * it.b] = it.first_item;
     p.info[2 * it.b + 1] = it.n;
   }
-  if (it.n > 1) {
-    const int64_t part = (int64_t)(unit / p.Hkv * p.Hkv + g) * p.RT + rt;
-    if (live) {
-#pragma unroll
-      for (int n = 0; n < NA; ++n) ((f32x4*)p.part)[(part * NA + n) * 64 + lane] = st.acc[n];
-      if (grp == 0) {
-        p.part_ml[part * 32 + col] = st.m;
-        p.part_ml[part * 32 + 16 + col] = st.l;
-      }
-    }
-    return;
-  }
   if (!live) return;
+  const int h = g * p.G + head;
   const float inv = len == 0 && it.span.ok ? 0.0f : 1.0f / st.l;
-  const int64_t h = g * p.G + head;
-  char* const to = p.out + (it.b * p.ob + h * p.oh) * T::ES;
+  const int64_t part = (int64_t)(unit / p.Hkv) * p.Hq + h, to = it.b * p.ob + h * p.oh;
 #pragma unroll
   for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int c = vb * T::CB + LC * (grp * 4 + r);
-      if (c >= p.d) continue;
-      Words<LW> w;
-      if constexpr (DT == SSA_F32) {
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int e = 0; e < LC; ++e) {
-          const float x = st.acc[vb * LC + e][r] * inv;
-          w.w[e] = __float_as_uint(x);
-        }
-      } else {
+      for (int e = 0; e < LC; e += 4) {
+        const int c = vb * T::CB + LC * (grp * 4 + r) + e;
+        if (c >= p.d) continue;
+        f32x4 x;
 #pragma unroll
-        for (int e = 0; e < LC; e += 2) {
-          const float x = st.acc[vb * LC + e][r] * inv, y = st.acc[vb * LC + e + 1][r] * inv;
-          unsigned short a, b;
-          if constexpr (DT == SSA_BF16) {
-            a = __builtin_bit_cast(unsigned short, (__bf16)x);
-            b = __builtin_bit_cast(unsigned short, (__bf16)y);
-          } else {
-            a = __builtin_bit_cast(unsigned short, (_Float16)x);
-            b = __builtin_bit_cast(unsigned short, (_Float16)y);
-          }
-          w.w[e / 2] = a | (unsigned int)b << 16;
+        for (int i = 0; i < 4; ++i) x[i] = st.acc[vb * LC + e + i][r];
+        if (it.n > 1) {
+          *(f32x4*)(p.part + part * DP + c) = x;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] *= inv;
+          store_row4<DT>(p.out, to + c, x);
         }
       }
-      store_words<LW>(to + c * T::ES, w);
-    }
-  if (p.lse && grp == 0)
+  if (grp != 0) return;
+  if (it.n > 1) {
+    p.part_ml[part * 2] = st.m;
+    p.part_ml[part * 2 + 1] = st.l;
+  } else if (p.lse) {
     p.lse[(int64_t)it.b * p.Hq + h] = len == 0 && it.span.ok ? -INFINITY
         : (st.m - T::kShift + __builtin_amdgcn_logf(st.l)) * kLn2;
+  }
 }
 
-// Joins a request's parts: a workgroup per accumulator of a (request, key head, row tile), its waves
-// taking every NW-th part. Rows without keys, and of lengths that do not fit, are answered here.
-template <int DT, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void paged_join_kernel(AttendParams p) {
-  using T = Tile<DT, DP>;
-  constexpr int NA = T::NA, LC = T::LC;
-  __shared__ f32x4 red[NW][64];
-  __shared__ float red_m[NW][64], red_l[NW][64];
-  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
-  const int col = lane & 15, grp = lane >> 4;
-  const int b = blockIdx.y, n = blockIdx.x % NA, g = blockIdx.x / NA / p.RT;
-  const int rt = blockIdx.x / NA % p.RT, head = rt * 16 + col;
-  const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
+constexpr int kJoinBatch = 8;
+
+// Joins a row's parts: a workgroup per (request, query head), DP / 4 threads across a part's row and
+// the parts shared out over the workgroup's splits, kJoinBatch of them on their way at a time. Rows
+// without keys, and of lengths that do not fit, are answered here.
+template <int DT, int DP, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(AttendParams p) {
+  constexpr int PER = DP / 4, NS = THREADS / PER, WAVES = THREADS / 64;
+  __shared__ f32x4 red[WAVES][PER < 64 ? PER : 64];
+  __shared__ float red_m[WAVES], red_l[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
+  const int h = blockIdx.x, b = blockIdx.y, c = tid % PER * 4, split = tid / PER;
+  const int len = p.lens[b], first = p.info[2 * b], parts = p.info[2 * b + 1];
+  const PagedSpan s = paged_span(len, p.window, p.cap);
   Softmax<1> st;
   st.m = -INFINITY;
   st.l = s.ok ? 0.0f : NAN;
   st.acc[0] = f32x4{0, 0, 0, 0};
   if (s.len > 0) {
-    const int first = p.info[2 * b], parts = p.info[2 * b + 1];
     if (parts <= 1) return;  // written by its one item
-    for (int i = wv; i < parts; i += NW) {
-      const int64_t part = ((int64_t)(first + i) * p.Hkv + g) * p.RT + rt;
-      if (head < p.G)
-        join(st, p.part_ml[part * 32 + col], p.part_ml[part * 32 + 16 + col],
-             (const f32x4*)p.part + (part * NA + n) * 64 + lane, 0);
-    }
-    red_m[wv][lane] = st.m;
-    red_l[wv][lane] = st.l;
-    red[wv][lane] = st.acc[0];
-    __syncthreads();
-    if (wv != 0) return;
-    for (int w = 1; w < NW; ++w) join(st, red_m[w][lane], red_l[w][lane], &red[w][lane], 0);
-  }
-  if (wv != 0 || head >= p.G) return;
-  const float inv = s.len == 0 && s.ok ? 0.0f : 1.0f / st.l;
-  const int64_t h = g * p.G + head;
+    for (int i = split; i < parts; i += NS * kJoinBatch) {
+      float m[kJoinBatch], l[kJoinBatch], mx = st.m;
+      f32x4 a[kJoinBatch];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int c = n / LC * T::CB + LC * (grp * 4 + r) + n % LC;
-    if (c < p.d) store_elem<DT>(p.out, b * p.ob + h * p.oh + c, st.acc[0][r] * inv);
+      for (int u = 0; u < kJoinBatch; ++u) {
+        const int at = i + u * NS;
+        const int64_t row = (int64_t)(first + at) * p.Hq + h;
+        const bool in = at < parts;
+        m[u] = in ? p.part_ml[row * 2] : -INFINITY;
+        l[u] = in ? p.part_ml[row * 2 + 1] : 0.0f;
+        a[u] = in ? *(const f32x4*)(p.part + row * DP + c) : f32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u) mx = fmaxf(mx, m[u]);
+      const float base = mx == -INFINITY ? 0.0f : mx, x = __builtin_amdgcn_exp2f(st.m - base);
+      st.m = mx;
+      st.l *= x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st.acc[0][r] *= x;
+#pragma unroll
+      for (int u = 0; u < kJoinBatch; ++u) {
+        const float y = __builtin_amdgcn_exp2f(m[u] - base);
+        st.l += l[u] * y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.acc[0][r] += a[u][r] * y;
+      }
+    }
+    // splits within a wave, then the waves' (past 256 columns a split is two waves)
+#pragma unroll
+    for (int off = 32; off >= PER; off >>= 1) {
+      f32x4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = lane_xor(st.acc[0][r], off);
+      const float m = lane_xor(st.m, off), l = lane_xor(st.l, off);
+      join(st, m, l, &o, 0);
+    }
+    constexpr int STEP = PER > 64 ? PER / 64 : 1;
+    if (lane < PER) red[wv][lane] = st.acc[0];
+    if (lane == 0) {
+      red_m[wv] = st.m;
+      red_l[wv] = st.l;
+    }
+    __syncthreads();
+    if (tid >= PER) return;
+#pragma unroll
+    for (int w = STEP; w < WAVES; w += STEP)
+      join(st, red_m[wv + w], red_l[wv + w], &red[wv + w][lane], 0);
   }
-  if (p.lse && grp == 0 && n == 0)
+  if (tid >= PER) return;
+  const float inv = s.len == 0 && s.ok ? 0.0f : 1.0f / st.l;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) st.acc[0][r] *= inv;
+  if (c < p.d) store_row4<DT>(p.out, b * p.ob + h * p.oh + c, st.acc[0]);
+  if (p.lse && tid == 0)
     p.lse[(int64_t)b * p.Hq + h] = s.len == 0 && s.ok ? -INFINITY
-        : (st.m - T::kShift + __builtin_amdgcn_logf(st.l)) * kLn2;
+        : (st.m - (DT == SSA_F16 ? kF16Shift : 0.0f) + __builtin_amdgcn_logf(st.l)) * kLn2;
 }
 
 bool fits_int(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
@@ -835,26 +905,30 @@ Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t 
   y.RT = (Hq / Hkv + 15) / 16;
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
   const int64_t units = paged_most_units(W * page, (int)window);
-  const int64_t target = y.dp <= 128 ? 1024 : y.dp <= 256 ? 512 : 256;
-  y.items = units <= 1 ? 0 : std::max<int64_t>(1, target / (Hkv * y.RT));
+  const int64_t target = y.dp == 64 ? (B == 1 ? 512 : 1024) : y.dp == 128 ? (B == 1 ? 512 : 1536) : y.dp == 256 ? 512 : 256;
+  y.items = units <= 4 || (units <= 16 && B * Hkv * y.RT >= 512) ? 0 : std::max<int64_t>(1, target / (Hkv * y.RT));
   y.max_items = y.items == 0 ? B : paged_most_items(B, y.items, units);
   if (y.items == 0) return y;
-  const size_t parts = (size_t)y.max_items * Hkv * y.RT;
-  y.part_ml = parts * 16 * y.dp * 4;
-  y.info = y.part_ml + parts * 32 * 4;
+  const size_t parts = (size_t)y.max_items * Hq;
+  y.part_ml = parts * y.dp * 4;
+  y.info = y.part_ml + parts * 2 * 4;
   y.bytes = (y.info + (size_t)B * 8 + 15) / 16 * 16;
   return y;
 }
 
 template <int DT, int DP, int WPE>
 int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
-  constexpr int NW = 4;
+  constexpr int NW = 4, MANY = DP <= 64 && DT != SSA_F32 ? 16 : DP <= 256 ? 8 : 4;
+  if (p.items == 0 && blocks < 512) {
+    paged_attend_kernel<DT, DP, MANY, 1><<<(unsigned)blocks, MANY * 64, 0, st>>>(p);
+    return launch_status("paged_attend_kernel");
+  }
   paged_attend_kernel<DT, DP, NW, WPE><<<(unsigned)blocks, NW * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_attend_kernel"));
   if (p.items == 0) return SSA_OK;
-  const dim3 grid((unsigned)(DP / 16 * p.RT * p.Hkv), (unsigned)p.B);
-  if (p.items > 32) paged_join_kernel<DT, DP, 16><<<grid, 1024, 0, st>>>(p);
-  else paged_join_kernel<DT, DP, 4><<<grid, 256, 0, st>>>(p);
+  const dim3 grid(p.Hq, p.B);
+  if ((int64_t)p.Hq * p.B < 64) paged_join_kernel<DT, DP, 1024><<<grid, 1024, 0, st>>>(p);
+  else paged_join_kernel<DT, DP, 256><<<grid, 256, 0, st>>>(p);
   return launch_status("paged_join_kernel");
 }
 
@@ -993,6 +1067,7 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   int64_t* const st[14] = {&p.qb, &p.qh, &p.kpp, &p.kph, &p.kps, &p.vpp, &p.vph,
                            &p.vps, &p.ob, &p.oh, &p.knb, &p.knh, &p.vnb, &p.vnh};
   for (int i = 0; i < (k_new ? 14 : 10); ++i) *st[i] = strides[i];
+  p.div = page_div((int)page / 16);
   p.RT = (int)y.RT;
   p.items = (int)y.items;
   p.part = (float*)workspace;
@@ -1001,8 +1076,8 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   const int64_t units = y.max_items * Hkv, blocks = (units + 7) / 8 * 8 * y.RT;
   SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_attend: too many rows in one call");
   p.units = (int)units;
-  hipStream_t stream_ = (hipStream_t)stream;
-  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, blocks, stream_);
-  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, blocks, stream_);
-  return run_attend_dim<SSA_BF16>(p, y.dp, blocks, stream_);
+  hipStream_t hs = (hipStream_t)stream;
+  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, blocks, hs);
+  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, blocks, hs);
+  return run_attend_dim<SSA_BF16>(p, y.dp, blocks, hs);
 }

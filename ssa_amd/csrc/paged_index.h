@@ -53,11 +53,15 @@ SSA_HD int64_t paged_most_items(int64_t B, int64_t items, int64_t most_units) {
 }
 
 // Units per item so that a call's `units` make at most `items` items besides one more per request.
-SSA_HD int paged_chunk(int64_t units, int64_t items) {
-  return units <= items ? 1 : (int)((units + items - 1) / items);
+SSA_HD int paged_chunk(int64_t units, int items) {
+  if (units <= items) return 1;
+  if (units <= 0x7fffffff) return (int)(((unsigned)units + (unsigned)items - 1) / (unsigned)items);
+  return (int)((units + items - 1) / items);
 }
 
-SSA_HD int paged_items(int units, int chunk) { return (units + chunk - 1) / chunk; }
+SSA_HD int paged_items(int units, int chunk) {
+  return (int)(((unsigned)units + (unsigned)chunk - 1) / (unsigned)chunk);
+}
 
 // Subtiles [begin, end) of item j of n: the request's units spread evenly over its items.
 struct PagedRange {
@@ -66,11 +70,32 @@ struct PagedRange {
 
 SSA_HD PagedRange paged_item_range(const PagedSpan& s, int units, int j, int n) {
   const int a = s.first / 16, last = (s.len - 1) / 16 + 1;
+  const int each = (int)((unsigned)units / (unsigned)n), more = units - each * n;
   PagedRange r;
-  r.begin = a + (int)((int64_t)units * j / n) * kPagedUnit;
-  r.end = a + (int)((int64_t)units * (j + 1) / n) * kPagedUnit;
+  r.begin = a + (j * each + (j < more ? j : more)) * kPagedUnit;
+  r.end = r.begin + (each + (j < more ? 1 : 0)) * kPagedUnit;
   if (r.end > last) r.end = last;
   return r;
+}
+
+// Division of a subtile's number (below 2^27: lengths are below 2^31) by the subtiles of a page, D up
+// to 4096, as a multiplication: mul = ceil(2^(31 + shift) / D), 2^shift <= D < 2^(shift + 1), is off
+// by less than 1 in 2^(31 + shift) / D > 2^30, more than any quotient's distance from the next.
+struct PageDiv {
+  unsigned mul;
+  int shift;
+};
+
+SSA_HD PageDiv page_div(int subtiles) {
+  PageDiv d{0, 0};
+  while ((2 << d.shift) <= subtiles) ++d.shift;
+  d.mul = (unsigned)((((uint64_t)1 << (31 + d.shift)) + (unsigned)subtiles - 1) /
+                     (unsigned)subtiles);
+  return d;
+}
+
+SSA_HD int page_of(int subtile, const PageDiv& d) {
+  return (int)(((uint64_t)((unsigned)subtile * 2u) * d.mul >> 32) >> d.shift);
 }
 
 }  // namespace ssa

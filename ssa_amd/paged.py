@@ -20,13 +20,13 @@ differentiable. The reference has no paged cache.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .ssa_kernel import _aligned
 
 RESIZE_ERRORS = {-1: "a length, the free count or the pool does not fit the table",
                  -2: "more new tokens than slots"}
@@ -52,38 +52,120 @@ def _launch(name, t, *args):
 
 
 def _one_device(first, *others):
-    _lib.require_device(first, *others)
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            _lib.require_device(first, *others)
             raise ValueError(f"tensors on {first.device} and {t.device}")
+    if index < 0:
+        _lib.require_device(first)
 
 
-def _int32(name, t, shape):
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} is {t.dtype}, expected torch.int32")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor, "
-                         f"got {tuple(t.shape)}")
+# The checks of shapes, strides and types depend on nothing else, and a serving loop makes the same
+# call again and again: what they give is kept by those (22 us a call on the host without, 12 with).
+
+def _int32(name, shape, stride, dtype, want):
+    if dtype != torch.int32:
+        raise TypeError(f"{name} is {dtype}, expected torch.int32")
+    if tuple(shape) != want or (len(want) and want[0] > 1 and stride != (1,)):
+        raise ValueError(f"{name} must be a contiguous {want} tensor, got {tuple(shape)}")
 
 
-def _table(table):
-    if table.dtype != torch.int32:
-        raise TypeError(f"table is {table.dtype}, expected torch.int32")
-    if table.dim() != 2 or table.stride(1) != 1:
+def _table(shape, stride, dtype):
+    """(B, W, elements a row)"""
+    if dtype != torch.int32:
+        raise TypeError(f"table is {dtype}, expected torch.int32")
+    if len(shape) != 2 or shape[1] > 1 and stride[1] != 1:
         raise ValueError("table must be (B, W) with a contiguous last dimension")
-    B, W = table.shape
-    return B, W, table.stride(0) if B > 1 else W
+    B, W = shape
+    return B, W, stride[0] if B > 1 else W
 
 
-def _pools(kpool, vpool):
-    if kpool.dim() != 4 or kpool.shape != vpool.shape:
+def _meta(t):
+    return (t.shape, t.stride(), t.dtype)
+
+
+def _pools(k, v):
+    (kshape, kstride, kdtype), (vshape, vstride, vdtype) = k, v
+    if len(kshape) != 4 or kshape != vshape:
         raise ValueError(f"kpool and vpool must share a (pages, Hkv, page, d) shape, got "
-                         f"{tuple(kpool.shape)} and {tuple(vpool.shape)}")
-    if kpool.dtype != vpool.dtype:
+                         f"{tuple(kshape)} and {tuple(vshape)}")
+    if kdtype != vdtype:
         raise TypeError("kpool and vpool must share a dtype")
-    if kpool.stride(3) != 1 or vpool.stride(3) != 1:
+    if kstride[3] != 1 or vstride[3] != 1:
         raise ValueError("the head dimension must be contiguous")
-    return kpool.shape
+    return kshape
+
+
+def _rows16(meta):
+    """Whether rows (the last dimension) start at multiples of 16 bytes, given an aligned base."""
+    shape, stride, dtype = meta
+    vec = 4 if dtype == torch.float32 else 8
+    return stride[-1] == 1 and all(s % vec == 0 for s in stride[:-1])
+
+
+@functools.lru_cache(maxsize=1024)
+def _resize_plan(lens, new_lens, table, free, nfree):
+    B, W, row = _table(*table)
+    _int32("lens", *lens, (B,))
+    _int32("new_lens", *new_lens, (B,))
+    _int32("nfree", *nfree, (1,))
+    _int32("free", *free, (free[0].numel(),))
+    return B, W, row, free[0].numel()
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_plan(k, v, kpool, vpool, slots):
+    """(constants of the call, whether k or v needs a copy)"""
+    pages, hkv, page, d = _pools(kpool, vpool)
+    dtype = kpool[2]
+    if k[2] != dtype or v[2] != dtype:
+        raise TypeError(f"k is {k[2]} and v {v[2]}, the cache holds {dtype}")
+    if slots[2] != torch.int64 or len(slots[0]) != 1 or slots[0][0] > 1 and slots[1] != (1,):
+        raise ValueError("slots must be a contiguous (T,) int64 tensor")
+    T = slots[0][0]
+    if k[0] != (T, hkv, d) or v[0] != (T, hkv, d):
+        raise ValueError(f"k and v must be ({T}, {hkv}, {d}), got {tuple(k[0])} and "
+                         f"{tuple(v[0])}")
+    strides = _lib.i64_array((*k[1][:2], *v[1][:2], *kpool[1][:3], *vpool[1][:3]))
+    return (_lib.dtype_code(dtype), T, hkv, d, pages, page, strides), \
+        not (_rows16(k) and _rows16(v))
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_plan(q, kpool, vpool, table, lens, out, k_new, v_new, window):
+    """(sizes of the call, table's, strides, workspace bytes, whether an input needs a copy)"""
+    pages, hkv, page, d = _pools(kpool, vpool)
+    dtype = kpool[2]
+    if len(q[0]) != 3 or q[0][2] != d:
+        raise ValueError(f"q must be (B, Hq, {d}), got {tuple(q[0])}")
+    B, hq, _ = q[0]
+    if q[2] != dtype:
+        raise TypeError(f"q is {q[2]}, the cache holds {dtype}")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
+    copy = not _rows16(q)
+    new = (0, 0, 0, 0)
+    if k_new is not None:
+        if k_new[2] != dtype or v_new[2] != dtype:
+            raise TypeError(f"k_new is {k_new[2]} and v_new {v_new[2]}, the cache holds {dtype}")
+        if k_new[0] != (B, hkv, d) or v_new[0] != (B, hkv, d):
+            raise ValueError(f"k_new and v_new must be ({B}, {hkv}, {d})")
+        copy = copy or not (_rows16(k_new) and _rows16(v_new))
+        new = (*k_new[1][:2], *v_new[1][:2])
+    rows, W, row = _table(*table)
+    if rows != B:
+        raise ValueError(f"table has {rows} rows for {B} requests")
+    _int32("lens", *lens, (B,))
+    to = (hq * d, d)
+    if out is not None:
+        if out[2] != dtype or out[0] != (B, hq, d) or not _rows16(out):
+            raise ValueError(f"out must be a ({B}, {hq}, {d}) {dtype} tensor with rows of 16-byte "
+                             "pieces")
+        to = out[1][:2]
+    strides = _lib.i64_array((*q[1][:2], *kpool[1][:3], *vpool[1][:3], *to, *new))
+    ws_bytes = _lib.query("ssa_paged_attend_workspace_size", B, hq, hkv, d, W, page, window)
+    return (_lib.dtype_code(dtype), B, hq, hkv, d, pages, page), (row, W), strides, ws_bytes, copy
 
 
 def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor,
@@ -102,18 +184,15 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
     Resized; `out` takes an earlier one of the same sizes to write into. All or nothing: if the
     growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
     slots are -1 and status says why."""
+    if out is None and torch.compiler.is_compiling():
+        from . import torch_ops as T
+        return Resized(*T.paged_resize(lens, new_lens, table, free, nfree, int(page), int(tokens)))
     _one_device(lens, new_lens, table, free, nfree)
-    B, W, row = _table(table)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens={tokens}")
-    _int32("lens", lens, (B,))
-    _int32("new_lens", new_lens, (B,))
-    _int32("nfree", nfree, (1,))
-    _int32("free", free, (free.numel(),))
-    if torch.compiler.is_compiling() and out is None:
-        from . import torch_ops as T
-        return Resized(*T.paged_resize(lens, new_lens, table, free, nfree, int(page), tokens))
+    B, W, row, pages = _resize_plan(_meta(lens), _meta(new_lens), _meta(table), _meta(free),
+                                    _meta(nfree))
     if out is None:
         dev = lens.device
         out = Resized(torch.empty(tokens, device=dev, dtype=torch.int64),
@@ -125,11 +204,10 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
         if out.slots.dtype != torch.int64 or out.slots.shape != (tokens,) \
                 or not out.slots.is_contiguous():
             raise ValueError(f"out.slots must be a contiguous ({tokens},) int64 tensor")
-        _int32("out.pos", out.pos, (tokens,))
-        _int32("out.cu", out.cu, (B + 1,))
-        _int32("out.status", out.status, (1,))
+        for name, n in (("pos", tokens), ("cu", B + 1), ("status", 1)):
+            _int32("out." + name, *_meta(getattr(out, name)), (n,))
     _launch("ssa_paged_resize", lens, lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(),
-            row, B, W, int(page), free.data_ptr(), free.numel(), nfree.data_ptr(),
+            row, B, W, int(page), free.data_ptr(), pages, nfree.data_ptr(),
             out.slots.data_ptr() if tokens else None, out.pos.data_ptr() if tokens else None,
             tokens, out.cu.data_ptr(), out.status.data_ptr())
     return out
@@ -142,29 +220,25 @@ def append_pages(k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: t
     The slots of a call must be distinct."""
     if torch.compiler.is_compiling():
         from . import torch_ops as T
-        return T.paged_append(k, v, kpool, vpool, slots)
-    return _append_pages_impl(k, v, kpool, vpool, slots)
+        T.paged_append(k, v, kpool, vpool, slots)
+    else:
+        _append_pages_impl(k, v, kpool, vpool, slots)
 
 
 def _append_pages_impl(k, v, kpool, vpool, slots):
     _one_device(kpool, vpool, k, v, slots)
-    pages, hkv, page, d = _pools(kpool, vpool)
-    if k.dtype != kpool.dtype or v.dtype != kpool.dtype:
-        raise TypeError(f"k is {k.dtype} and v {v.dtype}, the cache holds {kpool.dtype}")
-    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
-        raise ValueError("slots must be a contiguous (T,) int64 tensor")
-    T = slots.shape[0]
-    if k.shape != (T, hkv, d) or v.shape != (T, hkv, d):
-        raise ValueError(f"k and v must be ({T}, {hkv}, {d}), got {tuple(k.shape)} and "
-                         f"{tuple(v.shape)}")
-    if T == 0:
-        return
-    k, v = _aligned(k), _aligned(v)
-    strides = _lib.i64_array((*k.stride()[:2], *v.stride()[:2], *kpool.stride()[:3],
-                              *vpool.stride()[:3]))
-    _launch("ssa_paged_append", kpool, k.data_ptr(), v.data_ptr(), kpool.data_ptr(),
-            vpool.data_ptr(), _lib.dtype_code(kpool.dtype), T, hkv, d, pages, page, strides,
-            slots.data_ptr())
+    sizes, copy = _append_plan(_meta(k), _meta(v), _meta(kpool), _meta(vpool), _meta(slots))
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if copy or (kp | vp) & 15:
+        return _append_pages_impl(*(_own(t) for t in (k, v)), kpool, vpool, slots)
+    if sizes[1]:
+        _launch("ssa_paged_append", kpool, kp, vp, kpool.data_ptr(), vpool.data_ptr(), *sizes,
+                slots.data_ptr())
+
+
+def _own(t):
+    """A contiguous copy (allocations start at multiples of 16 bytes)."""
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor,
@@ -200,45 +274,27 @@ def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tabl
 def _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, return_lse,
                        out=None):
     _one_device(q, kpool, vpool, table, lens, k_new, v_new, out)
-    pages, hkv, page, d = _pools(kpool, vpool)
-    dtype = kpool.dtype
-    if q.dim() != 3 or q.shape[2] != d:
-        raise ValueError(f"q must be (B, Hq, {d}), got {tuple(q.shape)}")
-    B, hq, _ = q.shape
-    if q.dtype != dtype:
-        raise TypeError(f"q is {q.dtype}, the cache holds {dtype}")
-    if (k_new is None) != (v_new is None):
-        raise ValueError("k_new and v_new come together")
-    if k_new is not None:
-        if k_new.dtype != dtype or v_new.dtype != dtype:
-            raise TypeError(f"k_new is {k_new.dtype} and v_new {v_new.dtype}, the cache holds "
-                            f"{dtype}")
-        if k_new.shape != (B, hkv, d) or v_new.shape != (B, hkv, d):
-            raise ValueError(f"k_new and v_new must be ({B}, {hkv}, {d})")
-        k_new, v_new = _aligned(k_new), _aligned(v_new)
-    rows, W, row = _table(table)
-    if rows != B:
-        raise ValueError(f"table has {rows} rows for {B} requests")
-    _int32("lens", lens, (B,))
-    if out is None:
-        out = torch.empty(B, hq, d, device=q.device, dtype=dtype)
-    elif out.dtype != dtype or out.shape != (B, hq, d) or _aligned(out) is not out:
-        raise ValueError(f"out must be a ({B}, {hq}, {d}) {dtype} tensor with rows of 16-byte "
-                         "pieces")
-    lse = torch.empty(B, hq, device=q.device, dtype=torch.float32) if return_lse else None
-    if B == 0:
-        return (out, lse) if return_lse else out
-    q = _aligned(q)
-    new = (0, 0, 0, 0) if k_new is None else (*k_new.stride()[:2], *v_new.stride()[:2])
-    strides = _lib.i64_array((*q.stride()[:2], *kpool.stride()[:3], *vpool.stride()[:3],
-                              *out.stride()[:2], *new))
     window = int(window)
-    ws_bytes = _lib.query("ssa_paged_attend_workspace_size", B, hq, hkv, d, W, page, window)
-    ws = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    _launch("ssa_paged_attend", q, q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
-            out.data_ptr(), _lib.ptr(lse), _lib.dtype_code(dtype), B, hq, hkv, d, pages, page,
-            table.data_ptr(), row, W, lens.data_ptr(), _lib.ptr(k_new),
-            _lib.ptr(v_new), strides, float(scale), window, _lib.ptr(ws), ws_bytes)
+    sizes, rows, strides, ws_bytes, copy = _attend_plan(
+        _meta(q), _meta(kpool), _meta(vpool), _meta(table), _meta(lens),
+        None if out is None else _meta(out), None if k_new is None else _meta(k_new),
+        None if v_new is None else _meta(v_new), window)
+    qp = q.data_ptr()
+    kp, vp = (None, None) if k_new is None else (k_new.data_ptr(), v_new.data_ptr())
+    if copy or (qp if kp is None else qp | kp | vp) & 15:
+        k_new, v_new = (None if t is None else _own(t) for t in (k_new, v_new))
+        return _attend_pages_impl(_own(q), kpool, vpool, table, lens, k_new, v_new, scale, window,
+                                  return_lse, out)
+    _, B, hq, _, d, _, _ = sizes
+    dev = q.device
+    if out is None:
+        out = torch.empty(B, hq, d, device=dev, dtype=q.dtype)
+    lse = torch.empty(B, hq, device=dev, dtype=torch.float32) if return_lse else None
+    if B:
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+        _launch("ssa_paged_attend", q, qp, kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(),
+                _lib.ptr(lse), *sizes, table.data_ptr(), *rows, lens.data_ptr(), kp, vp, strides,
+                float(scale), window, _lib.ptr(ws), ws_bytes)
     return (out, lse) if return_lse else out
 
 

@@ -13,8 +13,7 @@ using namespace ssa;
 #define CHECK(x)                                                                            \
   do {                                                                                      \
     if (!(x)) {                                                                             \
-      std::printf("%s: batch %d, B=%d cap=%lld window=%d items=%lld\n", #x, batch, B,       \
-                  (long long)cap, window, (long long)items);                                \
+      std::printf("%s: batch %d, B=%d cap=%lld window=%d items=%d\n", #x, batch, B, (long long)cap, window, items);                                \
       return 1;                                                                             \
     }                                                                                       \
   } while (0)
@@ -27,7 +26,7 @@ int main() {
     const int64_t cap = page * (1 + upto(batch % 2 ? 12 : 3000));
     const int windows[] = {0, 0, 1, 2, 15, 16, 17, 100, 1000, 0x7fffffff};
     const int window = windows[upto(9)];
-    const int64_t items = 1 + upto(batch % 5 ? 40 : 1024);
+    const int items = 1 + (int)upto(batch % 5 ? 40 : 1024);
     std::vector<int> lens(B);
     for (int& n : lens) {
       const int edge[] = {0, 1, 15, 16, 17, (int)cap, (int)cap - 1, -1, (int)cap + 1, -0x7fffffff};
@@ -64,6 +63,17 @@ int main() {
       CHECK((at * 16 - 1) / page < cap / page);
     }
     CHECK(made <= paged_most_items(B, items, most));
+  }
+  for (int d = 1; d <= 4096; ++d) {
+    const PageDiv div = page_div(d);
+    for (int k = 0; k < 200; ++k) {
+      const int64_t q = k < 3 ? k : upto((1 << 27) / d);
+      for (int64_t x = q * d - 1; x <= q * d + 1; ++x)
+        if (x >= 0 && x < 1 << 27 && page_of((int)x, div) != x / d) {
+          std::printf("%lld / %d\n", (long long)x, d);
+          return 1;
+        }
+    }
   }
   std::puts("ok");
   return 0;

@@ -110,7 +110,7 @@ def test_another_device_is_made_current(monkeypatch):
     P._launch("x", NS(device=NS(index=0)), 1)
     P._launch("y", NS(device=NS(index=1)), 2)
     assert seen == [("x", 1, 40), ("in", 1), ("y", 2, 41), ("out", 1)]
-    a, b = (NS(device=NS(index=i), is_cuda=True) for i in (0, 1))
+    a, b = (NS(device=NS(index=i), is_cuda=True, get_device=lambda i=i: i) for i in (0, 1))
     with pytest.raises(ValueError, match="tensors on"):
         P._one_device(a, None, b)
 
