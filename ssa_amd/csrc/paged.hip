@@ -32,45 +32,87 @@ struct ResizeParams {
   int64_t T;
   int32_t* cu;
   int32_t* status;
+  PageDiv div;
 };
 
-constexpr int kResizeThreads = 1024;
+constexpr int kResizeThreads = 1024, kResizeWaves = kResizeThreads / 64;
 
-// Sum over the workgroup of three counts (every thread receives them).
-__device__ inline void block_sum3(int64_t (&x)[3], int64_t (*red)[3]) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-  for (int c = 0; c < 3; ++c) {
-    for (int off = 32; off >= 1; off >>= 1) x[c] += __shfl_xor(x[c], off);
-    if (lane == 0) red[wv][c] = x[c];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int c = 0; c < 3; ++c) {
-    x[c] = 0;
-    for (int w = 0; w < kResizeThreads / 64; ++w) x[c] += red[w][c];
-  }
-  __syncthreads();
+__device__ inline int other_lane(int x, int j) { return lane_xor(x, j); }
+__device__ inline int64_t other_lane(int64_t x, int j) {
+  const unsigned int lo = lane_xor((unsigned int)x, j), hi = lane_xor((unsigned int)(x >> 32), j);
+  return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// Exclusive prefix over the workgroup's threads; total: the sum over all of them.
-__device__ inline int block_scan(int x, int* red, int* total) {
+// Sums over the wave and up to (and with) each lane: a block of lanes takes the sum of the block
+// beside it, and its upper lanes add it to their prefix.
+template <class I>
+struct LaneSums {
+  I all, upto;
+};
+
+template <class I>
+__device__ inline LaneSums<I> lane_sums(I x) {
+  const int lane = threadIdx.x & 63;
+  LaneSums<I> s{x, x};
+  auto step = [&](I y, int off) {
+    s.upto += lane & off ? y : 0;
+    s.all += y;
+  };
+  step(other_lane(s.all, 1), 1);
+  step(other_lane(s.all, 2), 2);
+  step(other_lane(s.all, 4), 4);
+  step(other_lane(s.all, 8), 8);
+  step(other_lane(s.all, 16), 16);
+  step(other_lane(s.all, 32), 32);
+  return s;
+}
+
+// A request's change: pages taken, pages given back, new tokens.
+template <class I>
+struct Change {
+  I x[3];
+};
+
+template <class I>
+struct ScanRoom {
+  I of[3][kResizeWaves], all[3];
+};
+
+// Exclusive prefix of the threads' changes (c becomes it) and their sum; threads past n hold none.
+template <class I>
+__device__ inline Change<I> block_scan(Change<I>& c, int64_t n, ScanRoom<I>& room) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int s = x;
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(s, off);
-    if (lane >= off) s += y;
-  }
-  if (lane == 63) red[wv] = s;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kResizeThreads / 64; ++w) {
-    if (w < wv) before += red[w];
-    all += red[w];
+  if (wv * 64 < n) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const LaneSums<I> s = lane_sums(c.x[i]);
+      c.x[i] = s.upto - c.x[i];
+      if (lane == 63) room.of[i][wv] = s.upto;
+    }
+  } else if (lane < 3) {
+    room.of[lane][wv] = 0;
   }
   __syncthreads();
-  *total = all;
-  return before + s - x;
+  if (wv < 3) {
+    const I x = lane < kResizeWaves ? room.of[wv][lane] : 0;
+    const LaneSums<I> s = lane_sums(x);
+    if (lane < kResizeWaves) room.of[wv][lane] = s.upto - x;
+    if (lane == 0) room.all[wv] = s.all;
+  }
+  __syncthreads();
+  Change<I> all;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    c.x[i] += room.of[i][wv];
+    all.x[i] = room.all[i];
+  }
+  __syncthreads();
+  return all;
+}
+
+__device__ inline Change<int> change_of(int len, int new_len, const ResizeParams& p) {
+  const int have = paged_pages(len, p.page, p.div), need = paged_pages(new_len, p.page, p.div);
+  return Change<int>{{max(need - have, 0), max(have - need, 0), max(new_len - len, 0)}};
 }
 
 // The last i < n with at[i] <= x (at ascending, at[0] <= x): the request a page or token is of.
@@ -85,86 +127,179 @@ __device__ inline int last_at_most(It at, int n, int x) {
   return lo;
 }
 
-// One workgroup: totals first (all or nothing), then tiles of one request per thread whose pages
-// are shared out over the threads by a search in the tile's prefix sums. The free pages are a
+constexpr int kSlotsInside = 4 * kResizeThreads;  // more tokens' slots are a launch of their own
+
+// Calls f(request, its nth page, t) for the pages t < count of a tile of n requests whose prefix sums
+// are `at`; a thread's pages are consecutive, mostly of one request, so one search serves them.
+template <class F>
+__device__ inline void each_page(const int* at, int n, int count, F f) {
+  const int run = count > kResizeThreads ? 4 : 1;
+  for (int t0 = threadIdx.x * run; t0 < count; t0 += kResizeThreads * run) {
+    int i = 0, end = 0;
+    for (int t = t0; t < min(t0 + run, count); ++t) {
+      if (t >= end) {
+        i = last_at_most(at, n, t);
+        end = i + 1 < n ? at[i + 1] : count;
+      }
+      f(i, t - at[i], t);
+    }
+  }
+}
+
+// One workgroup: totals first (all or nothing), then tiles of one request per thread whose pages and
+// tokens are shared out over the threads by a search in the tile's prefix sums. The free pages are a
 // stack; a page given back lands where a take of the same order would find it, so growing and
 // shrinking back restores the stack. Takes are read before gives are written (they overlap).
+// Bound by its chain of memory latencies and, past some thousand pages, by one CU's instructions.
 __global__ __launch_bounds__(kResizeThreads) void paged_resize_kernel(ResizeParams p) {
-  __shared__ int64_t red3[kResizeThreads / 64][3];
-  __shared__ int red[kResizeThreads / 64];
-  __shared__ int s_at[kResizeThreads], s_have[kResizeThreads], s_need[kResizeThreads];
-  __shared__ int s_bad;
-  const int tid = threadIdx.x;
+  __shared__ ScanRoom<int> room;
+  __shared__ ScanRoom<int64_t> room64;
+  __shared__ int s_flags[kResizeWaves];
+  __shared__ int s_at[kResizeThreads], s_new[kResizeThreads], s_have[kResizeThreads],
+      s_len[kResizeThreads];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t cap = p.W * p.page;
   const int nfree = *p.nfree;
-  if (tid == 0) s_bad = nfree < 0 || nfree > p.P;
-  __syncthreads();
-  int64_t sum[3] = {0, 0, 0};  // taken, given, new tokens
+  const bool one = p.B <= kResizeThreads;  // one tile: its scan gives the totals
+  // bad: a length or count that does not fit; large: sums may pass 31 bits; many: more than a page or
+  // a token of one request
+  bool bad = nfree < 0 || nfree > p.P, large = !one, many = !one;
+  Change<int> before{{0, 0, 0}};
+  Change<int64_t> total{{0, 0, 0}};
+  int len = 0, want = 0;  // the tile's request of this thread
   for (int64_t b = tid; b < p.B; b += kResizeThreads) {
-    const PagedSpan o = paged_span(p.lens[b], 0, cap), n = paged_span(p.new_lens[b], 0, cap);
-    if (!o.ok || !n.ok) {
-      s_bad = 1;
-      continue;
+    len = p.lens[b];
+    want = p.new_lens[b];
+    const PagedSpan o = paged_span(len, 0, cap), n = paged_span(want, 0, cap);
+    bad |= !o.ok || !n.ok;
+    before = change_of(o.len, n.len, p);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      total.x[i] += before.x[i];
+      large |= before.x[i] >= 1 << 20;
+      many |= before.x[i] > 1;
     }
-    const int have = paged_pages(o.len, p.page), need = paged_pages(n.len, p.page);
-    sum[0] += max(need - have, 0);
-    sum[1] += max(have - need, 0);
-    sum[2] += max(n.len - o.len, 0);
   }
-  block_sum3(sum, red3);
-  const int64_t lack = sum[0] - nfree;
-  const int status = s_bad || nfree - sum[0] + sum[1] > p.P ? -1
-                     : sum[2] > p.T ? -2
+  const int flags = (__any(bad) ? 1 : 0) | (__any(large) ? 2 : 0) | (__any(many) ? 4 : 0);
+  if (lane == 0) s_flags[tid >> 6] = flags;
+  const Change<int> own = before;
+  Change<int> all = block_scan(before, p.B, room);
+  const int f = s_flags[lane & (kResizeWaves - 1)];
+  bad = __any(f & 1);
+  large = __any(f & 2);
+  many = __any(f & 4);
+  if (large) {
+    total = block_scan(total, kResizeThreads, room64);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) total.x[i] = all.x[i];
+  }
+  const int64_t lack = total.x[0] - nfree;
+  const int status = bad || nfree - total.x[0] + total.x[1] > p.P ? -1
+                     : total.x[2] > p.T ? -2
                      : lack > 0 ? (int)min(lack, (int64_t)0x7fffffff) : 0;
   if (tid == 0) *p.status = status;
+  const bool inside = p.T <= kSlotsInside;
+  const int live = status == 0 ? (int)total.x[2] : 0;  // slots that are written below
+  if (inside) {
+    for (int t = live + tid; t < p.T; t += kResizeThreads) {
+      p.slots[t] = -1;
+      if (p.pos) p.pos[t] = 0;
+    }
+  }
   if (status != 0) {
     for (int64_t b = tid; b <= p.B; b += kResizeThreads) p.cu[b] = 0;
     return;
   }
-  const int top = nfree - (int)sum[0], left = top + (int)sum[1];
-  int taken = 0, added = 0, given = 0;
+  const int top = nfree - (int)total.x[0], left = top + (int)total.x[1];
+  if (!many && inside) {  // a step of single tokens: every thread serves its own request
+    // the table entry of the page taken, given back or written to
+    const int e = own.x[1] ? paged_pages(want, p.page, p.div) : page_of(len / 16, p.div);
+    int32_t* const entry = p.table + tid * p.table_stride + e;
+    int pg = 0;
+    if (own.x[0]) pg = p.free_pages[nfree - 1 - before.x[0]];
+    else if (own.x[1] || own.x[2]) pg = *entry;
+    __syncthreads();  // takes are read before gives are written
+    if (own.x[0]) *entry = pg;
+    if (own.x[1]) {
+      *entry = -1;
+      p.free_pages[left - 1 - before.x[1]] = pg;
+    }
+    if (own.x[2]) {
+      p.slots[before.x[2]] = (int64_t)pg * p.page + (len - e * p.page);
+      if (p.pos) p.pos[before.x[2]] = len;
+    }
+    if (tid < p.B) {
+      p.cu[tid] = before.x[2];
+      p.lens[tid] = want;
+    }
+    if (tid == 0) {
+      p.cu[p.B] = all.x[2];
+      *p.nfree = left;
+    }
+    return;
+  }
+  int taken = 0, added = 0;
   for (int64_t b0 = 0; b0 < p.B; b0 += kResizeThreads) {
     const int64_t b = b0 + tid;
     const int n = (int)min(p.B - b0, (int64_t)kResizeThreads);
-    const int o = tid < n ? p.lens[b] : 0, w = tid < n ? p.new_lens[b] : 0;
-    const int have = paged_pages(o, p.page), need = paged_pages(w, p.page);
-    int all;
-    const int at_new = block_scan(max(w - o, 0), red, &all);
-    if (tid < n) p.cu[b] = added + at_new;
-    added += all;
-    s_have[tid] = have;
-    s_at[tid] = block_scan(max(need - have, 0), red, &all);
-    __syncthreads();
-    for (int t = tid; t < all; t += kResizeThreads) {
-      const int i = last_at_most(s_at, n, t);
-      p.table[(b0 + i) * p.table_stride + s_have[i] + t - s_at[i]] =
-          p.free_pages[nfree - 1 - (taken + t)];
+    if (large) {
+      len = tid < n ? p.lens[b] : 0;
+      want = tid < n ? p.new_lens[b] : 0;
+      before = change_of(len, want, p);
+      all = block_scan(before, n, room);
     }
-    taken += all;
+    s_have[tid] = paged_pages(len, p.page, p.div);
+    s_at[tid] = before.x[0];
+    s_new[tid] = before.x[2];
+    s_len[tid] = len;
+    if (tid < n) p.cu[b] = added + before.x[2];
+    __syncthreads();
+    each_page(s_at, n, all.x[0], [&](int i, int nth, int t) {
+      p.table[(b0 + i) * p.table_stride + s_have[i] + nth] = p.free_pages[nfree - 1 - (taken + t)];
+    });
+    if (inside) {
+      for (int t = tid; t < all.x[2]; t += kResizeThreads) {
+        const int i = last_at_most(s_new, n, t), pos = s_len[i] + t - s_new[i];
+        const int e = page_of(pos / 16, p.div), fresh = e - s_have[i];
+        // a page of this call from the stack it came from, an earlier one from the table
+        const int64_t pg = fresh >= 0 ? p.free_pages[nfree - 1 - (taken + s_at[i] + fresh)]
+                                      : p.table[(b0 + i) * p.table_stride + e];
+        p.slots[added + t] = pg * p.page + (pos - e * p.page);
+        if (p.pos) p.pos[added + t] = pos;
+      }
+    }
+    taken += all.x[0];
+    added += all.x[2];
     __syncthreads();
   }
   if (tid == 0) p.cu[p.B] = added;
-  if (sum[1] > 0) {
-    for (int64_t b0 = 0; b0 < p.B; b0 += kResizeThreads) {
-      const int64_t b = b0 + tid;
-      const int n = (int)min(p.B - b0, (int64_t)kResizeThreads);
-      const int have = paged_pages(tid < n ? p.lens[b] : 0, p.page);
-      const int need = paged_pages(tid < n ? p.new_lens[b] : 0, p.page);
-      int all;
-      s_need[tid] = need;
-      s_at[tid] = block_scan(max(have - need, 0), red, &all);
-      __syncthreads();
-      for (int t = tid; t < all; t += kResizeThreads) {
-        const int i = last_at_most(s_at, n, t);
-        int32_t* e = p.table + (b0 + i) * p.table_stride + s_need[i] + t - s_at[i];
-        p.free_pages[left - 1 - (given + t)] = *e;
-        *e = -1;
-      }
-      given += all;
-      __syncthreads();
+  int given = 0;
+  for (int64_t b0 = 0; total.x[1] > 0 && b0 < p.B; b0 += kResizeThreads) {
+    const int64_t b = b0 + tid;
+    const int n = (int)min(p.B - b0, (int64_t)kResizeThreads);
+    if (large) {
+      len = tid < n ? p.lens[b] : 0;
+      want = tid < n ? p.new_lens[b] : 0;
+      before = change_of(len, want, p);
+      all = block_scan(before, n, room);
     }
+    s_have[tid] = paged_pages(want, p.page, p.div);  // what is kept
+    s_at[tid] = before.x[1];
+    __syncthreads();
+    each_page(s_at, n, all.x[1], [&](int i, int nth, int t) {
+      int32_t* e = p.table + (b0 + i) * p.table_stride + s_have[i] + nth;
+      p.free_pages[left - 1 - (given + t)] = *e;
+      *e = -1;
+    });
+    given += all.x[1];
+    __syncthreads();
   }
-  for (int64_t b = tid; b < p.B; b += kResizeThreads) p.lens[b] = p.new_lens[b];
+  if (one) {
+    if (tid < p.B) p.lens[tid] = want;
+  } else {
+    for (int64_t b = tid; b < p.B; b += kResizeThreads) p.lens[b] = p.new_lens[b];
+  }
   if (tid == 0) *p.nfree = left;
 }
 
@@ -177,7 +312,7 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(ResizeParams p) {
   if (t < p.cu[p.B]) {
     const int b = last_at_most(p.cu, (int)p.B, (int)t);
     pos = p.lens[b] - p.cu[b + 1] + (int)t;
-    const int e = pos / p.page;
+    const int e = page_of(pos / 16, p.div);
     slot = (int64_t)p.table[b * p.table_stride + e] * p.page + (pos - e * p.page);
   }
   p.slots[t] = slot;
@@ -284,28 +419,6 @@ struct Item {
   int b, j, n, begin, end, first_item;
   PagedSpan span;
 };
-
-// Sums over the wave and up to (and with) each lane: a block of lanes takes the sum of the block
-// beside it, and its upper lanes add it to their prefix.
-struct LaneSums {
-  int all, upto;
-};
-
-__device__ inline LaneSums lane_sums(int x) {
-  const int lane = threadIdx.x & 63;
-  LaneSums s{x, x};
-  auto step = [&](int y, int off) {
-    s.upto += lane & off ? y : 0;
-    s.all += y;
-  };
-  step(lane_xor(s.all, 1), 1);
-  step(lane_xor(s.all, 2), 2);
-  step(lane_xor(s.all, 4), 4);
-  step(lane_xor(s.all, 8), 8);
-  step(lane_xor(s.all, 16), 16);
-  step(lane_xor(s.all, 32), 32);
-  return s;
-}
 
 // Finds item `index` from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. False past the last item.
@@ -965,12 +1078,12 @@ extern "C" int ssa_paged_resize(int32_t* lens, const int32_t* new_lens, int32_t*
               (long long)W);
   SSA_REQUIRE(fits_int(T) && (T == 0 || slots), SSA_ERR_INVALID,
               "ssa_paged_resize: T=%lld slots", (long long)T);
-  ResizeParams p{lens,  new_lens, table, table_stride, B,   W,     (int)page, free_pages,
-                 pages, nfree,    slots, pos,          T,   cu,    status};
+  ResizeParams p{lens,  new_lens, table, table_stride, B, W,  (int)page, free_pages,
+                 pages, nfree,    slots, pos,          T, cu, status,    page_div((int)page / 16)};
   hipStream_t st = (hipStream_t)stream;
   paged_resize_kernel<<<1, kResizeThreads, 0, st>>>(p);
   SSA_TRY(launch_status("paged_resize_kernel"));
-  if (T > 0) {
+  if (T > kSlotsInside) {
     paged_slots_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(p);
     SSA_TRY(launch_status("paged_slots_kernel"));
   }
@@ -1039,6 +1152,9 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
               SSA_ERR_INVALID, "ssa_paged_attend: rows must start at multiples of 16 bytes");
   SSA_REQUIRE(strides[4] < (1 << 24) && strides[7] < (1 << 24), SSA_ERR_UNSUPPORTED,
               "ssa_paged_attend: slots 2^24 elements apart or more");
+  SSA_REQUIRE(B * paged_most_units(W * page, (int)window) <= 0x7fffffff, SSA_ERR_UNSUPPORTED,
+              "ssa_paged_attend: %lld table rows of %lld tokens (2^38 in all at most)",
+              (long long)B, (long long)(W * page));
   const Layout y = layout(B, Hq, Hkv, d, W, page, window);
   SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
               SSA_ERR_WORKSPACE, "ssa_paged_attend: needs a 16-byte aligned workspace of %zu bytes, "

@@ -28,8 +28,6 @@ SSA_HD PagedSpan paged_span(int len, int window, int64_t cap) {
   return s;
 }
 
-SSA_HD int paged_pages(int len, int page) { return (int)(((int64_t)len + page - 1) / page); }
-
 // A request's keys are cut at multiples of 16 (a subtile, never across pages: pages hold a multiple
 // of 16 tokens) and dealt out in units of kPagedUnit subtiles.
 constexpr int kPagedUnit = 8;
@@ -78,7 +76,7 @@ SSA_HD PagedRange paged_item_range(const PagedSpan& s, int units, int j, int n) 
   return r;
 }
 
-// Division of a subtile's number (below 2^27: lengths are below 2^31) by the subtiles of a page, D up
+// Division of a subtile's number (below 2^28: lengths are below 2^31) by the subtiles of a page, D up
 // to 4096, as a multiplication: mul = ceil(2^(31 + shift) / D), 2^shift <= D < 2^(shift + 1), is off
 // by less than 1 in 2^(31 + shift) / D > 2^30, more than any quotient's distance from the next.
 struct PageDiv {
@@ -96,6 +94,11 @@ SSA_HD PageDiv page_div(int subtiles) {
 
 SSA_HD int page_of(int subtile, const PageDiv& d) {
   return (int)(((uint64_t)((unsigned)subtile * 2u) * d.mul >> 32) >> d.shift);
+}
+
+// Pages that hold len tokens.
+SSA_HD int paged_pages(int len, int page, const PageDiv& d) {
+  return page_of((int)(((unsigned)len + 15u) / 16u) + page / 16 - 1, d);
 }
 
 }  // namespace ssa

@@ -67,12 +67,17 @@ int main() {
   for (int d = 1; d <= 4096; ++d) {
     const PageDiv div = page_div(d);
     for (int k = 0; k < 200; ++k) {
-      const int64_t q = k < 3 ? k : upto((1 << 27) / d);
+      const int64_t q = k < 3 ? k : upto((1 << 28) / d);
       for (int64_t x = q * d - 1; x <= q * d + 1; ++x)
-        if (x >= 0 && x < 1 << 27 && page_of((int)x, div) != x / d) {
+        if (x >= 0 && x < 1 << 28 && page_of((int)x, div) != x / d) {
           std::printf("%lld / %d\n", (long long)x, d);
           return 1;
         }
+      const int64_t page = 16 * d, len = k < 4 ? 0x7fffffff - k : upto(k % 2 ? 5 * page : 0x7fffffff);
+      if (paged_pages((int)len, (int)page, div) != (len + page - 1) / page) {
+        std::printf("pages of %lld tokens at %d\n", (long long)len, (int)page);
+        return 1;
+      }
     }
   }
   std::puts("ok");

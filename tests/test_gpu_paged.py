@@ -68,6 +68,31 @@ def test_resize_equals_lists(cuda, requests, page, max_len):
     assert {0, -1} <= statuses
 
 
+@pytest.mark.parametrize("requests,pages", [(1, 4), (64, 150), (300, 400), (1024, 2000)])
+def test_resize_by_single_tokens(cuda, requests, pages):
+    """Steps in which no request changes by more than a token or a page: decode steps, tokens taken back,
+    requests that end; now and then refused."""
+    rng = random.Random(pages)
+    page = 16
+    cache = P.PagedCache(requests, 320, pages, 1, 8, page=page, device=cuda)
+    ref = U.PageState(requests, 20, pages, page)
+    lens = [rng.randrange(1 if pages < 500 else 33) for _ in range(requests)]
+    ref.resize(lens, sum(lens))
+    cache.resize(int32(lens, cuda), sum(lens))
+    statuses = set()
+    for step in range(60):
+        move = rng.choice(["grow", "grow", "all", "back", "mixed"])
+        new = [min(n + 1, 320) if move == "all" or move in ("grow", "mixed") and rng.random() < 0.7
+               else max(0, n - rng.randrange(page)) if move in ("back", "mixed") else n
+               for n in ref.lens]
+        room = requests + rng.choice([0, 3]) - (step % 20 == 7) * requests
+        want = ref.resize(new, room)
+        r = cache.resize(int32(new, cuda), room)
+        check_state(cache, ref, r, want)
+        statuses.add(min(want[3], 1))
+    assert -2 in statuses and 0 in statuses
+
+
 def test_resize_grown_and_shrunk_back_restores_the_state(cuda):
     cache = P.PagedCache(40, 1000, 800, 1, 8, page=16, device=cuda)
     rng = random.Random(4)
@@ -81,6 +106,41 @@ def test_resize_grown_and_shrunk_back_restores_the_state(cuda):
     cache.check()
     for x, y in zip((cache.lens, cache.table, cache.free, cache.nfree), held):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("requests", [3, 1100])
+def test_resize_sums_past_31_bits(cuda, requests):
+    """Lengths whose pages or tokens add up past 2^31 are counted, not wrapped; a request of more than a
+    million pages is served."""
+    i32 = dict(device=cuda, dtype=torch.int32)
+    width, pages = 2 ** 27 - 1, 1200000
+    table = torch.full((1, width), -1, **i32).expand(requests, width)  # refused before it is written
+    lens, free = torch.zeros(requests, **i32), torch.arange(pages, **i32)
+    nfree, new = torch.full((1,), pages, **i32), torch.full((requests,), width * 16, **i32)
+    ptr = lambda t: t.data_ptr()  # noqa: E731
+    out = torch.empty(8, device=cuda, dtype=torch.int64), torch.empty(requests + 1, **i32)
+    status = torch.empty(1, **i32)
+
+    # 2^31 - 16 tokens each, room for 8: the table is neither read nor written
+    _lib.call("ssa_paged_resize", ptr(lens), ptr(new), ptr(table), width, requests, width, 16,
+              ptr(free), pages, ptr(nfree), ptr(out[0]), None, 8, ptr(out[1]), ptr(status),
+              _lib.stream_of(lens))
+    assert status.item() == -2 and (out[0] == -1).all() and (out[1] == 0).all()
+    assert (lens == 0).all() and nfree.item() == pages
+    new.zero_()
+    new[0] = 17 * 10 ** 6
+    cache = P.PagedCache(requests, 17 * 10 ** 6, pages, 1, 8, page=16, dtype=torch.float16,
+                         device=cuda)
+    r = cache.resize(new, 17 * 10 ** 6 + 5)
+    assert r.status.item() == 0 and cache.nfree.item() == pages - 1062500
+    assert torch.equal(cache.table[0, :1062500], torch.arange(1062500, **i32))
+    at = torch.arange(17 * 10 ** 6, device=cuda)
+    assert torch.equal(r.slots[:-5], at) and (r.slots[-5:] == -1).all()
+    assert torch.equal(r.pos[:-5], at.to(torch.int32)) and r.cu[1].item() == 17 * 10 ** 6
+    cache.resize(torch.zeros_like(new), 0)
+    cache.check()
+    assert torch.equal(cache.free, torch.arange(pages, **i32).flip(0))
+    assert (cache.table == -1).all() and cache.nfree.item() == pages
 
 
 def test_resize_into_its_own_lengths_changes_nothing(cuda):
