@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "paged_index.h"
@@ -368,6 +369,7 @@ struct AttendParams {
   int64_t kpp, kph, kps, vpp, vph, vps;   // elements
   int64_t knb, knh, vnb, vnh;             // elements
   PageDiv div;           // by the subtiles of a page
+  int64_t stream_units;  // units of a key head from which a call streams
   int RT, items, units;  // row tiles of 16 heads; items aimed at (0: one per request); grid units
   float* part;           // (item, query head, DP): parts of rows that several items share
   float* part_ml;        // (item, query head, 2): their m and l
@@ -392,6 +394,7 @@ __device__ inline void store_row4(char* base, int64_t i, const f32x4& x) {
 }
 
 constexpr float kF16Shift = 14.0f;
+constexpr int64_t kStreamBytes = (int64_t)192 << 20;
 
 // How a call is laid out, by type and padded head dim DP. The 16-bit products take 32 keys at once
 // (two subtiles), the fp32 ones 4, so their tile is one subtile where registers are short.
@@ -417,6 +420,7 @@ __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x);
 // of the request's item 0 among all.
 struct Item {
   int b, j, n, begin, end, first_item;
+  bool stream;  // the call reads more than stays in the caches
   PagedSpan span;
 };
 
@@ -430,6 +434,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
     it.j = 0;
     it.n = 1;
     it.first_item = index;
+    it.stream = p.stream_units == 0;
     const int units = paged_units(it.span);
     const PagedRange r = paged_item_range(it.span, units, 0, 1);
     it.begin = r.begin;
@@ -440,7 +445,8 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
     const int len = lane < p.B ? p.lens[lane] : 0;
     const int units = paged_units(paged_span(len, p.window, p.cap));
     // 64 of at most 2^24 units fit 32 bits
-    const int n = paged_items(units, paged_chunk(lane_sums(units).all, p.items));
+    const int all = lane_sums(units).all, n = paged_items(units, paged_chunk(all, p.items));
+    it.stream = all >= p.stream_units;
     const int upto = lane_sums(n).upto;
     const unsigned long long past = __ballot(upto > index);
     if (past == 0) return false;
@@ -460,6 +466,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   for (int b = b0; b < b1; ++b) units += paged_units(paged_span(p.lens[b], p.window, p.cap));
   for (int off = 32; off >= 1; off >>= 1) units += __shfl_xor(units, off);
   const int chunk = paged_chunk(units, p.items);
+  it.stream = units >= p.stream_units;
   int mine = 0;
   for (int b = b0; b < b1; ++b)
     mine += paged_items(paged_units(paged_span(p.lens[b], p.window, p.cap)), chunk);
@@ -493,6 +500,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
 __device__ inline Item uniform(const Item& x) {
   return Item{uniform(x.b),     uniform(x.j),   uniform(x.n),
               uniform(x.begin), uniform(x.end), uniform(x.first_item),
+              uniform((int)x.stream) != 0,
               PagedSpan{uniform(x.span.first), uniform(x.span.len), uniform((int)x.span.ok) != 0}};
 }
 
@@ -566,16 +574,15 @@ __device__ inline Buffer buffer_at(const char* p) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, kSpan, 0x00027000);
 }
 
-__device__ inline u32x4 load16(Buffer b, int off) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
-}
+// AUX: 0, or kStream for the non-temporal hint.
+constexpr int kStream = 2;
 
-template <int W>
+template <int W, int AUX>
 __device__ inline Words<W> load_words(Buffer b, int off) {
   if constexpr (W == 4)
-    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, AUX));
   else
-    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
+    return __builtin_bit_cast(Words<W>, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, AUX));
 }
 
 // The rows of a lane's keys and values as they come from the cache, in the layouts of the products'
@@ -706,18 +713,19 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
     const int c = vb * T::CB * T::ES + col * LW * 4;
     vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
   }
-  auto load_k = [&](int i, int piece) {
+  auto load_k_as = [&](auto aux, int piece) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const Buffer src = buffer_at(kbase + (pg[t] * kpp + (int64_t)off[t] * kps));
 #pragma unroll
       for (int c = 0; c < NC / T::KP; ++c) {
         const int at = (piece * (NC / T::KP) + c) * 64;
-        rows.k[t][c] = load16(src, at + grp * 16 < row_bytes ? koff + at : kOutside);
+        rows.k[t][c] = __builtin_bit_cast(
+            u32x4, load_words<4, aux.value>(src, at + grp * 16 < row_bytes ? koff + at : kOutside));
       }
     }
   };
-  auto load_v = [&](int i) {
+  auto load_v_as = [&](auto aux, int i) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const Buffer src = buffer_at(vbase + (pg[t] * vpp + (int64_t)off[t] * vps));
@@ -729,14 +737,26 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
         const int n = grp * 4 + r, at = (unsigned)(n - lo) < (unsigned)max(count, 0) ? n * vps
                                                                                     : kOutside;
 #pragma unroll
-        for (int vb = 0; vb < VB; ++vb) rows.v[t][r][vb] = load_words<LW>(src, at + vcol[vb]);
+        for (int vb = 0; vb < VB; ++vb)
+          rows.v[t][r][vb] = load_words<LW, aux.value>(src, at + vcol[vb]);
       }
     }
+  };
+  constexpr bool kMayStream = DP < 512;  // there its second set of loads costs the registers
+  using Plain = std::integral_constant<int, 0>;
+  using Stream = std::integral_constant<int, kStream>;
+  auto load_k = [&](int piece) {
+    if (kMayStream && it.stream) load_k_as(Stream{}, piece);
+    else load_k_as(Plain{}, piece);
+  };
+  auto load_v = [&](int i) {
+    if (kMayStream && it.stream) load_v_as(Stream{}, i);
+    else load_v_as(Plain{}, i);
   };
 
   if (i0 < i1) {
     locate(i0);
-    load_k(i0, 0);
+    load_k(0);
     load_v(i0);
   }
   for (int i = i0; i < i1; ++i) {
@@ -750,7 +770,7 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       constexpr int per = NC / T::KP;
-      if (c > 0 && c % per == 0) load_k(i, c / per);
+      if (c > 0 && c % per == 0) load_k(c / per);
       u32x4 qc;
       if constexpr (T::kQInLds) qc = q_lds[c][lane];
       else qc = q[c];
@@ -771,7 +791,7 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
     const bool more = i + 1 < i1;
     if (more) {
       locate(i + 1);
-      load_k(i + 1, 0);
+      load_k(0);
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -1186,6 +1206,12 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   p.div = page_div((int)page / 16);
   p.RT = (int)y.RT;
   p.items = (int)y.items;
+  // What does not fit the 256 MB last-level cache is read past it, unless row tiles read it twice: 537
+  // MB 91 us with the hint, 101 without; 105 MB that the cache holds 30 and 27.
+  const int64_t unit_bytes = 2 * 16 * kPagedUnit * d * es * Hkv;
+  p.stream_units = y.RT > 1 ? INT64_MAX : kStreamBytes / unit_bytes;
+  if (y.items == 0 && B * paged_most_units(W * page, (int)window) >= p.stream_units)
+    p.stream_units = 0;
   p.part = (float*)workspace;
   p.part_ml = (float*)((char*)workspace + y.part_ml);
   p.info = (int32_t*)((char*)workspace + y.info);
