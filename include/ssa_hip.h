@@ -501,8 +501,11 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
  *   of the row's sum of exponentials. A row of length 0: out 0, lse -inf. A length outside
  *   [0, W * page] or an attended page id outside [0, pages): out and lse NaN. k_new, v_new (B, Hkv,
  *   d), both or none: the key and value at position len - 1, which the call stores into the pools
- *   and attends (that page must be one request's alone; earlier pages may be shared). strides[14] =
- *   q(b,h), kpool(page,head,slot), vpool(page,head,slot), out(b,h), k_new(b,h), v_new(b,h).
+ *   and attends (that page must be one request's alone; earlier pages may be shared). status, may be
+ *   NULL: the status of the resize that made room; if it is not 0 nothing is stored and every row is
+ *   NaN (the position len - 1 is then an older token's). strides[14] = q(b,h), kpool(page,head,slot),
+ *   vpool(page,head,slot), out(b,h), k_new(b,h), v_new(b,h). Slots lie fewer than 2^24 elements apart;
+ *   B table rows hold at most 2^38 tokens in all.
  *   Workspace: ssa_paged_attend_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
  * Rows start at multiples of 16 bytes (bases and strides).
  */
@@ -519,7 +522,8 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
                      int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t pages, int64_t page,
                      const int32_t* table, int64_t table_stride, int64_t W, const int32_t* lens,
                      const void* k_new, const void* v_new, const int64_t* strides, float scale,
-                     int64_t window, void* workspace, size_t workspace_bytes, ssa_stream_t stream);
+                     int64_t window, const int32_t* status, void* workspace,
+                     size_t workspace_bytes, ssa_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -101,7 +101,7 @@ _SIGNATURES = {
     "ssa_paged_append": (_c_int, [_c_p] * 4 + [_c_int] + [_c_i64] * 5 + [_c_p] * 3),
     "ssa_paged_attend_workspace_size": (_c_sz, [_c_i64] * 7),
     "ssa_paged_attend": (_c_int, [_c_p] * 5 + [_c_int] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] +
-                         [_c_p] * 4 + [_c_f, _c_i64, _c_p, _c_sz, _c_p]),
+                         [_c_p] * 4 + [_c_f, _c_i64, _c_p, _c_p, _c_sz, _c_p]),
 }
 
 _lock = threading.Lock()

@@ -362,6 +362,7 @@ struct AttendParams {
   const char* v_new;
   const int32_t* table;
   const int32_t* lens;
+  const int32_t* status;  // of the resize before, or NULL
   int64_t table_stride, cap, pages;
   int B, Hq, Hkv, G, d, page, window;
   float scale_log2;
@@ -424,13 +425,19 @@ struct Item {
   PagedSpan span;
 };
 
+// The tokens of a table row; none fits after a refused resize (every row is then answered as bad).
+__device__ inline int64_t row_cap(const AttendParams& p) {
+  return p.status && *p.status != 0 ? -1 : p.cap;
+}
+
 // Finds item `index` from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. False past the last item.
 __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   const int lane = threadIdx.x & 63;
+  const int64_t cap = row_cap(p);
   if (p.items == 0) {  // an item per request
     it.b = index;
-    it.span = paged_span(p.lens[index], p.window, p.cap);
+    it.span = paged_span(p.lens[index], p.window, cap);
     it.j = 0;
     it.n = 1;
     it.first_item = index;
@@ -443,7 +450,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   }
   if (p.B <= 64) {  // a request per lane
     const int len = lane < p.B ? p.lens[lane] : 0;
-    const int units = paged_units(paged_span(len, p.window, p.cap));
+    const int units = paged_units(paged_span(len, p.window, cap));
     // 64 of at most 2^24 units fit 32 bits
     const int all = lane_sums(units).all, n = paged_items(units, paged_chunk(all, p.items));
     it.stream = all >= p.stream_units;
@@ -451,7 +458,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
     const unsigned long long past = __ballot(upto > index);
     if (past == 0) return false;
     it.b = __builtin_ctzll(past);
-    it.span = paged_span(__builtin_amdgcn_readlane(len, it.b), p.window, p.cap);
+    it.span = paged_span(__builtin_amdgcn_readlane(len, it.b), p.window, cap);
     it.n = __builtin_amdgcn_readlane(n, it.b);
     it.first_item = __builtin_amdgcn_readlane(upto - n, it.b);
     it.j = index - it.first_item;
@@ -463,13 +470,13 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   }
   const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
   int64_t units = 0;
-  for (int b = b0; b < b1; ++b) units += paged_units(paged_span(p.lens[b], p.window, p.cap));
+  for (int b = b0; b < b1; ++b) units += paged_units(paged_span(p.lens[b], p.window, cap));
   for (int off = 32; off >= 1; off >>= 1) units += __shfl_xor(units, off);
   const int chunk = paged_chunk(units, p.items);
   it.stream = units >= p.stream_units;
   int mine = 0;
   for (int b = b0; b < b1; ++b)
-    mine += paged_items(paged_units(paged_span(p.lens[b], p.window, p.cap)), chunk);
+    mine += paged_items(paged_units(paged_span(p.lens[b], p.window, cap)), chunk);
   int upto = mine;
   for (int off = 1; off < 64; off <<= 1) {
     const int y = __shfl_up(upto, off);
@@ -480,7 +487,7 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   const int owner = __builtin_ctzll(past);
   int at = uniform(__builtin_amdgcn_readlane(upto - mine, owner));
   for (int b = uniform(owner * run);; ++b) {
-    const PagedSpan s = paged_span(p.lens[b], p.window, p.cap);
+    const PagedSpan s = paged_span(p.lens[b], p.window, cap);
     const int u = paged_units(s), n = paged_items(u, chunk);
     if (index < at + n) {
       it.b = b;
@@ -938,7 +945,7 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(AttendParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
   const int h = blockIdx.x, b = blockIdx.y, c = tid % PER * 4, split = tid / PER;
   const int len = p.lens[b], first = p.info[2 * b], parts = p.info[2 * b + 1];
-  const PagedSpan s = paged_span(len, p.window, p.cap);
+  const PagedSpan s = paged_span(len, p.window, row_cap(p));
   Softmax<1> st;
   st.m = -INFINITY;
   st.l = s.ok ? 0.0f : NAN;
@@ -1148,8 +1155,9 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
                                 int64_t pages, int64_t page, const int32_t* table,
                                 int64_t table_stride, int64_t W, const int32_t* lens,
                                 const void* k_new, const void* v_new, const int64_t* strides,
-                                float scale, int64_t window, void* workspace,
-                                size_t workspace_bytes, ssa_stream_t stream) {
+                                float scale, int64_t window, const int32_t* status,
+                                void* workspace, size_t workspace_bytes,
+                                ssa_stream_t stream) {
   SSA_REQUIRE(q && kpool && vpool && out && table && lens && strides, SSA_ERR_INVALID,
               "ssa_paged_attend: NULL argument");
   SSA_REQUIRE((k_new == nullptr) == (v_new == nullptr), SSA_ERR_INVALID,
@@ -1189,6 +1197,7 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   p.v_new = (const char*)v_new;
   p.table = table;
   p.lens = lens;
+  p.status = status;
   p.table_stride = table_stride;
   p.cap = W * page;
   p.pages = pages;

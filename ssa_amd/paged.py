@@ -97,6 +97,12 @@ def _pools(k, v):
     return kshape
 
 
+def _written(name, meta):
+    """Refuses a broadcast tensor (a stride of 0) where rows are written."""
+    if any(n > 1 and st == 0 for n, st in zip(*meta[:2])):
+        raise ValueError(f"{name} is written and must not be broadcast")
+
+
 def _rows16(meta):
     """Whether rows (the last dimension) start at multiples of 16 bytes, given an aligned base."""
     shape, stride, dtype = meta
@@ -111,6 +117,7 @@ def _resize_plan(lens, new_lens, table, free, nfree):
     _int32("new_lens", *new_lens, (B,))
     _int32("nfree", *nfree, (1,))
     _int32("free", *free, (free[0].numel(),))
+    _written("table", table)
     return B, W, row, free[0].numel()
 
 
@@ -123,6 +130,8 @@ def _append_plan(k, v, kpool, vpool, slots):
         raise TypeError(f"k is {k[2]} and v {v[2]}, the cache holds {dtype}")
     if slots[2] != torch.int64 or len(slots[0]) != 1 or slots[0][0] > 1 and slots[1] != (1,):
         raise ValueError("slots must be a contiguous (T,) int64 tensor")
+    _written("kpool", kpool)
+    _written("vpool", vpool)
     T = slots[0][0]
     if k[0] != (T, hkv, d) or v[0] != (T, hkv, d):
         raise ValueError(f"k and v must be ({T}, {hkv}, {d}), got {tuple(k[0])} and "
@@ -151,6 +160,8 @@ def _attend_plan(q, kpool, vpool, table, lens, out, k_new, v_new, window):
             raise TypeError(f"k_new is {k_new[2]} and v_new {v_new[2]}, the cache holds {dtype}")
         if k_new[0] != (B, hkv, d) or v_new[0] != (B, hkv, d):
             raise ValueError(f"k_new and v_new must be ({B}, {hkv}, {d})")
+        _written("kpool", kpool)
+        _written("vpool", vpool)
         copy = copy or not (_rows16(k_new) and _rows16(v_new))
         new = (*k_new[1][:2], *v_new[1][:2])
     rows, W, row = _table(*table)
@@ -162,6 +173,7 @@ def _attend_plan(q, kpool, vpool, table, lens, out, k_new, v_new, window):
         if out[2] != dtype or out[0] != (B, hq, d) or not _rows16(out):
             raise ValueError(f"out must be a ({B}, {hq}, {d}) {dtype} tensor with rows of 16-byte "
                              "pieces")
+        _written("out", out)
         to = out[1][:2]
     strides = _lib.i64_array((*q[1][:2], *kpool[1][:3], *vpool[1][:3], *to, *new))
     ws_bytes = _lib.query("ssa_paged_attend_workspace_size", B, hq, hkv, d, W, page, window)
@@ -244,7 +256,8 @@ def _own(t):
 def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor,
                  lens: torch.Tensor, k_new: torch.Tensor | None = None,
                  v_new: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
-                 return_lse: bool = False, out: torch.Tensor | None = None):
+                 return_lse: bool = False, out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None):
     """Attention of one token per request over its cached keys: q (B, Hq, d), out (B, Hq, d) in
     q's dtype; request b attends its keys j < lens[b] (with a window, the last `window` of them),
     softmax(scale * q.k) in fp32, query head h reading key head h // (Hq / Hkv). A request of
@@ -252,28 +265,31 @@ def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tabl
 
     k_new, v_new (B, Hkv, d): the token at position lens[b] - 1, stored into the cache by this
     call and attended with the rest (the page that holds that position must be the request's own;
-    earlier pages may be shared between requests). return_lse: also the natural log of each row's
+    earlier pages may be shared between requests). status (1,) int32: a resize's; if that resize was
+    refused, nothing is stored (lens[b] - 1 is then an older token's position) and every row is NaN.
+    return_lse: also the natural log of each row's
     sum of exponentials (B, Hq) fp32, with which partial results can be joined."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if torch.compiler.is_compiling():
         from . import torch_ops as T
         if k_new is None:
-            o, lse = T.paged_attend(q, kpool, vpool, table, lens, float(scale), int(window))
+            o, lse = T.paged_attend(q, kpool, vpool, table, lens, float(scale), int(window),
+                                    status)
         else:
             o, lse = T.paged_step(q, kpool, vpool, table, lens, k_new, v_new, float(scale),
-                                  int(window))
+                                  int(window), status)
         if out is not None:
             out.copy_(o)
             o = out
         return (o, lse) if return_lse else o
     return _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window,
-                              return_lse, out)
+                              return_lse, out, status)
 
 
 def _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, return_lse,
-                       out=None):
-    _one_device(q, kpool, vpool, table, lens, k_new, v_new, out)
+                       out=None, status=None):
+    _one_device(q, kpool, vpool, table, lens, k_new, v_new, out, status)
     window = int(window)
     sizes, rows, strides, ws_bytes, copy = _attend_plan(
         _meta(q), _meta(kpool), _meta(vpool), _meta(table), _meta(lens),
@@ -284,17 +300,19 @@ def _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window
     if copy or (qp if kp is None else qp | kp | vp) & 15:
         k_new, v_new = (None if t is None else _own(t) for t in (k_new, v_new))
         return _attend_pages_impl(_own(q), kpool, vpool, table, lens, k_new, v_new, scale, window,
-                                  return_lse, out)
+                                  return_lse, out, status)
     _, B, hq, _, d, _, _ = sizes
     dev = q.device
     if out is None:
         out = torch.empty(B, hq, d, device=dev, dtype=q.dtype)
     lse = torch.empty(B, hq, device=dev, dtype=torch.float32) if return_lse else None
+    if status is not None:
+        _int32("status", *_meta(status), (1,))
     if B:
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
         _launch("ssa_paged_attend", q, qp, kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(),
                 _lib.ptr(lse), *sizes, table.data_ptr(), *rows, lens.data_ptr(), kp, vp, strides,
-                float(scale), window, _lib.ptr(ws), ws_bytes)
+                float(scale), window, _lib.ptr(status), _lib.ptr(ws), ws_bytes)
     return (out, lse) if return_lse else out
 
 
@@ -308,8 +326,10 @@ class PagedCache:
         cache.append(layer, k, v, r.slots)                # a prompt's tokens, or
         o = cache.step(layer, q, k_new, v_new)            # one token of every request
 
-    A request ends by a resize to length 0. `check` raises if the last resize did not fit (it
-    synchronises; a caller that keeps count of the pages need not call it)."""
+    A request ends by a resize to length 0; q, k_new and v_new have a row for every request, idle ones
+    included. After a resize that did not fit, append and step store nothing and attend and step give
+    NaN, until a resize fits; `check` raises then (it synchronises; a caller that keeps count of the
+    pages need not call it)."""
 
     def __init__(self, requests, max_len, pages, hkv, d, page=64, layers=1, dtype=torch.bfloat16,
                  device="cuda", token_major=False):
@@ -355,7 +375,8 @@ class PagedCache:
     @torch.no_grad()
     def attend(self, layer: int, q: torch.Tensor, **kwargs):
         """attend_pages over a layer's pools (scale, window, return_lse, out as there)."""
-        return attend_pages(q, self.k[layer], self.v[layer], self.table, self.lens, **kwargs)
+        return attend_pages(q, self.k[layer], self.v[layer], self.table, self.lens,
+                            status=self.status, **kwargs)
 
     @torch.no_grad()
     def step(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,

@@ -22,8 +22,9 @@ dtypes. Run eagerly, the public functions call the library directly and skip the
     ssa_amd::paged_resize(lens!, new_lens, table!, free!, nfree!, page, tokens)
         -> (slots, pos, cu, status)
     ssa_amd::paged_append(k, v, kpool!, vpool!, slots)
-    ssa_amd::paged_attend(q, kpool, vpool, table, lens, scale, window) -> (out, lse)
-    ssa_amd::paged_step(q, kpool!, vpool!, table, lens, k_new, v_new, scale, window) -> (out, lse)
+    ssa_amd::paged_attend(q, kpool, vpool, table, lens, scale, window, status) -> (out, lse)
+    ssa_amd::paged_step(q, kpool!, vpool!, table, lens, k_new, v_new, scale, window, status)
+        -> (out, lse)
     (! = written in place; workspace None runs the allocation-free ssa_decode_step_static; the
     reference has no paged cache)
 """
@@ -185,26 +186,29 @@ def _(k, v, kpool, vpool, slots):
 
 @torch.library.custom_op("ssa_amd::paged_attend", mutates_args=())
 def paged_attend(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
-                 scale: float, window: int) -> tuple[Tensor, Tensor]:
+                 scale: float, window: int,
+                 status: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     from .paged import _attend_pages_impl
-    return _attend_pages_impl(q, kpool, vpool, table, lens, None, None, scale, window, True)
+    return _attend_pages_impl(q, kpool, vpool, table, lens, None, None, scale, window, True, None,
+                              status)
 
 
 @paged_attend.register_fake
-def _(q, kpool, vpool, table, lens, scale, window):
+def _(q, kpool, vpool, table, lens, scale, window, status=None):
     return (torch.empty_like(q, memory_format=torch.contiguous_format),
             q.new_empty(q.shape[:2], dtype=_F32))
 
 
 @torch.library.custom_op("ssa_amd::paged_step", mutates_args=("kpool", "vpool"))
 def paged_step(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
-               k_new: Tensor, v_new: Tensor, scale: float,
-               window: int) -> tuple[Tensor, Tensor]:
+               k_new: Tensor, v_new: Tensor, scale: float, window: int,
+               status: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     from .paged import _attend_pages_impl
-    return _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, True)
+    return _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window, True, None,
+                              status)
 
 
 @paged_step.register_fake
-def _(q, kpool, vpool, table, lens, k_new, v_new, scale, window):
+def _(q, kpool, vpool, table, lens, k_new, v_new, scale, window, status=None):
     return (torch.empty_like(q, memory_format=torch.contiguous_format),
             q.new_empty(q.shape[:2], dtype=_F32))

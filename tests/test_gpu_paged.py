@@ -511,6 +511,26 @@ def test_prompts_then_steps_then_ends(cuda, dtype, token_major):
         step()
 
 
+def test_refused_resize_stores_nothing(cuda):
+    """After a resize that did not fit, step and append leave the cache as it is and the rows are NaN."""
+    cache = P.PagedCache(3, 100, 6, 2, 64, page=16, dtype=torch.float16, device=cuda)
+    x = torch.randn(60, 2, 64, device=cuda).to(torch.float16)
+    q = torch.randn(3, 4, 64, device=cuda).to(torch.float16)
+    r = cache.resize(int32([40, 16, 0], cuda), 56)
+    cache.append(0, x[:56], x[:56], r.slots)
+    good = cache.attend(0, q)
+    held = cache.k.clone(), cache.v.clone()
+    r = cache.resize(cache.lens + int32([1, 1, 33], cuda), 60)  # 1 + 3 pages, 2 are free
+    assert r.status.item() == 2
+    cache.append(0, x, x, r.slots)
+    out, lse = cache.step(0, q, x[:3], x[:3], return_lse=True)
+    assert out.isnan().all() and lse.isnan().all()
+    assert cache.attend(0, q, window=20).isnan().all()
+    assert torch.equal(cache.k, held[0]) and torch.equal(cache.v, held[1])
+    cache.resize(cache.lens.clone(), 0)
+    assert torch.equal(cache.attend(0, q), good) and (good[2] == 0).all()
+
+
 def test_captured_step_replayed(cuda):
     """resize, step and attend captured in one graph and replayed with eager work between: each replay
     grows every live request by a token, as the eager cache beside it does."""
@@ -625,6 +645,13 @@ def test_arguments_are_refused(cuda):
         (TypeError, lambda: A(q, k, v, table, lens, k_new=new, v_new=new.float())),
         (ValueError, lambda: A(q, k, v, table, lens, out=torch.empty_like(q)[:1])),
         (ValueError, lambda: A(q, k, v, table, lens, out=torch.empty_like(q.float()))),
+        (ValueError, lambda: A(q, k, v, table, lens, out=torch.empty_like(q[:1]).expand_as(q))),
+        (ValueError, lambda: A(q, k[:, :1].expand_as(k), v, table, lens, k_new=new, v_new=new)),
+        (TypeError, lambda: A(q, k, v, table, lens, status=lens[:1].long())),
+        (ValueError, lambda: A(q, k, v, table, lens, status=lens)),
+        (ValueError, lambda: P.append_pages(new, new, k, v[:1].expand_as(v), lens.long())),
+        (ValueError, lambda: P.resize_pages(lens, lens, table[:1].expand_as(table), c.free, c.nfree,
+                                            16, 0)),
         (_lib.SSAError, lambda: A(q, k, v, table, lens, window=-1)),
         (_lib.SSAError, lambda: A(q[:, :3].contiguous(), k, v, table, lens)),
         (_lib.SSAError, lambda: A(q, k[:, :, :8], v[:, :, :8], table, lens)),

@@ -23,7 +23,7 @@ def attend(**kw):
              d=64, pages=10, page=16, table=FAKE, table_stride=8, W=8, lens=FAKE, k_new=NULL,
              v_new=NULL, strides=_lib.i64_array([256, 64, 2048, 1024, 64, 2048, 1024, 64, 256, 64,
                                                  128, 64, 128, 64]),
-             scale=0.125, window=0, ws=FAKE, ws_bytes=1 << 30)
+             scale=0.125, window=0, status=NULL, ws=FAKE, ws_bytes=1 << 30)
     a.update(kw)
     return status("ssa_paged_attend", *a.values(), None)
 
@@ -41,6 +41,13 @@ def attend(**kw):
     (dict(window=-1), _lib.SSA_ERR_INVALID), (dict(window=2 ** 31), _lib.SSA_ERR_INVALID),
     (dict(q=ctypes.c_void_p((1 << 20) + 8)), _lib.SSA_ERR_INVALID),
     (dict(strides=_lib.i64_array([256, 64, 2048, 1024, 60] + [64] * 9)), _lib.SSA_ERR_INVALID),
+    (dict(strides=_lib.i64_array([64] * 4 + [2 ** 24] + [64] * 9)), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(strides=_lib.i64_array([64] * 7 + [2 ** 24] + [64] * 6)), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(B=65536), _lib.SSA_ERR_INVALID), (dict(Hq=65536, Hkv=1), _lib.SSA_ERR_INVALID),
+    (dict(B=65535, W=2 ** 22, table_stride=2 ** 22), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(W=1000, table_stride=1000, ws_bytes=1000), _lib.SSA_ERR_WORKSPACE),
+    (dict(W=1000, table_stride=1000, ws=NULL), _lib.SSA_ERR_WORKSPACE),
+    (dict(W=1000, table_stride=1000, ws=ctypes.c_void_p((1 << 20) + 8)), _lib.SSA_ERR_WORKSPACE),
 ])
 def test_attend_refuses(change, code):
     assert attend(**change) == code
