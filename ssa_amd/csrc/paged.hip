@@ -448,60 +448,47 @@ __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
     it.end = units ? r.end : r.begin;
     return true;
   }
-  if (p.B <= 64) {  // a request per lane
-    const int len = lane < p.B ? p.lens[lane] : 0;
-    const int units = paged_units(paged_span(len, p.window, cap));
-    // 64 of at most 2^24 units fit 32 bits
-    const int all = lane_sums(units).all, n = paged_items(units, paged_chunk(all, p.items));
-    it.stream = all >= p.stream_units;
-    const int upto = lane_sums(n).upto;
-    const unsigned long long past = __ballot(upto > index);
-    if (past == 0) return false;
-    it.b = __builtin_ctzll(past);
-    it.span = paged_span(__builtin_amdgcn_readlane(len, it.b), p.window, cap);
-    it.n = __builtin_amdgcn_readlane(n, it.b);
-    it.first_item = __builtin_amdgcn_readlane(upto - n, it.b);
-    it.j = index - it.first_item;
-    const PagedRange r = paged_item_range(
-        it.span, __builtin_amdgcn_readlane(units, it.b), it.j, it.n);
-    it.begin = r.begin;
-    it.end = r.end;
-    return true;
-  }
+  // the requests in runs, a run per lane; up to 64 requests one each, whose numbers stay in registers
   const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
-  int64_t units = 0;
-  for (int b = b0; b < b1; ++b) units += paged_units(paged_span(p.lens[b], p.window, cap));
-  for (int off = 32; off >= 1; off >>= 1) units += __shfl_xor(units, off);
-  const int chunk = paged_chunk(units, p.items);
-  it.stream = units >= p.stream_units;
-  int mine = 0;
-  for (int b = b0; b < b1; ++b)
-    mine += paged_items(paged_units(paged_span(p.lens[b], p.window, cap)), chunk);
-  int upto = mine;
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(upto, off);
-    if (lane >= off) upto += y;
+  int len = 0, own = 0, units = 0, n = 0;
+  for (int b = b0; b < b1; ++b) {
+    len = p.lens[b];
+    own = paged_units(paged_span(len, p.window, cap));
+    units += own;
   }
+  const int all = lane_sums(units).all, chunk = paged_chunk(all, p.items);
+  it.stream = all >= p.stream_units;
+  if (run == 1) {
+    n = paged_items(own, chunk);
+  } else {
+    for (int b = b0; b < b1; ++b)
+      n += paged_items(paged_units(paged_span(p.lens[b], p.window, cap)), chunk);
+  }
+  const int upto = lane_sums(n).upto;
   const unsigned long long past = __ballot(upto > index);
   if (past == 0) return false;
   const int owner = __builtin_ctzll(past);
-  int at = uniform(__builtin_amdgcn_readlane(upto - mine, owner));
-  for (int b = uniform(owner * run);; ++b) {
-    const PagedSpan s = paged_span(p.lens[b], p.window, cap);
-    const int u = paged_units(s), n = paged_items(u, chunk);
-    if (index < at + n) {
-      it.b = b;
-      it.j = index - at;
-      it.n = n;
-      it.first_item = at;
-      it.span = s;
-      const PagedRange r = paged_item_range(s, u, it.j, n);
-      it.begin = r.begin;
-      it.end = r.end;
-      return true;
+  it.first_item = __builtin_amdgcn_readlane(upto - n, owner);
+  it.b = owner * run;
+  if (run == 1) {
+    len = __builtin_amdgcn_readlane(len, owner);
+    own = __builtin_amdgcn_readlane(own, owner);
+    it.n = __builtin_amdgcn_readlane(n, owner);
+  } else {
+    for (;; ++it.b) {
+      len = p.lens[it.b];
+      own = paged_units(paged_span(len, p.window, cap));
+      it.n = paged_items(own, chunk);
+      if (index < it.first_item + it.n) break;
+      it.first_item += it.n;
     }
-    at += n;
   }
+  it.span = paged_span(len, p.window, cap);
+  it.j = index - it.first_item;
+  const PagedRange r = paged_item_range(it.span, own, it.j, it.n);
+  it.begin = r.begin;
+  it.end = r.end;
+  return true;
 }
 
 __device__ inline Item uniform(const Item& x) {
@@ -768,7 +755,7 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
   }
   for (int i = i0; i < i1; ++i) {
     const int j0 = (it.begin + i * NT) * 16;
-    const bool edge = j0 < first || j0 + NT * 16 > len;
+    const bool edge = j0 < first || len - j0 < NT * 16;
     if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
     // scores: lane column a head, rows the keys 4 grp + r of each subtile
     f32x4 s[NT];
@@ -815,8 +802,9 @@ __global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams
       }
     mx = fmaxf(mx, lane_xor(mx, 16));
     mx = fmaxf(mx, lane_xor(mx, 32));
-    if (__any(mx > st.m)) {
-      const float m = fmaxf(st.m, mx), a = __builtin_amdgcn_exp2f(st.m - m);
+    if (__any(mx > st.m)) {  // a head without a finite score so far stays at -inf, its sums at 0
+      const float m = fmaxf(st.m, mx);
+      const float a = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.0f : m));
       st.m = m;
       st.l *= a;
 #pragma unroll

@@ -51,10 +51,9 @@ SSA_HD int64_t paged_most_items(int64_t B, int64_t items, int64_t most_units) {
 }
 
 // Units per item so that a call's `units` make at most `items` items besides one more per request.
-SSA_HD int paged_chunk(int64_t units, int items) {
-  if (units <= items) return 1;
-  if (units <= 0x7fffffff) return (int)(((unsigned)units + (unsigned)items - 1) / (unsigned)items);
-  return (int)((units + items - 1) / items);
+// (The units of a call are held below 2^31.)
+SSA_HD int paged_chunk(int units, int items) {
+  return units <= items ? 1 : (int)(((unsigned)units + (unsigned)items - 1) / (unsigned)items);
 }
 
 SSA_HD int paged_items(int units, int chunk) {

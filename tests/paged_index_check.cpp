@@ -32,7 +32,7 @@ int main() {
       const int edge[] = {0, 1, 15, 16, 17, (int)cap, (int)cap - 1, -1, (int)cap + 1, -0x7fffffff};
       n = upto(1) ? (int)upto(cap) : edge[upto(9)];
     }
-    int64_t units = 0;
+    int units = 0;
     for (int n : lens) units += paged_units(paged_span(n, window, cap));
     const int chunk = paged_chunk(units, items);
     CHECK(chunk >= 1);

@@ -357,6 +357,48 @@ def test_attend_infinities_and_nan(cuda, dtype, d):
         assert (lse[b].double().cpu() - torch.logsumexp(s, 1)).abs().max() < 1e-3
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 512])
+def test_attend_infinite_keys_per_head(cuda, dtype, d):
+    """Keys that score -inf for one head and +inf for another, all through the first tiles: the first
+    head's row is that of its other keys, the second's NaN."""
+    lens = [96, 3000]
+    q, cache = make(cuda, dtype, lens, 2, 1, d, 16, seed=11)
+    q = q.abs() + 1
+    q[:, 1] *= -1
+    for b, n in enumerate(lens):
+        for j in range(n - 30):
+            cache.k[0][int(cache.table[b, j // 16]), 0, j % 16, 0] = -math.inf
+    out, lse = cache.attend(0, q, return_lse=True)
+    torch.cuda.synchronize()
+    assert out[:, 1].isnan().all() and lse[:, 1].isnan().all()
+    for b, n in enumerate(lens):
+        k, v = (U.gather(x[0], cache.table[b], n)[0, n - 30:] for x in (cache.k, cache.v))
+        s = (k @ q[b, 0].double().cpu()) / math.sqrt(d)
+        assert (out[b, 0].double().cpu() - torch.softmax(s, 0) @ v).abs().max() < 2e-2
+        assert abs(float(lse[b, 0]) - float(torch.logsumexp(s, 0))) < 1e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_subnormal_values(cuda, dtype):
+    """Keys and values below the type's smallest normal number count as what they are."""
+    q, cache = make(cuda, dtype, [50, 700], 4, 2, 64, 16, seed=12)
+    tiny = torch.finfo(dtype).tiny
+    cache.v.mul_(tiny / 4)
+    cache.k.mul_(tiny / 4)
+    assert 0 < float(cache.v[cache.v > 0].min()) < tiny
+    check_attend(cache, q, scale=1.0 / tiny if dtype == torch.float16 else 1.0)
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 129])
+def test_attend_batch_sizes(cuda, B):
+    rng = random.Random(B)
+    lens = [rng.choice([0, 1, 500, rng.randrange(1, 3000)]) for _ in range(B)]
+    q, cache = make(cuda, torch.bfloat16, lens, 2, 1, 64, 16, seed=B)
+    check_attend(cache, q)
+    check_attend(cache, q, window=600)
+
+
 def test_attend_bad_lengths_and_pages_give_nan(cuda):
     """A length outside the table, a page id outside the pool: NaN for that row, nothing stored, the
     other rows as they were."""
