@@ -128,22 +128,17 @@ __device__ inline int last_at_most(It at, int n, int x) {
   return lo;
 }
 
-constexpr int kSlotsInside = 4 * kResizeThreads;  // more tokens' slots are a launch of their own
+// Slots of more tokens are a launch of their own: 3,840 tokens of 64 requests 10.7 us in this launch and
+// 11.5 in two, 15,000 of 1,000 requests 23.8 and 13.8 (each with the giving back).
+constexpr int kSlotsInside = 4 * kResizeThreads;
 
 // Calls f(request, its nth page, t) for the pages t < count of a tile of n requests whose prefix sums
-// are `at`; a thread's pages are consecutive, mostly of one request, so one search serves them.
+// are `at`.
 template <class F>
 __device__ inline void each_page(const int* at, int n, int count, F f) {
-  const int run = count > kResizeThreads ? 4 : 1;
-  for (int t0 = threadIdx.x * run; t0 < count; t0 += kResizeThreads * run) {
-    int i = 0, end = 0;
-    for (int t = t0; t < min(t0 + run, count); ++t) {
-      if (t >= end) {
-        i = last_at_most(at, n, t);
-        end = i + 1 < n ? at[i + 1] : count;
-      }
-      f(i, t - at[i], t);
-    }
+  for (int t = threadIdx.x; t < count; t += kResizeThreads) {
+    const int i = last_at_most(at, n, t);
+    f(i, t - at[i], t);
   }
 }
 
@@ -151,7 +146,8 @@ __device__ inline void each_page(const int* at, int n, int count, F f) {
 // tokens are shared out over the threads by a search in the tile's prefix sums. The free pages are a
 // stack; a page given back lands where a take of the same order would find it, so growing and
 // shrinking back restores the stack. Takes are read before gives are written (they overlap).
-// Bound by its chain of memory latencies and, past some thousand pages, by one CU's instructions.
+// Bound by its chain of memory latencies and, past some thousand pages, by one CU's instructions: 256
+// requests grown by a token 3 us, 13,000 pages taken for 64 prompts 8 to 10.
 __global__ __launch_bounds__(kResizeThreads) void paged_resize_kernel(ResizeParams p) {
   __shared__ ScanRoom<int> room;
   __shared__ ScanRoom<int64_t> room64;
@@ -334,7 +330,8 @@ struct AppendParams {
   int64_t kpp, kph, kps, vpp, vph, vps;                // bytes
 };
 
-// A thread moves one 16-byte piece of a key row and of its value row.
+// A thread moves one 16-byte piece of a key row and of its value row. Bound by memory: 65,436 tokens of
+// 2 heads of 64 (bf16, 67 MB in all) 11.8 us, 5.7 TB/s.
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per = p.Hkv * p.vecs;
@@ -611,14 +608,26 @@ __device__ inline void store_new(const AttendParams& p, int b, int g, int j) {
   wave_lds_sync();
 }
 
-// Attention over one item by NW waves. Scores are K Q^T: a product's result then has a head per lane
-// column and the keys in the very order that the second product, V^T P^T, takes its weights in, so
-// weights never move between lanes and a head's statistics belong to its lanes. Bound by the reading of K
-// and V: a wave's next keys are in flight while it weighs the current values and the other way round.
-template <int DT, int DP, int NW, int WPE>
-__global__ __launch_bounds__(NW * 64, WPE) void paged_attend_kernel(AttendParams p) {
+// With eight a unit's waves have a subtile each, half a tile: 128 requests of 2,000 to 9,000 keys, 20
+// heads on one, 97 us for 86.
+constexpr int kAttendWaves = 4;
+
+// Attention over one item by a workgroup, its tiles in four runs, one a wave. Scores are K Q^T: a
+// product's result then has a head per lane column and the keys in the very order that the second
+// product, V^T P^T, takes its weights in, so weights never move between lanes and a head's statistics
+// belong to its lanes. A lane's values are loaded a row at a time and turned into operands by
+// byte permutes: no LDS, no transposed copy. Bound by the reading of K and V: a wave's next keys are in
+// flight while it weighs the current values and the other way round; 16 lanes of 16 heads serve
+// any group of query heads, as the matrix units wait for memory anyway. 1,048,577 tokens (bf16, 14 / 2
+// heads of 64) 90 us with the join, 5.9 TB/s; a kernel that only reads as much takes 97 without the
+// non-temporal hint. Two tiles of heads per wave for more than 16 heads a key head (K and V read once) were
+// slower in five of eight cases (fewer, longer workgroups); equal shares that run on over several
+// requests cost every short call 1 us or more for 2 % of a mixed batch.
+template <int DT, int DP, int WPE>
+__global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(AttendParams p) {
   using T = Tile<DT, DP>;
   constexpr int NT = T::NT, NC = T::NC, VB = T::VB, LC = T::LC, LW = T::LW, NA = T::NA;
+  constexpr int NW = kAttendWaves;
   __shared__ f32x4 red[NW / 2][NA][64];
   __shared__ float red_m[NW / 2][64], red_l[NW / 2][64];
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
@@ -924,7 +933,8 @@ constexpr int kJoinBatch = 8;
 
 // Joins a row's parts: a workgroup per (request, query head), DP / 4 threads across a part's row and
 // the parts shared out over the workgroup's splits, kJoinBatch of them on their way at a time. Rows
-// without keys, and of lengths that do not fit, are answered here.
+// without keys, and of lengths that do not fit, are answered here. Bound by its chain of three memory
+// latencies: 3.5 us for 14 rows of 33 parts, 6 for 2,048 rows of 1 to 12.
 template <int DT, int DP, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(AttendParams p) {
   constexpr int PER = DP / 4, NS = THREADS / PER, WAVES = THREADS / 64;
@@ -1021,10 +1031,17 @@ int check_pool(const char* who, int dtype, int64_t Hkv, int64_t d, int64_t pages
 }
 
 // How a call of these sizes is cut: known on the host without the lengths.
+//   one launch, a request an item, where no request can pass 512 keys (8 us a call; parts and their
+//   join 11) or 2048 in 512 or more (request, key head, row tile) triples (256 x 1,000 keys, 4 key
+//   heads: 48 us; cut 60). With few triples and more keys the cut wins: 2,000 keys of 8 heads 12 and 24.
+//   otherwise items for about `target` workgroups, what the CUs hold at once (four a CU at head dim 64,
+//   two at 256, one at 512; three at 128, and there twice as many even out uneven lengths better: 64
+//   mixed requests 267 us for 1536, 286 for 768). A single request is even by itself and has the most
+//   parts to join: 512 (1M tokens 102 us, 106 for 1024).
 struct Layout {
   int64_t RT, items, max_items;  // items: 0 when every request is one item
   int dp;
-  size_t part, part_ml, info, bytes;  // offsets into the workspace
+  size_t part_ml, info, bytes;  // offsets into the workspace, which starts with the parts
 };
 
 Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
@@ -1033,10 +1050,14 @@ Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t 
   y.RT = (Hq / Hkv + 15) / 16;
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
   const int64_t units = paged_most_units(W * page, (int)window);
-  const int64_t target = y.dp == 64 ? (B == 1 ? 512 : 1024) : y.dp == 128 ? (B == 1 ? 512 : 1536) : y.dp == 256 ? 512 : 256;
-  y.items = units <= 4 || (units <= 16 && B * Hkv * y.RT >= 512) ? 0 : std::max<int64_t>(1, target / (Hkv * y.RT));
-  y.max_items = y.items == 0 ? B : paged_most_items(B, y.items, units);
-  if (y.items == 0) return y;
+  y.max_items = B;
+  if (units <= 4 || (units <= 16 && B * Hkv * y.RT >= 512)) return y;
+  const int64_t target = y.dp == 512             ? 256
+                         : y.dp == 256 || B == 1 ? 512
+                         : y.dp == 128           ? 1536
+                                                 : 1024;
+  y.items = std::max<int64_t>(1, target / (Hkv * y.RT));
+  y.max_items = paged_most_items(B, y.items, units);
   const size_t parts = (size_t)y.max_items * Hq;
   y.part_ml = parts * y.dp * 4;
   y.info = y.part_ml + parts * 2 * 4;
@@ -1046,17 +1067,13 @@ Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t 
 
 template <int DT, int DP, int WPE>
 int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
-  constexpr int NW = 4, MANY = DP <= 64 && DT != SSA_F32 ? 16 : DP <= 256 ? 8 : 4;
-  if (p.items == 0 && blocks < 512) {
-    paged_attend_kernel<DT, DP, MANY, 1><<<(unsigned)blocks, MANY * 64, 0, st>>>(p);
-    return launch_status("paged_attend_kernel");
-  }
-  paged_attend_kernel<DT, DP, NW, WPE><<<(unsigned)blocks, NW * 64, 0, st>>>(p);
+  paged_attend_kernel<DT, DP, WPE><<<(unsigned)blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_attend_kernel"));
   if (p.items == 0) return SSA_OK;
-  const dim3 grid(p.Hq, p.B);
-  if ((int64_t)p.Hq * p.B < 64) paged_join_kernel<DT, DP, 1024><<<grid, 1024, 0, st>>>(p);
-  else paged_join_kernel<DT, DP, 256><<<grid, 256, 0, st>>>(p);
+  // 16 to 4 splits of a row's parts; 1024 threads take 10 us more for 4,096 rows of a few parts, and
+  // 256 at head dim 512 (2 splits) 1.6 us more for 128 rows
+  constexpr int JOIN = DP <= 128 ? 256 : 512;
+  paged_join_kernel<DT, DP, JOIN><<<dim3(p.Hq, p.B), JOIN, 0, st>>>(p);
   return launch_status("paged_join_kernel");
 }
 
@@ -1203,8 +1220,9 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   p.div = page_div((int)page / 16);
   p.RT = (int)y.RT;
   p.items = (int)y.items;
-  // What does not fit the 256 MB last-level cache is read past it, unless row tiles read it twice: 537
-  // MB 91 us with the hint, 101 without; 105 MB that the cache holds 30 and 27.
+  // What does not fit the 256 MB last-level cache is read past it: 537 MB 91 us with the hint, 101
+  // without; 105 MB that the cache holds 30 and 27. Row tiles read it twice, the second time from L2:
+  // 300 MB with two of them 110 us with the hint, 83 without.
   const int64_t unit_bytes = 2 * 16 * kPagedUnit * d * es * Hkv;
   p.stream_units = y.RT > 1 ? INT64_MAX : kStreamBytes / unit_bytes;
   if (y.items == 0 && B * paged_most_units(W * page, (int)window) >= p.stream_units)
