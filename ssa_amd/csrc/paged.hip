@@ -620,18 +620,16 @@ constexpr int kAttendWaves = 4;
 // flight while it weighs the current values and the other way round; 16 lanes of 16 heads serve
 // any group of query heads, as the matrix units wait for memory anyway. 1,048,577 tokens (bf16, 14 / 2
 // heads of 64) 90 us with the join, 5.9 TB/s; a kernel that only reads as much takes 97 without the
-// non-temporal hint. Two tiles of heads per wave for more than 16 heads a key head (K and V read once) were
-// slower in five of eight cases (fewer, longer workgroups); equal shares that run on over several
-// requests cost every short call 1 us or more for 2 % of a mixed batch.
-template <int DT, int DP, int WPE>
+// non-temporal hint. Equal shares that run on over several requests cost every short call 1 us or more
+// for 2 % of a mixed batch. MT: tiles of 16 query heads served by one reading.
+template <int DT, int DP, int MT, int WPE>
 __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(AttendParams p) {
   using T = Tile<DT, DP>;
   constexpr int NT = T::NT, NC = T::NC, VB = T::VB, LC = T::LC, LW = T::LW, NA = T::NA;
   constexpr int NW = kAttendWaves;
-  __shared__ f32x4 red[NW / 2][NA][64];
-  __shared__ float red_m[NW / 2][64], red_l[NW / 2][64];
-  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
-  const int col = lane & 15, grp = lane >> 4;
+  __shared__ f32x4 red[NW / 2][MT][NA][64];
+  __shared__ float red_m[NW / 2][MT][64], red_l[NW / 2][MT][64];
+  const int wv = uniform(threadIdx.x >> 6);
   // row tiles of one (item, key head) are 8 workgroups apart: on one XCD, whose L2 they share
   const int id = blockIdx.x, rt = (id >> 3) % p.RT, unit = (id >> 3) / p.RT * 8 + (id & 7);
   const int g = unit % p.Hkv;
@@ -639,32 +637,41 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
   if (unit >= p.units || !find_item(p, unit / p.Hkv, found)) return;
   const Item it = uniform(found);
   const int first = it.span.first, len = it.span.len;
-  const int head = rt * 16 + col;
-  const bool live = head < p.G;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int head0 = rt * MT * 16 + col;  // of MT tiles of 16 heads
   const int tiles = (it.end - it.begin + NT - 1) / NT;
   const int i0 = uniform((int)((int64_t)tiles * wv / NW));
   const int i1 = uniform((int)((int64_t)tiles * (wv + 1) / NW));
 
-  __shared__ u32x4 q_lds[T::kQInLds ? NC : 1][64];
-  u32x4 q[T::kQInLds ? 1 : NC];
+  __shared__ u32x4 q_lds[T::kQInLds ? MT : 1][T::kQInLds ? NC : 1][64];
+  u32x4 q[MT][T::kQInLds ? 1 : NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (T::kQInLds && c % NW != wv) continue;
-    const int at = c * 64 + grp * 16;
-    u32x4 x = {0, 0, 0, 0};
-    if (live && at < p.d * T::ES)
-      x = *(const u32x4*)(p.q + (it.b * p.qb + (int64_t)(g * p.G + head) * p.qh) * T::ES + at);
-    if constexpr (T::kQInLds) q_lds[c][lane] = x;
-    else q[c] = x;
-  }
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (T::kQInLds && c % NW != wv) continue;
+      const int at = c * 64 + grp * 16, head = head0 + mt * 16;
+      u32x4 x = {0, 0, 0, 0};
+      if (head < p.G && at < p.d * T::ES)
+        x = *(const u32x4*)(p.q + (it.b * p.qb + (int64_t)(g * p.G + head) * p.qh) * T::ES + at);
+      if constexpr (T::kQInLds) q_lds[mt][c][lane] = x;
+      else q[mt][c] = x;
+    }
   if constexpr (T::kQInLds) __syncthreads();
 
   const char* const kbase = p.kpool + g * p.kph * T::ES;
   const char* const vbase = p.vpool + g * p.vph * T::ES;
   const int64_t kpp = p.kpp * T::ES, vpp = p.vpp * T::ES;
   const int kps = (int)p.kps * T::ES, vps = (int)p.vps * T::ES, row_bytes = p.d * T::ES;
-  const int32_t* const row = p.table + it.b * p.table_stride;
 
+  const int koff = col * kps + grp * 16;
+  int vcol[VB];
+#pragma unroll
+  for (int vb = 0; vb < VB; ++vb) {
+    const int c = vb * T::CB * T::ES + col * LW * 4;
+    vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
+  }
+  const int32_t* const row = p.table + it.b * p.table_stride;
   // page and offset of 64 subtiles at a time, one per lane; the next 64 are on their way
   int pid = 0, poff = 0, pid_next = 0, batch = it.begin + i0 * NT;
   unsigned long long bad = 0;
@@ -686,11 +693,14 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
   }
 
   Rows<DT, DP> rows;
-  Softmax<NA> st;
-  st.m = -INFINITY;
-  st.l = 0.0f;
+  Softmax<NA> st[MT];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) st.acc[i] = f32x4{0, 0, 0, 0};
+  for (int mt = 0; mt < MT; ++mt) {
+    st[mt].m = -INFINITY;
+    st[mt].l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) st[mt].acc[i] = f32x4{0, 0, 0, 0};
+  }
 
   // pages of tile i's subtiles (the last one again past the wave's end)
   int64_t pg[NT];
@@ -709,13 +719,6 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
       off[t] = __builtin_amdgcn_readlane(poff, x);
     }
   };
-  const int koff = col * kps + grp * 16;
-  int vcol[VB];
-#pragma unroll
-  for (int vb = 0; vb < VB; ++vb) {
-    const int c = vb * T::CB * T::ES + col * LW * 4;
-    vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
-  }
   auto load_k_as = [&](auto aux, int piece) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -767,27 +770,33 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
     const bool edge = j0 < first || len - j0 < NT * 16;
     if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
     // scores: lane column a head, rows the keys 4 grp + r of each subtile
-    f32x4 s[NT];
+    f32x4 s[MT][NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s[t] = f32x4{0, 0, 0, 0};
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[mt][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       constexpr int per = NC / T::KP;
       if (c > 0 && c % per == 0) load_k(c / per);
-      u32x4 qc;
-      if constexpr (T::kQInLds) qc = q_lds[c][lane];
-      else qc = q[c];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (DT == SSA_F32) {
+      for (int mt = 0; mt < MT; ++mt) {
+        u32x4 qc;
+        if constexpr (T::kQInLds) qc = q_lds[mt][c][lane];
+        else qc = q[mt][c];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned int a = rows.k[t][c % per][e], b = qc[e];
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b),
-                                                        s[t], 0, 0, 0);
+        for (int t = 0; t < NT; ++t) {
+          f32x4& x = s[mt][t];
+          if constexpr (DT == SSA_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned int a = rows.k[t][c % per][e], b = qc[e];
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), x,
+                                                       0, 0, 0);
+            }
+          } else {
+            x = mfma16(rows.k[t][c % per], qc, x, DT == SSA_BF16);
           }
-        } else {
-          s[t] = mfma16(rows.k[t][c % per], qc, s[t], DT == SSA_BF16);
         }
       }
     }
@@ -796,67 +805,73 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
       locate(i + 1);
       load_k(0);
     }
-    float mx = -INFINITY;
+    u32x4 hi[MT], lo[MT];  // the weights in 16-bit parts
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = s[t][r] * p.scale_log2;
-        if (edge) {
-          const int j = j0 + t * 16 + grp * 4 + r;
-          if (j < first || j >= len) x = -INFINITY;
-        }
-        s[t][r] = x;
-        mx = fmaxf(mx, x);
-      }
-    mx = fmaxf(mx, lane_xor(mx, 16));
-    mx = fmaxf(mx, lane_xor(mx, 32));
-    if (__any(mx > st.m)) {  // a head without a finite score so far stays at -inf, its sums at 0
-      const float m = fmaxf(st.m, mx);
-      const float a = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.0f : m));
-      st.m = m;
-      st.l *= a;
-#pragma unroll
-      for (int n = 0; n < NA; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st.acc[n][r] *= a;
-    }
-    const float base = (st.m == -INFINITY ? 0.0f : st.m) - T::kShift;
-    float sum = 0.0f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
-        sum += s[t][r];
-      }
-    st.l += sum;
-    if constexpr (DT == SSA_F32) {
+    for (int mt = 0; mt < MT; ++mt) {
+      Softmax<NA>& o = st[mt];
+      float mx = -INFINITY;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int vb = 0; vb < VB; ++vb)
-#pragma unroll
-            for (int e = 0; e < LC; ++e)
-              st.acc[vb * LC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  __uint_as_float(rows.v[t][r][vb].w[e]), s[t][r], st.acc[vb * LC + e], 0, 0, 0);
-    } else {
-      u32x4 hi, lo;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          unsigned int a, b;
-          split2<DT>(s[t][2 * h], s[t][2 * h + 1], a, b);
-          hi[2 * t + h] = a;
-          lo[2 * t + h] = b;
+        for (int r = 0; r < 4; ++r) {
+          float x = s[mt][t][r] * p.scale_log2;
+          if (edge) {
+            const int j = j0 + t * 16 + grp * 4 + r;
+            if (j < first || j >= len) x = -INFINITY;
+          }
+          s[mt][t][r] = x;
+          mx = fmaxf(mx, x);
         }
+      mx = fmaxf(mx, lane_xor(mx, 16));
+      mx = fmaxf(mx, lane_xor(mx, 32));
+      if (__any(mx > o.m)) {  // a head without a finite score so far stays at -inf, its sums at 0
+        const float m = fmaxf(o.m, mx);
+        const float a = __builtin_amdgcn_exp2f(o.m - (m == -INFINITY ? 0.0f : m));
+        o.m = m;
+        o.l *= a;
 #pragma unroll
-      for (int vb = 0; vb < VB; ++vb)
+        for (int n = 0; n < NA; ++n)
 #pragma unroll
-        for (int e = 0; e < LC; ++e) {
+          for (int r = 0; r < 4; ++r) o.acc[n][r] *= a;
+      }
+      const float base = (o.m == -INFINITY ? 0.0f : o.m) - T::kShift;
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[mt][t][r] = __builtin_amdgcn_exp2f(s[mt][t][r] - base);
+          sum += s[mt][t][r];
+        }
+      o.l += sum;
+      if constexpr (DT != SSA_F32) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned int a, b;
+            split2<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], a, b);
+            hi[mt][2 * t + h] = a;
+            lo[mt][2 * t + h] = b;
+          }
+      }
+    }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int e = 0; e < LC; ++e) {
+        if constexpr (DT == SSA_F32) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                f32x4& acc = st[mt].acc[vb * LC + e];
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    __uint_as_float(rows.v[t][r][vb].w[e]), s[mt][t][r], acc, 0, 0, 0);
+              }
+        } else {
           // column e of the lane's values, key after key
           u32x4 vt;
 #pragma unroll
@@ -866,28 +881,41 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
               vt[2 * t + h] = __builtin_amdgcn_perm(
                   rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
                   e % 2 ? 0x07060302u : 0x05040100u);
-          f32x4& acc = st.acc[vb * LC + e];
-          acc = mfma16(vt, hi, acc, DT == SSA_BF16);
-          acc = mfma16(vt, lo, acc, DT == SSA_BF16);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            f32x4& acc = st[mt].acc[vb * LC + e];
+            acc = mfma16(vt, hi[mt], acc, DT == SSA_BF16);
+            acc = mfma16(vt, lo[mt], acc, DT == SSA_BF16);
+          }
         }
-    }
+      }
     if (more) load_v(i + 1);
   }
-  st.l += lane_xor(st.l, 16);
-  st.l += lane_xor(st.l, 32);
-  if (bad != 0 || !it.span.ok) st.l = NAN;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    st[mt].l += lane_xor(st[mt].l, 16);
+    st[mt].l += lane_xor(st[mt].l, 32);
+    if (bad != 0 || !it.span.ok) st[mt].l = NAN;
+  }
 
   // the waves' results, half of them into the other half at a time
 #pragma unroll
   for (int half = NW / 2; half >= 1; half >>= 1) {
     if (wv >= half && wv < 2 * half) {
-      red_m[wv - half][lane] = st.m;
-      red_l[wv - half][lane] = st.l;
 #pragma unroll
-      for (int n = 0; n < NA; ++n) red[wv - half][n][lane] = st.acc[n];
+      for (int mt = 0; mt < MT; ++mt) {
+        red_m[wv - half][mt][lane] = st[mt].m;
+        red_l[wv - half][mt][lane] = st[mt].l;
+#pragma unroll
+        for (int n = 0; n < NA; ++n) red[wv - half][mt][n][lane] = st[mt].acc[n];
+      }
     }
     __syncthreads();
-    if (wv < half) join(st, red_m[wv][lane], red_l[wv][lane], &red[wv][0][lane], 64);
+    if (wv < half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        join(st[mt], red_m[wv][mt][lane], red_l[wv][mt][lane], &red[wv][mt][0][lane], 64);
+    }
     __syncthreads();
   }
   if (wv != 0) return;
@@ -896,36 +924,40 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
     p.info[2 * it.b] = it.first_item;
     p.info[2 * it.b + 1] = it.n;
   }
-  if (!live) return;
-  const int h = g * p.G + head;
-  const float inv = len == 0 && it.span.ok ? 0.0f : 1.0f / st.l;
-  const int64_t part = (int64_t)(unit / p.Hkv) * p.Hq + h, to = it.b * p.ob + h * p.oh;
 #pragma unroll
-  for (int vb = 0; vb < VB; ++vb)
+  for (int mt = 0; mt < MT; ++mt) {
+    const Softmax<NA>& o = st[mt];
+    const int h = g * p.G + head0 + mt * 16;
+    if (head0 + mt * 16 >= p.G) break;
+    const float inv = len == 0 && it.span.ok ? 0.0f : 1.0f / o.l;
+    const int64_t part = (int64_t)(unit / p.Hkv) * p.Hq + h, to = it.b * p.ob + h * p.oh;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-      for (int e = 0; e < LC; e += 4) {
-        const int c = vb * T::CB + LC * (grp * 4 + r) + e;
-        if (c >= p.d) continue;
-        f32x4 x;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = st.acc[vb * LC + e + i][r];
-        if (it.n > 1) {
-          *(f32x4*)(p.part + part * DP + c) = x;
-        } else {
+        for (int e = 0; e < LC; e += 4) {
+          const int c = vb * T::CB + LC * (grp * 4 + r) + e;
+          if (c >= p.d) continue;
+          f32x4 x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] *= inv;
-          store_row4<DT>(p.out, to + c, x);
+          for (int i = 0; i < 4; ++i) x[i] = o.acc[vb * LC + e + i][r];
+          if (it.n > 1) {
+            *(f32x4*)(p.part + part * DP + c) = x;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] *= inv;
+            store_row4<DT>(p.out, to + c, x);
+          }
         }
-      }
-  if (grp != 0) return;
-  if (it.n > 1) {
-    p.part_ml[part * 2] = st.m;
-    p.part_ml[part * 2 + 1] = st.l;
-  } else if (p.lse) {
-    p.lse[(int64_t)it.b * p.Hq + h] = len == 0 && it.span.ok ? -INFINITY
-        : (st.m - T::kShift + __builtin_amdgcn_logf(st.l)) * kLn2;
+    if (grp != 0) continue;
+    if (it.n > 1) {
+      p.part_ml[part * 2] = o.m;
+      p.part_ml[part * 2 + 1] = o.l;
+    } else if (p.lse) {
+      p.lse[(int64_t)it.b * p.Hq + h] = len == 0 && it.span.ok ? -INFINITY
+          : (o.m - T::kShift + __builtin_amdgcn_logf(o.l)) * kLn2;
+    }
   }
 }
 
@@ -1030,6 +1062,20 @@ int check_pool(const char* who, int dtype, int64_t Hkv, int64_t d, int64_t pages
   return SSA_OK;
 }
 
+// Whether a wave serves two tiles of 16 query heads from one reading of the keys and values (past head
+// dim 128 their registers do not fit). It makes fewer, longer workgroups: 16-bit calls that may read
+// more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 76 us for 83;
+// 64 of 2,000 to 20,000, 48 on two: 122 for 137), smaller ones lose (64 of 500 to 4,000, 32 on one: 23
+// for 19); in fp32 the matrix products count as well (8 of 2,000 to 9,000, 40 on two: 26 for 31).
+bool may_serve_two(int64_t G, int64_t d) { return G > 16 && d <= 128; }
+
+bool serve_two(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
+               int64_t window) {
+  const int64_t keys = B * paged_most_units(W * page, (int)window) * 16 * kPagedUnit;
+  return may_serve_two(Hq / Hkv, d) &&
+         (dtype == SSA_F32 || keys >= kStreamBytes / (2 * dtype_size(dtype) * d * Hkv));
+}
+
 // How a call of these sizes is cut: known on the host without the lengths.
 //   one launch, a request an item, where no request can pass 512 keys (8 us a call; parts and their
 //   join 11) or 2048 in 512 or more (request, key head, row tile) triples (256 x 1,000 keys, 4 key
@@ -1045,16 +1091,16 @@ struct Layout {
 };
 
 Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
-              int64_t window) {
+              int64_t window, bool two) {
   Layout y{};
-  y.RT = (Hq / Hkv + 15) / 16;
+  y.RT = (Hq / Hkv + (two ? 31 : 15)) / (two ? 32 : 16);
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
   const int64_t units = paged_most_units(W * page, (int)window);
   y.max_items = B;
   if (units <= 4 || (units <= 16 && B * Hkv * y.RT >= 512)) return y;
   const int64_t target = y.dp == 512             ? 256
                          : y.dp == 256 || B == 1 ? 512
-                         : y.dp == 128           ? 1536
+                         : y.dp == 128           ? (two ? 1024 : 1536)
                                                  : 1024;
   y.items = std::max<int64_t>(1, target / (Hkv * y.RT));
   y.max_items = paged_most_items(B, y.items, units);
@@ -1065,9 +1111,9 @@ Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t 
   return y;
 }
 
-template <int DT, int DP, int WPE>
+template <int DT, int DP, int MT, int WPE>
 int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
-  paged_attend_kernel<DT, DP, WPE><<<(unsigned)blocks, kAttendWaves * 64, 0, st>>>(p);
+  paged_attend_kernel<DT, DP, MT, WPE><<<(unsigned)blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_attend_kernel"));
   if (p.items == 0) return SSA_OK;
   // 16 to 4 splits of a row's parts; 1024 threads take 10 us more for 4,096 rows of a few parts, and
@@ -1078,12 +1124,16 @@ int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
 }
 
 template <int DT>
-int run_attend_dim(const AttendParams& p, int dp, int64_t blocks, hipStream_t st) {
+int run_attend_dim(const AttendParams& p, int dp, bool two, int64_t blocks, hipStream_t st) {
   switch (dp) {
-    case 64: return run_attend<DT, 64, DT == SSA_F32 ? 3 : 4>(p, blocks, st);
-    case 128: return run_attend<DT, 128, 3>(p, blocks, st);
-    case 256: return run_attend<DT, 256, 2>(p, blocks, st);
-    default: return run_attend<DT, 512, 1>(p, blocks, st);
+    case 64:
+      if (two) return run_attend<DT, 64, 2, DT == SSA_F32 ? 2 : 3>(p, blocks, st);
+      return run_attend<DT, 64, 1, DT == SSA_F32 ? 3 : 4>(p, blocks, st);
+    case 128:
+      if (two) return run_attend<DT, 128, 2, 2>(p, blocks, st);
+      return run_attend<DT, 128, 1, 3>(p, blocks, st);
+    case 256: return run_attend<DT, 256, 1, 2>(p, blocks, st);
+    default: return run_attend<DT, 512, 1, 1>(p, blocks, st);
   }
 }
 
@@ -1152,7 +1202,9 @@ extern "C" size_t ssa_paged_attend_workspace_size(int64_t B, int64_t Hq, int64_t
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 || W <= 0 || page <= 0 ||
       !fits_int(window) || W > 0x7fffffff / page)
     return 0;
-  return layout(B, Hq, Hkv, d, W, page, window).bytes;
+  const size_t one = layout(B, Hq, Hkv, d, W, page, window, false).bytes;
+  return may_serve_two(Hq / Hkv, d)
+             ? std::max(one, layout(B, Hq, Hkv, d, W, page, window, true).bytes) : one;
 }
 
 extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* lse,
@@ -1188,7 +1240,8 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   SSA_REQUIRE(B * paged_most_units(W * page, (int)window) <= 0x7fffffff, SSA_ERR_UNSUPPORTED,
               "ssa_paged_attend: %lld table rows of %lld tokens (2^38 in all at most)",
               (long long)B, (long long)(W * page));
-  const Layout y = layout(B, Hq, Hkv, d, W, page, window);
+  const bool two = serve_two(dtype, B, Hq, Hkv, d, W, page, window);
+  const Layout y = layout(B, Hq, Hkv, d, W, page, window, two);
   SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
               SSA_ERR_WORKSPACE, "ssa_paged_attend: needs a 16-byte aligned workspace of %zu bytes, "
               "got %zu", y.bytes, workspace_bytes);
@@ -1234,7 +1287,7 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_attend: too many rows in one call");
   p.units = (int)units;
   hipStream_t hs = (hipStream_t)stream;
-  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, blocks, hs);
-  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, blocks, hs);
-  return run_attend_dim<SSA_BF16>(p, y.dp, blocks, hs);
+  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, two, blocks, hs);
+  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, two, blocks, hs);
+  return run_attend_dim<SSA_BF16>(p, y.dp, two, blocks, hs);
 }

@@ -271,6 +271,30 @@ def test_attend_long_and_uneven(cuda, dtype, lens, hq, hkv, d, page):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(17, 1, 64), (32, 1, 128), (66, 2, 128), (100, 2, 72)])
+def test_attend_many_heads_on_one_key_head(cuda, dtype, hq, hkv, d):
+    """More than 16 query heads a key head, with room for more keys than the caches hold (a wide table)
+    and without: the two ways to serve them."""
+    lens = [1, 33, 0, 2500, 700, 128]
+    page = 256
+    q, cache = make(cuda, dtype, lens, hq, hkv, d, page, seed=hq)
+    narrow = cache.table
+    wide = torch.full((6, (1 << 28) // (6 * page * d * hkv)), -1, device=cuda, dtype=torch.int32)
+    wide[:, :narrow.shape[1]] = narrow
+    for table in (narrow, wide):
+        cache.table = table
+        for window in (0, 100):
+            print(dtype, hq, hkv, d, table.shape[1], window, flush=True)
+            check_attend(cache, q, window=window)
+    x = torch.randn(6, 2 * hkv * d, device=cuda).to(dtype)
+    k_new, v_new = (x[:, i * hkv * d:(i + 1) * hkv * d].view(6, hkv, d) for i in (0, 1))
+    out = cache.step(0, q, k_new, v_new)
+    want, _, tol, _ = U.attend(q, cache.k[0], cache.v[0], narrow, cache.lens, 1 / math.sqrt(d))
+    U.close(out, want, tol)
+    assert torch.equal(cache.k[0, int(narrow[3, 9]), :, 2499 % page], k_new[3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_many_requests(cuda, dtype):
     rng = random.Random(2)
     lens = [rng.choice([0, 1, rng.randrange(1, 60), rng.randrange(1, 400)]) for _ in range(700)]
