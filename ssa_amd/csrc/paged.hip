@@ -128,8 +128,8 @@ __device__ inline int last_at_most(It at, int n, int x) {
   return lo;
 }
 
-// Slots of more tokens are a launch of their own: 3,840 tokens of 64 requests 10.7 us in this launch and
-// 11.5 in two, 15,000 of 1,000 requests 23.8 and 13.8 (each with the giving back).
+// Slots of more tokens are a launch of their own: 3,840 tokens of 64 requests 10.7 us in this launch
+// and 11.5 in two, 15,000 of 1,000 requests 23.8 and 13.8 (each with the giving back).
 constexpr int kSlotsInside = 4 * kResizeThreads;
 
 // Calls f(request, its nth page, t) for the pages t < count of a tile of n requests whose prefix sums
@@ -1064,9 +1064,9 @@ int check_pool(const char* who, int dtype, int64_t Hkv, int64_t d, int64_t pages
 
 // Whether a wave serves two tiles of 16 query heads from one reading of the keys and values (past head
 // dim 128 their registers do not fit). It makes fewer, longer workgroups: 16-bit calls that may read
-// more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 76 us for 83;
-// 64 of 2,000 to 20,000, 48 on two: 122 for 137), smaller ones lose (64 of 500 to 4,000, 32 on one: 23
-// for 19); in fp32 the matrix products count as well (8 of 2,000 to 9,000, 40 on two: 26 for 31).
+// more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 76 us
+// for 83; 64 of 2,000 to 20,000, 48 on two: 122 for 137), smaller ones lose (64 of 500 to 4,000, 32 on
+// one: 23 for 19); in fp32 the matrix products count too (8 of 2,000 to 9,000, 40 on two: 26 for 31).
 bool may_serve_two(int64_t G, int64_t d) { return G > 16 && d <= 128; }
 
 bool serve_two(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,

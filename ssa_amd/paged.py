@@ -94,6 +94,8 @@ def _pools(k, v):
         raise TypeError("kpool and vpool must share a dtype")
     if kstride[3] != 1 or vstride[3] != 1:
         raise ValueError("the head dimension must be contiguous")
+    if kshape[3] % 8 or kshape[3] > 512:
+        raise ValueError(f"head dim {kshape[3]}: a multiple of 8 up to 512 is wanted")
     return kshape
 
 
@@ -196,9 +198,14 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
     Resized; `out` takes an earlier one of the same sizes to write into. All or nothing: if the
     growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
     slots are -1 and status says why."""
-    if out is None and torch.compiler.is_compiling():
+    if torch.compiler.is_compiling():
         from . import torch_ops as T
-        return Resized(*T.paged_resize(lens, new_lens, table, free, nfree, int(page), int(tokens)))
+        r = T.paged_resize(lens, new_lens, table, free, nfree, int(page), int(tokens))
+        if out is not None:
+            for to, x in zip(out, r):
+                to.copy_(x)
+            return out
+        return Resized(*r)
     _one_device(lens, new_lens, table, free, nfree)
     tokens = int(tokens)
     if tokens < 0:
@@ -267,8 +274,8 @@ def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tabl
     call and attended with the rest (the page that holds that position must be the request's own;
     earlier pages may be shared between requests). status (1,) int32: a resize's; if that resize was
     refused, nothing is stored (lens[b] - 1 is then an older token's position) and every row is NaN.
-    return_lse: also the natural log of each row's
-    sum of exponentials (B, Hq) fp32, with which partial results can be joined."""
+    return_lse: also the natural log of each row's sum of exponentials (B, Hq) fp32, with which
+    partial results can be joined. Under torch.compile `out` costs a copy."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if torch.compiler.is_compiling():

@@ -13,7 +13,8 @@ using namespace ssa;
 #define CHECK(x)                                                                            \
   do {                                                                                      \
     if (!(x)) {                                                                             \
-      std::printf("%s: batch %d, B=%d cap=%lld window=%d items=%d\n", #x, batch, B, (long long)cap, window, items);                                \
+      std::printf("%s: batch %d, B=%d cap=%lld window=%d items=%d\n", #x, batch, B,       \
+                  (long long)cap, window, items);                                           \
       return 1;                                                                             \
     }                                                                                       \
   } while (0)

@@ -684,9 +684,17 @@ def test_compiled_step_equals_eager(cuda):
 
     slots = torch.tensor([int(a.table[0, 0]) * 16 + 3, -1], device=cuda)
     args = [dict(k=c.k[0], v=c.v[0], table=c.table, lens=c.lens, slots=slots) for c in (a, b)]
+    def resize(c, new):
+        return P.resize_pages(c["lens"], new, c["table"], c["free"], c["nfree"], 16, 3)
+
     want = f(args[0], q, x)
     got = torch.compile(f, backend="aot_eager")(args[1], q, x)
     assert torch.equal(got, want) and torch.equal(a.k.view(torch.int16), b.k.view(torch.int16))
+    state = [dict(lens=c.lens, table=c.table, free=c.free, nfree=c.nfree.fill_(0)) for c in (a, b)]
+    r = resize(state[0], int32([99, 35], cuda))
+    rc = torch.compile(resize, backend="aot_eager")(state[1], int32([99, 35], cuda))
+    assert r.status.item() == 0 and all(torch.equal(x, y) for x, y in zip(r, rc))
+    assert all(torch.equal(state[0][x], state[1][x]) for x in state[0])
 
 
 # ---- refusals -----------------------------------------------------------------------------------
@@ -735,5 +743,11 @@ def test_arguments_are_refused(cuda):
         with pytest.raises(error):
             call()
             pytest.fail(f"case {i} was not refused")
+    odd = torch.zeros(2, 4, 60, device=cuda, dtype=torch.bfloat16)  # rows that no copy can align
+    pool = torch.zeros(3, 2, 16, 60, device=cuda, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="head dim 60"):
+        A(odd, pool, pool, table, lens)
+    with pytest.raises(ValueError, match="head dim 60"):
+        P.append_pages(odd[:, :2], odd[:, :2], pool, pool, lens.long())
     assert A(q[:0], k, v, table[:0], lens[:0]).shape == (0, 4, 64)
     P.append_pages(new[:0], new[:0], k, v, lens[:0].long())

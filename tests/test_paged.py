@@ -165,7 +165,7 @@ def test_items_cover_every_key_once(tmp_path):
     if cxx is None:
         pytest.skip("no host compiler")
     exe = tmp_path / "check"
-    subprocess.run([cxx, "-std=c++17", "-O1", f"-I{root / 'ssa_amd' / 'csrc'}", str(root / "tests/paged_index_check.cpp"),
-                    "-o", str(exe)], check=True)
+    subprocess.run([cxx, "-std=c++17", "-O1", f"-I{root / 'ssa_amd' / 'csrc'}",
+                    str(root / "tests/paged_index_check.cpp"), "-o", str(exe)], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
     assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
