@@ -485,6 +485,79 @@ def test_attend_layouts_and_shared_pages(cuda):
     U.close(cache.attend(0, q2.transpose(0, 1).contiguous().transpose(0, 1)), want, tol)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (2, 1, 128), (20, 1, 128), (2, 1, 256)])
+def test_attend_more_than_the_caches_hold(cuda, dtype, hq, hkv, d):
+    """Calls that read past the last-level cache load with another hint: the requests share their pages,
+    so that the pool is small."""
+    n = 12000
+    row = 2 * n * hkv * d * (4 if dtype == torch.float32 else 2)
+    B = (200 << 20) // row + 1
+    q, cache = make(cuda, dtype, [n], hq, hkv, d, 16, seed=d, spread=2.0)
+    q = torch.cat([q * (1 + b % 3) * 0.5 for b in range(B)]).to(dtype)
+    cache.table = cache.table.expand(B, -1).contiguous()
+    cache.lens = int32([n - b % 40 for b in range(B)], cuda)
+    print(dtype, hq, hkv, d, B, flush=True)
+    pick = list(range(0, B, max(1, B // 6)))
+    for window in (0, n - 100):
+        out, lse = cache.attend(0, q, window=window, return_lse=True)
+        torch.cuda.synchronize()
+        want, wlse, tol, ltol = U.attend(q[pick], cache.k[0], cache.v[0], cache.table[pick],
+                                         cache.lens[pick], 1 / math.sqrt(d), window)
+        U.close(out[pick], want, tol)
+        U.close(lse[pick], wlse, ltol)
+
+
+def test_attend_wide_batch_of_short_windows(cuda):
+    """The one-launch form with that hint: many (request, key head) pairs, a window of 1,000 keys."""
+    q, cache = make(cuda, torch.float16, [1500], 8, 8, 128, 64, seed=2)
+    B = 128
+    q = torch.cat([q * (1 + b % 3) * 0.5 for b in range(B)])
+    cache.table = cache.table.expand(B, -1).contiguous()
+    cache.lens = int32([1500 - 7 * b for b in range(B)], cuda)
+    out = cache.attend(0, q, window=1000)
+    pick = [0, 1, 63, 100, 127]
+    want, _, tol, _ = U.attend(q[pick], cache.k[0], cache.v[0], cache.table[pick],
+                               cache.lens[pick], 1 / math.sqrt(128), 1000)
+    U.close(out[pick], want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attend_at_the_longest_lengths(cuda, dtype):
+    """Positions up to 2^31 - 17, the last a table row can hold, through a window (every page but the last
+    is the same)."""
+    page, d = 16, 8
+    cap = 2 ** 31 - 16
+    g = torch.Generator(device=cuda).manual_seed(1)
+    k, v = (torch.randn(2, 1, page, d, device=cuda, generator=g).to(dtype) for _ in range(2))
+    table = torch.zeros(1, cap // page, device=cuda, dtype=torch.int32)
+    q = torch.randn(1, 2, d, device=cuda, generator=g).to(dtype)
+    new = torch.randn(1, 1, d, device=cuda, generator=g).to(dtype)
+    for n, window in ((cap, 40), (cap - 1, 1), (cap - 15, 200), (cap - 16, 17), (cap - 17, 3000)):
+        table[0, (n - 1) // page] = 1
+        out, lse = P.attend_pages(q, k, v, table, int32([n], cuda), window=window, k_new=new,
+                                  v_new=new, return_lse=True)
+        torch.cuda.synchronize()
+        table[0, (n - 1) // page] = 0
+        assert torch.equal(k[1, 0, (n - 1) % page], new[0, 0])
+        # the same keys at the start of a short row: n and its stand-in agree modulo the page
+        m = window + 32 - (window - n) % page
+        assert (m - n) % page == 0
+        short = torch.zeros(1, m // page + 2, dtype=torch.int32)
+        short[0, (m - 1) // page] = 1
+        want, wlse, tol, ltol = U.attend(q, k, v, short, int32([m], "cpu"), 1 / math.sqrt(d),
+                                         window)
+        U.close(out, want, tol)
+        U.close(lse, wlse, ltol)
+    # all 2^31 - 16 keys, of equal weight: the mean of the page's values
+    q.zero_()
+    out = P.attend_pages(q, k, v, table, int32([cap], cuda))
+    mean = v[0, 0].double().mean(0)
+    assert (out[0].double() - mean).abs().max() < 2e-2
+    bad = P.attend_pages(q, k, v, table, int32([cap + 1], cuda))
+    assert bad.isnan().all()
+
+
 def test_pool_beyond_32_bit_offsets(cuda):
     """Pages whose elements lie past 2^32 bytes and 2^31 elements into the pool."""
     page, d, hkv = 256, 512, 2
