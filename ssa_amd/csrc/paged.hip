@@ -621,27 +621,29 @@ constexpr int kAttendWaves = 4;
 // any group of query heads, as the matrix units wait for memory anyway. 1,048,577 tokens (bf16, 14 / 2
 // heads of 64) 90 us with the join, 5.9 TB/s; a kernel that only reads as much takes 97 without the
 // non-temporal hint. Equal shares that run on over several requests cost every short call 1 us or more
-// for 2 % of a mixed batch. MT: tiles of 16 query heads served by one reading.
-template <int DT, int DP, int MT, int WPE>
+// for 2 % of a mixed batch. MT: tiles of 16 query heads served by one reading. ACROSS: the waves take
+// a key head each, over all of the item's tiles.
+template <int DT, int DP, int MT, bool ACROSS, int WPE>
 __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(AttendParams p) {
   using T = Tile<DT, DP>;
   constexpr int NT = T::NT, NC = T::NC, VB = T::VB, LC = T::LC, LW = T::LW, NA = T::NA;
-  constexpr int NW = kAttendWaves;
-  __shared__ f32x4 red[NW / 2][MT][NA][64];
-  __shared__ float red_m[NW / 2][MT][64], red_l[NW / 2][MT][64];
+  constexpr int NW = kAttendWaves, HEADS = ACROSS ? NW : 1, NR = ACROSS ? 1 : NW / 2;
+  __shared__ f32x4 red[NR][MT][ACROSS ? 1 : NA][64];
+  __shared__ float red_m[NR][MT][64], red_l[NR][MT][64];
   const int wv = uniform(threadIdx.x >> 6);
   // row tiles of one (item, key head) are 8 workgroups apart: on one XCD, whose L2 they share
   const int id = blockIdx.x, rt = (id >> 3) % p.RT, unit = (id >> 3) / p.RT * 8 + (id & 7);
-  const int g = unit % p.Hkv;
+  const int groups = p.Hkv / HEADS, item = unit / groups;
+  const int g = unit % groups * HEADS + (ACROSS ? wv : 0);
   Item found;
-  if (unit >= p.units || !find_item(p, unit / p.Hkv, found)) return;
+  if (unit >= p.units || !find_item(p, item, found)) return;
   const Item it = uniform(found);
   const int first = it.span.first, len = it.span.len;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int head0 = rt * MT * 16 + col;  // of MT tiles of 16 heads
   const int tiles = (it.end - it.begin + NT - 1) / NT;
-  const int i0 = uniform((int)((int64_t)tiles * wv / NW));
-  const int i1 = uniform((int)((int64_t)tiles * (wv + 1) / NW));
+  const int i0 = ACROSS ? 0 : uniform((int)((int64_t)tiles * wv / NW));
+  const int i1 = ACROSS ? tiles : uniform((int)((int64_t)tiles * (wv + 1) / NW));
 
   __shared__ u32x4 q_lds[T::kQInLds ? MT : 1][T::kQInLds ? NC : 1][64];
   u32x4 q[MT][T::kQInLds ? 1 : NC];
@@ -898,27 +900,29 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
     if (bad != 0 || !it.span.ok) st[mt].l = NAN;
   }
 
-  // the waves' results, half of them into the other half at a time
+  if constexpr (!ACROSS) {
+    // the waves' results, half of them into the other half at a time
 #pragma unroll
-  for (int half = NW / 2; half >= 1; half >>= 1) {
-    if (wv >= half && wv < 2 * half) {
+    for (int half = NW / 2; half >= 1; half >>= 1) {
+      if (wv >= half && wv < 2 * half) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        red_m[wv - half][mt][lane] = st[mt].m;
-        red_l[wv - half][mt][lane] = st[mt].l;
+        for (int mt = 0; mt < MT; ++mt) {
+          red_m[wv - half][mt][lane] = st[mt].m;
+          red_l[wv - half][mt][lane] = st[mt].l;
 #pragma unroll
-        for (int n = 0; n < NA; ++n) red[wv - half][mt][n][lane] = st[mt].acc[n];
+          for (int n = 0; n < NA; ++n) red[wv - half][mt][n][lane] = st[mt].acc[n];
+        }
       }
-    }
-    __syncthreads();
-    if (wv < half) {
+      __syncthreads();
+      if (wv < half) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        join(st[mt], red_m[wv][mt][lane], red_l[wv][mt][lane], &red[wv][mt][0][lane], 64);
+        for (int mt = 0; mt < MT; ++mt)
+          join(st[mt], red_m[wv][mt][lane], red_l[wv][mt][lane], &red[wv][mt][0][lane], 64);
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    if (wv != 0) return;
   }
-  if (wv != 0) return;
 
   if (p.items != 0 && it.j == 0 && g == 0 && rt == 0 && lane == 0) {
     p.info[2 * it.b] = it.first_item;
@@ -930,7 +934,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
     const int h = g * p.G + head0 + mt * 16;
     if (head0 + mt * 16 >= p.G) break;
     const float inv = len == 0 && it.span.ok ? 0.0f : 1.0f / o.l;
-    const int64_t part = (int64_t)(unit / p.Hkv) * p.Hq + h, to = it.b * p.ob + h * p.oh;
+    const int64_t part = (int64_t)item * p.Hq + h, to = it.b * p.ob + h * p.oh;
 #pragma unroll
     for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
@@ -1062,28 +1066,56 @@ int check_pool(const char* who, int dtype, int64_t Hkv, int64_t d, int64_t pages
   return SSA_OK;
 }
 
+// Bytes of the keys and values of one unit of every key head.
+int64_t unit_bytes(int dtype, int64_t d, int64_t Hkv) {
+  return 2 * 16 * kPagedUnit * dtype_size(dtype) * d * Hkv;
+}
+
+// Whether a call is one launch, a request an item: no request passes 512 keys (8 us a call; parts and
+// their join 11), or 2048 in 512 or more (request, key head, row tile) triples (256 x 1,000 keys, 4 key
+// heads: 48 us; cut 60). With few triples and more keys the cut wins: 2,000 keys of 8 heads 12 and 24.
+bool one_launch(int64_t triples, int64_t units) {
+  return units <= 4 || (units <= 16 && triples >= 512);
+}
+
 // Whether a wave serves two tiles of 16 query heads from one reading of the keys and values (past head
 // dim 128 their registers do not fit). It makes fewer, longer workgroups: 16-bit calls that may read
 // more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 76 us
 // for 83; 64 of 2,000 to 20,000, 48 on two: 122 for 137), smaller ones lose (64 of 500 to 4,000, 32 on
 // one: 23 for 19); in fp32 the matrix products count too (8 of 2,000 to 9,000, 40 on two: 26 for 31).
-bool may_serve_two(int64_t G, int64_t d) { return G > 16 && d <= 128; }
+//
+// A workgroup's waves take a key head each instead of a run of keys each where a token's heads lie side
+// by side (token-major pools): four rows of 128 or 256 bytes are then read at about the same time, one at
+// a time leaves memory at 5.4 TB/s of 6.1: 64 requests of 64 to 32,768 keys (8 heads of 128, 16-bit)
+// 236 us for 256, 16 of 8,192 100 for 113 (of head dim 64 55 for 67). Longer rows gain nothing (fp32 63 for
+// 61), heads that lie apart lose (235 for 219), and so do calls of little to read, whose waves then have
+// four tiles each to begin with (one of 4,096 keys 15 for 13; one of 32,768 33 for 30).
+constexpr int64_t kAcrossBytes = (int64_t)32 << 20;
 
-bool serve_two(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
-               int64_t window) {
-  const int64_t keys = B * paged_most_units(W * page, (int)window) * 16 * kPagedUnit;
-  return may_serve_two(Hq / Hkv, d) &&
-         (dtype == SSA_F32 || keys >= kStreamBytes / (2 * dtype_size(dtype) * d * Hkv));
+enum Serve { kOneTile, kTwoTiles, kAcross };
+
+bool may_serve_two(int64_t G, int64_t d) { return G > 16 && d <= 128; }
+bool may_serve_across(int64_t G, int64_t Hkv, int64_t d) {
+  return G <= 16 && Hkv % kAttendWaves == 0 && d <= 128;
+}
+
+// strides: kpool's and vpool's (page, head, slot)
+Serve serve(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
+            int64_t window, const int64_t* strides) {
+  const int64_t units = paged_most_units(W * page, (int)window);
+  const int64_t bytes = B * units * unit_bytes(dtype, d, Hkv);  // read at most
+  if (may_serve_two(Hq / Hkv, d) && (dtype == SSA_F32 || bytes >= kStreamBytes)) return kTwoTiles;
+  if (may_serve_across(Hq / Hkv, Hkv, d) && dtype != SSA_F32 && strides[1] < strides[2] &&
+      strides[4] < strides[5] && B > 1 && bytes >= kAcrossBytes && !one_launch(B * Hkv, units))
+    return kAcross;
+  return kOneTile;
 }
 
 // How a call of these sizes is cut: known on the host without the lengths.
-//   one launch, a request an item, where no request can pass 512 keys (8 us a call; parts and their
-//   join 11) or 2048 in 512 or more (request, key head, row tile) triples (256 x 1,000 keys, 4 key
-//   heads: 48 us; cut 60). With few triples and more keys the cut wins: 2,000 keys of 8 heads 12 and 24.
-//   otherwise items for about `target` workgroups, what the CUs hold at once (four a CU at head dim 64,
-//   two at 256, one at 512; three at 128, and there twice as many even out uneven lengths better: 64
-//   mixed requests 267 us for 1536, 286 for 768). A single request is even by itself and has the most
-//   parts to join: 512 (1M tokens 102 us, 106 for 1024).
+// Unless it is one launch, items for about `target` workgroups, what the CUs hold at once (four a CU at
+// head dim 64, two at 256, one at 512; three at 128, and there twice as many even out uneven lengths
+// better: 64 mixed requests 267 us for 1536, 286 for 768). A single request is even by itself and has the
+// most parts to join: 512 (1M tokens 102 us, 106 for 1024).
 struct Layout {
   int64_t RT, items, max_items;  // items: 0 when every request is one item
   int dp;
@@ -1091,18 +1123,20 @@ struct Layout {
 };
 
 Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
-              int64_t window, bool two) {
+              int64_t window, Serve how) {
   Layout y{};
+  const bool two = how == kTwoTiles;
+  const int64_t heads = how == kAcross ? Hkv / kAttendWaves : Hkv;  // of a workgroup each
   y.RT = (Hq / Hkv + (two ? 31 : 15)) / (two ? 32 : 16);
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
   const int64_t units = paged_most_units(W * page, (int)window);
   y.max_items = B;
-  if (units <= 4 || (units <= 16 && B * Hkv * y.RT >= 512)) return y;
+  if (one_launch(B * Hkv * y.RT, units)) return y;
   const int64_t target = y.dp == 512             ? 256
                          : y.dp == 256 || B == 1 ? 512
                          : y.dp == 128           ? (two ? 1024 : 1536)
                                                  : 1024;
-  y.items = std::max<int64_t>(1, target / (Hkv * y.RT));
+  y.items = std::max<int64_t>(1, target / (heads * y.RT));
   y.max_items = paged_most_items(B, y.items, units);
   const size_t parts = (size_t)y.max_items * Hq;
   y.part_ml = parts * y.dp * 4;
@@ -1111,9 +1145,9 @@ Layout layout(int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t 
   return y;
 }
 
-template <int DT, int DP, int MT, int WPE>
+template <int DT, int DP, int MT, bool ACROSS, int WPE>
 int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
-  paged_attend_kernel<DT, DP, MT, WPE><<<(unsigned)blocks, kAttendWaves * 64, 0, st>>>(p);
+  paged_attend_kernel<DT, DP, MT, ACROSS, WPE><<<(unsigned)blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_attend_kernel"));
   if (p.items == 0) return SSA_OK;
   // 16 to 4 splits of a row's parts; 1024 threads take 10 us more for 4,096 rows of a few parts, and
@@ -1124,16 +1158,22 @@ int run_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
 }
 
 template <int DT>
-int run_attend_dim(const AttendParams& p, int dp, bool two, int64_t blocks, hipStream_t st) {
+int run_attend_dim(const AttendParams& p, int dp, Serve how, int64_t blocks, hipStream_t st) {
+  const bool two = how == kTwoTiles;
+  if constexpr (DT != SSA_F32) {
+    if (how == kAcross)
+      return dp == 64 ? run_attend<DT, 64, 1, true, 4>(p, blocks, st)
+                      : run_attend<DT, 128, 1, true, 3>(p, blocks, st);
+  }
   switch (dp) {
     case 64:
-      if (two) return run_attend<DT, 64, 2, DT == SSA_F32 ? 2 : 3>(p, blocks, st);
-      return run_attend<DT, 64, 1, DT == SSA_F32 ? 3 : 4>(p, blocks, st);
+      if (two) return run_attend<DT, 64, 2, false, DT == SSA_F32 ? 2 : 3>(p, blocks, st);
+      return run_attend<DT, 64, 1, false, DT == SSA_F32 ? 3 : 4>(p, blocks, st);
     case 128:
-      if (two) return run_attend<DT, 128, 2, 2>(p, blocks, st);
-      return run_attend<DT, 128, 1, 3>(p, blocks, st);
-    case 256: return run_attend<DT, 256, 1, 2>(p, blocks, st);
-    default: return run_attend<DT, 512, 1, 1>(p, blocks, st);
+      if (two) return run_attend<DT, 128, 2, false, 2>(p, blocks, st);
+      return run_attend<DT, 128, 1, false, 3>(p, blocks, st);
+    case 256: return run_attend<DT, 256, 1, false, 2>(p, blocks, st);
+    default: return run_attend<DT, 512, 1, false, 1>(p, blocks, st);
   }
 }
 
@@ -1202,9 +1242,12 @@ extern "C" size_t ssa_paged_attend_workspace_size(int64_t B, int64_t Hq, int64_t
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 || W <= 0 || page <= 0 ||
       !fits_int(window) || W > 0x7fffffff / page)
     return 0;
-  const size_t one = layout(B, Hq, Hkv, d, W, page, window, false).bytes;
-  return may_serve_two(Hq / Hkv, d)
-             ? std::max(one, layout(B, Hq, Hkv, d, W, page, window, true).bytes) : one;
+  const size_t one = layout(B, Hq, Hkv, d, W, page, window, kOneTile).bytes;
+  if (may_serve_two(Hq / Hkv, d))
+    return std::max(one, layout(B, Hq, Hkv, d, W, page, window, kTwoTiles).bytes);
+  if (may_serve_across(Hq / Hkv, Hkv, d))
+    return std::max(one, layout(B, Hq, Hkv, d, W, page, window, kAcross).bytes);
+  return one;
 }
 
 extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* lse,
@@ -1240,8 +1283,8 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   SSA_REQUIRE(B * paged_most_units(W * page, (int)window) <= 0x7fffffff, SSA_ERR_UNSUPPORTED,
               "ssa_paged_attend: %lld table rows of %lld tokens (2^38 in all at most)",
               (long long)B, (long long)(W * page));
-  const bool two = serve_two(dtype, B, Hq, Hkv, d, W, page, window);
-  const Layout y = layout(B, Hq, Hkv, d, W, page, window, two);
+  const Serve how = serve(dtype, B, Hq, Hkv, d, W, page, window, strides + 2);
+  const Layout y = layout(B, Hq, Hkv, d, W, page, window, how);
   SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
               SSA_ERR_WORKSPACE, "ssa_paged_attend: needs a 16-byte aligned workspace of %zu bytes, "
               "got %zu", y.bytes, workspace_bytes);
@@ -1276,18 +1319,18 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   // What does not fit the 256 MB last-level cache is read past it: 537 MB 91 us with the hint, 101
   // without; 105 MB that the cache holds 30 and 27. Row tiles read it twice, the second time from L2:
   // 300 MB with two of them 110 us with the hint, 83 without.
-  const int64_t unit_bytes = 2 * 16 * kPagedUnit * d * es * Hkv;
-  p.stream_units = y.RT > 1 ? INT64_MAX : kStreamBytes / unit_bytes;
+  p.stream_units = y.RT > 1 ? INT64_MAX : kStreamBytes / unit_bytes(dtype, d, Hkv);
   if (y.items == 0 && B * paged_most_units(W * page, (int)window) >= p.stream_units)
     p.stream_units = 0;
   p.part = (float*)workspace;
   p.part_ml = (float*)((char*)workspace + y.part_ml);
   p.info = (int32_t*)((char*)workspace + y.info);
-  const int64_t units = y.max_items * Hkv, blocks = (units + 7) / 8 * 8 * y.RT;
+  const int64_t units = y.max_items * (how == kAcross ? Hkv / kAttendWaves : Hkv);
+  const int64_t blocks = (units + 7) / 8 * 8 * y.RT;
   SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_attend: too many rows in one call");
   p.units = (int)units;
   hipStream_t hs = (hipStream_t)stream;
-  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, two, blocks, hs);
-  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, two, blocks, hs);
-  return run_attend_dim<SSA_BF16>(p, y.dp, two, blocks, hs);
+  if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, how, blocks, hs);
+  if (dtype == SSA_F16) return run_attend_dim<SSA_F16>(p, y.dp, how, blocks, hs);
+  return run_attend_dim<SSA_BF16>(p, y.dp, how, blocks, hs);
 }

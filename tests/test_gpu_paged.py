@@ -508,6 +508,34 @@ def test_attend_more_than_the_caches_hold(cuda, dtype, hq, hkv, d):
         U.close(lse[pick], wlse, ltol)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,page", [(32, 8, 128, 16), (4, 4, 64, 48), (16, 8, 80, 16),
+                                           (16, 16, 40, 256)])
+def test_attend_heads_side_by_side(cuda, dtype, hq, hkv, d, page):
+    """Token-major pools with room for many keys: a wave serves a key head of its own."""
+    lens = EDGES + [3000, 129]
+    q, cache = make(cuda, dtype, lens, hq, hkv, d, page, token_major=True, seed=d, spread=2.0)
+    B = len(lens)
+    wide = torch.full((B, (1 << 25) // (B * page * d * hkv) + 200), -1, device=cuda,
+                      dtype=torch.int32)
+    wide[:, :cache.table.shape[1]] = cache.table
+    cache.table = wide
+    for window in (0, 20, 2500):
+        print(dtype, hq, hkv, d, page, window, flush=True)
+        check_attend(cache, q, window=window)
+    x = torch.randn(B, 2 * hkv * d, device=cuda).to(dtype)
+    k_new, v_new = (x[:, i * hkv * d:(i + 1) * hkv * d].view(B, hkv, d) for i in (0, 1))
+    check_attend(cache, q, k_new=k_new, v_new=v_new)
+    for b, n in enumerate(lens):
+        if n:
+            at = int(cache.table[b, (n - 1) // page]), slice(None), (n - 1) % page
+            assert torch.equal(cache.k[0][at], k_new[b]) and torch.equal(cache.v[0][at], v_new[b])
+    cache.table = cache.table.clone()
+    cache.table[B - 2, 3] = -1  # a bad page: this row and no other
+    out = cache.attend(0, q)
+    assert out[B - 2].isnan().all() and not out[[b for b in range(B) if b != B - 2]].isnan().any()
+
+
 def test_attend_wide_batch_of_short_windows(cuda):
     """The one-launch form with that hint: many (request, key head) pairs, a window of 1,000 keys."""
     q, cache = make(cuda, torch.float16, [1500], 8, 8, 128, 64, seed=2)
