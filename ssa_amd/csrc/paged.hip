@@ -1046,11 +1046,11 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(AttendParams p) {
 
 bool fits_int(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
 
-// Rows of 16-byte pieces: the base and every stride (elements) a multiple of 16 bytes.
+// Rows of 16-byte pieces: the base and every stride (elements, none negative) a multiple of 16 bytes.
 bool rows16(const void* base, const int64_t* strides, int n, int es) {
   if (!aligned16(base)) return false;
   for (int i = 0; i < n; ++i)
-    if (strides[i] * es % 16 != 0) return false;
+    if (strides[i] < 0 || strides[i] * es % 16 != 0) return false;
   return true;
 }
 
@@ -1103,10 +1103,11 @@ bool may_serve_across(int64_t G, int64_t Hkv, int64_t d) {
 Serve serve(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t page,
             int64_t window, const int64_t* strides) {
   const int64_t units = paged_most_units(W * page, (int)window);
-  const int64_t bytes = B * units * unit_bytes(dtype, d, Hkv);  // read at most
-  if (may_serve_two(Hq / Hkv, d) && (dtype == SSA_F32 || bytes >= kStreamBytes)) return kTwoTiles;
+  // whether the call may read so much
+  auto reads = [&](int64_t bytes) { return B * units >= bytes / unit_bytes(dtype, d, Hkv); };
+  if (may_serve_two(Hq / Hkv, d) && (dtype == SSA_F32 || reads(kStreamBytes))) return kTwoTiles;
   if (may_serve_across(Hq / Hkv, Hkv, d) && dtype != SSA_F32 && strides[1] < strides[2] &&
-      strides[4] < strides[5] && B > 1 && bytes >= kAcrossBytes && !one_launch(B * Hkv, units))
+      strides[4] < strides[5] && B > 1 && reads(kAcrossBytes) && !one_launch(B * Hkv, units))
     return kAcross;
   return kOneTile;
 }

@@ -43,6 +43,7 @@ def attend(**kw):
     (dict(strides=_lib.i64_array([256, 64, 2048, 1024, 60] + [64] * 9)), _lib.SSA_ERR_INVALID),
     (dict(strides=_lib.i64_array([64] * 4 + [2 ** 24] + [64] * 9)), _lib.SSA_ERR_UNSUPPORTED),
     (dict(strides=_lib.i64_array([64] * 7 + [2 ** 24] + [64] * 6)), _lib.SSA_ERR_UNSUPPORTED),
+    (dict(strides=_lib.i64_array([64] * 4 + [-64] + [64] * 9)), _lib.SSA_ERR_INVALID),
     (dict(B=65536), _lib.SSA_ERR_INVALID), (dict(Hq=65536, Hkv=1), _lib.SSA_ERR_INVALID),
     (dict(B=65535, W=2 ** 22, table_stride=2 ** 22), _lib.SSA_ERR_UNSUPPORTED),
     (dict(W=1000, table_stride=1000, ws_bytes=1000), _lib.SSA_ERR_WORKSPACE),
