@@ -414,6 +414,28 @@ def test_attend_subnormal_values(cuda, dtype):
     check_attend(cache, q, scale=1.0 / tiny if dtype == torch.float16 else 1.0)
 
 
+@pytest.mark.parametrize("d,chain", [(64, 32), (128, 32), (256, 64), (512, 128)])
+def test_attend_adds_fp32_products_in_chains(cuda, d, chain):
+    """fp32 products are added in chains shorter than the head: one of 2^24 hides the products of 1 in
+    its own chain only (2^24 + 1 rounds back), the others' sum counts. Key 0 has the ones and key 1 has
+    none, so its weight is 1 / (1 + exp(-(d - 1) 2^-17)), of slope 1/4: off by the chain's chain - 1
+    products, 2 for joining the chains and 2 for the two scores of 185 in log2 units (half of 2^-16
+    each), in units of 2^-17, over 4. One chain would lose all d - 1."""
+    q, cache = make(cuda, torch.float32, [2], 2, 1, d, 16)
+    q.fill_(1.0)
+    page = int(cache.table[0, 0])
+    cache.k[0, page, 0, :2] = 0.0
+    cache.k[0, page, 0, :2, 0] = 2.0**24
+    cache.k[0, page, 0, 0, 1:] = 1.0
+    cache.v[0, page, 0, 0] = 1.0
+    cache.v[0, page, 0, 1] = 0.0
+    out = cache.attend(0, q, scale=2.0**-17)
+    want = 1 / (1 + math.exp(-(d - 1) * 2.0**-17))
+    tol = (chain - 1 + 4) * 2.0**-17 / 4
+    assert tol < (want - 0.5) * 0.6
+    assert float((out.double() - want).abs().max()) <= tol
+
+
 @pytest.mark.parametrize("B", [63, 64, 65, 129])
 def test_attend_batch_sizes(cuda, B):
     rng = random.Random(B)
