@@ -362,10 +362,13 @@ class PagedCache:
 
     @torch.no_grad()
     def resize(self, new_lens: torch.Tensor, tokens: int, out: Resized | None = None) -> Resized:
-        """resize_pages on this cache's state."""
+        """resize_pages on this cache's state. The status that attend, step and check go by is
+        the cache's own tensor, like its lengths: a captured call finds the last resize's there,
+        whether that one ran eagerly or in a replay."""
         r = resize_pages(self.lens, new_lens, self.table, self.free, self.nfree, self.page,
                          tokens, out)
-        self.status = r.status
+        # r's own may be written by another cache's resize; added, not copied: a kernel in a graph too
+        torch.add(r.status, 0, out=self.status)
         return r
 
     def check(self) -> None:

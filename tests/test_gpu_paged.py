@@ -760,6 +760,93 @@ def test_captured_step_replayed(cuda):
         torch.empty(1 << 20, device=cuda).normal_().sum().item()
 
 
+def test_captured_step_between_eager_resizes(cuda):
+    """step alone captured, resizes run eagerly between its replays with other small tensors made where
+    an earlier status lay: each replay equals the eager cache beside it, a refused resize's replay stores
+    nothing and gives NaN, and the next that fits serves again."""
+    hq, hkv, d, page = 4, 2, 64, 16
+    a, b = (P.PagedCache(3, 200, 12, hkv, d, page=page, dtype=torch.float16, device=cuda)
+            for _ in range(2))
+    x = torch.randn(60, hkv, d, device=cuda).to(torch.float16)
+    q = torch.randn(3, hq, d, device=cuda).to(torch.float16)
+    kn, vn = (torch.randn(3, hkv, d, device=cuda).to(torch.float16) for _ in range(2))
+    for c in (a, b):
+        r = c.resize(int32([40, 0, 20], cuda), 60)
+        c.append(0, x, x, r.slots)
+    one = int32([1, 0, 1], cuda)
+    a.resize(a.lens + one, 2)
+    b.resize(b.lens + one, 2)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(0, q, kn, vn, out=out)
+    graph.replay()
+    assert torch.equal(out, b.step(0, q, kn, vn))
+    kept = []
+    for rep in range(12):
+        grow = int32([1, 500, 1] if rep % 4 == 2 else [1, 0, 1], cuda)  # 500: past the table
+        for c in (a, b):
+            r = c.resize(c.lens + grow, 600)
+            assert r.status.item() == (-1 if rep % 4 == 2 else 0)
+            if rep % 2:
+                kept.append(r)  # its status is kept as well as dropped
+        junk = [torch.full((n,), 7, device=cuda, dtype=torch.int32) for n in (1, 1, 1, 3, 60, 128)]
+        for t in (q, kn, vn):
+            t.normal_()
+        held = a.k.clone(), a.v.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = b.step(0, q, kn, vn)
+        if rep % 4 == 2:
+            assert out.isnan().all() and want.isnan().all(), rep
+            assert torch.equal(a.k, held[0]) and torch.equal(a.v, held[1]), rep
+            with pytest.raises(RuntimeError, match="does not fit the table"):
+                a.check()
+        else:
+            assert torch.equal(out, want) and not out.isnan().any(), rep
+            assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v), rep
+            a.check()
+        del junk
+
+
+def test_captured_resize_refused_on_replay(cuda):
+    """A captured resize replayed after an eager one: its refusal is what check, an eager step and an eager
+    attend go by, and the next eager resize that fits ends it."""
+    cache = P.PagedCache(2, 100, 5, 2, 64, page=16, dtype=torch.bfloat16, device=cuda)
+    x = torch.randn(40, 2, 64, device=cuda).to(torch.bfloat16)
+    q = torch.randn(2, 4, 64, device=cuda).to(torch.bfloat16)
+    grow = int32([1, 1], cuda)
+    r = cache.resize(int32([20, 20], cuda), 40)
+    cache.append(0, x, x, r.slots)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = cache.resize(cache.lens + grow, 60)
+    for rep in range(3):
+        cache.resize(int32([20, 20], cuda), 0)
+        cache.check()
+        good = cache.attend(0, q)
+        grow.fill_(1)
+        graph.replay()
+        torch.empty(1 << 20, device=cuda).normal_().sum().item()
+        cache.check()
+        assert cache.lens.tolist() == [21, 21] and not cache.attend(0, q).isnan().any()
+        cache.resize(int32([20, 20], cuda), 0)
+        grow.fill_(28)  # two pages more, one is free
+        held = cache.k.clone(), cache.v.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert inside.status.item() == 1 and cache.lens.tolist() == [20, 20], rep
+        with pytest.raises(RuntimeError, match="1 pages lacking"):
+            cache.check()
+        assert cache.step(0, q, x[:2], x[:2]).isnan().all() and cache.attend(0, q).isnan().all()
+        assert torch.equal(cache.k, held[0]) and torch.equal(cache.v, held[1]), rep
+        cache.resize(cache.lens.clone(), 0)
+        cache.check()
+        assert torch.equal(cache.attend(0, q), good), rep
+
+
 def test_two_graphs_with_one_memory_pool(cuda):
     """Two captured attentions whose workspaces may share memory, replayed in turn."""
     q, a = make(cuda, torch.float16, [9000, 3], 8, 2, 128, 16, seed=3)

@@ -96,6 +96,39 @@ def test_cpu_tensors_raise():
                             **kw})
 
 
+def test_cache_keeps_its_tensors(monkeypatch):
+    """A captured step holds the addresses of the cache's tensors: resizes write them in place, the
+    status among them, and a Resized given to another cache as `out` leaves this one's alone."""
+    outcome = []
+
+    def resize(lens, new_lens, table, free, nfree, page, tokens, out=None):
+        if out is None:
+            out = P.Resized(torch.zeros(tokens, dtype=torch.int64),
+                            *(torch.zeros(n, dtype=torch.int32) for n in (tokens, 4, 1)))
+        out.status.fill_(outcome.pop(0))
+        return out
+
+    monkeypatch.setattr(P, "resize_pages", resize)
+    a, b = (P.PagedCache(3, 40, 9, 1, 8, page=16, device="cpu") for _ in range(2))
+    state = lambda c: [t.data_ptr() for t in (c.k, c.v, c.lens, c.table, c.free,  # noqa: E731
+                                              c.nfree, c.status)]
+    held = state(a)
+    outcome += [0, 2, 5, -1, 0, 0]
+    r = a.resize(a.lens, 5)
+    first = a.resize(a.lens, 5)
+    assert state(a) == held and a.status.item() == 2 and r.status.item() == 0
+    with pytest.raises(RuntimeError, match="2 pages lacking"):
+        a.check()
+    b.resize(b.lens, 5, out=first)
+    assert a.status.item() == 2 and b.status.item() == first.status.item() == 5
+    assert a.resize(a.lens, 5, out=r) is r
+    assert state(a) == held and a.status.item() == r.status.item() == -1
+    b.resize(b.lens, 5)
+    a.resize(a.lens, 5)
+    assert state(a) == held and a.status.item() == b.status.item() == 0
+    a.check()
+
+
 def test_another_device_is_made_current(monkeypatch):
     """A call for tensors of a device that is not the current one runs with that device current."""
     from types import SimpleNamespace as NS
