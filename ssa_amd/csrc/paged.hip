@@ -527,27 +527,46 @@ __device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c, b
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A weight as the sum of two 16-bit parts, both positive where it is: the first takes the leading
-// bits of a little less than the weight, the second the rest. With one 16-bit weight the output
-// would be off by as much again as its own rounding; a second part of the other sign, or zero, would
-// turn an infinite value into NaN.
+// A weight's 16-bit parts: bf16 holds 8 of its 24 bits, fp16 11 (of 22: the output rounds to 11).
 template <int DT>
-__device__ inline void split2(float p0, float p1, unsigned int& hi, unsigned int& lo) {
+constexpr int kParts = DT == SSA_BF16 ? 3 : 2;
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Two weights as sums of 16-bit parts, none negative and none zero where the weight is not: one of
+// another sign, or zero, would turn an infinite value into NaN. bf16: each part the leading bits of what
+// is left, so that the three hold the weight exactly; with two 0.4 % of the outputs fell on the other side
+// of their rounding, with three 0.05 %, as many as in plain fp32 operations. The third's product costs up
+// to 2.5 % (one request of 1M tokens 90.2 -> 92.4 us, 128 of 2,000 to 9,000 with 20 heads on one 75.7 ->
+// 77.1, 64 mixed ones 0.2 %). A part that would be zero is the smallest subnormal instead, 2^-133. fp16:
+// the first takes the leading bits of a little less than the weight, the second the rest.
+template <int DT>
+__device__ inline void split(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
   if constexpr (DT == SSA_BF16) {
-    const float less = 1.0f - 0x1p-8f;
-    const unsigned int a = __float_as_uint(p0 * less) & 0xffff0000u;
-    const unsigned int b = __float_as_uint(p1 * less) & 0xffff0000u;
-    hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned int a = __float_as_uint(p0) & 0xffff0000u;
+      const unsigned int b = __float_as_uint(p1) & 0xffff0000u;
+      w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      p0 -= __uint_as_float(a);
+      p1 -= __uint_as_float(b);
+    }
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 r = {(__bf16)(p0 - __uint_as_float(a)), (__bf16)(p1 - __uint_as_float(b))};
-    lo = __builtin_bit_cast(unsigned int, r);
+    const bf16x2 r = {(__bf16)p0, (__bf16)p1};
+    w[2] = __builtin_bit_cast(unsigned int, r);
+    const u16x2 one = {1, 1};
+    const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w[0]), one);
+#pragma unroll
+    for (int i = 1; i < 3; ++i)
+      w[i] = __builtin_bit_cast(
+          unsigned int, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w[i]), least));
   } else {
     const float less = 1.0f - 0x1p-11f;
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 * less, p1 * less));
-    hi = __builtin_bit_cast(unsigned int, h);
-    lo = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0],
-                                                                     p1 - (float)h[1]));
+    w[0] = __builtin_bit_cast(unsigned int, h);
+    w[1] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0],
+                                                                       p1 - (float)h[1]));
   }
 }
 
@@ -619,7 +638,7 @@ constexpr int kAttendWaves = 4;
 // byte permutes: no LDS, no transposed copy. Bound by the reading of K and V: a wave's next keys are in
 // flight while it weighs the current values and the other way round; 16 lanes of 16 heads serve
 // any group of query heads, as the matrix units wait for memory anyway. 1,048,577 tokens (bf16, 14 / 2
-// heads of 64) 90 us with the join, 5.9 TB/s; a kernel that only reads as much takes 97 without the
+// heads of 64) 92 us with the join, 5.8 TB/s; a kernel that only reads as much takes 97 without the
 // non-temporal hint. Equal shares that run on over several requests cost every short call 1 us or more
 // for 2 % of a mixed batch. MT: tiles of 16 query heads served by one reading. ACROSS: the waves take
 // a key head each, over all of the item's tiles.
@@ -814,7 +833,8 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
       locate(i + 1);
       load_k(0);
     }
-    u32x4 hi[MT], lo[MT];  // the weights in 16-bit parts
+    constexpr int PARTS = kParts<DT>;
+    u32x4 w[MT][PARTS];  // the weights in 16-bit parts
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       Softmax<NA>& o = st[mt];
@@ -862,10 +882,10 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            unsigned int a, b;
-            split2<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], a, b);
-            hi[mt][2 * t + h] = a;
-            lo[mt][2 * t + h] = b;
+            unsigned int x[PARTS];
+            split<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], x);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) w[mt][i][2 * t + h] = x[i];
           }
       }
     }
@@ -897,8 +917,8 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             f32x4& acc = st[mt].acc[vb * LC + e];
-            acc = mfma16(vt, hi[mt], acc, DT == SSA_BF16);
-            acc = mfma16(vt, lo[mt], acc, DT == SSA_BF16);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) acc = mfma16(vt, w[mt][i], acc, DT == SSA_BF16);
           }
         }
       }

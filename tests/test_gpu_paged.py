@@ -404,6 +404,46 @@ def test_attend_infinite_keys_per_head(cuda, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,width,token_major", [
+    (4, 4, 64, 1, False), (2, 1, 128, 1, False), (4, 2, 256, 1, False), (2, 2, 512, 1, False),
+    (20, 1, 64, 2000, False), (20, 1, 128, 2000, False), (4, 4, 64, 2000, True),
+    (4, 4, 128, 2000, True), (4, 2, 80, 300, False)])
+def test_attend_weights_keep_their_bits(cuda, dtype, hq, hkv, d, width, token_major):
+    """Outputs round as fp32 weights make them round. Three keys a request, a score the product of two
+    16-bit numbers below 1 (exact), so that little but the weights' own bits is off, u = 2^-24:
+      a weight    2 u |score| for the scale in log2 units, 0.7 u |exponent| for its difference from the
+                  maximum (up to 3, in fp16 17 with the shift by 14), 2 u for exp2: 7 u, in fp16 16 u;
+                  its parts: bf16 three of 8 bits, 2 u at most for the last one's rounding; fp16 two
+                  of 11, the first up to 2^-9 below the weight, 16 u: 9 u, in fp16 32 u
+      numerator   three terms of up to three parts, 2 u each: 18 u, and 4 u for the joins' factors
+      quotient    3 u for the denominator's sum, 4 u for its joins, 2 u for division and product
+    with the weights' counted for numerator and denominator: 18 + 31 = 49 u, in fp16 64 + 31 = 95 u, times
+    A = sum w |v| / sum w. A weight of 16 bits (2^-16 of it off) left 0.2 % of the outputs outside."""
+    B, page, u = 256, 16, 2.0**-24
+    g = torch.Generator(device=cuda).manual_seed(d + hq)
+    cache = P.PagedCache(B, width * page, B, hkv, d, page=page, dtype=dtype, device=cuda,
+                         token_major=token_major)
+    cache.table[:, 0] = torch.randperm(B, device=cuda, generator=g).to(torch.int32)
+    cache.lens.fill_(3)
+    rows = cache.table[:, 0].long()
+    q = torch.zeros(B, hq, d, device=cuda, dtype=dtype)
+    q[..., 0] = (torch.rand(B, hq, device=cuda, generator=g) * 2 - 1).to(dtype)
+    k = (torch.rand(B, hkv, 3, device=cuda, generator=g) * 2 - 1).to(dtype)
+    v = torch.randn(B, hkv, 3, d, device=cuda, generator=g).to(dtype)
+    cache.k[0, rows, :, :3, 0] = k
+    cache.v[0, rows, :, :3] = v
+    out = cache.attend(0, q, scale=1.0)
+    s = q[..., 0].double().view(B, hkv, -1, 1) * k.double()[:, :, None]  # (B, hkv, group, 3)
+    w = torch.softmax(s, 3)[..., None]
+    v = v.double()[:, :, None]
+    want, size = ((w * x).sum(3).view(B, hq, d) for x in (v, v.abs()))
+    # and u of the value, as the bounds below pass through fp32 on their way to the type
+    t = size * (49 if dtype == torch.bfloat16 else 95) * u + want.abs() * 2 * u
+    wrong = (out < (want - t).to(dtype)) | (out > (want + t).to(dtype))
+    assert int(wrong.sum()) == 0, f"{int(wrong.sum())} of {wrong.numel()}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_attend_subnormal_values(cuda, dtype):
     """Keys and values below the type's smallest normal number count as what they are."""
     q, cache = make(cuda, dtype, [50, 700], 4, 2, 64, 16, seed=12)
