@@ -498,8 +498,8 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
  * ssa_paged_attend: one query row per head and request, q, out (B, Hq, d), over keys j of
  *   [max(0, len - window), len) (window 0: all), len = lens[b] (B) int32: softmax(scale * q.k) in
  *   fp32, query head h reading key head h / (Hq / Hkv). The 16-bit types' weights meet their values as
- *   sums of 16-bit parts: bf16 all 24 bits, fp16 20, and none of a weight below 2^-38 of the row's
- *   largest. lse (B, Hq) fp32, may be NULL: natural log of the row's sum of exponentials. A row of
+ *   sums of 16-bit parts: bf16 all 24 bits, fp16 22, and none of a weight below 2^-38 of the largest
+ *   so far. lse (B, Hq) fp32, may be NULL: natural log of the row's sum of exponentials. A row of
  *   length 0: out 0, lse -inf. A length outside [0, W * page] or an attended page id outside
  *   [0, pages): out and lse NaN. k_new, v_new (B, Hkv, d), both or none: the key and value at position
  *   len - 1, which the call stores into the pools and attends (that page must be one request's alone;

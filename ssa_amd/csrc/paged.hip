@@ -532,14 +532,16 @@ template <int DT>
 constexpr int kParts = DT == SSA_BF16 ? 3 : 2;
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// Two weights as sums of 16-bit parts, none negative and none zero where the weight is not: one of
-// another sign, or zero, would turn an infinite value into NaN. bf16: each part the leading bits of what
-// is left, so that the three hold the weight exactly; with two 0.4 % of the outputs fell on the other side
-// of their rounding, with three 0.05 %, as many as in plain fp32 operations. The third's product costs up
-// to 2.5 % (one request of 1M tokens 90.2 -> 92.4 us, 128 of 2,000 to 9,000 with 20 heads on one 75.7 ->
-// 77.1, 64 mixed ones 0.2 %). A part that would be zero is the smallest subnormal instead, 2^-133. fp16:
-// the first takes the leading bits of a little less than the weight, the second the rest.
+// Two weights as sums of 16-bit parts, each the leading bits of what the ones before leave. bf16: three
+// hold the weight exactly; with two 0.4 % of the outputs fell on the other side of their rounding, with
+// three 0.05 %, as many as in plain fp32 operations. The third's product costs up to 2.5 % (one request of
+// 1M tokens 90.2 -> 92.4 us, 128 of 2,000 to 9,000 with 20 heads on one 75.7 -> 77.1, 64 mixed ones 0.2 %).
+// A part of another sign than the first, or zero where that is not, would turn an infinite value into NaN:
+// none is negative, and instead of zero they are the smallest subnormal (fp16: 2^-38 of the largest
+// weight; below that the first part is zero too and such a value gives NaN).
 template <int DT>
 __device__ inline void split(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
   if constexpr (DT == SSA_BF16) {
@@ -551,23 +553,19 @@ __device__ inline void split(float p0, float p1, unsigned int (&w)[kParts<DT>]) 
       p0 -= __uint_as_float(a);
       p1 -= __uint_as_float(b);
     }
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 r = {(__bf16)p0, (__bf16)p1};
-    w[2] = __builtin_bit_cast(unsigned int, r);
-    const u16x2 one = {1, 1};
-    const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w[0]), one);
-#pragma unroll
-    for (int i = 1; i < 3; ++i)
-      w[i] = __builtin_bit_cast(
-          unsigned int, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w[i]), least));
+    w[2] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
   } else {
-    const float less = 1.0f - 0x1p-11f;
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 * less, p1 * less));
+    const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
     w[0] = __builtin_bit_cast(unsigned int, h);
-    w[1] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0],
-                                                                       p1 - (float)h[1]));
+    w[1] = __builtin_bit_cast(unsigned int, f16x2{(_Float16)(p0 - (float)h[0]),
+                                                  (_Float16)(p1 - (float)h[1])});
   }
+  const u16x2 one = {1, 1};
+  const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w[0]), one);
+#pragma unroll
+  for (int i = 1; i < kParts<DT>; ++i)
+    w[i] = __builtin_bit_cast(
+        unsigned int, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w[i]), least));
 }
 
 template <int W>

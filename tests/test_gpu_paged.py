@@ -382,6 +382,40 @@ def test_attend_infinities_and_nan(cuda, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,d", [(2, 64), (20, 64), (2, 128), (20, 128), (2, 256), (2, 512)])
+def test_attend_infinite_values_far_below_the_maximum(cuda, dtype, hq, d):
+    """A value that is infinite makes its column infinite however small its key's weight: the score lies
+    `gap` below the row's largest, up to 2^-37 of it in fp16 and 2^-120 in the others (a weight below 2^-126
+    is zero in fp32, below 2^-38 in fp16). The other columns hold ones: 1, off by the additions of up to 40
+    terms of three parts (2 u each, u = 2^-24), 40 u for the denominator's, 8 u for joins and division, 4 u
+    for a weight's parts (300 u in all), and half a step of the type."""
+    gaps = [0.5, 6.0, 13.0, 17.0, 19.0, 21.0, 23.0, 25.0]
+    gaps += [25.6] if dtype == torch.float16 else [30.0, 50.0, 70.0, 83.0]
+    page, n = 16, 40
+    cache = P.PagedCache(len(gaps), 4000, 3 * len(gaps), 1, d, page=page, dtype=dtype, device=cuda)
+    cache.resize(int32([n] * len(gaps), cuda), n * len(gaps))
+    q = torch.zeros(len(gaps), hq, d, device=cuda, dtype=dtype)
+    q[:, :, 0] = 1.0
+    cache.v.fill_(1.0)
+    at = lambda b, j: (0, int(cache.table[b, j // page]), 0, j % page)  # noqa: E731
+    for b, gap in enumerate(gaps):
+        for j in range(n):
+            cache.k[at(b, j)][0] = -gap
+        for j in (3, 37):  # the largest score is 0
+            cache.k[at(b, j)][0] = 0.0
+        cache.v[at(b, 5)][1] = math.inf
+        cache.v[at(b, 20)][2] = -math.inf
+        cache.v[at(b, 39)][d - 1] = math.inf
+    out = cache.attend(0, q, scale=1.0).double().cpu()
+    for b, gap in enumerate(gaps):
+        print(dtype, hq, d, gap, flush=True)
+        assert (out[b, :, 1] == math.inf).all() and (out[b, :, 2] == -math.inf).all()
+        assert (out[b, :, d - 1] == math.inf).all()
+        cols = [c for c in range(d) if c not in (1, 2, d - 1)]
+        assert (out[b][:, cols] - 1).abs().max() <= 300 * 2.0**-24 + torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128, 512])
 def test_attend_infinite_keys_per_head(cuda, dtype, d):
     """Keys that score -inf for one head and +inf for another, all through the first tiles: the first
@@ -414,10 +448,10 @@ def test_attend_weights_keep_their_bits(cuda, dtype, hq, hkv, d, width, token_ma
       a weight    2 u |score| for the scale in log2 units, 0.7 u |exponent| for its difference from the
                   maximum (up to 3, in fp16 17 with the shift by 14), 2 u for exp2: 7 u, in fp16 16 u;
                   its parts: bf16 three of 8 bits, 2 u at most for the last one's rounding; fp16 two
-                  of 11, the first up to 2^-9 below the weight, 16 u: 9 u, in fp16 32 u
+                  of 11, 4 u, and 2^-38: 9 u, in fp16 21 u
       numerator   three terms of up to three parts, 2 u each: 18 u, and 4 u for the joins' factors
       quotient    3 u for the denominator's sum, 4 u for its joins, 2 u for division and product
-    with the weights' counted for numerator and denominator: 18 + 31 = 49 u, in fp16 64 + 31 = 95 u, times
+    with the weights' counted for numerator and denominator: 18 + 31 = 49 u, in fp16 42 + 31 = 73 u, times
     A = sum w |v| / sum w. A weight of 16 bits (2^-16 of it off) left 0.2 % of the outputs outside."""
     B, page, u = 256, 16, 2.0**-24
     g = torch.Generator(device=cuda).manual_seed(d + hq)
@@ -438,7 +472,7 @@ def test_attend_weights_keep_their_bits(cuda, dtype, hq, hkv, d, width, token_ma
     v = v.double()[:, :, None]
     want, size = ((w * x).sum(3).view(B, hq, d) for x in (v, v.abs()))
     # and u of the value, as the bounds below pass through fp32 on their way to the type
-    t = size * (49 if dtype == torch.bfloat16 else 95) * u + want.abs() * 2 * u
+    t = size * (49 if dtype == torch.bfloat16 else 73) * u + want.abs() * 2 * u
     wrong = (out < (want - t).to(dtype)) | (out > (want + t).to(dtype))
     assert int(wrong.sum()) == 0, f"{int(wrong.sum())} of {wrong.numel()}"
 
