@@ -225,6 +225,11 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
             raise ValueError(f"out.slots must be a contiguous ({tokens},) int64 tensor")
         for name, n in (("pos", tokens), ("cu", B + 1), ("status", 1)):
             _int32("out." + name, *_meta(getattr(out, name)), (n,))
+    if B == 0:  # no requests, no new tokens
+        out.slots.fill_(-1)
+        for x in out[1:]:
+            x.zero_()
+        return out
     _launch("ssa_paged_resize", lens, lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(),
             row, B, W, int(page), free.data_ptr(), pages, nfree.data_ptr(),
             out.slots.data_ptr() if tokens else None, out.pos.data_ptr() if tokens else None,

@@ -152,6 +152,20 @@ def test_resize_into_its_own_lengths_changes_nothing(cuda):
     assert torch.equal(cache.table, held) and cache.lens.tolist() == [3, 0, 16, 17, 99]
 
 
+def test_empty_batch_through_the_run(cuda):
+    """No requests: resize, append and attend all answer an empty batch and leave the pool alone."""
+    cache = P.PagedCache(2, 64, 6, 1, 64, page=16, device=cuda)
+    lens, table = cache.lens[:0], cache.table[:0]
+    r = P.resize_pages(lens, lens.clone(), table, cache.free, cache.nfree, 16, 5)
+    assert r.slots.tolist() == [-1] * 5 and r.pos.tolist() == [0] * 5
+    assert r.cu.tolist() == [0] and r.status.tolist() == [0]
+    assert cache.nfree.item() == 6 and sorted(cache.free.tolist()) == list(range(6))
+    x = torch.ones(5, 1, 64, device=cuda, dtype=torch.bfloat16)
+    cache.append(0, x, x, r.slots)
+    out, lse = P.attend_pages(x[:0], cache.k[0], cache.v[0], table, lens, return_lse=True)
+    assert out.shape == (0, 1, 64) and lse.shape == (0, 1) and (cache.k == 0).all()
+
+
 def test_resize_refuses_a_bad_free_count(cuda):
     cache = P.PagedCache(2, 100, 10, 1, 8, page=16, device=cuda)
     for n in (-1, 11, 2 ** 31 - 1):

@@ -129,6 +129,21 @@ def test_cache_keeps_its_tensors(monkeypatch):
     a.check()
 
 
+@pytest.mark.parametrize("tokens,given", [(0, False), (3, False), (3, True)])
+def test_resize_of_no_requests(monkeypatch, tokens, given):
+    """An empty batch is resized as it is appended and attended: nothing changes, every slot is padding."""
+    monkeypatch.setattr(P, "_one_device", lambda *a: None)
+    monkeypatch.setattr(P, "_launch", lambda *a: pytest.fail("launched"))
+    i32 = lambda *n: torch.full(n, 7, dtype=torch.int32)  # noqa: E731
+    lens, table, free, nfree = i32(0), i32(0, 4), i32(9), i32(1)
+    out = P.Resized(i32(tokens).long(), i32(tokens), i32(1), i32(1)) if given else None
+    r = P.resize_pages(lens, lens.clone(), table, free, nfree, 16, tokens, out)
+    assert out is None or r is out
+    assert r.slots.tolist() == [-1] * tokens and r.pos.tolist() == [0] * tokens
+    assert r.cu.tolist() == [0] and r.status.tolist() == [0]
+    assert nfree.item() == 7 and (free == 7).all()
+
+
 def test_another_device_is_made_current(monkeypatch):
     """A call for tensors of a device that is not the current one runs with that device current."""
     from types import SimpleNamespace as NS
