@@ -493,8 +493,8 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
  *   tokens). Pages given back in a call can be taken from the next call on. The table's entries of
  *   different requests must not overlap in memory; new_lens may be lens itself.
  * ssa_paged_append: keys and values k, v (T, Hkv, d) of new tokens into the pools at slots (T) int64
- *   (distinct; rows whose slot lies outside the pool are skipped). strides[10] = k(t,h), v(t,h),
- *   kpool(page,head,slot), vpool(page,head,slot).
+ *   (distinct; rows whose slot lies outside the pool are skipped), fewer than 64 GiB of keys a call.
+ *   strides[10] = k(t,h), v(t,h), kpool(page,head,slot), vpool(page,head,slot).
  * ssa_paged_attend: one query row per head and request, q, out (B, Hq, d), over keys j of
  *   [max(0, len - window), len) (window 0: all), len = lens[b] (B) int32: softmax(scale * q.k) in
  *   fp32, query head h reading key head h / (Hq / Hkv). The 16-bit types' weights meet their values as
@@ -506,7 +506,9 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
  *   earlier pages may be shared). status, may be NULL: the status of the resize that made room; if it
  *   is not 0 nothing is stored and every row is NaN (the position len - 1 is then an older token's).
  *   strides[14] = q(b,h), kpool(page,head,slot), vpool(page,head,slot), out(b,h), k_new(b,h),
- *   v_new(b,h). Slots lie fewer than 2^24 elements apart; B table rows hold at most 2^38 tokens in all.
+ *   v_new(b,h). Slots lie fewer than 2^24 elements apart; B table rows hold at most 2^38 tokens in all;
+ *   B and Hq are at most 65535, and a call of 2^24 workgroups (one or more a request and key head) is
+ *   refused.
  *   Workspace: ssa_paged_attend_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
  * Rows start at multiples of 16 bytes (bases and strides).
  */

@@ -1075,6 +1075,9 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(AttendParams p) {
 
 bool fits_int(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
 
+// Whether a launch's threads can be counted: in 32 bits.
+bool fits_launch(int64_t blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+
 // Rows of 16-byte pieces: the base and every stride (elements, none negative) a multiple of 16 bytes.
 bool rows16(const void* base, const int64_t* strides, int n, int es) {
   if (!aligned16(base)) return false;
@@ -1261,7 +1264,7 @@ extern "C" int ssa_paged_append(const void* k, const void* v, void* kpool, void*
                  strides[4] * es, strides[5] * es, strides[6] * es, strides[7] * es,
                  strides[8] * es, strides[9] * es};
   const int64_t blocks = (T * p.Hkv * p.vecs + 255) / 256;
-  SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_append: %lld tokens in one call",
+  SSA_REQUIRE(fits_launch(blocks, 256), SSA_ERR_UNSUPPORTED, "ssa_paged_append: %lld tokens in one call",
               (long long)T);
   paged_append_kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(p);
   return launch_status("paged_append_kernel");
@@ -1357,7 +1360,8 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   p.info = (int32_t*)((char*)workspace + y.info);
   const int64_t units = y.max_items * (how == kAcross ? Hkv / kAttendWaves : Hkv);
   const int64_t blocks = (units + 7) / 8 * 8 * y.RT;
-  SSA_REQUIRE(fits_int(blocks), SSA_ERR_UNSUPPORTED, "ssa_paged_attend: too many rows in one call");
+  SSA_REQUIRE(fits_launch(blocks, kAttendWaves * 64), SSA_ERR_UNSUPPORTED,
+              "ssa_paged_attend: too many rows in one call");
   p.units = (int)units;
   hipStream_t hs = (hipStream_t)stream;
   if (dtype == SSA_F32) return run_attend_dim<SSA_F32>(p, y.dp, how, blocks, hs);

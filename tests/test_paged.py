@@ -55,6 +55,23 @@ def test_attend_refuses(change, code):
     assert b"ssa_paged_attend" in _lib.lib().ssa_last_error()
 
 
+def test_launches_past_32_bits_are_refused():
+    """A launch counts its threads in 32 bits: calls with more are refused by name, and the largest that
+    fits is left to the launch (which fails without a GPU)."""
+    if torch.cuda.is_available():
+        pytest.skip("would launch")
+    wide = dict(B=65535, d=8, W=1, table_stride=1, ws_bytes=1 << 40)
+    assert attend(Hq=256, Hkv=256, **wide) == _lib.SSA_ERR_HIP  # 65,535 x 256 workgroups
+    assert attend(Hq=257, Hkv=257, **wide) == _lib.SSA_ERR_UNSUPPORTED
+    assert b"too many rows" in _lib.lib().ssa_last_error()
+    st = _lib.i64_array([0, 0, 0, 0] + [1 << 20] * 6)
+    ap = lambda T: status("ssa_paged_append", FAKE, FAKE, FAKE, FAKE, _lib.F32, T, 1,  # noqa: E731
+                          512, 10, 16, st, FAKE, None)
+    assert ap((1 << 25) - 2) == _lib.SSA_ERR_HIP  # 128 threads a token
+    assert ap(1 << 25) == _lib.SSA_ERR_UNSUPPORTED
+    assert b"tokens in one call" in _lib.lib().ssa_last_error()
+
+
 def test_append_and_resize_refuse():
     st = _lib.i64_array([128, 64, 128, 64, 2048, 1024, 64, 2048, 1024, 64])
     ap = lambda k, dt, T, d, page, s=st: status(  # noqa: E731
