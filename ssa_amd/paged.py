@@ -112,6 +112,15 @@ def _rows16(meta):
     return stride[-1] == 1 and all(s % vec == 0 for s in stride[:-1])
 
 
+def _given(out, tokens, B):
+    """Refuses an `out` of resize_pages that is not what a call of these sizes returns."""
+    if out.slots.dtype != torch.int64 or out.slots.shape != (tokens,) \
+            or not out.slots.is_contiguous():
+        raise ValueError(f"out.slots must be a contiguous ({tokens},) int64 tensor")
+    for name, n in (("pos", tokens), ("cu", B + 1), ("status", 1)):
+        _int32("out." + name, *_meta(getattr(out, name)), (n,))
+
+
 @functools.lru_cache(maxsize=1024)
 def _resize_plan(lens, new_lens, table, free, nfree):
     B, W, row = _table(*table)
@@ -153,8 +162,6 @@ def _attend_plan(q, kpool, vpool, table, lens, out, k_new, v_new, window):
     B, hq, _ = q[0]
     if q[2] != dtype:
         raise TypeError(f"q is {q[2]}, the cache holds {dtype}")
-    if (k_new is None) != (v_new is None):
-        raise ValueError("k_new and v_new come together")
     copy = not _rows16(q)
     new = (0, 0, 0, 0)
     if k_new is not None:
@@ -198,18 +205,20 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
     Resized; `out` takes an earlier one of the same sizes to write into. All or nothing: if the
     growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
     slots are -1 and status says why."""
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError(f"tokens={tokens}")
     if torch.compiler.is_compiling():
         from . import torch_ops as T
-        r = T.paged_resize(lens, new_lens, table, free, nfree, int(page), int(tokens))
+        if out is not None:
+            _given(out, tokens, lens.shape[0])
+        r = T.paged_resize(lens, new_lens, table, free, nfree, int(page), tokens)
         if out is not None:
             for to, x in zip(out, r):
                 to.copy_(x)
             return out
         return Resized(*r)
     _one_device(lens, new_lens, table, free, nfree)
-    tokens = int(tokens)
-    if tokens < 0:
-        raise ValueError(f"tokens={tokens}")
     B, W, row, pages = _resize_plan(_meta(lens), _meta(new_lens), _meta(table), _meta(free),
                                     _meta(nfree))
     if out is None:
@@ -220,11 +229,7 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
                       torch.empty(1, device=dev, dtype=torch.int32))
     else:
         _one_device(lens, *out)
-        if out.slots.dtype != torch.int64 or out.slots.shape != (tokens,) \
-                or not out.slots.is_contiguous():
-            raise ValueError(f"out.slots must be a contiguous ({tokens},) int64 tensor")
-        for name, n in (("pos", tokens), ("cu", B + 1), ("status", 1)):
-            _int32("out." + name, *_meta(getattr(out, name)), (n,))
+        _given(out, tokens, B)
     if B == 0:  # no requests, no new tokens
         out.slots.fill_(-1)
         for x in out[1:]:
@@ -283,8 +288,12 @@ def attend_pages(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tabl
     partial results can be joined. Under torch.compile `out` costs a copy."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new come together")
     if torch.compiler.is_compiling():
         from . import torch_ops as T
+        if out is not None and (out.dtype != q.dtype or out.shape != q.shape):
+            raise ValueError(f"out must be a {tuple(q.shape)} {q.dtype} tensor")
         if k_new is None:
             o, lse = T.paged_attend(q, kpool, vpool, table, lens, float(scale), int(window),
                                     status)

@@ -995,6 +995,38 @@ def test_compiled_step_equals_eager(cuda):
     assert all(torch.equal(state[0][x], state[1][x]) for x in state[0])
 
 
+def test_compiled_cache_equals_eager(cuda):
+    """PagedCache's own calls traced: a step that grows every request, one that is refused (the status kept
+    in place, nothing stored) and one into a given Resized."""
+    lens = [100, 33, 0]
+    q, a = make(cuda, torch.float16, lens, 4, 2, 64, 16, seed=4)
+    _, b = make(cuda, torch.float16, lens, 4, 2, 64, 16, seed=4)
+    spare = set(range(a.k.shape[1])) - set(a.table.flatten().tolist())
+    for c in (a, b):
+        c.free[:len(spare)] = int32(sorted(spare), cuda)
+        c.nfree.fill_(len(spare))
+    x = torch.randn(3, 2, 64, device=cuda).to(torch.float16)
+
+    def step(c, grow, x, out):
+        r = c.resize(c.lens + grow, 4, out)
+        return r, c.step(0, q, x, x, window=50)
+
+    held = b.status.data_ptr()
+    compiled = torch.compile(step, backend="aot_eager")
+    out = [None, None]
+    for i, grow in enumerate(([1, 1, 0], [0, 5, 0], [1, 1, 1], [1, 1, 0])):
+        grow = int32(grow, cuda)
+        r, want = step(a, grow, x, out[0])
+        rc, got = compiled(b, grow, x, out[1])
+        assert r.status.item() == rc.status.item() == b.status.item() == (-2 if i == 1 else 0)
+        assert b.status.data_ptr() == held and all(torch.equal(s, t) for s, t in zip(r, rc))
+        assert torch.equal(got.isnan(), want.isnan()) and want.isnan().all() == (i == 1)
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
+        assert torch.equal(a.lens, b.lens) and torch.equal(a.table, b.table)
+        assert torch.equal(a.k.view(torch.int16), b.k.view(torch.int16))
+        out = [r, rc] if i == 2 else [None, None]
+
+
 # ---- refusals -----------------------------------------------------------------------------------
 
 def test_arguments_are_refused(cuda):

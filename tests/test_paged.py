@@ -208,6 +208,37 @@ def test_registered_operators_give_shapes():
     assert ops.paged_append(new, new, pool, pool.clone(), slots[:3]) is None
 
 
+def test_compiled_calls_refuse_what_eager_ones_refuse(monkeypatch):
+    """A given `out` of another size or type is refused when traced too: copies into it would broadcast and
+    convert."""
+    monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    m = dict(device="meta")
+    i32 = lambda *n: torch.empty(n, dtype=torch.int32, **m)  # noqa: E731
+    q = torch.empty(2, 4, 64, dtype=torch.float16, **m)
+    pool = torch.empty(9, 2, 16, 64, dtype=torch.float16, **m)
+    lens, table, free, nfree = i32(2), i32(2, 4), i32(9), i32(1)
+    resize = lambda n, out: P.resize_pages(lens, lens.clone(), table, free, nfree, 16,  # noqa: E731
+                                           n, out)
+    good = [torch.empty(1, dtype=torch.int64, **m), i32(1), i32(3), i32(1)]
+    assert resize(1, P.Resized(*good)).slots is good[0]
+    for i, bad in ((0, torch.empty(5, dtype=torch.int64, **m)), (0, i32(1)), (1, i32(4)),
+                   (2, i32(4)), (2, torch.empty(3, **m)), (3, i32(2))):
+        with pytest.raises((ValueError, TypeError)):
+            resize(1, P.Resized(*good[:i], bad, *good[i + 1:]))
+    with pytest.raises(ValueError, match="tokens=-1"):
+        resize(-1, None)
+    new = torch.empty(2, 2, 64, dtype=torch.float16, **m)
+    for kw in ({}, dict(k_new=new, v_new=new)):
+        out = torch.empty_like(q)
+        assert P.attend_pages(q, pool, pool.clone(), table, lens, out=out, **kw) is out
+        for bad in (q.float(), torch.empty(3, 2, 4, 64, dtype=q.dtype, **m)):
+            with pytest.raises(ValueError, match="out must be"):
+                P.attend_pages(q, pool, pool.clone(), table, lens, out=bad, **kw)
+        for k, v in ((new, None), (None, new)):
+            with pytest.raises(ValueError, match="come together"):
+                P.attend_pages(q, pool, pool.clone(), table, lens, k_new=k, v_new=v)
+
+
 def test_plain_state_keeps_every_page_once():
     import random
     rng = random.Random(0)
