@@ -491,7 +491,9 @@ int ssa_masked_attn_bwd(const void* q, const void* k, const void* v, const void*
  *   last. *status: 0; or nothing was changed (cu all 0, slots all -1): the number of pages lacking,
  *   -1 (a length outside [0, W * page], or counts that do not fit the pool), -2 (more than T new
  *   tokens). Pages given back in a call can be taken from the next call on. The table's entries of
- *   different requests must not overlap in memory; new_lens may be lens itself.
+ *   different requests must not overlap in memory; new_lens may be lens itself. A page given back is
+ *   free, whichever other rows list it: a request that shares pages may shrink to the length of these,
+ *   and below it only as their last holder.
  * ssa_paged_append: keys and values k, v (T, Hkv, d) of new tokens into the pools at slots (T) int64
  *   (distinct; rows whose slot lies outside the pool are skipped), fewer than 64 GiB of keys a call.
  *   strides[10] = k(t,h), v(t,h), kpool(page,head,slot), vpool(page,head,slot).

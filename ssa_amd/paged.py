@@ -204,7 +204,12 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
     tokens: room for the new tokens (at least the sum of the growths; more is padding). Returns a
     Resized; `out` takes an earlier one of the same sizes to write into. All or nothing: if the
     growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
-    slots are -1 and status says why."""
+    slots are -1 and status says why.
+
+    A page given back is free: nothing counts how many rows list it. Pages that requests share (a common
+    prefix, set by the caller in their table rows and lengths; attend_pages reads them as any others) go
+    back once, by the last request that holds them. Any other is brought to the length of its shared
+    pages here, which gives back its own, and taken out by the caller: its row to -1, its length to 0."""
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens={tokens}")
@@ -347,8 +352,8 @@ class PagedCache:
         cache.append(layer, k, v, r.slots)                # a prompt's tokens, or
         o = cache.step(layer, q, k_new, v_new)            # one token of every request
 
-    A request ends by a resize to length 0; q, k_new and v_new have a row for every request, idle ones
-    included. After a resize that did not fit, append and step store nothing and attend and step give
+    A request ends by a resize to length 0 (one that shares pages: as resize_pages says); q, k_new and
+    v_new have a row for every request, idle ones included. After a resize that did not fit, append and step store nothing and attend and step give
     NaN, until a resize fits; `check` raises then (it synchronises; a caller that keeps count of the
     pages need not call it)."""
 

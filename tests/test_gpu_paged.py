@@ -788,6 +788,48 @@ def test_prompts_then_steps_then_ends(cuda, dtype, token_major):
         step()
 
 
+def test_requests_that_share_a_prefix(cuda):
+    """A prefix of two pages held by three requests, as resize_pages describes: they grow on pages of their
+    own, attend the shared ones, end one by one, and every page is free exactly once at the end."""
+    page, hkv, d = 16, 2, 64
+    g = torch.Generator(device=cuda).manual_seed(2)
+    cache = P.PagedCache(3, 200, 14, hkv, d, page=page, dtype=torch.float16, device=cuda)
+    x = torch.randn(32, hkv, d, device=cuda, generator=g).to(torch.float16)
+    r = cache.resize(int32([32, 0, 0], cuda), 32)
+    cache.append(0, x, x, r.slots)
+    for b in (1, 2):  # the caller's part
+        cache.table[b, :2] = cache.table[0, :2]
+        cache.lens[b] = 32
+    y = torch.randn(40, hkv, d, device=cuda, generator=g).to(torch.float16)
+    r = cache.resize(int32([37, 50, 32 + 17], cuda), 40)
+    cache.check()
+    cache.append(0, y, y, r.slots)
+    q = torch.randn(3, 4, d, device=cuda, generator=g).to(torch.float16)
+    new = torch.randn(3, hkv, d, device=cuda, generator=g).to(torch.float16)
+    cache.resize(cache.lens + 1, 3)
+    shared = cache.table[0, :2].tolist()
+    out = cache.step(0, q, new, new)
+    cu = [0, 5, 23, 40]
+    for b in range(3):
+        own = torch.cat([x, y[cu[b]:cu[b + 1]], new[b:b + 1]]).transpose(0, 1)[None]
+        want, _, tol, _ = U.attend(q[b:b + 1], own, own, torch.tensor([[0]]),
+                                   torch.tensor([own.shape[2]]), 1 / math.sqrt(d))
+        U.close(out[b:b + 1], want, tol)
+    for b in (1, 0):
+        new_lens = cache.lens.clone()
+        new_lens[b] = 32  # its own pages back
+        cache.resize(new_lens, 0)
+        cache.check()
+        cache.table[b, :2] = -1  # the caller's part again
+        cache.lens[b] = 0
+    held = cache.table[2, :4].tolist()
+    assert held[:2] == shared and cache.nfree.item() == 10
+    assert sorted(cache.free[:10].tolist() + held) == list(range(14))
+    cache.resize(torch.zeros_like(cache.lens), 0)  # the last holder
+    cache.check()
+    assert sorted(cache.free.tolist()) == list(range(14)) and (cache.table == -1).all()
+
+
 def test_refused_resize_stores_nothing(cuda):
     """After a resize that did not fit, step and append leave the cache as it is and the rows are NaN."""
     cache = P.PagedCache(3, 100, 6, 2, 64, page=16, dtype=torch.float16, device=cuda)
