@@ -377,7 +377,8 @@ class PagedCache:
         self.lens = torch.zeros(requests, **i32)
         self.free = torch.arange(pages, **i32).flip(0).contiguous()  # page 0 on top
         self.nfree = torch.full((1,), pages, **i32)
-        self.status = torch.zeros(1, **i32)
+        with torch.inference_mode(False):  # torch writes it, inside and outside inference mode
+            self.status = torch.zeros(1, **i32)
 
     @torch.no_grad()
     def resize(self, new_lens: torch.Tensor, tokens: int, out: Resized | None = None) -> Resized:

@@ -146,6 +146,22 @@ def test_cache_keeps_its_tensors(monkeypatch):
     a.check()
 
 
+@pytest.mark.parametrize("made", [False, True])
+@pytest.mark.parametrize("used", [False, True])
+def test_cache_in_and_out_of_inference_mode(monkeypatch, made, used):
+    i32 = lambda n: torch.full((n,), 3, dtype=torch.int32)  # noqa: E731
+    monkeypatch.setattr(P, "resize_pages",
+                        lambda *a: a[7] or P.Resized(i32(5).long(), i32(5), i32(3), i32(1)))
+    with torch.inference_mode(made):
+        cache = P.PagedCache(2, 40, 9, 1, 8, page=16, device="cpu")
+        given = P.Resized(i32(5).long(), i32(5), i32(3), i32(1))
+    with torch.inference_mode(used):
+        for out in (None, given):
+            cache.status.zero_()
+            cache.resize(cache.lens, 5, out)
+            assert cache.status.item() == 3
+
+
 @pytest.mark.parametrize("tokens,given", [(0, False), (3, False), (3, True)])
 def test_resize_of_no_requests(monkeypatch, tokens, given):
     """An empty batch is resized as it is appended and attended: nothing changes, every slot is padding."""
