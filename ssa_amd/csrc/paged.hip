@@ -428,7 +428,11 @@ __device__ inline int64_t row_cap(const AttendParams& p) {
 }
 
 // Finds item `index` from the lengths alone, each wave for itself: every lane sums a run of
-// requests, the wave adds the runs up. False past the last item.
+// requests, the wave adds the runs up. False past the last item. Up to 64 requests the lengths are one
+// load; past that the time grows with the square of the batch, as every workgroup reads all lengths: 256
+// requests of 20 to 200 keys in a table 4,096 tokens wide 16 us, 1,024 65, 4,096 600, 16,384 7.8 ms (in a
+// table of 208, an item per request: 7, 17, 61, 233 us); 1,024 of 500 to 1,500 keys 135 us and 97, 4,096
+// of these 880 and 350.
 __device__ inline bool find_item(const AttendParams& p, int index, Item& it) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = row_cap(p);
@@ -636,8 +640,8 @@ constexpr int kAttendWaves = 4;
 // byte permutes: no LDS, no transposed copy. Bound by the reading of K and V: a wave's next keys are in
 // flight while it weighs the current values and the other way round; 16 lanes of 16 heads serve
 // any group of query heads, as the matrix units wait for memory anyway. 1,048,577 tokens (bf16, 14 / 2
-// heads of 64) 92 us with the join, 5.8 TB/s; a kernel that only reads as much takes 97 without the
-// non-temporal hint. Equal shares that run on over several requests cost every short call 1 us or more
+// heads of 64) 92 us with the join, 5.8 TB/s; a kernel that only reads as much takes 96 without the
+// non-temporal hint and 88 with it. Equal shares that run on over several requests cost every short call 1 us or more
 // for 2 % of a mixed batch. MT: tiles of 16 query heads served by one reading. ACROSS: the waves take
 // a key head each, over all of the item's tiles.
 template <int DT, int DP, int MT, bool ACROSS, int WPE>
@@ -791,7 +795,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_attend_kernel(At
     // scores: lane column a head, rows the keys 4 grp + r of each subtile
     // fp32 adds its products in kChains chains: against 64 bits one over the whole head left up to
     // 3.1 times the error of the same in plain operations, four 1.3 times at most, for 1.5% more
-    // time or less (eight requests of up to 16K keys, 106.4 -> 107.9 us). At 64 columns two are as
+    // time or less (eight requests of up to 16K keys, 106.4 -> 107.9 us, on another box 110.3 -> 110.6). At 64 columns two are as
     // short, and four spilled.
     constexpr int kChains = DT != SSA_F32 ? 1 : DP == 64 ? 2 : 4;
     f32x4 s[MT][NT], chain[MT][NT][kChains];
@@ -1106,20 +1110,23 @@ int64_t unit_bytes(int dtype, int64_t d, int64_t Hkv) {
 // Whether a call is one launch, a request an item: no request passes 512 keys (8 us a call; parts and
 // their join 11), or 2048 in 512 or more (request, key head, row tile) triples (256 x 1,000 keys, 4 key
 // heads: 48 us; cut 60). With few triples and more keys the cut wins: 2,000 keys of 8 heads 12 and 24.
+// What a request may reach counts, the table's width, as the lengths are the device's: 64 requests of 100
+// to 500 keys (8 key heads of 128) 18.8 us in a table of 496, 24.6 in one of 32,768; of 2 heads of 64 7.7
+// and 10.1.
 bool one_launch(int64_t triples, int64_t units) {
   return units <= 4 || (units <= 16 && triples >= 512);
 }
 
 // Whether a wave serves two tiles of 16 query heads from one reading of the keys and values (past head
 // dim 128 their registers do not fit). It makes fewer, longer workgroups: 16-bit calls that may read
-// more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 76 us
-// for 83; 64 of 2,000 to 20,000, 48 on two: 122 for 137), smaller ones lose (64 of 500 to 4,000, 32 on
+// more than the caches hold win (128 requests of 2,000 to 9,000 keys, 20 heads of 128 on one: 77 us
+// for 84; 64 of 2,000 to 20,000, 48 on two: 124 for 137), smaller ones lose (64 of 500 to 4,000, 32 on
 // one: 23 for 19); in fp32 the matrix products count too (8 of 2,000 to 9,000, 40 on two: 26 for 31).
 //
 // A workgroup's waves take a key head each instead of a run of keys each where a token's heads lie side
 // by side (token-major pools): four rows of 128 or 256 bytes are then read at about the same time, one at
 // a time leaves memory at 5.4 TB/s of 6.1: 64 requests of 64 to 32,768 keys (8 heads of 128, 16-bit)
-// 236 us for 256, 16 of 8,192 100 for 113 (of head dim 64 55 for 67). Longer rows gain nothing (fp32 63 for
+// 235 us for 250, 16 of 8,192 100 for 114 (of head dim 64 55 for 67). Longer rows gain nothing (fp32 63 for
 // 61), heads that lie apart lose (235 for 219), and so do calls of little to read, whose waves then have
 // four tiles each to begin with (one of 4,096 keys 15 for 13; one of 32,768 33 for 30).
 constexpr int64_t kAcrossBytes = (int64_t)32 << 20;
@@ -1349,7 +1356,7 @@ extern "C" int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* o
   p.div = page_div((int)page / 16);
   p.RT = (int)y.RT;
   p.items = (int)y.items;
-  // What does not fit the 256 MB last-level cache is read past it: 537 MB 91 us with the hint, 101
+  // What does not fit the 256 MB last-level cache is read past it: 537 MB 94 us with the hint, 102
   // without; 105 MB that the cache holds 30 and 27. Row tiles read it twice, the second time from L2:
   // 300 MB with two of them 110 us with the hint, 83 without.
   p.stream_units = y.RT > 1 ? INT64_MAX : kStreamBytes / unit_bytes(dtype, d, Hkv);
