@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define SSA_ABI_VERSION 8
+#define SSA_ABI_VERSION 9
 
 typedef void* ssa_stream_t; /* hipStream_t */
 
@@ -529,6 +529,81 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
                      const void* k_new, const void* v_new, const int64_t* strides, float scale,
                      int64_t window, const int32_t* status, void* workspace,
                      size_t workspace_bytes, ssa_stream_t stream);
+
+/*
+ * Drafted tokens over the paged cache: several new tokens of every request, each attending the context
+ * and some of the others (a tree that one step of the model verifies, a chain, the next piece of a
+ * prompt). Request b's are rows [cu[b], cu[b + 1]) of N (cu (B + 1) int32, as ssa_paged_resize writes
+ * it) and, stored by ssa_paged_append, the last n = cu[b + 1] - cu[b] of its lens[b] tokens in the
+ * cache; ctx = lens[b] - n are before them. What does not fit is found on the device: offsets that
+ * descend or pass N make a request none, 0 <= n <= lens[b] <= W * page and n <= 32 * words must hold.
+ *
+ * ssa_paged_draft_masks: parents (N) int32, of each drafted token the place of the one it continues
+ *   among its request's (less than its own), or -1 for the context. masks (N, words) int32, words 1 to
+ *   32: bit i % 32 of word i / 32 says that the token attends drafted token i: itself and its
+ *   ancestors; pos (N) int32: its position, ctx + the ancestors. Of a token with a parent that does not
+ *   fit, of those that continue it and of requests that do not fit: 0 and -1; of rows behind the last
+ *   request's: 0 and 0.
+ * ssa_paged_attend_drafts: q, out (N, Hq, d). Row t of request b attends the keys j < ctx and the
+ *   drafted ones of its mask (masks (N, words), pos (N), or all NULL with words 0: the drafted tokens
+ *   up to itself, one after the other from position ctx on); with a window only those at positions past
+ *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, precision, head
+ *   layout, lse (N, Hq), status, page ids and strides as ssa_paged_attend. A row that attends nothing:
+ *   out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request that does
+ *   not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
+ *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
+ *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq / 4 workgroups or more than 2^24 are
+ *   refused. Workspace: ssa_paged_attend_drafts_workspace_size bytes, 16-byte aligned, nothing in it
+ *   needs to be set.
+ * ssa_paged_keep: moves the accepted drafted tokens together: drafted token path[b][i] of request b to
+ *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
+ *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the
+ *   resize that gives back the pages behind; -1, and nothing moved, where a path, a count, the lengths
+ *   or a page id do not fit. strides[8] = kpool(layer,page,head,slot), vpool(layer,page,head,slot).
+ *
+ * Requests that share pages:
+ * ssa_paged_fork: row b of the table becomes the first new_lens[b] tokens of what row src[b] was (src,
+ *   new_lens (B) int32; src NULL: row b; 0 tokens: an empty row, whatever src): a fork, a prefix shared, beams
+ *   reordered; with src[b] = b a request cut short or ended. Whole pages are listed by both. A last,
+ *   partly filled page that another row lists too is taken anew, so that every row can grow by
+ *   ssa_paged_resize: source[b], target[b], tokens[b] (B) say what ssa_paged_copy has to copy (-1, -1, 0
+ *   where nothing); the lowest row keeps the page if no row lists it whole. With r such rows before it
+ *   (rows in order) the page is free_pages[*nfree - 1 - r]. Pages that no row lists any more are given
+ *   back as ssa_paged_resize does, each by the lowest row that listed it; forking and ending the forks
+ *   restores the stack. *status: 0; or nothing was changed (source, target -1): the number of pages
+ *   lacking, or -1 (a length, a row, a held page id or a count that does not fit). Workspace:
+ *   ssa_paged_fork_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
+ * ssa_paged_copy: the first tokens[i] (NULL: all) tokens of page source[i] to page target[i], i < n, in
+ *   every layer, keys and values. Pairs with an id outside the pool are skipped; a target is listed once
+ *   and is nobody's source. strides as ssa_paged_keep.
+ */
+int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu, const int32_t* lens, int64_t B,
+                          int64_t N, int64_t words, int32_t* masks, int32_t* pos,
+                          ssa_stream_t stream);
+size_t ssa_paged_attend_drafts_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+                                              int64_t d, int64_t W, int64_t page, int64_t window);
+int ssa_paged_attend_drafts(const void* q, const void* kpool, const void* vpool, void* out,
+                            float* lse, int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+                            int64_t d, int64_t pages, int64_t page, const int32_t* table,
+                            int64_t table_stride, int64_t W, const int32_t* lens,
+                            const int32_t* cu, const int32_t* masks, const int32_t* pos,
+                            int64_t words, const int64_t* strides, float scale, int64_t window,
+                            const int32_t* status, int clear_rest, void* workspace,
+                            size_t workspace_bytes, ssa_stream_t stream);
+int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv, int64_t d,
+                   int64_t pages, int64_t page, const int64_t* strides, const int32_t* table,
+                   int64_t table_stride, int64_t W, const int32_t* lens, const int32_t* cu,
+                   int64_t B, const int32_t* path, int64_t path_stride, int64_t width,
+                   const int32_t* counts, int32_t* new_lens, ssa_stream_t stream);
+size_t ssa_paged_fork_workspace_size(int64_t B, int64_t W, int64_t pages);
+int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32_t* lens, int32_t* table,
+                   int64_t table_stride, int64_t B, int64_t W, int64_t page, int32_t* free_pages,
+                   int64_t pages, int32_t* nfree, int32_t* source, int32_t* target,
+                   int32_t* tokens, int32_t* status, void* workspace, size_t workspace_bytes,
+                   ssa_stream_t stream);
+int ssa_paged_copy(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv, int64_t d,
+                   int64_t pages, int64_t page, const int64_t* strides, const int32_t* source,
+                   const int32_t* target, const int32_t* tokens, int64_t n, ssa_stream_t stream);
 
 #ifdef __cplusplus
 }

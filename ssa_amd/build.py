@@ -21,7 +21,7 @@ LIB = PKG / "libssa_hip.so"
 ARCH = "gfx950"
 
 SOURCES = ["abi.hip", "summary.hip", "route.hip", "attn.hip", "decode.hip", "swap.hip", "ivf.hip",
-           "tree.hip", "ccc.hip", "paged.hip"]
+           "tree.hip", "ccc.hip", "paged.hip", "paged_drafts.hip", "paged_fork.hip"]
 
 
 def hipcc() -> str:

@@ -1,0 +1,1144 @@
+// Drafted tokens over the paged key-value cache: their masks and positions from their parents, their
+// attention over the cache (every one over the context and its own ancestors), and the accepted ones
+// moved together.
+//
+// Request b's drafted tokens are rows [cu[b], cu[b + 1]) of a call's N and the last n = cu[b + 1] -
+// cu[b] of its lens[b] tokens of the cache.
+#include <float.h>
+
+#include <algorithm>
+
+#include "paged_parts.h"
+
+namespace ssa {
+namespace {
+
+constexpr int kMaxWords = 32;  // of a mask: 1024 drafted tokens a request
+
+// ---- parents -> masks, positions ---------------------------------------------------------------
+
+struct MaskParams {
+  const int32_t* parents;
+  const int32_t* cu;
+  const int32_t* lens;
+  int32_t* masks;
+  int32_t* pos;
+  int64_t N;
+  int B, words;
+};
+
+// A token's way up so far: the next ancestor's place plus 1 (0: none), the tokens on the way, and
+// whether one of them has a parent that does not fit.
+__device__ inline unsigned int way(int anc, int steps, bool bad) {
+  return (unsigned)(anc + 1) | (unsigned)steps << 16 | (bad ? 1u << 31 : 0);
+}
+
+// A workgroup for a request and four words of its masks, a thread a token. Every round joins a token's
+// way with that of the ancestor where it ends, so its length doubles: a chain of 1024 takes ten rounds.
+// The last workgroups clear the rows behind the last token. Bound by launch and barrier latency.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_draft_masks_kernel(MaskParams p) {
+  __shared__ unsigned int ways[THREADS];
+  __shared__ u32x4 seen[THREADS];
+  const int b = blockIdx.x, t = threadIdx.x, w0 = blockIdx.y * 4;
+  const int count = min(4, p.words - w0);
+  auto store = [&](int64_t row, const u32x4& m, int pos) {
+    for (int i = 0; i < count; ++i) p.masks[row * p.words + w0 + i] = m[i];
+    if (w0 == 0) p.pos[row] = pos;
+  };
+  if (b == p.B) {
+    const int end = p.cu[p.B];
+    for (int64_t row = max(end, 0) + t; row < p.N; row += THREADS) store(row, u32x4{}, 0);
+    return;
+  }
+  const int c0 = p.cu[b];
+  const DraftSpan s = draft_span(p.lens[b], c0, p.cu[b + 1], p.N, 0, p.words, 0x7fffffff);
+  if (!s.span.ok) {
+    for (int i = t; i < s.n; i += THREADS) store((int64_t)c0 + i, u32x4{}, -1);
+    return;
+  }
+  const bool mine = t < s.n;
+  const int parent = mine ? p.parents[(int64_t)c0 + t] : -1;
+  const bool bad = parent < -1 || parent >= t;
+  unsigned int own = way(bad ? -1 : parent, 1, mine && bad);
+  u32x4 m{};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = t >> 5 == w0 + i ? 1u << (t & 31) : 0;
+  ways[t] = own;
+  seen[t] = m;
+  while (__syncthreads_or((own & 0xffff) != 0)) {
+    const int at = (int)(own & 0xffff) - 1;
+    if (at >= 0) {
+      const unsigned int up = ways[at];
+      m |= seen[at];
+      own = (up & 0xffff) | (own & 0x7fff0000u) + (up & 0x7fff0000u) | ((own | up) & 1u << 31);
+    }
+    __syncthreads();
+    ways[t] = own;
+    seen[t] = m;
+  }
+  if (!mine) return;
+  const bool fits = own >> 31 == 0;
+  store((int64_t)c0 + t, fits ? m : u32x4{}, fits ? s.ctx + (int)(own >> 16 & 0x7fff) - 1 : -1);
+}
+
+// ---- attention of drafted tokens ---------------------------------------------------------------
+
+struct DraftParams {
+  const char* q;
+  const char* kpool;
+  const char* vpool;
+  char* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  const int32_t* masks;   // NULL: a chain
+  const int32_t* pos;
+  const int32_t* status;  // of the resize before, or NULL
+  int64_t table_stride, cap, pages, N;
+  int B, Hq, Hkv, G, d, page, window, words;
+  bool clear;  // rows behind the last token become zeros
+  float scale_log2;
+  int64_t qt, qh, ot, oh;                // elements
+  int64_t kpp, kph, kps, vpp, vph, vps;  // elements
+  PageDiv div;           // by the subtiles of a page
+  int64_t stream_units;  // units of a key head from which a call streams
+  int64_t items;         // items aimed at, 0: no row tile is cut
+  int64_t blocks;        // workgroups for row tiles; kRestBlocks more follow
+  int64_t max_parts;     // row tiles of parts that the workspace holds
+  float* part;           // (part, row of the tile, DP)
+  float* part_ml;        // (part, row of the tile, 2): their m and l
+  int32_t* info;         // per request: its first part and the splits of its row tiles
+};
+
+constexpr int kRestBlocks = 8;
+
+// What one workgroup does: split j of n of a row tile of request b and key head g.
+struct DraftItem {
+  int b, g, tile, tiles, j, n, begin, end, first_part, c0;
+  bool stream;
+  DraftSpan s;
+};
+
+__device__ inline DraftSpan draft_of(const DraftParams& p, int b) {
+  return draft_span(p.lens[b], p.cu[b], p.cu[b + 1], p.N, p.window, p.words, p.cap);
+}
+
+// Finds workgroup `id`'s item from the lengths alone, each wave for itself: every lane sums a run of
+// requests, the wave adds the runs up. Of the call's row tiles an XCD takes a run, the tiles of the
+// same keys next to each other: its L2 serves them together. False past the last one.
+template <int M>
+__device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
+  const int lane = threadIdx.x & 63;
+  const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
+  DraftSpan own{};
+  int units = 0;
+  int64_t tiles = 0, work = 0;
+  for (int b = b0; b < b1; ++b) {
+    own = draft_of(p, b);
+    units = draft_units(own);
+    tiles = draft_tiles(own, p.G, M);
+    work += tiles * units;
+  }
+  int chunk = 0x7fffffff;
+  it.stream = p.stream_units == 0;
+  if (p.items != 0) {
+    const int64_t all = lane_sums(work).all;
+    chunk = draft_chunk(all, p.items);
+    it.stream = all >= p.stream_units;
+  }
+  int64_t n = 0, parts = 0;
+  auto count = [&](int64_t of, int u) {
+    const int splits = paged_items(u, chunk);
+    n += of * splits;
+    parts += splits > 1 ? of * splits : 0;
+    return splits;
+  };
+  if (run == 1) {
+    count(tiles, units);
+  } else {
+    for (int b = b0; b < b1; ++b) {
+      const DraftSpan s = draft_of(p, b);
+      count(draft_tiles(s, p.G, M), draft_units(s));
+    }
+  }
+  const LaneSums<int64_t> sums = lane_sums(n);
+  const int64_t all = sums.all * p.Hkv, per = (all + 7) / 8, index = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || index >= all) return false;
+  const unsigned long long past = __ballot(sums.upto * p.Hkv > index);
+  if (past == 0) return false;
+  const int owner = __builtin_ctzll(past);
+  const LaneSums<int64_t> part_sums = lane_sums(parts);
+  auto pick = [&](int64_t x) {
+    const unsigned int lo = __builtin_amdgcn_readlane((unsigned int)x, owner);
+    const unsigned int hi = __builtin_amdgcn_readlane((unsigned int)(x >> 32), owner);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+  };
+  int64_t first = pick(sums.upto - n), part = pick(part_sums.upto - parts);
+  it.b = owner * run;
+  for (;; ++it.b) {
+    it.s = draft_of(p, it.b);
+    units = draft_units(it.s);
+    tiles = draft_tiles(it.s, p.G, M);
+    it.n = paged_items(units, chunk);
+    if (run == 1 || index < (first + tiles * it.n) * p.Hkv) break;
+    first += tiles * it.n;
+    part += it.n > 1 ? tiles * it.n : 0;
+  }
+  it.c0 = p.cu[it.b];
+  it.tiles = (int)tiles;
+  const int64_t at = index - first * p.Hkv, row = at / tiles;
+  it.tile = (int)(at - row * tiles);
+  it.j = (int)(row / p.Hkv);
+  it.g = (int)(row - (int64_t)it.j * p.Hkv);
+  it.stream = it.stream && it.tiles == 1;
+  // parts that the workspace does not hold (offsets that do not ascend): the join answers
+  part *= p.Hkv;
+  it.first_part = it.n > 1 && part + tiles * it.n * p.Hkv > p.max_parts ? -1 : (int)part;
+  it.begin = it.end = 0;
+  if (it.s.span.ok) {
+    const PagedRange r = paged_item_range(it.s.span, units, it.j, it.n);
+    it.begin = r.begin;
+    it.end = r.end;
+  }
+  return true;
+}
+
+__device__ inline DraftItem uniform(const DraftItem& x) {
+  return DraftItem{uniform(x.b),     uniform(x.g),   uniform(x.tile), uniform(x.tiles),
+                   uniform(x.j),     uniform(x.n),   uniform(x.begin), uniform(x.end),
+                   uniform(x.first_part), uniform(x.c0), uniform((int)x.stream) != 0,
+                   DraftSpan{uniform(x.s.ctx), uniform(x.s.n),
+                             PagedSpan{uniform(x.s.span.first), uniform(x.s.span.len),
+                                       uniform((int)x.s.span.ok) != 0}}};
+}
+
+// Rows that no request holds: zeros where the call wants them cleared; every row NaN after a refused
+// resize. Block `id` of kRestBlocks.
+template <int DT>
+__device__ inline void rest_rows(const DraftParams& p, int id) {
+  constexpr int ES = DT == SSA_F32 ? 4 : 2;
+  const bool refused = p.status && *p.status != 0;
+  if (!refused && !p.clear) return;
+  const int per = p.d * ES / 16;
+  const float x = refused ? NAN : 0.0f;
+  const int64_t first = refused ? 0 : max(p.cu[p.B], 0), rows = (p.N - first) * p.Hq;
+  for (int64_t i = id * 256 + (int)threadIdx.x; i < rows * per; i += kRestBlocks * 256) {
+    const int64_t row = i / per, t = first + row / p.Hq, h = row % p.Hq;
+    const int64_t to = t * p.ot + h * p.oh + (i - row * per) * (16 / ES);
+    const f32x4 v = {x, x, x, x};
+    store_row4<DT>(p.out, to, v);
+    if constexpr (ES == 2) store_row4<DT>(p.out, to + 4, v);
+    if (p.lse && i == row * per) p.lse[t * p.Hq + h] = refused ? NAN : -INFINITY;
+  }
+}
+
+// The value a row's sums give: m -INFINITY: no key is attended; l NaN: the row is answered as bad.
+__device__ inline float row_scale(float m, float l) {
+  return l != l ? NAN : m == -INFINITY ? 0.0f : 1.0f / l;
+}
+
+__device__ inline float row_lse(float m, float l, float shift) {
+  return l != l ? NAN : m == -INFINITY ? -INFINITY
+                                       : (m - shift + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Whether a 16-bit (two a word) or 32-bit value is infinite or NaN.
+template <int DT>
+__device__ inline bool not_finite(unsigned int w) {
+  if constexpr (DT == SSA_F32) return (w & 0x7f800000u) == 0x7f800000u;
+  constexpr unsigned int e = DT == SSA_BF16 ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w & e << 16) == e << 16;
+}
+
+// The value with what is infinite or NaN made zero.
+template <int DT>
+__device__ inline unsigned int finite_part(unsigned int w) {
+  if constexpr (DT == SSA_F32) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+  constexpr unsigned int e = DT == SSA_BF16 ? 0x7f80u : 0x7c00u;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w & e << 16) == e << 16) w &= 0xffffu;
+  return w;
+}
+
+// What is not finite in the value as a number of the type: 1 for +inf, 2^8 for -inf, 2^15 for NaN, 0.
+template <int DT>
+__device__ inline unsigned int kind_of(unsigned int w) {
+  if constexpr (DT == SSA_F32) {
+    const unsigned int x = w & 0x7fffffffu;
+    return x < 0x7f800000u ? 0u : x > 0x7f800000u ? 0x47000000u : w >> 31 ? 0x43800000u : 0x3f800000u;
+  } else {
+    constexpr unsigned int e = DT == SSA_BF16 ? 0x7f80u : 0x7c00u;
+    constexpr unsigned int pos = DT == SSA_BF16 ? 0x3f80u : 0x3c00u;
+    constexpr unsigned int neg = DT == SSA_BF16 ? 0x4380u : 0x5c00u;
+    constexpr unsigned int nan = DT == SSA_BF16 ? 0x4700u : 0x7800u;
+    auto half = [&](unsigned int h) {
+      const unsigned int x = h & 0x7fffu;
+      return x < e ? 0u : x > e ? nan : h >> 15 ? neg : pos;
+    };
+    return half(w & 0xffffu) | half(w >> 16) << 16;
+  }
+}
+
+// Zeros and ones as two 16-bit numbers.
+template <int DT>
+__device__ inline unsigned int pack16(float a, float b) {
+  constexpr unsigned int one = DT == SSA_BF16 ? 0x3f80u : 0x3c00u;
+  return (a != 0.0f ? one : 0u) | (b != 0.0f ? one << 16 : 0u);
+}
+
+// Attention of a row tile (MT times 16 rows, a row a drafted token's query head of the key head) over
+// an item's keys, its tiles of keys in four runs, one a wave; the layout of products and loads is
+// paged_attend_kernel's, a row where that has a head. Tiles of keys that some row does not attend (the
+// drafted ones, the last, a window's first) take their masks from the rows' words; their lowest score
+// -FLT_MAX stands for attended keys, so that -INFINITY means a row without any. A value that is infinite
+// or NaN there would reach the rows that do not attend it as 0 x infinity: such values are taken out of
+// the product and added to the rows that attend them.
+template <int DT, int DP, int MT, int WPE>
+__global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(DraftParams p) {
+  using T = Tile<DT, DP>;
+  constexpr int NT = T::NT, NC = T::NC, VB = T::VB, LC = T::LC, LW = T::LW, NA = T::NA;
+  constexpr int NW = kAttendWaves, NR = NW / 2, M = MT * 16;
+  __shared__ f32x4 red[NR][MT][NA][64];
+  __shared__ float red_m[NR][MT][64], red_l[NR][MT][64];
+  const int wv = uniform(threadIdx.x >> 6);
+  if (blockIdx.x >= p.blocks) {
+    rest_rows<DT>(p, (int)(blockIdx.x - p.blocks));
+    return;
+  }
+  if (p.status && *p.status != 0) return;
+  DraftItem found;
+  if (!find_draft<M>(p, blockIdx.x, found)) return;
+  const DraftItem it = uniform(found);
+  const int ctx = it.s.ctx, n = it.s.n, first = it.s.span.first, len = it.s.span.len;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const int tiles = (it.end - it.begin + NT - 1) / NT;
+  const int i0 = uniform((int)((int64_t)tiles * wv / NW));
+  const int i1 = uniform((int)((int64_t)tiles * (wv + 1) / NW));
+
+  // this lane's rows: drafted token, head, position and first key; past the last row the last again
+  int tok[MT], head[MT], rpos[MT], start[MT];
+  bool real[MT];
+  int late = 0;  // the latest first key of the tile's rows
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int64_t x = (int64_t)it.tile * M + mt * 16 + col;
+    const int t = (int)(x / p.G);
+    real[mt] = t < n;
+    tok[mt] = min(t, n - 1);
+    head[mt] = it.g * p.G + (int)(x - (int64_t)t * p.G);
+    rpos[mt] = !p.masks ? ctx + tok[mt] : p.pos[(int64_t)it.c0 + tok[mt]];
+    start[mt] = p.window > 0 && rpos[mt] >= p.window ? rpos[mt] - p.window + 1 : 0;
+    late = max(late, start[mt]);
+  }
+  if (p.window > 0) {
+    late = max(late, lane_xor(late, 1));
+    late = max(late, lane_xor(late, 2));
+    late = max(late, lane_xor(late, 4));
+    late = max(late, lane_xor(late, 8));
+  }
+  late = uniform(late);
+
+  __shared__ u32x4 q_lds[T::kQInLds ? MT : 1][T::kQInLds ? NC : 1][64];
+  u32x4 q[MT][T::kQInLds ? 1 : NC];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (T::kQInLds && c % NW != wv) continue;
+      const int at = c * 64 + grp * 16;
+      u32x4 x = {0, 0, 0, 0};
+      if (real[mt] && at < p.d * T::ES)
+        x = *(const u32x4*)(p.q + (((int64_t)it.c0 + tok[mt]) * p.qt + head[mt] * p.qh) * T::ES + at);
+      if constexpr (T::kQInLds) q_lds[mt][c][lane] = x;
+      else q[mt][c] = x;
+    }
+  if constexpr (T::kQInLds) __syncthreads();
+
+  const char* const kbase = p.kpool + it.g * p.kph * T::ES;
+  const char* const vbase = p.vpool + it.g * p.vph * T::ES;
+  const int64_t kpp = p.kpp * T::ES, vpp = p.vpp * T::ES;
+  const int kps = (int)p.kps * T::ES, vps = (int)p.vps * T::ES, row_bytes = p.d * T::ES;
+
+  const int koff = col * kps + grp * 16;
+  int vcol[VB];
+#pragma unroll
+  for (int vb = 0; vb < VB; ++vb) {
+    const int c = vb * T::CB * T::ES + col * LW * 4;
+    vcol[vb] = c < row_bytes ? c : 0;  // columns past d are computed and not written
+  }
+  const int32_t* const row = p.table + it.b * p.table_stride;
+  // page and offset of 64 subtiles at a time, one per lane; the next 64 are on their way
+  int pid = 0, poff = 0, pid_next = 0, batch = it.begin + i0 * NT;
+  unsigned long long bad = 0;
+  const int sub_end = min(it.begin + i1 * NT, it.end);
+  auto pages_at = [&](int s) {
+    s += lane;
+    return s < sub_end ? row[page_of(s, p.div)] : 0;
+  };
+  auto take_pages = [&](int x) {
+    bad |= __ballot(x < 0 || x >= p.pages);
+    pid = x < 0 || x >= p.pages ? 0 : x;
+    poff = (batch + lane) * 16 - page_of(batch + lane, p.div) * p.page;
+  };
+  if (i0 < i1) {
+    const int x = pages_at(batch);
+    pid_next = pages_at(batch + 64);
+    take_pages(x);
+  }
+
+  Rows<DT, DP> rows;
+  Softmax<NA> st[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    st[mt].m = -INFINITY;
+    st[mt].l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) st[mt].acc[i] = f32x4{0, 0, 0, 0};
+  }
+
+  // pages of tile i's subtiles (the last one again past the wave's end)
+  int64_t pg[NT];
+  int off[NT];
+  auto locate = [&](int i) {
+    const int s = it.begin + i * NT;
+    if (s >= batch + 64) {
+      batch += 64;
+      take_pages(pid_next);
+      pid_next = pages_at(batch + 64);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int x = min(s + t, sub_end - 1) - batch;
+      pg[t] = __builtin_amdgcn_readlane(pid, x);
+      off[t] = __builtin_amdgcn_readlane(poff, x);
+    }
+  };
+  auto load_k_as = [&](auto aux, int piece) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Buffer src = buffer_at(kbase + (pg[t] * kpp + (int64_t)off[t] * kps));
+#pragma unroll
+      for (int c = 0; c < NC / T::KP; ++c) {
+        const int at = (piece * (NC / T::KP) + c) * 64;
+        rows.k[t][c] = __builtin_bit_cast(
+            u32x4, load_words<4, aux.value>(src, at + grp * 16 < row_bytes ? koff + at : kOutside));
+      }
+    }
+  };
+  auto load_v_as = [&](auto aux, int i) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Buffer src = buffer_at(vbase + (pg[t] * vpp + (int64_t)off[t] * vps));
+      // rows that do not count may hold anything: read as zero
+      const int lo = max(first - (it.begin + i * NT + t) * 16, 0);
+      const int count = min(len - (it.begin + i * NT + t) * 16, 16) - lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int x = grp * 4 + r, at = (unsigned)(x - lo) < (unsigned)max(count, 0) ? x * vps
+                                                                                    : kOutside;
+#pragma unroll
+        for (int vb = 0; vb < VB; ++vb)
+          rows.v[t][r][vb] = load_words<LW, aux.value>(src, at + vcol[vb]);
+      }
+    }
+  };
+  constexpr bool kMayStream = DP < 512 && MT == 1;
+  using Plain = std::integral_constant<int, 0>;
+  using Stream = std::integral_constant<int, kStream>;
+  auto load_k = [&](int piece) {
+    if (kMayStream && it.stream) load_k_as(Stream{}, piece);
+    else load_k_as(Plain{}, piece);
+  };
+  auto load_v = [&](int i) {
+    if (kMayStream && it.stream) load_v_as(Stream{}, i);
+    else load_v_as(Plain{}, i);
+  };
+  // which of this lane's keys of the tile from j0 on its row attends: bit 4 t + r
+  auto attended = [&](int mt, int j0) {
+    unsigned int bits = 0;
+    const int32_t* const words = p.masks + ((int64_t)it.c0 + tok[mt]) * p.words;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = j0 + t * 16 + grp * 4 + r, i = j - ctx;
+        bool yes = i < 0 ? j >= start[mt] : false;
+        if (i >= 0 && j < len) {
+          if (!p.masks) yes = i <= tok[mt] && j >= start[mt];
+          else yes = (words[i >> 5] >> (i & 31) & 1) &&
+                     (p.window == 0 || p.pos[(int64_t)it.c0 + i] >= start[mt]);
+        }
+        bits |= yes ? 1u << (t * 4 + r) : 0;
+      }
+    return bits;
+  };
+
+  auto each_value = [&](auto f) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+          for (int x = 0; x < LW; ++x) f(rows.v[t][r][vb].w[x]);
+  };
+  // Adds the tile's infinite and NaN values to the rows that attend them: products of their kinds, as
+  // numbers (1, 2^8 and 2^15 add up without carries), with ones at the keys of a weight, and with ones
+  // at the keys whose weight is zero, where 0 x infinity is NaN.
+  auto add_not_finite = [&](const f32x4 (&s)[MT][NT], const unsigned int (&allow)[MT]) {
+    f32x4 some[MT][NT], none[MT][NT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool yes = allow[mt] >> (t * 4 + r) & 1;
+          some[mt][t][r] = yes && !(s[mt][t][r] == 0.0f) ? 1.0f : 0.0f;
+          none[mt][t][r] = yes && s[mt][t][r] == 0.0f ? 1.0f : 0.0f;
+        }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int e = 0; e < LC; ++e)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          f32x4 x{}, y{};
+          if constexpr (DT == SSA_F32) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float kind = __uint_as_float(kind_of<DT>(rows.v[t][r][vb].w[e]));
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(kind, some[mt][t][r], x, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x4f32(kind, none[mt][t][r], y, 0, 0, 0);
+              }
+          } else {
+            u32x4 kinds, a, b;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                kinds[2 * t + h] = kind_of<DT>(__builtin_amdgcn_perm(
+                    rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
+                    e % 2 ? 0x07060302u : 0x05040100u));
+                a[2 * t + h] = pack16<DT>(some[mt][t][2 * h], some[mt][t][2 * h + 1]);
+                b[2 * t + h] = pack16<DT>(none[mt][t][2 * h], none[mt][t][2 * h + 1]);
+              }
+            x = mfma16(kinds, a, x, DT == SSA_BF16);
+            y = mfma16(kinds, b, y, DT == SSA_BF16);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int kinds = (int)x[r];
+            const bool nan = kinds >= 1 << 15 || y[r] > 0.0f;
+            float v = nan ? NAN : 0.0f;
+            if (kinds & 0xff) v += INFINITY;
+            if (kinds & 0x7f00) v -= INFINITY;
+            st[mt].acc[vb * LC + e][r] += v;
+          }
+        }
+  };
+
+  if (i0 < i1) {
+    locate(i0);
+    load_k(0);
+    load_v(i0);
+  }
+  for (int i = i0; i < i1; ++i) {
+    const int j0 = (it.begin + i * NT) * 16;
+    const bool edge = j0 < late || j0 + NT * 16 > ctx;
+    if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
+    // scores: lane column a row, rows the keys 4 grp + r of each subtile; fp32 in kChains chains, as
+    // paged_attend_kernel
+    constexpr int kChains = DT != SSA_F32 ? 1 : DP == 64 ? 2 : 4;
+    f32x4 s[MT][NT], chain[MT][NT][kChains];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < kChains; ++e) chain[mt][t][e] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      constexpr int per = NC / T::KP;
+      if (c > 0 && c % per == 0) load_k(c / per);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        u32x4 qc;
+        if constexpr (T::kQInLds) qc = q_lds[mt][c][lane];
+        else qc = q[mt][c];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (DT == SSA_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f32x4& x = chain[mt][t][e % kChains];
+              const unsigned int a = rows.k[t][c % per][e], b = qc[e];
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), x,
+                                                       0, 0, 0);
+            }
+          } else {
+            chain[mt][t][0] = mfma16(rows.k[t][c % per], qc, chain[mt][t][0], DT == SSA_BF16);
+          }
+        }
+      }
+    }
+    const bool more = i + 1 < i1;
+    if (more) {
+      locate(i + 1);
+      load_k(0);
+    }
+    constexpr int PARTS = kParts<DT>;
+    u32x4 w[MT][PARTS];  // the weights in 16-bit parts
+    unsigned int allow[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      Softmax<NA>& o = st[mt];
+      allow[mt] = edge ? attended(mt, j0) : 0xffu;
+      float mx = allow[mt] ? -FLT_MAX : -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const auto& of = chain[mt][t];
+          float x = of[0][r];
+          if constexpr (kChains == 2) x += of[1][r];
+          if constexpr (kChains == 4) x = (x + of[1][r]) + (of[2][r] + of[3][r]);
+          x *= p.scale_log2;
+          if (edge && !(allow[mt] >> (t * 4 + r) & 1)) x = -INFINITY;
+          s[mt][t][r] = x;
+          mx = fmaxf(mx, x);
+        }
+      mx = fmaxf(mx, lane_xor(mx, 16));
+      mx = fmaxf(mx, lane_xor(mx, 32));
+      if (__any(mx > o.m)) {  // a row without a key so far stays at -inf, its sums at 0
+        const float m = fmaxf(o.m, mx);
+        const float a = __builtin_amdgcn_exp2f(o.m - (m == -INFINITY ? 0.0f : m));
+        o.m = m;
+        o.l *= a;
+#pragma unroll
+        for (int x = 0; x < NA; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o.acc[x][r] *= a;
+      }
+      const float base = (o.m == -INFINITY ? 0.0f : o.m) - T::kShift;
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[mt][t][r] = __builtin_amdgcn_exp2f(s[mt][t][r] - base);
+          sum += s[mt][t][r];
+        }
+      o.l += sum;
+      if constexpr (DT != SSA_F32) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned int x[PARTS];
+            split<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], x);
+#pragma unroll
+            for (int y = 0; y < PARTS; ++y) w[mt][y][2 * t + h] = x[y];
+          }
+      }
+    }
+    if (edge) {
+      bool odd = false;
+      each_value([&](unsigned int& v) { odd |= not_finite<DT>(v); });
+      if (__any(odd)) {
+        add_not_finite(s, allow);
+        each_value([&](unsigned int& v) { v = finite_part<DT>(v); });
+      }
+    }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int e = 0; e < LC; ++e) {
+        if constexpr (DT == SSA_F32) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                f32x4& acc = st[mt].acc[vb * LC + e];
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    __uint_as_float(rows.v[t][r][vb].w[e]), s[mt][t][r], acc, 0, 0, 0);
+              }
+        } else {
+          // column e of the lane's values, key after key
+          u32x4 vt;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              vt[2 * t + h] = __builtin_amdgcn_perm(
+                  rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
+                  e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            f32x4& acc = st[mt].acc[vb * LC + e];
+#pragma unroll
+            for (int y = 0; y < PARTS; ++y) acc = mfma16(vt, w[mt][y], acc, DT == SSA_BF16);
+          }
+        }
+      }
+    if (more) load_v(i + 1);
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    st[mt].l += lane_xor(st[mt].l, 16);
+    st[mt].l += lane_xor(st[mt].l, 32);
+    if (bad != 0 || !it.s.span.ok || rpos[mt] < ctx) st[mt].l = NAN;
+  }
+
+  // the waves' results, half of them into the other half at a time
+#pragma unroll
+  for (int half = NW / 2; half >= 1; half >>= 1) {
+    if (wv >= half && wv < 2 * half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        red_m[wv - half][mt][lane] = st[mt].m;
+        red_l[wv - half][mt][lane] = st[mt].l;
+#pragma unroll
+        for (int x = 0; x < NA; ++x) red[wv - half][mt][x][lane] = st[mt].acc[x];
+      }
+    }
+    __syncthreads();
+    if (wv < half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        join(st[mt], red_m[wv][mt][lane], red_l[wv][mt][lane], &red[wv][mt][0][lane], 64);
+    }
+    __syncthreads();
+  }
+  if (wv != 0) return;
+
+  if (p.items != 0 && it.j == 0 && it.g == 0 && it.tile == 0 && lane == 0) {
+    p.info[2 * it.b] = it.first_part;
+    p.info[2 * it.b + 1] = it.n;
+  }
+  if (it.n > 1 && it.first_part < 0) return;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const Softmax<NA>& o = st[mt];
+    if (!real[mt]) continue;
+    const float inv = row_scale(o.m, o.l);
+    const int64_t token = (int64_t)it.c0 + tok[mt], to = token * p.ot + head[mt] * p.oh;
+    const int64_t part =
+        ((int64_t)it.first_part + ((int64_t)it.j * p.Hkv + it.g) * it.tiles + it.tile) * M +
+        mt * 16 + col;
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < LC; e += 4) {
+          const int c = vb * T::CB + LC * (grp * 4 + r) + e;
+          if (c >= p.d) continue;
+          f32x4 x;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[y] = o.acc[vb * LC + e + y][r];
+          if (it.n > 1) {
+            *(f32x4*)(p.part + part * DP + c) = x;
+          } else {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[y] *= inv;
+            store_row4<DT>(p.out, to + c, x);
+          }
+        }
+    if (grp != 0) continue;
+    if (it.n > 1) {
+      p.part_ml[part * 2] = o.m;
+      p.part_ml[part * 2 + 1] = o.l;
+    } else if (p.lse) {
+      p.lse[token * p.Hq + head[mt]] = row_lse(o.m, o.l, T::kShift);
+    }
+  }
+}
+
+constexpr int kJoinRows = 8;  // parts of a row on their way at a time
+
+// Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
+// the columns, four waves a workgroup.
+template <int DT, int DP, int M>
+__global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
+  constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  const int64_t row = id / p.Hq;
+  if (row >= p.N || (p.status && *p.status != 0)) return;
+  const int h = (int)(id - row * p.Hq), g = h / p.G;
+  const int b = last_at_most(p.cu, p.B, (int)row), c0 = p.cu[b], c1 = p.cu[b + 1];
+  const DraftSpan s = draft_of(p, b);
+  if (row < c0 || row >= c1 || s.n == 0) return;
+  const int first = p.info[2 * b], parts = p.info[2 * b + 1];
+  if (parts <= 1) return;  // written by its one item
+  const int64_t x = (row - c0) * p.G + (h - g * p.G), tiles = draft_tiles(s, p.G, M);
+  const int64_t tile = x / M, step = tiles * p.Hkv;
+  const bool held = first >= 0 && first + step * parts <= p.max_parts;
+  const int64_t at = ((held ? first : 0) + g * tiles + tile) * M + x % M;
+  const int split = lane / PER % NS, c = lane % PER * 4;
+  Softmax<NV> st;
+  st.m = -INFINITY;
+  st.l = held ? 0.0f : NAN;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) st.acc[v] = f32x4{0, 0, 0, 0};
+  for (int i = split; held && i < parts; i += NS * kJoinRows) {
+    float m[kJoinRows], l[kJoinRows], mx = st.m;
+    f32x4 a[kJoinRows][NV];
+#pragma unroll
+    for (int u = 0; u < kJoinRows; ++u) {
+      const bool in = i + u * NS < parts;
+      const int64_t from = at + (in ? i + u * NS : 0) * step * M;
+      m[u] = in ? p.part_ml[from * 2] : -INFINITY;
+      l[u] = in ? p.part_ml[from * 2 + 1] : 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        a[u][v] = in ? *(const f32x4*)(p.part + from * DP + v * 256 + c) : f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinRows; ++u) mx = fmaxf(mx, m[u]);
+    const float base = mx == -INFINITY ? 0.0f : mx, y = __builtin_amdgcn_exp2f(st.m - base);
+    st.m = mx;
+    st.l *= y;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st.acc[v][r] *= y;
+#pragma unroll
+    for (int u = 0; u < kJoinRows; ++u) {
+      const float z = __builtin_amdgcn_exp2f(m[u] - base);
+      st.l += l[u] * z;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.acc[v][r] += a[u][v][r] * z;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= PER; off >>= 1) {
+    f32x4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = lane_xor(st.acc[0][r], off);
+    const float m = lane_xor(st.m, off), l = lane_xor(st.l, off);
+    Softmax<1> one{st.m, st.l, {st.acc[0]}};
+    join(one, m, l, &o, 0);
+    st.m = one.m;
+    st.l = one.l;
+    st.acc[0] = one.acc[0];
+  }
+  const float inv = row_scale(st.m, st.l);
+  const int64_t to = row * p.ot + h * p.oh;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) st.acc[v][r] *= inv;
+    if (lane < PER && v * 256 + c < p.d) store_row4<DT>(p.out, to + v * 256 + c, st.acc[v]);
+  }
+  if (p.lse && lane == 0)
+    p.lse[row * p.Hq + h] = row_lse(st.m, st.l, DT == SSA_F16 ? kF16Shift : 0.0f);
+}
+
+// How a call of these sizes is cut: known on the host without the lengths.
+struct DraftLayout {
+  int64_t items, blocks, max_parts;  // items: 0 when no row tile is cut
+  int dp, M;
+  size_t part_ml, info, bytes;  // offsets into the workspace, which starts with the parts
+};
+
+// Two tiles of 16 rows a wave where requests have more rows on average (past head dim 128 their
+// registers do not fit).
+DraftLayout draft_layout(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+                         int64_t page, int64_t window) {
+  DraftLayout y{};
+  const int64_t G = Hq / Hkv;
+  y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
+  y.M = y.dp <= 128 && N * G > 16 * B ? 32 : 16;
+  const int64_t tiles = draft_most_tiles(B, N, G, y.M) * Hkv;
+  const int64_t cap = W * page;
+  const int64_t units = paged_most_units(window > 0 ? std::min(cap, window + N + 15) : cap, 0);
+  const auto rounded = [](int64_t x) { return (x + 7) / 8 * 8; };  // an XCD's run each
+  y.blocks = rounded(tiles);
+  if (units <= 4 || (units <= 16 && tiles >= 512)) return y;
+  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 || B == 1 ? 512 : 1024;
+  y.items = std::max<int64_t>(1, target / Hkv);
+  y.blocks = rounded(std::min(tiles + y.items * Hkv, tiles * units));
+  y.max_parts = std::min(2 * y.items * Hkv, y.blocks);
+  const size_t rows = (size_t)y.max_parts * y.M;
+  y.part_ml = rows * y.dp * 4;
+  y.info = y.part_ml + rows * 2 * 4;
+  y.bytes = (y.info + (size_t)B * 8 + 15) / 16 * 16;
+  return y;
+}
+
+template <int DT, int DP, int MT, int WPE>
+int run_drafts(const DraftParams& p, hipStream_t st) {
+  paged_drafts_kernel<DT, DP, MT, WPE>
+      <<<(unsigned)(p.blocks + kRestBlocks), kAttendWaves * 64, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_drafts_kernel"));
+  if (p.items == 0) return SSA_OK;
+  paged_drafts_join_kernel<DT, DP, MT * 16>
+      <<<(unsigned)((p.N * p.Hq + 3) / 4), 256, 0, st>>>(p);
+  return launch_status("paged_drafts_join_kernel");
+}
+
+template <int DT>
+int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
+  switch (y.dp) {
+    case 64:
+      if (y.M == 32) return run_drafts<DT, 64, 2, 2>(p, st);
+      return run_drafts<DT, 64, 1, 3>(p, st);
+    case 128:
+      if (y.M == 32) return run_drafts<DT, 128, 2, 2>(p, st);
+      return run_drafts<DT, 128, 1, 2>(p, st);
+    case 256: return run_drafts<DT, 256, 1, 1>(p, st);
+    default: return run_drafts<DT, 512, 1, 1>(p, st);
+  }
+}
+
+// ---- accepted tokens moved together ------------------------------------------------------------
+
+struct KeepParams {
+  char* kpool;
+  char* vpool;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  const int32_t* path;
+  const int32_t* counts;
+  int32_t* new_lens;
+  int64_t table_stride, path_stride, cap, pages;
+  int width;                                           // of a path
+  int page, Hkv, vecs, columns;                        // vecs: 16-byte pieces of a row
+  int64_t kpl, kpp, kph, kps, vpl, vpp, vph, vps;      // bytes
+  PageDiv div;
+};
+
+constexpr int kKeepThreads = 256, kKeepBatch = 8;
+
+// A workgroup for a request and 256 columns (a column: 16 bytes of a layer's keys or values of a head,
+// over all tokens), a thread a column. An accepted token never moves up and they move in order, so a
+// column's tokens are read kKeepBatch at a time before any of these is written, and none that is
+// written is read again. All or nothing: every workgroup of a request checks its whole path first.
+__global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
+  __shared__ int s_page[2][kKeepThreads], s_slot[2][kKeepThreads];
+  __shared__ int s_first;
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int len = p.lens[b], c0 = p.cu[b], c1 = p.cu[b + 1], count = p.counts[b];
+  const int n = c1 - c0, ctx = len - n;
+  bool bad = c0 < 0 || c1 < c0 || len < 0 || len > p.cap || n > len || count < 0 || count > n ||
+             count > p.width;
+  const int32_t* const path = p.path + b * p.path_stride;
+  const int32_t* const row = p.table + b * p.table_stride;
+  auto place = [&](int at, int& page, int& slot) {  // of drafted token `at`
+    const int j = ctx + at, e = page_of(j / 16, p.div);
+    page = row[e];
+    slot = j - e * p.page;
+    return page >= 0 && page < p.pages;
+  };
+  if (tid == 0) s_first = 0x7fffffff;
+  __syncthreads();
+  if (!bad) {
+    bool wrong = false;
+    int moved = 0x7fffffff;
+    for (int i = tid; i < count; i += kKeepThreads) {
+      const int at = path[i], before = i > 0 ? path[i - 1] : -1;
+      int page, slot;
+      if (before >= at || at < 0 || at >= n || !place(at, page, slot) || !place(i, page, slot))
+        wrong = true;
+      else if (at != i) moved = min(moved, i);
+    }
+    if (moved != 0x7fffffff) atomicMin(&s_first, moved);
+    bad = __syncthreads_or(wrong);
+  }
+  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = bad ? -1 : ctx + count;
+  if (bad || s_first >= count) return;
+  const int first = s_first, column = blockIdx.x * kKeepThreads + tid;
+  const int c = column % p.vecs, of = column / p.vecs, h = of % p.Hkv, lv = of / p.Hkv;
+  const bool mine = column < p.columns, v = lv & 1;
+  const int64_t pp = v ? p.vpp : p.kpp, ps = v ? p.vps : p.kps;
+  char* const base = (v ? p.vpool : p.kpool) + (lv >> 1) * (v ? p.vpl : p.kpl) +
+                     h * (v ? p.vph : p.kph) + c * 16;
+  for (int i0 = first; i0 < count; i0 += kKeepThreads) {
+    const int m = min(count - i0, kKeepThreads);
+    __syncthreads();
+    if (tid < m) {
+      place(path[i0 + tid], s_page[0][tid], s_slot[0][tid]);
+      place(i0 + tid, s_page[1][tid], s_slot[1][tid]);
+    }
+    __syncthreads();
+    if (!mine) continue;
+    for (int i = 0; i < m; i += kKeepBatch) {
+      u32x4 x[kKeepBatch];
+#pragma unroll
+      for (int u = 0; u < kKeepBatch; ++u)
+        if (i + u < m)
+          x[u] = *(const u32x4*)(base + s_page[0][i + u] * pp + s_slot[0][i + u] * ps);
+#pragma unroll
+      for (int u = 0; u < kKeepBatch; ++u)
+        if (i + u < m) *(u32x4*)(base + s_page[1][i + u] * pp + s_slot[1][i + u] * ps) = x[u];
+    }
+  }
+}
+
+int check_table(const char* who, int64_t W, int64_t table_stride, int64_t page) {
+  SSA_REQUIRE(W > 0 && table_stride >= W && W <= 0x7fffffff / page, SSA_ERR_INVALID,
+              "%s: table of %lld pages a row, stride %lld (at most 2^31 - 1 tokens)", who,
+              (long long)W, (long long)table_stride);
+  return SSA_OK;
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu,
+                                     const int32_t* lens, int64_t B, int64_t N, int64_t words,
+                                     int32_t* masks, int32_t* pos, ssa_stream_t stream) {
+  SSA_REQUIRE(cu && lens && (N == 0 || (parents && masks && pos)), SSA_ERR_INVALID,
+              "ssa_paged_draft_masks: NULL argument");
+  SSA_REQUIRE(B > 0 && B < 0x7fffffff && fits_int(N), SSA_ERR_INVALID,
+              "ssa_paged_draft_masks: bad shape (B=%lld, N=%lld)", (long long)B, (long long)N);
+  SSA_REQUIRE(words > 0 && words <= kMaxWords, SSA_ERR_UNSUPPORTED,
+              "ssa_paged_draft_masks: masks of %lld words (1 to %d)", (long long)words, kMaxWords);
+  const int threads = words <= 2 ? 64 : words <= 8 ? 256 : 1024;
+  SSA_REQUIRE(fits_launch((B + 1) * ((words + 3) / 4), threads), SSA_ERR_UNSUPPORTED,
+              "ssa_paged_draft_masks: %lld requests in one call", (long long)B);
+  if (N == 0) return SSA_OK;
+  MaskParams p{parents, cu, lens, masks, pos, N, (int)B, (int)words};
+  const dim3 grid((unsigned)(B + 1), (unsigned)((words + 3) / 4));
+  hipStream_t st = (hipStream_t)stream;
+  if (threads == 64) paged_draft_masks_kernel<64><<<grid, 64, 0, st>>>(p);
+  else if (threads == 256) paged_draft_masks_kernel<256><<<grid, 256, 0, st>>>(p);
+  else paged_draft_masks_kernel<1024><<<grid, 1024, 0, st>>>(p);
+  return launch_status("paged_draft_masks_kernel");
+}
+
+extern "C" size_t ssa_paged_attend_drafts_workspace_size(int64_t B, int64_t N, int64_t Hq,
+                                                         int64_t Hkv, int64_t d, int64_t W,
+                                                         int64_t page, int64_t window) {
+  if (B <= 0 || N <= 0 || !fits_int(N) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 ||
+      W <= 0 || page <= 0 || !fits_int(window) || W > 0x7fffffff / page)
+    return 0;
+  return draft_layout(B, N, Hq, Hkv, d, W, page, window).bytes;
+}
+
+extern "C" int ssa_paged_attend_drafts(const void* q, const void* kpool, const void* vpool,
+                                       void* out, float* lse, int dtype, int64_t B, int64_t N,
+                                       int64_t Hq, int64_t Hkv, int64_t d, int64_t pages,
+                                       int64_t page, const int32_t* table, int64_t table_stride,
+                                       int64_t W, const int32_t* lens, const int32_t* cu,
+                                       const int32_t* masks, const int32_t* pos, int64_t words,
+                                       const int64_t* strides, float scale, int64_t window,
+                                       const int32_t* status, int clear_rest, void* workspace,
+                                       size_t workspace_bytes, ssa_stream_t stream) {
+  const char* const who = "ssa_paged_attend_drafts";
+  SSA_REQUIRE(q && kpool && vpool && out && table && lens && cu && strides, SSA_ERR_INVALID,
+              "%s: NULL argument", who);
+  SSA_REQUIRE((masks == nullptr) == (pos == nullptr) && (masks == nullptr) == (words == 0),
+              SSA_ERR_INVALID, "%s: masks, pos and words come together", who);
+  SSA_REQUIRE(words >= 0 && words <= kMaxWords, SSA_ERR_UNSUPPORTED,
+              "%s: masks of %lld words (1 to %d)", who, (long long)words, kMaxWords);
+  SSA_TRY(check_pool(who, dtype, Hkv, d, pages, page));
+  SSA_REQUIRE(B > 0 && B <= 65535 && N > 0 && fits_int(N) && Hq > 0 && Hq <= 65535 &&
+                  Hq % Hkv == 0, SSA_ERR_INVALID,
+              "%s: B=%lld, N=%lld, Hq=%lld, Hkv=%lld (at most 65535 requests; Hq a multiple of "
+              "Hkv)", who, (long long)B, (long long)N, (long long)Hq, (long long)Hkv);
+  SSA_TRY(check_table(who, W, table_stride, page));
+  SSA_REQUIRE(fits_int(window), SSA_ERR_INVALID, "%s: window %lld", who, (long long)window);
+  const int es = dtype_size(dtype);
+  // strides: q(t,h), kpool(page,head,slot), vpool(page,head,slot), out(t,h)
+  SSA_REQUIRE(rows16(q, strides, 2, es) && rows16(kpool, strides + 2, 3, es) &&
+                  rows16(vpool, strides + 5, 3, es) && rows16(out, strides + 8, 2, es),
+              SSA_ERR_INVALID, "%s: rows must start at multiples of 16 bytes", who);
+  SSA_REQUIRE(strides[4] < (1 << 24) && strides[7] < (1 << 24), SSA_ERR_UNSUPPORTED,
+              "%s: slots 2^24 elements apart or more", who);
+  const DraftLayout y = draft_layout(B, N, Hq, Hkv, d, W, page, window);
+  SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
+              SSA_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who,
+              y.bytes, workspace_bytes);
+  SSA_REQUIRE(fits_launch(y.blocks + kRestBlocks, kAttendWaves * 64) &&
+                  fits_launch((N * Hq + 3) / 4, 256), SSA_ERR_UNSUPPORTED,
+              "%s: too many rows in one call", who);
+  DraftParams p{};
+  p.q = (const char*)q;
+  p.kpool = (const char*)kpool;
+  p.vpool = (const char*)vpool;
+  p.out = (char*)out;
+  p.lse = lse;
+  p.table = table;
+  p.lens = lens;
+  p.cu = cu;
+  p.masks = masks;
+  p.pos = pos;
+  p.status = status;
+  p.table_stride = table_stride;
+  p.cap = W * page;
+  p.pages = pages;
+  p.N = N;
+  p.B = (int)B;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.G = (int)(Hq / Hkv);
+  p.d = (int)d;
+  p.page = (int)page;
+  p.window = (int)window;
+  p.words = (int)words;
+  p.clear = clear_rest != 0;
+  p.scale_log2 = scale * kLog2e;
+  int64_t* const st[10] = {&p.qt,  &p.qh,  &p.kpp, &p.kph, &p.kps,
+                           &p.vpp, &p.vph, &p.vps, &p.ot,  &p.oh};
+  for (int i = 0; i < 10; ++i) *st[i] = strides[i];
+  p.div = page_div((int)page / 16);
+  p.stream_units = kStreamBytes / unit_bytes(dtype, d, Hkv);
+  p.items = y.items;
+  p.blocks = y.blocks;
+  p.max_parts = y.max_parts;
+  p.part = (float*)workspace;
+  p.part_ml = (float*)((char*)workspace + y.part_ml);
+  p.info = (int32_t*)((char*)workspace + y.info);
+  hipStream_t hs = (hipStream_t)stream;
+  if (dtype == SSA_F32) return run_drafts_dim<SSA_F32>(p, y, hs);
+  if (dtype == SSA_F16) return run_drafts_dim<SSA_F16>(p, y, hs);
+  return run_drafts_dim<SSA_BF16>(p, y, hs);
+}
+
+extern "C" int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
+                              int64_t d, int64_t pages, int64_t page, const int64_t* strides,
+                              const int32_t* table, int64_t table_stride, int64_t W,
+                              const int32_t* lens, const int32_t* cu, int64_t B,
+                              const int32_t* path, int64_t path_stride, int64_t width,
+                              const int32_t* counts, int32_t* new_lens, ssa_stream_t stream) {
+  const char* const who = "ssa_paged_keep";
+  SSA_REQUIRE(kpool && vpool && strides && table && lens && cu && counts && new_lens &&
+                  (path || width == 0), SSA_ERR_INVALID, "%s: NULL argument", who);
+  SSA_TRY(check_pool(who, dtype, Hkv, d, pages, page));
+  SSA_REQUIRE(B > 0 && B <= 65535 && layers > 0 && fits_int(layers) && fits_int(width) &&
+                  path_stride >= 0, SSA_ERR_INVALID,
+              "%s: B=%lld, layers=%lld, paths of %lld (at most 65535 requests)", who, (long long)B,
+              (long long)layers, (long long)width);
+  SSA_TRY(check_table(who, W, table_stride, page));
+  const int es = dtype_size(dtype);
+  // strides: kpool(layer,page,head,slot), vpool(layer,page,head,slot)
+  SSA_REQUIRE(rows16(kpool, strides, 4, es) && rows16(vpool, strides + 4, 4, es), SSA_ERR_INVALID,
+              "%s: rows must start at multiples of 16 bytes", who);
+  const int64_t vecs = d * es / 16, columns = 2 * layers * Hkv * vecs;
+  const int64_t blocks = (columns + kKeepThreads - 1) / kKeepThreads;
+  SSA_REQUIRE(fits_int(columns) && fits_launch(blocks * B, kKeepThreads), SSA_ERR_UNSUPPORTED,
+              "%s: %lld layers of %lld requests in one call", who, (long long)layers, (long long)B);
+  KeepParams p{(char*)kpool, (char*)vpool, table, lens, cu, path, counts, new_lens,
+               table_stride, path_stride, W * page, pages, (int)width,
+               (int)page, (int)Hkv, (int)vecs, (int)columns,
+               strides[0] * es, strides[1] * es, strides[2] * es, strides[3] * es,
+               strides[4] * es, strides[5] * es, strides[6] * es, strides[7] * es,
+               page_div((int)page / 16)};
+  paged_keep_kernel<<<dim3((unsigned)blocks, (unsigned)B), kKeepThreads, 0, (hipStream_t)stream>>>(p);
+  return launch_status("paged_keep_kernel");
+}

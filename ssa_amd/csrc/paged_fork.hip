@@ -1,0 +1,435 @@
+// Requests of the paged key-value cache that share pages: forked, cut short and ended, with the pages that
+// no request lists any more given back; and the pages that have to be copied for it.
+#include <algorithm>
+
+#include "paged_parts.h"
+
+namespace ssa {
+namespace {
+
+// ---- rows of the table from other rows ---------------------------------------------------------
+
+// What the call's rows say of a page: the first row that listed it and changes, the first row that will
+// hold it as its last, partly filled page, whether a row will hold it whole.
+struct PageUse {
+  int holder, first_part, whole, unused;
+};
+
+struct ForkParams {
+  const int32_t* src;  // NULL: every row itself
+  const int32_t* new_lens;
+  int32_t* lens;
+  int32_t* table;
+  int64_t table_stride, W, cap;
+  int B, page;
+  int32_t* free_pages;
+  int64_t P;
+  int32_t* nfree;
+  int32_t* source;
+  int32_t* target;
+  int32_t* tokens;
+  int32_t* status;
+  PageDiv div;
+  // workspace
+  PageUse* use;       // (P)
+  int32_t* old;       // (B, W): the held entries of the table before
+  int32_t* old_lens;  // (B)
+  int32_t* given;     // (units): pages given back, then the sum of those before
+  int32_t* bad;       // (units)
+  int32_t* taken;     // (B): whether a page is taken, then its place on the stack
+  int32_t* left;      // (1): free pages after, -1: nothing changes
+  int64_t units;      // of at most kForkEntries entries of a row
+  int chunks;         // of a row
+};
+
+constexpr int kForkEntries = 1024, kForkLoads = kForkEntries / 64;
+
+// A row's change, from its lengths alone.
+struct ForkRow {
+  int from, len, want, have, whole, need;  // pages held before, to hold whole and to hold
+  bool ok, same;
+};
+
+__device__ inline ForkRow fork_row(const ForkParams& p, const int32_t* lens, int b) {
+  ForkRow r;
+  r.len = lens[b];
+  r.want = p.new_lens[b];
+  r.from = p.src ? p.src[b] : b;
+  r.ok = r.len >= 0 && r.len <= p.cap && r.want >= 0;
+  if (r.want > 0) {
+    r.ok = r.ok && r.from >= 0 && r.from < p.B;
+    const int of = r.ok ? lens[r.from] : 0;
+    r.ok = r.ok && of <= p.cap && r.want <= of;
+  }
+  r.have = r.ok ? paged_pages(r.len, p.page, p.div) : 0;
+  r.need = r.ok ? paged_pages(r.want, p.page, p.div) : 0;
+  r.whole = r.need - (r.want > r.need * p.page - p.page && r.want < r.need * p.page ? 1 : 0);
+  r.same = r.ok && r.want == r.len && (r.want == 0 || r.from == b);
+  return r;
+}
+
+// f(k, entry) for this lane's entries of a chunk below `end`; k counts to kForkLoads.
+template <class F>
+__device__ inline void each_entry(int chunk, int end, F f) {
+  const int first = chunk * kForkEntries, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < kForkLoads; ++k) {
+    if (first + k * 64 >= end) return;
+    const int e = first + k * 64 + lane;
+    if (e < end) f(k, e);
+  }
+}
+
+// The steps, each a wave for a unit (a chunk of a row's entries). Between two of them all units are done.
+// 1: the table's held entries are kept, the uses of their pages cleared.
+__device__ inline void fork_clear(const ForkParams& p, int unit) {
+  const int b = unit / p.chunks, chunk = unit - b * p.chunks;
+  const ForkRow r = fork_row(p, p.lens, b);
+  bool bad = !r.ok;
+  const int32_t* const row = p.table + b * p.table_stride;
+  int id[kForkLoads];
+  each_entry(chunk, r.have, [&](int k, int e) { id[k] = row[e]; });
+  each_entry(chunk, r.have, [&](int k, int e) {
+    p.old[b * p.W + e] = id[k];
+    if (id[k] < 0 || id[k] >= p.P) bad = true;
+    else p.use[id[k]] = PageUse{0x7fffffff, 0x7fffffff, 0, 0};
+  });
+  const bool any = __any(bad);
+  if ((threadIdx.x & 63) == 0) {
+    p.bad[unit] = any;
+    if (chunk == 0) p.old_lens[b] = p.lens[b];
+  }
+}
+
+// 2: the uses of the pages.
+__device__ inline void fork_mark(const ForkParams& p, int unit) {
+  const int b = unit / p.chunks, chunk = unit - b * p.chunks;
+  const ForkRow r = fork_row(p, p.old_lens, b);
+  const bool here = r.from >= 0 && r.from < p.B;
+  const int32_t* const mine = p.old + b * p.W;
+  const int32_t* const theirs = p.old + (here ? r.from : 0) * p.W;
+  int id[kForkLoads];
+  each_entry(chunk, r.need, [&](int k, int e) { id[k] = theirs[e]; });
+  each_entry(chunk, r.need, [&](int k, int e) {
+    if (id[k] < 0 || id[k] >= p.P) return;
+    if (e < r.whole) p.use[id[k]].whole = 1;
+    else atomicMin(&p.use[id[k]].first_part, b);
+  });
+  if (r.same) return;
+  each_entry(chunk, r.have, [&](int k, int e) { id[k] = mine[e]; });
+  each_entry(chunk, r.have, [&](int k, int e) {
+    if (id[k] >= 0 && id[k] < p.P) atomicMin(&p.use[id[k]].holder, b);
+  });
+}
+
+// Whether row b gives back a page of this use.
+__device__ inline bool gives(const PageUse& u, int b) {
+  return !u.whole && u.first_part == 0x7fffffff && u.holder == b;
+}
+
+// Whether row b needs a copy of its last page: another row holds it whole or was first.
+__device__ inline bool copies(const PageUse& u, int b) { return u.whole || u.first_part != b; }
+
+// 3: pages given back by the unit, and whether its row takes one.
+__device__ inline void fork_count(const ForkParams& p, int unit) {
+  const int b = unit / p.chunks, chunk = unit - b * p.chunks, lane = threadIdx.x & 63;
+  const ForkRow r = fork_row(p, p.old_lens, b);
+  if (chunk == 0 && lane == 0) {
+    bool take = false;
+    if (r.whole < r.need) {
+      const int id = p.old[(int64_t)r.from * p.W + r.whole];
+      take = id >= 0 && id < p.P && copies(p.use[id], b);
+    }
+    p.taken[b] = take;
+  }
+  int n = 0;
+  if (!r.same) {
+    int id[kForkLoads];
+    each_entry(chunk, r.have, [&](int k, int e) { id[k] = p.old[b * p.W + e]; });
+    each_entry(chunk, r.have, [&](int k, int e) {
+      if (id[k] >= 0 && id[k] < p.P) n += gives(p.use[id[k]], b);
+    });
+  }
+  n = lane_sums(n).all;
+  if (lane == 0) p.given[unit] = n;
+}
+
+constexpr int kForkThreads = 1024, kForkWaves = kForkThreads / 64;
+
+// 4, by one workgroup: sums of the units and rows before each, the status (all or nothing), and the
+// pages taken off the stack.
+__device__ inline void fork_sum(const ForkParams& p) {
+  __shared__ int64_t s_wave[kForkWaves];
+  __shared__ int64_t s_all;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  bool bad = false;
+  for (int64_t u = tid; u < p.units; u += kForkThreads) bad |= p.bad[u] != 0;
+  bad = __syncthreads_or(bad);
+  // x becomes the sum before it, running on from `sum`
+  auto scan = [&](int32_t* x, int64_t n) {
+    int64_t sum = 0;
+    for (int64_t i0 = 0; i0 < n; i0 += kForkThreads) {
+      const int64_t i = i0 + tid;
+      const int64_t v = i < n ? x[i] : 0;
+      const LaneSums<int64_t> s = lane_sums(v);
+      __syncthreads();
+      if (lane == 63) s_wave[wv] = s.upto;
+      __syncthreads();
+      if (wv == 0) {
+        const int64_t w = lane < kForkWaves ? s_wave[lane] : 0;
+        const LaneSums<int64_t> t = lane_sums(w);
+        if (lane < kForkWaves) s_wave[lane] = t.upto - w;
+        if (lane == 0) s_all = t.all;
+      }
+      __syncthreads();
+      // a row that takes no page keeps -1
+      if (i < n) x[i] = x == p.taken && v == 0 ? -1 : (int)min(sum + s_wave[wv] + s.upto - v,
+                                                               (int64_t)0x7fffffff);
+      sum += s_all;
+    }
+    return sum;
+  };
+  const int64_t taken = scan(p.taken, p.B), given = scan(p.given, p.units);
+  const int nfree = *p.nfree;
+  const int64_t lack = taken - nfree, left = nfree - taken + given;
+  const int status = bad || nfree < 0 || nfree > p.P || left > p.P ? -1 : lack > 0 ? (int)lack : 0;
+  __syncthreads();
+  for (int64_t b = tid; b < p.B; b += kForkThreads) {
+    const int nth = status == 0 ? p.taken[b] : -1;
+    int from = -1, to = -1, n = 0;
+    if (nth >= 0) {
+      const ForkRow r = fork_row(p, p.old_lens, (int)b);
+      from = p.old[(int64_t)r.from * p.W + r.whole];
+      to = p.free_pages[nfree - 1 - nth];
+      n = r.want - r.whole * p.page;
+    }
+    p.source[b] = from;
+    p.target[b] = to;
+    p.tokens[b] = n;
+  }
+  if (tid == 0) {
+    *p.status = status;
+    *p.left = status == 0 ? (int)left : -1;
+    if (status == 0) *p.nfree = (int)left;
+  }
+}
+
+// 5: pages onto the stack, the new rows, the new lengths.
+__device__ inline void fork_write(const ForkParams& p, int unit) {
+  const int left = *p.left;
+  if (left < 0) return;
+  const int b = unit / p.chunks, chunk = unit - b * p.chunks, lane = threadIdx.x & 63;
+  const ForkRow r = fork_row(p, p.old_lens, b);
+  const int fresh = p.target[b];
+  int32_t* const row = p.table + b * p.table_stride;
+  if (!r.same) {
+    int at = left - 1 - p.given[unit];
+    const int first = chunk * kForkEntries;
+#pragma unroll 1
+    for (int e = first + lane; e - lane < min(r.have, first + kForkEntries); e += 64) {
+      const int id = e < r.have ? p.old[b * p.W + e] : -1;
+      const unsigned long long all = __ballot(id >= 0 && gives(p.use[id], b));
+      if (all >> lane & 1) p.free_pages[at - __popcll(all & ((1ull << lane) - 1))] = id;
+      at -= __popcll(all);
+    }
+    const int32_t* const theirs = p.old + (int64_t)max(r.from, 0) * p.W;
+    each_entry(chunk, max(r.have, r.need), [&](int, int e) {
+      row[e] = e >= r.need ? -1 : e == r.whole && fresh >= 0 ? fresh : theirs[e];
+    });
+    if (chunk == 0 && lane == 0) p.lens[b] = r.want;
+  } else if (fresh >= 0 && chunk == r.whole / kForkEntries && lane == 0) {
+    row[r.whole] = fresh;
+  }
+}
+
+// Makes this workgroup's writes and atomics visible to its later reads.
+__device__ inline void fork_step() {
+  __threadfence();
+  __syncthreads();
+  __threadfence();
+}
+
+// The whole call by one workgroup, a wave a unit at a time.
+__global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkParams p) {
+  const int wv = uniform(threadIdx.x >> 6);
+  for (int u = wv; u < p.units; u += kForkWaves) fork_clear(p, u);
+  fork_step();
+  for (int u = wv; u < p.units; u += kForkWaves) fork_mark(p, u);
+  fork_step();
+  for (int u = wv; u < p.units; u += kForkWaves) fork_count(p, u);
+  fork_step();
+  fork_sum(p);
+  fork_step();
+  for (int u = wv; u < p.units; u += kForkWaves) fork_write(p, u);
+}
+
+// The steps as launches of their own, four units a workgroup.
+__global__ __launch_bounds__(256) void paged_fork_clear_kernel(ForkParams p) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (u < p.units) fork_clear(p, (int)u);
+}
+__global__ __launch_bounds__(256) void paged_fork_mark_kernel(ForkParams p) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (u < p.units) fork_mark(p, (int)u);
+}
+__global__ __launch_bounds__(256) void paged_fork_count_kernel(ForkParams p) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (u < p.units) fork_count(p, (int)u);
+}
+__global__ __launch_bounds__(kForkThreads) void paged_fork_sum_kernel(ForkParams p) { fork_sum(p); }
+__global__ __launch_bounds__(256) void paged_fork_write_kernel(ForkParams p) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (u < p.units) fork_write(p, (int)u);
+}
+
+constexpr int64_t kForkInside = 64;
+
+struct ForkLayout {
+  int64_t chunks, units;
+  size_t old, old_lens, given, bad, taken, left, bytes;
+};
+
+ForkLayout fork_layout(int64_t B, int64_t W, int64_t pages) {
+  ForkLayout y{};
+  y.chunks = (W + kForkEntries - 1) / kForkEntries;
+  y.units = B * y.chunks;
+  y.old = (size_t)pages * sizeof(PageUse);
+  y.old_lens = y.old + (size_t)B * W * 4;
+  y.given = y.old_lens + (size_t)B * 4;
+  y.bad = y.given + (size_t)y.units * 4;
+  y.taken = y.bad + (size_t)y.units * 4;
+  y.left = y.taken + (size_t)B * 4;
+  y.bytes = (y.left + 4 + 15) / 16 * 16;
+  return y;
+}
+
+// ---- pages copied ------------------------------------------------------------------------------
+
+struct CopyParams {
+  char* kpool;
+  char* vpool;
+  const int32_t* source;
+  const int32_t* target;
+  const int32_t* tokens;  // NULL: whole pages
+  int64_t pages;
+  int page, Hkv, vecs, layers;                     // vecs: 16-byte pieces of a row
+  int64_t kpl, kpp, kph, kps, vpl, vpp, vph, vps;  // bytes
+};
+
+constexpr int kCopyBatch = 4;
+
+// A thread moves 16-byte pieces of the copied tokens' keys and values, kCopyBatch of them on their way
+// at a time; a workgroup row (y) a page, x over a page's pieces of all layers.
+__global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
+  const int i = blockIdx.y;
+  const int64_t from = p.source[i], to = p.target[i];
+  const int n = p.tokens ? min(p.tokens[i], p.page) : p.page;
+  if (from < 0 || from >= p.pages || to < 0 || to >= p.pages || from == to || n <= 0) return;
+  const int per = n * p.vecs;  // pieces of a layer's keys or values of a head
+  const int64_t all = (int64_t)2 * p.layers * p.Hkv * per, step = (int64_t)gridDim.x * 256;
+  for (int64_t x0 = (int64_t)blockIdx.x * 256 + threadIdx.x; x0 < all; x0 += step * kCopyBatch) {
+    u32x4 v[kCopyBatch];
+    char* at[kCopyBatch];
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u) {
+      const int64_t x = x0 + u * step;
+      if (x >= all) continue;
+      const int of = (int)(x / per), r = (int)(x - (int64_t)of * per), slot = r / p.vecs;
+      const int lv = of / p.Hkv, h = of - lv * p.Hkv, c = r - slot * p.vecs;
+      const bool val = lv & 1;
+      char* const base = (val ? p.vpool : p.kpool) + (lv >> 1) * (val ? p.vpl : p.kpl) +
+                         h * (val ? p.vph : p.kph) + slot * (val ? p.vps : p.kps) + c * 16;
+      const int64_t pp = val ? p.vpp : p.kpp;
+      v[u] = *(const u32x4*)(base + from * pp);
+      at[u] = base + to * pp;
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u)
+      if (x0 + u * step < all) *(u32x4*)at[u] = v[u];
+  }
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" size_t ssa_paged_fork_workspace_size(int64_t B, int64_t W, int64_t pages) {
+  if (B <= 0 || W <= 0 || pages <= 0 || !fits_int(B) || !fits_int(W) || !fits_int(pages)) return 0;
+  return fork_layout(B, W, pages).bytes;
+}
+
+extern "C" int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32_t* lens,
+                              int32_t* table, int64_t table_stride, int64_t B, int64_t W,
+                              int64_t page, int32_t* free_pages, int64_t pages, int32_t* nfree,
+                              int32_t* source, int32_t* target, int32_t* tokens, int32_t* status,
+                              void* workspace, size_t workspace_bytes, ssa_stream_t stream) {
+  const char* const who = "ssa_paged_fork";
+  SSA_REQUIRE(new_lens && lens && table && free_pages && nfree && source && target &&
+                  tokens && status, SSA_ERR_INVALID, "%s: NULL argument", who);
+  SSA_REQUIRE(B > 0 && fits_int(B) && W > 0 && table_stride >= W && pages > 0 && fits_int(pages),
+              SSA_ERR_INVALID, "%s: bad shape (B=%lld, W=%lld, pages=%lld)", who, (long long)B,
+              (long long)W, (long long)pages);
+  SSA_REQUIRE(page > 0 && page % 16 == 0 && page <= 65536, SSA_ERR_UNSUPPORTED,
+              "%s: page of %lld tokens (a multiple of 16 up to 65536)", who, (long long)page);
+  SSA_REQUIRE(W <= 0x7fffffff / page, SSA_ERR_UNSUPPORTED,
+              "%s: a table row of %lld pages holds more than 2^31 - 1 tokens", who, (long long)W);
+  const ForkLayout y = fork_layout(B, W, pages);
+  SSA_REQUIRE(fits_int(y.units) && fits_launch((y.units + 3) / 4, 256), SSA_ERR_UNSUPPORTED,
+              "%s: %lld table rows of %lld pages", who, (long long)B, (long long)W);
+  SSA_REQUIRE(workspace_bytes >= y.bytes && workspace && aligned16(workspace), SSA_ERR_WORKSPACE,
+              "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, y.bytes,
+              workspace_bytes);
+  char* const ws = (char*)workspace;
+  ForkParams p{src, new_lens, lens, table, table_stride, W, W * page, (int)B, (int)page,
+               free_pages, pages, nfree, source, target, tokens, status,
+               page_div((int)page / 16), (PageUse*)ws, (int32_t*)(ws + y.old),
+               (int32_t*)(ws + y.old_lens), (int32_t*)(ws + y.given), (int32_t*)(ws + y.bad),
+               (int32_t*)(ws + y.taken), (int32_t*)(ws + y.left), y.units, (int)y.chunks};
+  hipStream_t st = (hipStream_t)stream;
+  if (y.units <= kForkInside) {
+    paged_fork_kernel<<<1, kForkThreads, 0, st>>>(p);
+    return launch_status("paged_fork_kernel");
+  }
+  const unsigned grid = (unsigned)((y.units + 3) / 4);
+  paged_fork_clear_kernel<<<grid, 256, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_fork_clear_kernel"));
+  paged_fork_mark_kernel<<<grid, 256, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_fork_mark_kernel"));
+  paged_fork_count_kernel<<<grid, 256, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_fork_count_kernel"));
+  paged_fork_sum_kernel<<<1, kForkThreads, 0, st>>>(p);
+  SSA_TRY(launch_status("paged_fork_sum_kernel"));
+  paged_fork_write_kernel<<<grid, 256, 0, st>>>(p);
+  return launch_status("paged_fork_write_kernel");
+}
+
+extern "C" int ssa_paged_copy(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
+                              int64_t d, int64_t pages, int64_t page, const int64_t* strides,
+                              const int32_t* source, const int32_t* target, const int32_t* tokens,
+                              int64_t n, ssa_stream_t stream) {
+  const char* const who = "ssa_paged_copy";
+  SSA_REQUIRE(kpool && vpool && strides && source && target, SSA_ERR_INVALID, "%s: NULL argument",
+              who);
+  SSA_TRY(check_pool(who, dtype, Hkv, d, pages, page));
+  SSA_REQUIRE(n >= 0 && n <= 65535 && layers > 0 && fits_int(layers), SSA_ERR_INVALID,
+              "%s: %lld pages of %lld layers (at most 65535 pages)", who, (long long)n,
+              (long long)layers);
+  const int es = dtype_size(dtype);
+  // strides: kpool(layer,page,head,slot), vpool(layer,page,head,slot)
+  SSA_REQUIRE(rows16(kpool, strides, 4, es) && rows16(vpool, strides + 4, 4, es), SSA_ERR_INVALID,
+              "%s: rows must start at multiples of 16 bytes", who);
+  SSA_REQUIRE(fits_int(2 * layers * Hkv), SSA_ERR_UNSUPPORTED, "%s: %lld layers", who,
+              (long long)layers);
+  if (n == 0) return SSA_OK;
+  const int64_t vecs = d * es / 16, pieces = 2 * layers * Hkv * page * vecs;
+  // at most eight workgroups a CU for all pages, each with kCopyBatch pieces a thread or more
+  const int64_t blocks = std::max<int64_t>(
+      1, std::min((pieces + 256 * kCopyBatch - 1) / (256 * kCopyBatch), (2048 + n - 1) / n));
+  CopyParams p{(char*)kpool, (char*)vpool, source, target, tokens, pages, (int)page, (int)Hkv,
+               (int)vecs, (int)layers,
+               strides[0] * es, strides[1] * es, strides[2] * es, strides[3] * es,
+               strides[4] * es, strides[5] * es, strides[6] * es, strides[7] * es};
+  paged_copy_kernel<<<dim3((unsigned)blocks, (unsigned)n), 256, 0, (hipStream_t)stream>>>(p);
+  return launch_status("paged_copy_kernel");
+}

@@ -75,6 +75,51 @@ SSA_HD PagedRange paged_item_range(const PagedSpan& s, int units, int j, int n) 
   return r;
 }
 
+// Drafted tokens: request b's are rows [cu[b], cu[b + 1]) of the call's N, its last n tokens of the
+// cache. ctx: the tokens before them, the first at position ctx. Keys [span.first, span.len) are
+// attended by some of its rows: a row's position is ctx or later, its window ends there.
+// n is 0 where the offsets do not fit N; span.ok: the tokens fit the cache and the masks (of `words`
+// 32-bit words a row; 0: every token attends those before it).
+struct DraftSpan {
+  int ctx, n;
+  PagedSpan span;
+};
+
+SSA_HD DraftSpan draft_span(int len, int c0, int c1, int64_t N, int window, int words,
+                            int64_t cap) {
+  DraftSpan s{0, c0 >= 0 && c1 >= c0 && (int64_t)c1 <= N ? c1 - c0 : 0, {0, 0, false}};
+  if (s.n == 0) return s;
+  s.span.ok = len >= s.n && (int64_t)len <= cap && (words == 0 || (int64_t)s.n <= 32ll * words);
+  if (!s.span.ok) return s;
+  s.ctx = len - s.n;
+  s.span.len = len;
+  s.span.first = window > 0 && s.ctx >= window ? s.ctx - window + 1 : 0;
+  return s;
+}
+
+// Units of keys; one where rows are only answered (a length that does not fit).
+SSA_HD int draft_units(const DraftSpan& s) {
+  return s.n == 0 ? 0 : s.span.ok ? paged_units(s.span) : 1;
+}
+
+// Tiles of M rows, a row a drafted token and one of the G query heads of a key head.
+SSA_HD int64_t draft_tiles(const DraftSpan& s, int64_t G, int M) {
+  return ((int64_t)s.n * G + M - 1) / M;
+}
+
+// Units per item so that `work` units (of every row tile) make at most `items` items besides one more
+// per row tile.
+SSA_HD int draft_chunk(int64_t work, int64_t items) {
+  const int64_t c = work <= items ? 1 : (work + items - 1) / items;
+  return c > (1 << 30) ? 1 << 30 : (int)c;
+}
+
+// The most row tiles that N tokens of B requests make, and the most items of requests that are cut
+// in more than one (each of their parts is kept for the join): fewer than two per item aimed at.
+SSA_HD int64_t draft_most_tiles(int64_t B, int64_t N, int64_t G, int M) {
+  return N * G / M + (B < N ? B : N);
+}
+
 // Division of a subtile's number (below 2^28: lengths are below 2^31) by the subtiles of a page, D up
 // to 4096, as a multiplication: mul = ceil(2^(31 + shift) / D), 2^shift <= D < 2^(shift + 1), is off
 // by less than 1 in 2^(31 + shift) / D > 2^30, more than any quotient's distance from the next.

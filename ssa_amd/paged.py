@@ -3,6 +3,11 @@
     resize_pages(lens, new_lens, table, free, nfree, page, tokens)   pages taken and given back
     append_pages(k, v, kpool, vpool, slots)                          new tokens into their slots
     attend_pages(q, kpool, vpool, table, lens, ...)                  one new token per request
+    draft_masks(parents, cu, lens, most)                             trees of drafted tokens
+    attend_drafts(q, kpool, vpool, table, lens, cu, drafts, ...)     several tokens per request
+    keep_drafts(kpool, vpool, table, lens, cu, path, counts)         the accepted ones kept
+    fork_pages(src, new_lens, lens, table, free, nfree, page)        requests that share pages
+    copy_pages(kpool, vpool, source, target, tokens)                 what a fork has to copy
     PagedCache                                                       the state these work on
 
 A pool is a (pages, Hkv, page, d) tensor (any strides with a contiguous last dimension, so a
@@ -11,12 +16,14 @@ table[b, j // page] at slot j % page, and its slot number is table[b, j // page]
 The lengths live on the device: every call is asynchronous on the current stream of the tensors'
 device, works under graph capture and synchronises with nothing. What a call can only find out on
 the device (a length beyond the table, too few free pages, a page id outside the pool) is answered
-there: resize_pages changes nothing and writes a status, append_pages skips the row, attend_pages
-returns NaN for the row; no call follows a bad length or page id.
+there: resize_pages and fork_pages change nothing and write a status, append_pages skips the row,
+attend_pages and attend_drafts return NaN for the row, keep_drafts moves nothing and gives a length of
+-1; no call follows a bad length or page id.
 
 attend_pages is the dense counterpart of attend_rows and dense_decode (ivf_decode) for batches of
-requests: the decode of the layers that a routed model leaves dense or sliding. It is not
-differentiable. The reference has no paged cache.
+requests: the decode of the layers that a routed model leaves dense or sliding. attend_drafts is that
+for several new tokens of every request, a tree of drafted ones that a step verifies or the next piece
+of a prompt. They are not differentiable. The reference has no paged cache.
 """
 from __future__ import annotations
 
@@ -39,6 +46,20 @@ class Resized(NamedTuple):
     pos: torch.Tensor     # (tokens,) int32, 0 past the last new token
     cu: torch.Tensor      # (B + 1,) int32
     status: torch.Tensor  # (1,) int32: 0, the number of pages lacking, or a key of RESIZE_ERRORS
+
+
+class Drafts(NamedTuple):
+    """Of every drafted token which of its request's it attends, and its position (draft_masks)."""
+    masks: torch.Tensor   # (N, words) int32: bit i % 32 of word i / 32 for drafted token i
+    pos: torch.Tensor     # (N,) int32: -1 for a token that does not fit, 0 behind the last
+
+
+class Forked(NamedTuple):
+    """What fork_pages returns: of every row the page that has to be copied for it, and the status."""
+    source: torch.Tensor  # (B,) int32, -1 where nothing is copied
+    target: torch.Tensor  # (B,) int32, -1 where nothing is copied
+    tokens: torch.Tensor  # (B,) int32: how many of the page's tokens
+    status: torch.Tensor  # (1,) int32: 0, the number of pages lacking, or -1
 
 
 def _launch(name, t, *args):
@@ -206,10 +227,9 @@ def resize_pages(lens: torch.Tensor, new_lens: torch.Tensor, table: torch.Tensor
     growth does not fit the free pages or `tokens`, or a length its table row, nothing changes, all
     slots are -1 and status says why.
 
-    A page given back is free: nothing counts how many rows list it. Pages that requests share (a common
-    prefix, set by the caller in their table rows and lengths; attend_pages reads them as any others) go
-    back once, by the last request that holds them. Any other is brought to the length of its shared
-    pages here, which gives back its own, and taken out by the caller: its row to -1, its length to 0."""
+    A page given back is free: nothing counts here how many rows list it. Pages that requests share (by
+    fork_pages, or set by the caller in their table rows and lengths) go back once: fork_pages, which
+    looks at all rows, ends and shortens such requests."""
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens={tokens}")
@@ -342,6 +362,286 @@ def _attend_pages_impl(q, kpool, vpool, table, lens, k_new, v_new, scale, window
     return (out, lse) if return_lse else out
 
 
+@functools.lru_cache(maxsize=1024)
+def _masks_plan(parents, cu, lens):
+    """(B, N)"""
+    N, B = parents[0].numel(), lens[0].numel()
+    _int32("parents", *parents, (N,))
+    _int32("cu", *cu, (B + 1,))
+    _int32("lens", *lens, (B,))
+    return B, N
+
+
+def draft_masks(parents: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, most: int) -> Drafts:
+    """Masks and positions of drafted tokens for attend_drafts, once a step for all layers.
+
+    parents (N,) int32: of every drafted token (request by request, cu (B + 1,) int32 their offsets as
+    resize_pages gives them, lens (B,) the lengths with the drafted tokens) the place, among its
+    request's drafted tokens, of the one it continues; -1 for one that continues the context. A token
+    comes after the one it continues. most: the most drafted tokens of a request, up to 1024.
+
+    A token attends itself and its ancestors; its position is the context's length + its ancestors. A
+    parent that does not fit, and what continues it, gives no mask and position -1 (attend_drafts: NaN),
+    as does a request of more than `most` (rounded up to 32) or more than its length. Rows behind the
+    last request's: 0."""
+    if not 1 <= most <= 1024:
+        raise ValueError(f"most={most}: 1 to 1024 drafted tokens a request are served")
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        return Drafts(*T.paged_draft_masks(parents, cu, lens, int(most)))
+    _one_device(parents, cu, lens)
+    B, N = _masks_plan(_meta(parents), _meta(cu), _meta(lens))
+    words = -(-int(most) // 32)
+    new = torch.empty if B else torch.zeros
+    masks = new(N, words, device=parents.device, dtype=torch.int32)
+    pos = new(N, device=parents.device, dtype=torch.int32)
+    if B and N:
+        _launch("ssa_paged_draft_masks", parents, parents.data_ptr(), cu.data_ptr(),
+                lens.data_ptr(), B, N, words, masks.data_ptr(), pos.data_ptr())
+    return Drafts(masks, pos)
+
+
+@functools.lru_cache(maxsize=1024)
+def _drafts_plan(q, kpool, vpool, table, lens, cu, masks, pos, out, window):
+    """(sizes of the call, table's, words, strides, workspace bytes, whether q needs a copy)"""
+    pages, hkv, page, d = _pools(kpool, vpool)
+    dtype = kpool[2]
+    if len(q[0]) != 3 or q[0][2] != d:
+        raise ValueError(f"q must be (N, Hq, {d}), got {tuple(q[0])}")
+    N, hq, _ = q[0]
+    if q[2] != dtype:
+        raise TypeError(f"q is {q[2]}, the cache holds {dtype}")
+    B, W, row = _table(*table)
+    _int32("lens", *lens, (B,))
+    _int32("cu", *cu, (B + 1,))
+    words = 0
+    if masks is not None:
+        if masks[2] != torch.int32:
+            raise TypeError(f"masks is {masks[2]}, expected torch.int32")
+        if len(masks[0]) != 2 or masks[0][0] != N or not 1 <= masks[0][1] <= 32 \
+                or N > 1 and masks[1] != (masks[0][1], 1):
+            raise ValueError(f"masks must be a contiguous ({N}, 1 to 32) tensor, got "
+                             f"{tuple(masks[0])}")
+        words = masks[0][1]
+        _int32("pos", *pos, (N,))
+    to = (hq * d, d)
+    if out is not None:
+        if out[2] != dtype or out[0] != (N, hq, d) or not _rows16(out):
+            raise ValueError(f"out must be a ({N}, {hq}, {d}) {dtype} tensor with rows of 16-byte "
+                             "pieces")
+        _written("out", out)
+        to = out[1][:2]
+    strides = _lib.i64_array((*q[1][:2], *kpool[1][:3], *vpool[1][:3], *to))
+    ws_bytes = _lib.query("ssa_paged_attend_drafts_workspace_size", B, N, hq, hkv, d, W, page,
+                          window)
+    return (_lib.dtype_code(dtype), B, N, hq, hkv, d, pages, page), (row, W), words, strides, \
+        ws_bytes, not _rows16(q)
+
+
+def attend_drafts(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor,
+                  lens: torch.Tensor, cu: torch.Tensor, drafts: Drafts | None = None,
+                  scale: float | None = None, window: int = 0, return_lse: bool = False,
+                  out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Attention of several new tokens per request over its cached keys: q (N, Hq, d), request by
+    request, request b's in rows cu[b] to cu[b + 1] (cu (B + 1,) int32, as resize_pages gives it). They
+    are the last tokens of its lens[b] in the cache (append_pages stores them first).
+
+    Each attends the context, the tokens before the drafted ones, and of the drafted ones those of its
+    mask (draft_masks, or any other masks and positions), without `drafts` those before it and itself.
+    With a window only the keys at the last `window` positions, its own among them, count. Scores, types
+    and heads as attend_pages. A row that attends nothing gets zeros and a log-sum of -inf; values that
+    a row does not attend do not reach it, infinite or NaN ones either. Rows behind the last request's
+    are zeros and -inf; in a given `out` they are left as they were.
+
+    status (1,) int32: a resize's; if that was refused, every row is NaN, as are the rows of a request
+    whose length or pages do not fit. For one token a request attend_pages is the faster call; prompts
+    from their start are sparse_attention's and dense's (ssa_kernel)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    masks, pos = (None, None) if drafts is None else drafts
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        if out is not None and (out.dtype != q.dtype or out.shape != q.shape):
+            raise ValueError(f"out must be a {tuple(q.shape)} {q.dtype} tensor")
+        args = (q, kpool, vpool, table, lens, cu, masks, pos, float(scale), int(window), status)
+        if out is None:
+            out, lse = T.paged_attend_drafts(*args)
+        else:
+            lse = T.paged_attend_drafts_into(*args, out)
+        return (out, lse) if return_lse else out
+    return _attend_drafts_impl(q, kpool, vpool, table, lens, cu, masks, pos, scale, window,
+                               return_lse, out, status)
+
+
+def _attend_drafts_impl(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, return_lse,
+                        out=None, status=None):
+    _one_device(q, kpool, vpool, table, lens, cu, masks, pos, out, status)
+    window = int(window)
+    sizes, rows, words, strides, ws_bytes, copy = _drafts_plan(
+        _meta(q), _meta(kpool), _meta(vpool), _meta(table), _meta(lens), _meta(cu),
+        None if masks is None else _meta(masks), None if pos is None else _meta(pos),
+        None if out is None else _meta(out), window)
+    if copy or q.data_ptr() & 15:
+        return _attend_drafts_impl(_own(q), kpool, vpool, table, lens, cu, masks, pos, scale,
+                                   window, return_lse, out, status)
+    _, B, N, hq, _, d, _, _ = sizes
+    dev = q.device
+    clear = out is None
+    new = torch.empty if B else torch.zeros
+    if out is None:
+        out = new(N, hq, d, device=dev, dtype=q.dtype)
+    lse = torch.empty(N, hq, device=dev, dtype=torch.float32) if return_lse else None
+    if return_lse and (not B or not clear):
+        lse.fill_(-math.inf)
+    if status is not None:
+        _int32("status", *_meta(status), (1,))
+    if B and N:
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+        _launch("ssa_paged_attend_drafts", q, q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
+                out.data_ptr(), _lib.ptr(lse), *sizes, table.data_ptr(), *rows, lens.data_ptr(),
+                cu.data_ptr(), _lib.ptr(masks), _lib.ptr(pos), words, strides, float(scale),
+                window, _lib.ptr(status), int(clear), _lib.ptr(ws), ws_bytes)
+    return (out, lse) if return_lse else out
+
+
+def _layered(meta):
+    """A pool (pages, Hkv, page, d) as one of one layer."""
+    shape, stride, dtype = meta
+    return meta if len(shape) != 4 else ((1, *shape), (0, *stride), dtype)
+
+
+@functools.lru_cache(maxsize=1024)
+def _layers_plan(kpool, vpool):
+    """(dtype, layers, Hkv, d, pages, page, strides) of pools with or without layers"""
+    k, v = _layered(kpool), _layered(vpool)
+    if len(k[0]) != 5 or k[0] != v[0]:
+        raise ValueError(f"kpool and vpool must share a (layers, pages, Hkv, page, d) or (pages, Hkv, "
+                         f"page, d) shape, got {tuple(kpool[0])} and {tuple(vpool[0])}")
+    pages, hkv, page, d = _pools((k[0][1:], k[1][1:], k[2]), (v[0][1:], v[1][1:], v[2]))
+    for name, t in (("kpool", k), ("vpool", v)):
+        _written(name, t)
+    return (_lib.dtype_code(k[2]), k[0][0], hkv, d, pages, page,
+            _lib.i64_array((*k[1][:4], *v[1][:4])))
+
+
+@functools.lru_cache(maxsize=1024)
+def _keep_plan(table, lens, cu, path, counts):
+    """(table's row and width, B, path's row and width)"""
+    B, W, row = _table(*table)
+    _int32("lens", *lens, (B,))
+    _int32("cu", *cu, (B + 1,))
+    _int32("counts", *counts, (B,))
+    if path[2] != torch.int32:
+        raise TypeError(f"path is {path[2]}, expected torch.int32")
+    if len(path[0]) != 2 or path[0][0] != B or path[0][1] > 1 and path[1][1] != 1 \
+            or B > 1 and path[1][0] < 0:
+        raise ValueError(f"path must be ({B}, K) with a contiguous last dimension, got "
+                         f"{tuple(path[0])}")
+    K = path[0][1]
+    # a path that all requests share (expanded) is read by each
+    return row, W, B, path[1][0] if B > 1 else K, K
+
+
+def keep_drafts(kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                cu: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+    """Keeps the accepted ones of the drafted tokens: moves token path[b, i] of request b's (their
+    places among them, ascending; a way down a tree is) to place i, for i < counts[b], in every layer
+    of kpool, vpool (layers, pages, Hkv, page, d), or of one layer's (pages, Hkv, page, d).
+
+    path (B, K), counts (B,) int32, lens and cu as attend_drafts. Returns the lengths after (B,) int32,
+    for the resize_pages that gives back the pages behind them; -1, and nothing is moved, for a request
+    whose path, count, length or pages do not fit. The pages of the drafted tokens must be the request's
+    own."""
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        return T.paged_keep(kpool, vpool, table, lens, cu, path, counts)
+    _one_device(kpool, vpool, table, lens, cu, path, counts)
+    sizes = _layers_plan(_meta(kpool), _meta(vpool))
+    row, W, B, prow, K = _keep_plan(_meta(table), _meta(lens), _meta(cu), _meta(path),
+                                    _meta(counts))
+    new_lens = torch.empty(B, device=lens.device, dtype=torch.int32)
+    if B:
+        _launch("ssa_paged_keep", lens, kpool.data_ptr(), vpool.data_ptr(), *sizes,
+                table.data_ptr(), row, W, lens.data_ptr(), cu.data_ptr(), B,
+                path.data_ptr() if K else None, prow, K, counts.data_ptr(), new_lens.data_ptr())
+    return new_lens
+
+
+@functools.lru_cache(maxsize=1024)
+def _fork_plan(src, new_lens, lens, table, free, nfree):
+    """(table's row, B, W, pages, workspace bytes)"""
+    B, W, row = _table(*table)
+    if src is not None:
+        _int32("src", *src, (B,))
+    _int32("new_lens", *new_lens, (B,))
+    _int32("lens", *lens, (B,))
+    _int32("nfree", *nfree, (1,))
+    _int32("free", *free, (free[0].numel(),))
+    _written("table", table)
+    pages = free[0].numel()
+    return row, B, W, pages, _lib.query("ssa_paged_fork_workspace_size", B, W, pages)
+
+
+def fork_pages(src: torch.Tensor | None, new_lens: torch.Tensor, lens: torch.Tensor,
+               table: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, page: int) -> Forked:
+    """Makes row b of the table the first new_lens[b] tokens of what row src[b] was, on the device: a
+    fork (an answer more for a prompt, a prefix that requests share), beams reordered, and with
+    src[b] = b (src None: all rows) a request cut short or, at 0 tokens, ended.
+
+    src, new_lens (B,) int32; lens, table, free, nfree as resize_pages, and updated. Pages are shared,
+    but a last, partly filled page that another row lists too is taken anew for this one (the lowest row
+    keeps it, if none holds it whole), so that every row grows by resize_pages into pages of its own:
+    copy_pages copies what Forked lists. Pages that no row lists any more are given back; what is taken
+    comes off the stack row by row, and ending forks again restores it.
+
+    All or nothing: if the pages do not suffice, a length is more than its source's, or what the table
+    holds does not fit the pool, nothing changes, nothing is listed, and status says why (-1 is the
+    latter two)."""
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        return Forked(*T.paged_fork(src, new_lens, lens, table, free, nfree, int(page)))
+    _one_device(lens, src, new_lens, table, free, nfree)
+    row, B, W, pages, ws_bytes = _fork_plan(None if src is None else _meta(src), _meta(new_lens),
+                                            _meta(lens), _meta(table), _meta(free), _meta(nfree))
+    new = torch.empty if B else torch.zeros
+    i32 = dict(device=lens.device, dtype=torch.int32)
+    out = Forked(*(new(n, **i32) for n in (B, B, B, 1)))
+    if B:
+        ws = torch.empty(ws_bytes, device=lens.device, dtype=torch.uint8)
+        _launch("ssa_paged_fork", lens, _lib.ptr(src), new_lens.data_ptr(), lens.data_ptr(),
+                table.data_ptr(), row, B, W, int(page), free.data_ptr(), pages, nfree.data_ptr(),
+                *(t.data_ptr() for t in out), ws.data_ptr(), ws_bytes)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _copy_plan(source, target, tokens):
+    n = source[0].numel()
+    _int32("source", *source, (n,))
+    _int32("target", *target, (n,))
+    if tokens is not None:
+        _int32("tokens", *tokens, (n,))
+    return n
+
+
+def copy_pages(kpool: torch.Tensor, vpool: torch.Tensor, source: torch.Tensor,
+               target: torch.Tensor, tokens: torch.Tensor | None = None) -> None:
+    """Copies page source[i] to page target[i], its first tokens[i] tokens (None: all), keys and
+    values, in every layer of kpool, vpool (layers, pages, Hkv, page, d), or of one layer's. source,
+    target, tokens (n,) int32; a pair with an id outside the pool, as -1, is skipped. A target is listed
+    once and is no source."""
+    if torch.compiler.is_compiling():
+        from . import torch_ops as T
+        T.paged_copy(kpool, vpool, source, target, tokens)
+        return
+    _one_device(kpool, vpool, source, target, tokens)
+    sizes = _layers_plan(_meta(kpool), _meta(vpool))
+    n = _copy_plan(_meta(source), _meta(target), None if tokens is None else _meta(tokens))
+    if n:
+        _launch("ssa_paged_copy", kpool, kpool.data_ptr(), vpool.data_ptr(), *sizes,
+                source.data_ptr(), target.data_ptr(), _lib.ptr(tokens), n)
+
+
 class PagedCache:
     """The keys and values of up to `requests` requests in `pages` pages per layer.
 
@@ -352,10 +652,19 @@ class PagedCache:
         cache.append(layer, k, v, r.slots)                # a prompt's tokens, or
         o = cache.step(layer, q, k_new, v_new)            # one token of every request
 
-    A request ends by a resize to length 0 (one that shares pages: as resize_pages says); q, k_new and
-    v_new have a row for every request, idle ones included. After a resize that did not fit, append and step store nothing and attend and step give
-    NaN, until a resize fits; `check` raises then (it synchronises; a caller that keeps count of the
-    pages need not call it)."""
+    Several tokens a request, drafted ones that the step verifies, are stored and attended alike, and
+    the accepted ones kept:
+
+        r = cache.resize(cache.lens + drafted, tokens)
+        drafts = draft_masks(parents, r.cu, cache.lens, most)
+        cache.append(layer, k, v, r.slots)                # layer by layer
+        o = cache.attend_drafts(layer, q, r.cu, drafts)
+        cache.accept(r.cu, path, counts)                  # every layer at once
+
+    A request ends by a resize to length 0, or by a fork to it where requests share pages (`fork`); q,
+    k_new and v_new have a row for every request, idle ones included. After a resize or fork that did
+    not fit, append and step store nothing and attend, attend_drafts and step give NaN, until one fits;
+    `check` raises then (it synchronises; a caller that keeps count of the pages need not call it)."""
 
     def __init__(self, requests, max_len, pages, hkv, d, page=64, layers=1, dtype=torch.bfloat16,
                  device="cuda", token_major=False):
@@ -392,10 +701,10 @@ class PagedCache:
         return r
 
     def check(self) -> None:
-        """Raises if the last resize changed nothing because it did not fit. Synchronises."""
+        """Raises if the last resize or fork changed nothing because it did not fit. Synchronises."""
         status = int(self.status)
         if status:
-            raise RuntimeError("resize: " + RESIZE_ERRORS.get(status, f"{status} pages lacking"))
+            raise RuntimeError("resize or fork: " + RESIZE_ERRORS.get(status, f"{status} pages lacking"))
 
     @torch.no_grad()
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -414,5 +723,28 @@ class PagedCache:
         """attend with the newest token of every request stored first."""
         return self.attend(layer, q, k_new=k_new, v_new=v_new, **kwargs)
 
+    @torch.no_grad()
+    def attend_drafts(self, layer: int, q: torch.Tensor, cu: torch.Tensor,
+                      drafts: Drafts | None = None, **kwargs):
+        """attend_drafts over a layer's pools (scale, window, return_lse, out as there)."""
+        return attend_drafts(q, self.k[layer], self.v[layer], self.table, self.lens, cu, drafts,
+                             status=self.status, **kwargs)
 
-__all__ = ["resize_pages", "append_pages", "attend_pages", "PagedCache", "Resized"]
+    @torch.no_grad()
+    def accept(self, cu: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> Resized:
+        """keep_drafts in every layer, and the resize to the lengths it gives. A path or count that does
+        not fit refuses the resize (status -1); the other requests' tokens are moved then."""
+        return self.resize(keep_drafts(self.k, self.v, self.table, self.lens, cu, path, counts), 0)
+
+    @torch.no_grad()
+    def fork(self, src: torch.Tensor | None, new_lens: torch.Tensor) -> Forked:
+        """fork_pages on this cache's state and copy_pages in every layer. attend, attend_drafts, step
+        and check go by its status as by a resize's."""
+        f = fork_pages(src, new_lens, self.lens, self.table, self.free, self.nfree, self.page)
+        torch.add(f.status, 0, out=self.status)
+        copy_pages(self.k, self.v, f.source, f.target, f.tokens)
+        return f
+
+
+__all__ = ["resize_pages", "append_pages", "attend_pages", "draft_masks", "attend_drafts",
+           "keep_drafts", "fork_pages", "copy_pages", "PagedCache", "Resized", "Drafts", "Forked"]

@@ -25,6 +25,14 @@ dtypes. Run eagerly, the public functions call the library directly and skip the
     ssa_amd::paged_attend(q, kpool, vpool, table, lens, scale, window, status) -> (out, lse)
     ssa_amd::paged_step(q, kpool!, vpool!, table, lens, k_new, v_new, scale, window, status)
         -> (out, lse)
+    ssa_amd::paged_draft_masks(parents, cu, lens, most) -> (masks, pos)
+    ssa_amd::paged_attend_drafts(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, status)
+        -> (out, lse)
+    ssa_amd::paged_attend_drafts_into(..., out!) -> lse
+    ssa_amd::paged_keep(kpool!, vpool!, table, lens, cu, path, counts) -> new_lens
+    ssa_amd::paged_fork(src, new_lens, lens!, table!, free!, nfree!, page)
+        -> (source, target, tokens, status)
+    ssa_amd::paged_copy(kpool!, vpool!, source, target, tokens)
     (! = written in place; workspace None runs the allocation-free ssa_decode_step_static; the
     reference has no paged cache)
 """
@@ -212,3 +220,83 @@ def paged_step(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Ten
 def _(q, kpool, vpool, table, lens, k_new, v_new, scale, window, status=None):
     return (torch.empty_like(q, memory_format=torch.contiguous_format),
             q.new_empty(q.shape[:2], dtype=_F32))
+
+
+@torch.library.custom_op("ssa_amd::paged_draft_masks", mutates_args=())
+def paged_draft_masks(parents: Tensor, cu: Tensor, lens: Tensor,
+                      most: int) -> tuple[Tensor, Tensor]:
+    from .paged import draft_masks
+    return tuple(draft_masks(parents, cu, lens, most))
+
+
+@paged_draft_masks.register_fake
+def _(parents, cu, lens, most):
+    N = parents.shape[0]
+    return parents.new_empty(N, -(-most // 32)), parents.new_empty(N)
+
+
+@torch.library.custom_op("ssa_amd::paged_attend_drafts", mutates_args=())
+def paged_attend_drafts(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
+                        cu: Tensor, masks: Optional[Tensor], pos: Optional[Tensor], scale: float,
+                        window: int, status: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    from .paged import _attend_drafts_impl
+    return _attend_drafts_impl(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, True,
+                               None, status)
+
+
+@paged_attend_drafts.register_fake
+def _(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, status=None):
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            q.new_empty(q.shape[:2], dtype=_F32))
+
+
+@torch.library.custom_op("ssa_amd::paged_attend_drafts_into", mutates_args=("out",))
+def paged_attend_drafts_into(q: Tensor, kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor,
+                             cu: Tensor, masks: Optional[Tensor], pos: Optional[Tensor],
+                             scale: float, window: int, status: Optional[Tensor],
+                             out: Tensor) -> Tensor:
+    from .paged import _attend_drafts_impl
+    return _attend_drafts_impl(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, True,
+                               out, status)[1]
+
+
+@paged_attend_drafts_into.register_fake
+def _(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, status, out):
+    return q.new_empty(q.shape[:2], dtype=_F32)
+
+
+@torch.library.custom_op("ssa_amd::paged_keep", mutates_args=("kpool", "vpool"))
+def paged_keep(kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor, cu: Tensor, path: Tensor,
+               counts: Tensor) -> Tensor:
+    from .paged import keep_drafts
+    return keep_drafts(kpool, vpool, table, lens, cu, path, counts)
+
+
+@paged_keep.register_fake
+def _(kpool, vpool, table, lens, cu, path, counts):
+    return lens.new_empty(lens.shape[0])
+
+
+@torch.library.custom_op("ssa_amd::paged_fork", mutates_args=("lens", "table", "free", "nfree"))
+def paged_fork(src: Optional[Tensor], new_lens: Tensor, lens: Tensor, table: Tensor, free: Tensor,
+               nfree: Tensor, page: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    from .paged import fork_pages
+    return tuple(fork_pages(src, new_lens, lens, table, free, nfree, page))
+
+
+@paged_fork.register_fake
+def _(src, new_lens, lens, table, free, nfree, page):
+    B = lens.shape[0]
+    return lens.new_empty(B), lens.new_empty(B), lens.new_empty(B), lens.new_empty(1)
+
+
+@torch.library.custom_op("ssa_amd::paged_copy", mutates_args=("kpool", "vpool"))
+def paged_copy(kpool: Tensor, vpool: Tensor, source: Tensor, target: Tensor,
+               tokens: Optional[Tensor]) -> None:
+    from .paged import copy_pages
+    copy_pages(kpool, vpool, source, target, tokens)
+
+
+@paged_copy.register_fake
+def _(kpool, vpool, source, target, tokens):
+    return None

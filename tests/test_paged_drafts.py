@@ -1,0 +1,220 @@
+"""Drafted tokens and shared pages over the paged cache without a GPU: arguments refused at the C ABI and in
+Python, shapes of the registered operators, and the plain restatements that the GPU tests compare with."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from ssa_amd import _lib
+from ssa_amd import paged as P
+from tests import drafts_util as D
+from tests.test_paged import FAKE, NULL, status
+
+ODD = ctypes.c_void_p((1 << 20) + 8)
+INVALID, UNSUPPORTED, SPACE = _lib.SSA_ERR_INVALID, _lib.SSA_ERR_UNSUPPORTED, _lib.SSA_ERR_WORKSPACE
+
+
+def attend(**kw):
+    a = dict(q=FAKE, kpool=FAKE, vpool=FAKE, out=FAKE, lse=NULL, dtype=_lib.BF16, B=2, N=9, Hq=4,
+             Hkv=2, d=64, pages=10, page=16, table=FAKE, table_stride=8, W=8, lens=FAKE, cu=FAKE,
+             masks=FAKE, pos=FAKE, words=1,
+             strides=_lib.i64_array([256, 64, 2048, 1024, 64, 2048, 1024, 64, 256, 64]),
+             scale=0.125, window=0, status=NULL, clear=1, ws=FAKE, ws_bytes=1 << 40)
+    a.update(kw)
+    return status("ssa_paged_attend_drafts", *a.values(), None)
+
+
+WIDE = dict(W=1000, table_stride=1000)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(q=NULL), INVALID), (dict(lens=NULL), INVALID), (dict(cu=NULL), INVALID),
+    (dict(masks=NULL), INVALID), (dict(pos=NULL), INVALID), (dict(words=0), INVALID),
+    (dict(masks=NULL, pos=NULL), INVALID), (dict(words=33), UNSUPPORTED),
+    (dict(words=-1), UNSUPPORTED), (dict(dtype=7), UNSUPPORTED), (dict(d=60), UNSUPPORTED),
+    (dict(d=520), UNSUPPORTED), (dict(page=24), UNSUPPORTED), (dict(Hq=3), INVALID),
+    (dict(B=0), INVALID), (dict(B=65536), INVALID), (dict(N=0), INVALID), (dict(N=2 ** 31), INVALID),
+    (dict(pages=0), INVALID), (dict(W=0), INVALID), (dict(W=9), INVALID),
+    (dict(W=2 ** 27, table_stride=2 ** 27), INVALID), (dict(window=-1), INVALID),
+    (dict(window=2 ** 31), INVALID), (dict(q=ODD), INVALID), (dict(out=ODD), INVALID),
+    (dict(strides=_lib.i64_array([256, 64, 2048, 1024, 60] + [64] * 5)), INVALID),
+    (dict(strides=_lib.i64_array([64] * 4 + [-64] + [64] * 5)), INVALID),
+    (dict(strides=_lib.i64_array([64] * 4 + [2 ** 24] + [64] * 5)), UNSUPPORTED),
+    (dict(strides=_lib.i64_array([64] * 7 + [2 ** 24] + [64] * 2)), UNSUPPORTED),
+    (dict(N=2 ** 31 - 1, Hq=64, Hkv=64), UNSUPPORTED),
+    (dict(ws_bytes=1000, **WIDE), SPACE), (dict(ws=NULL, **WIDE), SPACE), (dict(ws=ODD, **WIDE), SPACE),
+])
+def test_attend_refuses(change, code):
+    assert attend(**change) == code
+    assert b"ssa_paged_attend_drafts" in _lib.lib().ssa_last_error()
+
+
+def test_masks_refuse():
+    f = lambda parents=FAKE, cu=FAKE, B=2, N=9, words=1: status(  # noqa: E731
+        "ssa_paged_draft_masks", parents, cu, FAKE, B, N, words, FAKE, FAKE, None)
+    assert f(parents=NULL) == INVALID and f(cu=NULL) == INVALID
+    assert f(B=0) == INVALID and f(N=-1) == INVALID and f(N=2 ** 31) == INVALID
+    assert f(words=0) == UNSUPPORTED and f(words=33) == UNSUPPORTED
+    assert f(B=2 ** 30) == UNSUPPORTED
+    assert f(parents=NULL, N=0) == _lib.SSA_OK  # nothing to do, nothing launched
+    with pytest.raises(ValueError, match="most=0"):
+        P.draft_masks(None, None, None, 0)
+    with pytest.raises(ValueError, match="most=1025"):
+        P.draft_masks(None, None, None, 1025)
+
+
+S8 = _lib.i64_array([20480, 2048, 1024, 64] * 2)
+
+
+def test_keep_refuses():
+    def f(kpool=FAKE, dtype=_lib.F16, layers=1, hkv=2, d=64, pages=10, page=16, st=S8, W=8, B=2,
+          path=FAKE, stride=3, width=3):
+        return status("ssa_paged_keep", kpool, FAKE, dtype, layers, hkv, d, pages, page, st, FAKE, 8,
+                      W, FAKE, FAKE, B, path, stride, width, FAKE, FAKE, None)
+    assert f(kpool=NULL) == INVALID and f(path=NULL) == INVALID and f(B=0) == INVALID
+    assert f(B=65536) == INVALID and f(layers=0) == INVALID and f(width=-1) == INVALID
+    assert f(stride=-3) == INVALID and f(W=9) == INVALID and f(kpool=ODD) == INVALID
+    assert f(dtype=5) == UNSUPPORTED and f(d=20) == UNSUPPORTED and f(page=20) == UNSUPPORTED
+    assert f(layers=2 ** 30) == UNSUPPORTED and f(layers=2 ** 20, B=65535) == UNSUPPORTED
+    assert f(st=_lib.i64_array([64, 64, 64, 60] * 2)) == INVALID
+
+
+def test_fork_and_copy_refuse():
+    def f(new=FAKE, stride=8, B=2, W=8, page=16, pages=10, ws=FAKE, n=1 << 40):
+        return status("ssa_paged_fork", NULL, new, FAKE, FAKE, stride, B, W, page, FAKE, pages,
+                      FAKE, FAKE, FAKE, FAKE, FAKE, ws, n, None)
+    assert f(new=NULL) == INVALID and f(B=0) == INVALID and f(stride=7) == INVALID
+    assert f(pages=0) == INVALID and f(pages=2 ** 31) == INVALID
+    assert f(page=17) == UNSUPPORTED and f(W=2 ** 27, stride=2 ** 27) == UNSUPPORTED
+    assert f(B=2 ** 30, W=2 ** 13, stride=2 ** 13) == UNSUPPORTED
+    assert f(ws=NULL) == SPACE and f(ws=ODD) == SPACE and f(n=100) == SPACE
+    assert _lib.query("ssa_paged_fork_workspace_size", 0, 1, 1) == 0
+
+    def c(kpool=FAKE, dtype=_lib.F16, layers=1, d=64, page=16, st=S8, n=3):
+        return status("ssa_paged_copy", kpool, FAKE, dtype, layers, 2, d, 10, page, st, FAKE, FAKE,
+                      NULL, n, None)
+    assert c(kpool=NULL) == INVALID and c(n=-1) == INVALID and c(n=65536) == INVALID
+    assert c(layers=0) == INVALID and c(kpool=ODD) == INVALID
+    assert c(dtype=5) == UNSUPPORTED and c(d=20) == UNSUPPORTED and c(page=20) == UNSUPPORTED
+    assert c(layers=2 ** 30) == UNSUPPORTED
+    assert c(n=0) == _lib.SSA_OK
+
+
+def test_python_refuses(monkeypatch):
+    """Shapes and types are refused before anything is launched (on tensors of one device)."""
+    monkeypatch.setattr(P, "_one_device", lambda *a: None)
+    monkeypatch.setattr(P, "_launch", lambda *a: pytest.fail("launched"))
+    i32 = lambda *n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    pool, q = torch.zeros(9, 2, 16, 64), torch.zeros(5, 4, 64)
+    lens, cu, table = i32(3), i32(4), i32(3, 2)
+    good = dict(q=q, kpool=pool, vpool=pool, table=table, lens=lens, cu=cu, drafts=None)
+    for kw in (dict(q=q[0]), dict(q=q[..., :32]), dict(q=q.half()), dict(lens=lens[:2]),
+               dict(cu=lens), dict(cu=cu.long()), dict(table=table.float()),
+               dict(drafts=P.Drafts(i32(4, 1), i32(5))), dict(drafts=P.Drafts(i32(5, 1), i32(4))),
+               dict(drafts=P.Drafts(i32(5, 33), i32(5))), dict(drafts=P.Drafts(i32(5), i32(5))),
+               dict(drafts=P.Drafts(i32(5, 1).long(), i32(5))),
+               dict(drafts=P.Drafts(i32(1, 5).t(), i32(5))[:1] + (i32(5).long(),)),
+               dict(drafts=P.Drafts(i32(2, 5).t(), i32(5))), dict(vpool=pool[:8]),
+               dict(out=q.half()), dict(out=q[:4]), dict(out=q[:1].expand(5, 4, 64))):
+        with pytest.raises((ValueError, TypeError)):
+            P.attend_drafts(**{**good, **kw})
+    for parents, c, n in ((i32(5, 1)[:, 0].long(), cu, lens), (i32(5), lens, lens),
+                          (i32(5), cu.long(), lens)):
+        with pytest.raises((ValueError, TypeError)):
+            P.draft_masks(parents, c, n, 5)
+    path, layers = i32(3, 2), torch.zeros(2, 9, 2, 16, 64)
+    for kw in (dict(path=path.long()), dict(path=path[:2]), dict(path=i32(3)), dict(counts=cu),
+               dict(path=i32(2, 3).t()), dict(kpool=layers), dict(kpool=layers[0].half()),
+               dict(kpool=layers[0, :1].expand(9, 2, 16, 64)), dict(cu=lens)):
+        a = dict(kpool=pool, vpool=pool, table=table, lens=lens, cu=cu, path=path, counts=lens)
+        with pytest.raises((ValueError, TypeError)):
+            P.keep_drafts(**{**a, **kw})
+    for kw in (dict(src=cu), dict(src=lens.long()), dict(new_lens=cu), dict(lens=lens[:2]),
+               dict(table=i32(3, 1).expand(3, 2)), dict(nfree=cu), dict(free=i32(2, 9).t())):
+        a = dict(src=lens, new_lens=lens, lens=lens, table=table, free=i32(9), nfree=i32(1), page=16)
+        with pytest.raises((ValueError, TypeError)):
+            P.fork_pages(**{**a, **kw})
+    for args in ((cu, lens, None), (lens, lens.long(), None), (lens, lens, cu)):
+        with pytest.raises((ValueError, TypeError)):
+            P.copy_pages(layers, layers.clone(), *args)
+    empty = P.fork_pages(None, i32(0), i32(0), i32(0, 2), i32(9), i32(1), 16)
+    assert [x.tolist() for x in empty] == [[], [], [], [0]]
+
+
+def test_cpu_tensors_raise():
+    i = torch.zeros(1, dtype=torch.int32)
+    pool, q, cu = torch.zeros(2, 2, 16, 64), torch.zeros(1, 2, 64), torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: P.attend_drafts(q, pool, pool, i.view(1, 1), i, cu),
+                 lambda: P.draft_masks(i, cu, i, 4),
+                 lambda: P.keep_drafts(pool, pool, i.view(1, 1), i, cu, i.view(1, 1), i),
+                 lambda: P.fork_pages(i, i, i, i.view(1, 1), i, i, 16),
+                 lambda: P.copy_pages(pool, pool, i, i)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+def test_registered_operators_give_shapes():
+    import ssa_amd  # noqa: F401  (registers the ops)
+    ops = torch.ops.ssa_amd
+    m = dict(device="meta")
+    i32 = lambda *n: torch.empty(n, dtype=torch.int32, **m)  # noqa: E731
+    q = torch.empty(5, 4, 64, dtype=torch.float16, **m)
+    pool = torch.empty(9, 2, 16, 64, dtype=torch.float16, **m)
+    masks, pos = ops.paged_draft_masks(i32(5), i32(4), i32(3), 40)
+    assert masks.shape == (5, 2) and pos.shape == (5,) and masks.dtype == torch.int32
+    for a in ((None, None), (masks, pos)):
+        out, lse = ops.paged_attend_drafts(q, pool, pool, i32(3, 2), i32(3), i32(4), *a, 0.1, 0, None)
+        assert out.shape == q.shape and out.dtype == q.dtype
+        assert lse.shape == (5, 4) and lse.dtype == torch.float32
+        lse = ops.paged_attend_drafts_into(q, pool, pool, i32(3, 2), i32(3), i32(4), *a, 0.1, 0,
+                                           None, torch.empty_like(q))
+        assert lse.shape == (5, 4)
+    new = ops.paged_keep(pool, pool.clone(), i32(3, 2), i32(3), i32(4), i32(3, 2), i32(3))
+    assert new.shape == (3,) and new.dtype == torch.int32
+    for src in (None, i32(3)):
+        f = ops.paged_fork(src, i32(3), i32(3), i32(3, 2), i32(9), i32(1), 16)
+        assert [tuple(x.shape) for x in f] == [(3,), (3,), (3,), (1,)]
+    assert ops.paged_copy(pool, pool.clone(), i32(3), i32(3), None) is None
+
+
+def test_plain_fork_keeps_every_page_once():
+    """After any run of resizes and forks a page is free or listed, the last partly filled ones by one
+    row each."""
+    rng = random.Random(0)
+    s = D.ForkState(6, 10, 40, 16)
+    for step in range(300):
+        if step % 2:
+            new = [min(160, n + rng.randrange(40)) for n in s.lens]
+            s.resize(new, 2000)
+        else:
+            src = [rng.randrange(6) for _ in range(6)]
+            s.fork(src, [rng.choice([s.lens[a], rng.randrange(s.lens[a] + 1), 0]) for a in src])
+        held = [row[:-(-n // 16)] for row, n in zip(s.table, s.lens)]
+        assert sorted(set(sum(held, [])) | set(s.free)) == list(range(40))
+        assert len(set(s.free)) == len(s.free) and not set(s.free) & set(sum(held, []))
+        last = [row[-1] for row, n in zip(held, s.lens) if n % 16]
+        assert all(sum(x in row for row in held) == 1 for x in last)
+
+
+def test_plain_attention_is_the_softmax_of_the_attended_keys():
+    """The restatement against a loop over rows, with what is not attended left out."""
+    torch.manual_seed(0)
+    pool = torch.randn(4, 1, 16, 8)
+    table, lens = torch.tensor([[2, 0], [3, -1]]), torch.tensor([21, 9])
+    cu, q = torch.tensor([0, 5, 8]), torch.randn(8, 2, 8)
+    parents = [-1, 0, 0, -1, 2, -1, 0, 0]
+    masks, pos = D.masks_and_pos(parents, [5, 3], [21, 9], 1, 8)
+    for window in (0, 3):
+        out, lse, _, _ = D.attend(q, pool, pool, table, lens, cu, 0.3, window,
+                                  torch.tensor(masks), torch.tensor(pos))
+        for row, (b, see) in enumerate([(0, x) for x in D.ancestors(parents[:5])]
+                                       + [(1, x) for x in D.ancestors(parents[5:])]):
+            ctx = (16, 6)[b]
+            keys = [j for j in range(ctx) if not window or j > pos[row] - window]
+            keys += [ctx + i for i in see if not window or pos[cu[b] + i] > pos[row] - window]
+            k = torch.stack([pool[table[b, j // 16], 0, j % 16] for j in keys]).double()
+            for h in range(2):
+                s = k @ q[row, h].double() * 0.3
+                torch.testing.assert_close(out[row, h], torch.softmax(s, 0) @ k)
+                torch.testing.assert_close(lse[row, h], torch.logsumexp(s, 0))
