@@ -580,8 +580,9 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
 int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu, const int32_t* lens, int64_t B,
                           int64_t N, int64_t words, int32_t* masks, int32_t* pos,
                           ssa_stream_t stream);
-size_t ssa_paged_attend_drafts_workspace_size(int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
-                                              int64_t d, int64_t W, int64_t page, int64_t window);
+size_t ssa_paged_attend_drafts_workspace_size(int dtype, int64_t B, int64_t N, int64_t Hq,
+                                              int64_t Hkv, int64_t d, int64_t W, int64_t page,
+                                              int64_t window);
 int ssa_paged_attend_drafts(const void* q, const void* kpool, const void* vpool, void* out,
                             float* lse, int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
                             int64_t d, int64_t pages, int64_t page, const int32_t* table,

@@ -103,7 +103,7 @@ _SIGNATURES = {
     "ssa_paged_attend": (_c_int, [_c_p] * 5 + [_c_int] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] +
                          [_c_p] * 4 + [_c_f, _c_i64, _c_p, _c_p, _c_sz, _c_p]),
     "ssa_paged_draft_masks": (_c_int, [_c_p] * 3 + [_c_i64] * 3 + [_c_p] * 3),
-    "ssa_paged_attend_drafts_workspace_size": (_c_sz, [_c_i64] * 8),
+    "ssa_paged_attend_drafts_workspace_size": (_c_sz, [_c_int] + [_c_i64] * 8),
     "ssa_paged_attend_drafts": (_c_int, [_c_p] * 5 + [_c_int] + [_c_i64] * 7 +
                                 [_c_p, _c_i64, _c_i64] + [_c_p] * 4 +
                                 [_c_i64, _c_p, _c_f, _c_i64, _c_p, _c_int, _c_p, _c_sz, _c_p]),

@@ -214,6 +214,34 @@ __device__ inline DraftItem uniform(const DraftItem& x) {
                                        uniform((int)x.s.span.ok) != 0}}};
 }
 
+// Which of the 64 keys from j0 on a row attends: bit j - j0. tok, pos, start: the row's place among its
+// request's n drafted tokens, its position and its first key.
+__device__ inline uint64_t attended_keys(const DraftParams& p, const DraftItem& it, int tok, int start,
+                                         int j0) {
+  const int ctx = it.s.ctx, i0 = j0 - ctx;  // the first key's place among the drafted ones
+  auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
+  const uint64_t context = below(-(int64_t)i0) & ~below((int64_t)start - j0);
+  if (i0 + 64 <= 0) return context;
+  uint64_t bits;
+  if (!p.masks) {
+    bits = below((int64_t)tok - i0 + 1) & ~below((int64_t)start - j0);
+  } else {
+    const int32_t* const words = p.masks + ((int64_t)it.c0 + tok) * p.words;
+    auto word = [&](int w) { return w >= 0 && w < p.words ? (uint64_t)(unsigned)words[w] : 0ull; };
+    const int w = i0 >> 5, r = i0 & 31;
+    const uint64_t lo = word(w) | word(w + 1) << 32;
+    bits = r ? lo >> r | word(w + 2) << (64 - r) : lo;
+    bits &= below((int64_t)it.s.n - i0);
+    if (p.window > 0) {
+      for (uint64_t left = bits; left; left &= left - 1) {
+        const int x = __builtin_ctzll(left);
+        if (p.pos[(int64_t)it.c0 + i0 + x] < start) bits &= ~(1ull << x);
+      }
+    }
+  }
+  return context | (bits & ~below(-(int64_t)i0) & below((int64_t)it.s.n - i0));
+}
+
 // Rows that no request holds: zeros where the call wants them cleared; every row NaN after a refused
 // resize. Block `id` of kRestBlocks.
 template <int DT>
@@ -281,11 +309,20 @@ __device__ inline unsigned int kind_of(unsigned int w) {
   }
 }
 
-// Zeros and ones as two 16-bit numbers.
+// Two 16-bit numbers, 0 or 1.
 template <int DT>
-__device__ inline unsigned int pack16(float a, float b) {
+__device__ inline unsigned int pack16(bool a, bool b) {
   constexpr unsigned int one = DT == SSA_BF16 ? 0x3f80u : 0x3c00u;
-  return (a != 0.0f ? one : 0u) | (b != 0.0f ? one << 16 : 0u);
+  return (a ? one : 0u) | (b ? one << 16 : 0u);
+}
+
+// What sums of kinds say: with[r] over keys of a weight, without over those of weight zero.
+__device__ inline float not_finite_sum(float with, float without) {
+  const int kinds = (int)with;
+  float v = kinds >= 1 << 15 || without > 0.0f ? NAN : 0.0f;
+  if (kinds & 0xff) v += INFINITY;
+  if (kinds & 0x7f00) v -= INFINITY;
+  return v;
 }
 
 // Attention of a row tile (MT times 16 rows, a row a drafted token's query head of the key head) over
@@ -457,24 +494,12 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   };
   // which of this lane's keys of the tile from j0 on its row attends: bit 4 t + r
   auto attended = [&](int mt, int j0) {
+    const uint64_t keys = attended_keys(p, it, tok[mt], start[mt], j0) >> grp * 4;
     unsigned int bits = 0;
-    const int32_t* const words = p.masks + ((int64_t)it.c0 + tok[mt]) * p.words;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = j0 + t * 16 + grp * 4 + r, i = j - ctx;
-        bool yes = i < 0 ? j >= start[mt] : false;
-        if (i >= 0 && j < len) {
-          if (!p.masks) yes = i <= tok[mt] && j >= start[mt];
-          else yes = (words[i >> 5] >> (i & 31) & 1) &&
-                     (p.window == 0 || p.pos[(int64_t)it.c0 + i] >= start[mt]);
-        }
-        bits |= yes ? 1u << (t * 4 + r) : 0;
-      }
+    for (int t = 0; t < NT; ++t) bits |= (unsigned)(keys >> t * 16 & 15) << t * 4;
     return bits;
   };
-
   auto each_value = [&](auto f) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -525,21 +550,14 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
                 kinds[2 * t + h] = kind_of<DT>(__builtin_amdgcn_perm(
                     rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
                     e % 2 ? 0x07060302u : 0x05040100u));
-                a[2 * t + h] = pack16<DT>(some[mt][t][2 * h], some[mt][t][2 * h + 1]);
-                b[2 * t + h] = pack16<DT>(none[mt][t][2 * h], none[mt][t][2 * h + 1]);
+                a[2 * t + h] = pack16<DT>(some[mt][t][2 * h] != 0.0f, some[mt][t][2 * h + 1] != 0.0f);
+                b[2 * t + h] = pack16<DT>(none[mt][t][2 * h] != 0.0f, none[mt][t][2 * h + 1] != 0.0f);
               }
             x = mfma16(kinds, a, x, DT == SSA_BF16);
             y = mfma16(kinds, b, y, DT == SSA_BF16);
           }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int kinds = (int)x[r];
-            const bool nan = kinds >= 1 << 15 || y[r] > 0.0f;
-            float v = nan ? NAN : 0.0f;
-            if (kinds & 0xff) v += INFINITY;
-            if (kinds & 0x7f00) v -= INFINITY;
-            st[mt].acc[vb * LC + e][r] += v;
-          }
+          for (int r = 0; r < 4; ++r) st[mt].acc[vb * LC + e][r] += not_finite_sum(x[r], y[r]);
         }
   };
 
@@ -762,6 +780,333 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   }
 }
 
+// ---- many rows -----------------------------------------------------------------------------------
+
+// A tile of kKeys keys in LDS as rows of DP 16-bit numbers; 16-byte chunk c of row r lies at chunk
+// c ^ tile_swz(r), so that the 16 lanes of a ds_read_b128 phase (rows r..r + 15) and the 32 of a
+// transposing read (four rows, four chunks) meet every bank once.
+constexpr int kKeys = 64;
+
+template <int DP>
+__device__ inline int tile_swz(int r) {
+  if constexpr (DP == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);  // two rows fill the banks
+  return (r & 3) << 2 | (r >> 2 & 3);
+}
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// Weights of two keys as exact 16-bit parts (bf16: three, cut; fp16: two of 22 bits).
+template <int DT>
+__device__ inline void cut(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
+  if constexpr (DT == SSA_BF16) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const unsigned int a = __float_as_uint(p0), b = __float_as_uint(p1);
+      w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      p0 -= __uint_as_float(a & 0xffff0000u);
+      p1 -= __uint_as_float(b & 0xffff0000u);
+    }
+  } else {
+    const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+    w[0] = __builtin_bit_cast(unsigned int, h);
+    w[1] = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0],
+                                                                       p1 - (float)h[1]));
+  }
+}
+
+__device__ inline f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c, bool bf16) {
+  if (bf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Attention of 128 rows over an item's keys, a wave's 32 rows against all of them: tiles of 64 keys go
+// from memory to LDS, one ahead of the products, and serve the four waves. Scores are K Q^T: lane column
+// a row, so its statistics and its weights stay in its lanes and are the second product's operand as they
+// are; values are transposed by the LDS reads. A row's maximum is raised only where it grows by more
+// than kGrow, and nothing looks for infinite or NaN values: where a result is NaN, the item is done
+// again with care (values that are not finite taken out of the products, as paged_drafts_kernel does).
+template <int DT, int DP, int WPE>
+__global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams p) {
+  constexpr int M = 128, NW = 4, KD = DP / 16, DB = DP / 32, ROW = DP * 2, TILE = kKeys * ROW;
+  constexpr int CH = ROW / 16, RPI = 64 / CH, LPW = kKeys / RPI / NW;  // chunks, rows and loads a wave
+  constexpr float kShift = DT == SSA_F16 ? kF16Shift : 0.0f;
+  constexpr float kGrow = DT == SSA_F16 ? 1.0f : 8.0f;  // fp16 weights end at 2^16
+  __shared__ __attribute__((aligned(1024))) unsigned char kst0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char vst0[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char kst1[TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char vst1[TILE];
+  if (blockIdx.x >= p.blocks) {
+    rest_rows<DT>(p, (int)(blockIdx.x - p.blocks));
+    return;
+  }
+  if (p.status && *p.status != 0) return;
+  DraftItem found;
+  if (!find_draft<M>(p, blockIdx.x, found)) return;
+  const DraftItem it = uniform(found);
+  const int wv = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
+  const int ctx = it.s.ctx, n = it.s.n, first = it.s.span.first, len = it.s.span.len;
+  const int tiles = (it.end - it.begin + 3) / 4;
+
+  const int64_t x = (int64_t)it.tile * M + wv * 32 + col;
+  const int t0 = (int)(x / p.G), tok = min(t0, n - 1), head = it.g * p.G + (int)(x - (int64_t)t0 * p.G);
+  const bool real = t0 < n, any = __any(real);  // a wave without rows loads and waits with the others
+  const int rpos = !p.masks ? ctx + tok : p.pos[(int64_t)it.c0 + tok];
+  const int start = p.window > 0 && rpos >= p.window ? rpos - p.window + 1 : 0;
+  int late = start;
+  if (p.window > 0) {
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) late = max(late, lane_xor(late, i));
+  }
+  late = uniform(late);
+
+  // the queries take the scale's sign, so that larger products are larger scores; one of 0 is next to it
+  const unsigned int sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+  const float scale = fmaxf(fabsf(p.scale_log2), FLT_MIN);
+  u32x4 q[KD];
+#pragma unroll
+  for (int c = 0; c < KD; ++c) {
+    const int at = c * 32 + hi * 16;
+    q[c] = u32x4{};
+    if (real && at < p.d * 2)
+      q[c] = *(const u32x4*)(p.q + (((int64_t)it.c0 + tok) * p.qt + head * p.qh) * 2 + at) ^ sign;
+  }
+
+  const char* const kbase = p.kpool + it.g * p.kph * 2;
+  const char* const vbase = p.vpool + it.g * p.vph * 2;
+  const int64_t kpp = p.kpp * 2, vpp = p.vpp * 2;
+  const int kps = (int)p.kps * 2, vps = (int)p.vps * 2, row_bytes = p.d * 2;
+  const int32_t* const row = p.table + it.b * p.table_stride;
+
+  // page and offset of 64 subtiles at a time, one per lane; the next 64 are on their way
+  int pid = 0, poff = 0, pid_next = 0, batch = 0;
+  unsigned long long bad = 0;
+  auto pages_at = [&](int s) {
+    s += lane;
+    return s < it.end ? row[page_of(s, p.div)] : 0;
+  };
+  auto take_pages = [&](int v) {
+    bad |= __ballot(v < 0 || v >= p.pages);
+    pid = v < 0 || v >= p.pages ? 0 : v;
+    poff = (batch + lane) * 16 - page_of(batch + lane, p.div) * p.page;
+  };
+
+  // load j of this wave: rows (j NW + wv) RPI.. of the tile, a lane a chunk; a row's place in its
+  // subtile of 16 and so its swizzle are the same for every j
+  const int lrow = (wv * RPI + lane / CH) & 15, lchunk = (lane % CH) ^ tile_swz<DP>(lrow);
+  const int koff = lrow * kps + lchunk * 16, voff = lrow * vps + lchunk * 16;
+  const bool inside = lchunk * 16 < row_bytes;
+  auto issue = [&](unsigned char* kdst, unsigned char* vdst, int i) __attribute__((always_inline)) {
+    const int s0 = it.begin + i * 4;
+    if (s0 >= batch + 64) {
+      batch += 64;
+      take_pages(pid_next);
+      pid_next = pages_at(batch + 64);
+    }
+    const bool full = DP == p.d && s0 * 16 >= first && s0 * 16 + kKeys <= len && s0 + 4 <= it.end;
+#pragma unroll
+    for (int j = 0; j < LPW; ++j) {
+      const int u = j * NW + wv, s = s0 + u * RPI / 16, at = min(s, it.end - 1) - batch;
+      const int64_t pg = __builtin_amdgcn_readlane(pid, at);
+      const int64_t off = __builtin_amdgcn_readlane(poff, at);
+      const char* k = kbase + (pg * kpp + off * kps) + koff;
+      const char* v = vbase + (pg * vpp + off * vps) + voff;
+      if (!full) {  // columns past d and rows that do not count are read as zero
+        const int key = s * 16 + lrow;
+        const char* const zero = (const char*)kZeroRow + (lane % CH) * 16;
+        if (!inside) k = zero;
+        if (!inside || s >= it.end || key < first || key >= len) v = zero;
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)k,
+                                       (LdsPtr)(kdst + u * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)v,
+                                       (LdsPtr)(vdst + u * 1024), 16, 0, 0);
+    }
+  };
+
+  // LDS reads: keys row 32 t + col, chunk 2 c + hi; values (transposing) rows 16 s + 4 hi + (0..3, then
+  // 8 on), columns 32 db + 16 (lane / 16 % 2)..
+  const int kswz = (tile_swz<DP>(col & 15) ^ hi) * 16, krow = col * ROW;
+  const int vrow = 4 * hi + (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+  const int vat0 = vrow * ROW + (lane & 1) * 8, vswz0 = (tile_swz<DP>(vrow) ^ vchunk) * 16;
+  const int vat1 = vat0 + 8 * ROW, vswz1 = (tile_swz<DP>(vrow + 8) ^ vchunk) * 16;
+
+  float m, l;
+  f32x16 acc[DB];
+  auto compute = [&](const unsigned char* ks, const unsigned char* vs, int i,
+                     auto careful) __attribute__((always_inline)) {
+    const int j0 = (it.begin + i * 4) * 16;
+    const bool edge = j0 < late || j0 + kKeys > ctx || it.begin + i * 4 + 4 > it.end;
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int c = 0; c < KD; ++c)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 a = *(const u32x4*)(ks + t * 32 * ROW + krow + (kswz ^ c * 32));
+        s[t] = mfma32(a, q[c], s[t], DT == SSA_BF16);
+      }
+    // bit 8 g + r of word t: whether the row attends key 32 t + 8 g + 4 hi + r
+    unsigned int allow[2] = {0x0f0f0f0fu, 0x0f0f0f0fu};
+    float mx = -FLT_MAX;
+    if (edge) {
+      uint64_t keys = attended_keys(p, it, tok, start, j0);
+      const int own = (it.end - it.begin - i * 4) * 16;  // past the item's end the next item's keys lie
+      if (own < kKeys) keys &= (1ull << own) - 1;
+      keys = keys >> 4 * hi & 0x0f0f0f0f0f0f0f0full;
+      allow[0] = (unsigned)keys;
+      allow[1] = (unsigned)(keys >> 32);
+      if (keys == 0) mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[t][r] = allow[t] & 1u << (8 * (r >> 2) + (r & 3)) ? s[t][r] : -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+    mx = fmaxf(mx, top * scale);
+    mx = fmaxf(mx, lane_xor(mx, 32));
+    if (__any(mx > m + kGrow)) {
+      const float up = fmaxf(m, mx);
+      const float a = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
+      m = up;
+      l *= a;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] *= a;
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - kShift;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], scale, -base));
+        sum += s[t][r];
+      }
+    l += sum;
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      constexpr int PARTS = kParts<DT>;
+      u32x4 w[PARTS];
+#pragma unroll
+      for (int i2 = 0; i2 < 4; ++i2) {
+        unsigned int y[PARTS];
+        const int r = 8 * (st & 1) + 2 * i2;
+        cut<DT>(s[st >> 1][r], s[st >> 1][r + 1], y);
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) w[k][i2] = y[k];
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint2 lo = lds_read_tr(vs + st * 16 * ROW + vat0 + (vswz0 ^ db * 64));
+        const uint2 up = lds_read_tr(vs + st * 16 * ROW + vat1 + (vswz1 ^ db * 64));
+        u32x4 v = {lo.x, lo.y, up.x, up.y};
+        if constexpr (careful.value) {
+          u32x4 kinds, some, none;
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) {
+            kinds[i2] = kind_of<DT>(v[i2]);
+            v[i2] = finite_part<DT>(v[i2]);
+            const int r = 8 * (st & 1) + 2 * i2;
+            const float w0 = s[st >> 1][r], w1 = s[st >> 1][r + 1];
+            const unsigned int yes = allow[st >> 1] >> (8 * (r >> 2) + (r & 3));
+            some[i2] = pack16<DT>(yes & 1 && !(w0 == 0.0f), yes & 2 && !(w1 == 0.0f));
+            none[i2] = pack16<DT>(yes & 1 && w0 == 0.0f, yes & 2 && w1 == 0.0f);
+          }
+          if (__any((kinds[0] | kinds[1] | kinds[2] | kinds[3]) != 0)) {
+            f32x16 a{}, b{};
+            a = mfma32(kinds, some, a, DT == SSA_BF16);
+            b = mfma32(kinds, none, b, DT == SSA_BF16);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[db][r] += not_finite_sum(a[r], b[r]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) acc[db] = mfma32(v, w[k], acc[db], DT == SSA_BF16);
+      }
+    }
+  };
+  auto begin = [&] {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+    batch = it.begin;
+    const int v = pages_at(batch);
+    pid_next = pages_at(batch + 64);
+    take_pages(v);
+  };
+  begin();
+  if (tiles > 0) issue(kst0, vst0, 0);
+  for (int i = 0; i < tiles; i += 2) {
+    dma_barrier();  // tile i is there for all waves; tile i - 1 is read no more
+    if (i + 1 < tiles) issue(kst1, vst1, i + 1);
+    if (any) compute(kst0, vst0, i, std::false_type{});
+    if (i + 1 >= tiles) break;
+    dma_barrier();
+    if (i + 2 < tiles) issue(kst0, vst0, i + 2);
+    if (any) compute(kst1, vst1, i + 1, std::false_type{});
+  }
+  bool nan = false;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) nan |= acc[db][r] != acc[db][r];
+  if (__syncthreads_or(nan && real)) {
+    begin();
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+      __syncthreads();
+      issue(kst0, vst0, i);
+      dma_barrier();
+      if (any) compute(kst0, vst0, i, std::true_type{});
+    }
+  }
+  l += lane_xor(l, 32);
+  if (bad != 0 || !it.s.span.ok || rpos < ctx) l = NAN;
+
+  if (p.items != 0 && it.j == 0 && it.g == 0 && it.tile == 0 && threadIdx.x == 0) {
+    p.info[2 * it.b] = it.first_part;
+    p.info[2 * it.b + 1] = it.n;
+  }
+  if (!real || (it.n > 1 && it.first_part < 0)) return;
+  const float inv = row_scale(m, l);
+  const int64_t token = (int64_t)it.c0 + tok, to = token * p.ot + head * p.oh;
+  const int64_t part = ((int64_t)it.first_part + ((int64_t)it.j * p.Hkv + it.g) * it.tiles + it.tile) * M +
+                       wv * 32 + col;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * db + 8 * g + 4 * hi;
+      if (c >= p.d) continue;
+      f32x4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = acc[db][4 * g + r];
+      if (it.n > 1) {
+        *(f32x4*)(p.part + part * DP + c) = y;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] *= inv;
+        store_row4<DT>(p.out, to + c, y);
+      }
+    }
+  if (hi != 0) return;
+  if (it.n > 1) {
+    p.part_ml[part * 2] = m;
+    p.part_ml[part * 2 + 1] = l;
+  } else if (p.lse) {
+    p.lse[token * p.Hq + head] = row_lse(m, l, kShift);
+  }
+}
+
 constexpr int kJoinRows = 8;  // parts of a row on their way at a time
 
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
@@ -854,19 +1199,20 @@ struct DraftLayout {
 
 // Two tiles of 16 rows a wave where requests have more rows on average (past head dim 128 their
 // registers do not fit).
-DraftLayout draft_layout(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
                          int64_t page, int64_t window) {
   DraftLayout y{};
   const int64_t G = Hq / Hkv;
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
-  y.M = y.dp <= 128 && N * G > 16 * B ? 32 : 16;
+  const bool many = N * G > 16 * B;
+  y.M = y.dp > 128 || !many ? 16 : dtype == SSA_F32 ? 32 : 128;
   const int64_t tiles = draft_most_tiles(B, N, G, y.M) * Hkv;
   const int64_t cap = W * page;
   const int64_t units = paged_most_units(window > 0 ? std::min(cap, window + N + 15) : cap, 0);
   const auto rounded = [](int64_t x) { return (x + 7) / 8 * 8; };  // an XCD's run each
   y.blocks = rounded(tiles);
   if (units <= 4 || (units <= 16 && tiles >= 512)) return y;
-  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 || B == 1 ? 512 : 1024;
+  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 || B == 1 || y.M == 128 ? 512 : 1024;
   y.items = std::max<int64_t>(1, target / Hkv);
   y.blocks = rounded(std::min(tiles + y.items * Hkv, tiles * units));
   y.max_parts = std::min(2 * y.items * Hkv, y.blocks);
@@ -877,28 +1223,33 @@ DraftLayout draft_layout(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t 
   return y;
 }
 
-template <int DT, int DP, int MT, int WPE>
+template <int DT, int DP, int M, int WPE>
 int run_drafts(const DraftParams& p, hipStream_t st) {
-  paged_drafts_kernel<DT, DP, MT, WPE>
-      <<<(unsigned)(p.blocks + kRestBlocks), kAttendWaves * 64, 0, st>>>(p);
+  const unsigned blocks = (unsigned)(p.blocks + kRestBlocks);
+  if constexpr (M == 128)
+    paged_drafts_tile_kernel<DT, DP, WPE><<<blocks, 256, 0, st>>>(p);
+  else
+    paged_drafts_kernel<DT, DP, M / 16, WPE><<<blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_drafts_kernel"));
   if (p.items == 0) return SSA_OK;
-  paged_drafts_join_kernel<DT, DP, MT * 16>
+  paged_drafts_join_kernel<DT, DP, M>
       <<<(unsigned)((p.N * p.Hq + 3) / 4), 256, 0, st>>>(p);
   return launch_status("paged_drafts_join_kernel");
 }
 
 template <int DT>
 int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
+  constexpr bool f32 = DT == SSA_F32;
+  constexpr int kMany = f32 ? 32 : 128;
   switch (y.dp) {
     case 64:
-      if (y.M == 32) return run_drafts<DT, 64, 2, 2>(p, st);
-      return run_drafts<DT, 64, 1, 3>(p, st);
+      if (y.M == kMany) return run_drafts<DT, 64, kMany, f32 ? 2 : 3>(p, st);
+      return run_drafts<DT, 64, 16, 3>(p, st);
     case 128:
-      if (y.M == 32) return run_drafts<DT, 128, 2, 2>(p, st);
-      return run_drafts<DT, 128, 1, 2>(p, st);
-    case 256: return run_drafts<DT, 256, 1, 1>(p, st);
-    default: return run_drafts<DT, 512, 1, 1>(p, st);
+      if (y.M == kMany) return run_drafts<DT, 128, kMany, 2>(p, st);
+      return run_drafts<DT, 128, 16, 2>(p, st);
+    case 256: return run_drafts<DT, 256, 16, 1>(p, st);
+    default: return run_drafts<DT, 512, 16, 1>(p, st);
   }
 }
 
@@ -1021,13 +1372,13 @@ extern "C" int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu,
   return launch_status("paged_draft_masks_kernel");
 }
 
-extern "C" size_t ssa_paged_attend_drafts_workspace_size(int64_t B, int64_t N, int64_t Hq,
+extern "C" size_t ssa_paged_attend_drafts_workspace_size(int dtype, int64_t B, int64_t N, int64_t Hq,
                                                          int64_t Hkv, int64_t d, int64_t W,
                                                          int64_t page, int64_t window) {
-  if (B <= 0 || N <= 0 || !fits_int(N) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 ||
+  if (dtype_size(dtype) == 0 || B <= 0 || N <= 0 || !fits_int(N) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 512 ||
       W <= 0 || page <= 0 || !fits_int(window) || W > 0x7fffffff / page)
     return 0;
-  return draft_layout(B, N, Hq, Hkv, d, W, page, window).bytes;
+  return draft_layout(dtype, B, N, Hq, Hkv, d, W, page, window).bytes;
 }
 
 extern "C" int ssa_paged_attend_drafts(const void* q, const void* kpool, const void* vpool,
@@ -1060,7 +1411,7 @@ extern "C" int ssa_paged_attend_drafts(const void* q, const void* kpool, const v
               SSA_ERR_INVALID, "%s: rows must start at multiples of 16 bytes", who);
   SSA_REQUIRE(strides[4] < (1 << 24) && strides[7] < (1 << 24), SSA_ERR_UNSUPPORTED,
               "%s: slots 2^24 elements apart or more", who);
-  const DraftLayout y = draft_layout(B, N, Hq, Hkv, d, W, page, window);
+  const DraftLayout y = draft_layout(dtype, B, N, Hq, Hkv, d, W, page, window);
   SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
               SSA_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who,
               y.bytes, workspace_bytes);

@@ -432,8 +432,8 @@ def _drafts_plan(q, kpool, vpool, table, lens, cu, masks, pos, out, window):
         _written("out", out)
         to = out[1][:2]
     strides = _lib.i64_array((*q[1][:2], *kpool[1][:3], *vpool[1][:3], *to))
-    ws_bytes = _lib.query("ssa_paged_attend_drafts_workspace_size", B, N, hq, hkv, d, W, page,
-                          window)
+    ws_bytes = _lib.query("ssa_paged_attend_drafts_workspace_size", _lib.dtype_code(dtype), B, N,
+                          hq, hkv, d, W, page, window)
     return (_lib.dtype_code(dtype), B, N, hq, hkv, d, pages, page), (row, W), words, strides, \
         ws_bytes, not _rows16(q)
 
