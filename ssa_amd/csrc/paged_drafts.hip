@@ -782,30 +782,29 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
 
 // ---- many rows -----------------------------------------------------------------------------------
 
-// A tile of kKeys keys in LDS as rows of DP 16-bit numbers; 16-byte chunk c of row r lies at chunk
+// A tile of keys or values in LDS is rows of DP 16-bit numbers; 16-byte chunk c of row r lies at chunk
 // c ^ tile_swz(r), so that the 16 lanes of a ds_read_b128 phase (rows r..r + 15) and the 32 of a
-// transposing read (four rows, four chunks) meet every bank once.
-constexpr int kKeys = 64;
-
+// transposing read (four rows and four chunks, or eight and two) meet every bank once.
 template <int DP>
 __device__ inline int tile_swz(int r) {
-  if constexpr (DP == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);  // two rows fill the banks
-  return (r & 3) << 2 | (r >> 2 & 3);
+  if constexpr (DP == 64)  // two rows fill the banks
+    return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+  return (r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
 }
 
 typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef const __attribute__((address_space(1))) void* MemPtr;
 
-// Weights of two keys as exact 16-bit parts (bf16: three, cut; fp16: two of 22 bits).
+// Weights of two keys as 16-bit parts, two for either type: bf16's, rounded to nearest, leave 2^-18 of a
+// weight at most, fp16's, cut, 2^-20. The output keeps 8 and 11 bits. (bf16's third part, which holds
+// what is left, made trees of 64 tokens 17 % slower and 16 tokens over 1M 12 %.)
 template <int DT>
-__device__ inline void cut(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
+__device__ inline void parts_of(float p0, float p1, unsigned int (&w)[2]) {
   if constexpr (DT == SSA_BF16) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const unsigned int a = __float_as_uint(p0), b = __float_as_uint(p1);
-      w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-      p0 -= __uint_as_float(a & 0xffff0000u);
-      p1 -= __uint_as_float(b & 0xffff0000u);
-    }
+    w[0] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
+    p0 -= __uint_as_float(w[0] << 16);
+    p1 -= __uint_as_float(w[0] & 0xffff0000u);
+    w[1] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
   } else {
     const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
     w[0] = __builtin_bit_cast(unsigned int, h);
@@ -814,30 +813,56 @@ __device__ inline void cut(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
   }
 }
 
-__device__ inline f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c, bool bf16) {
-  if (bf16)
+// Products of RW x RW numbers over 1024 / RW columns (32 bytes of 16 lanes each, or 16 of 32).
+template <int DT>
+__device__ inline f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return mfma16(a, b, c, DT == SSA_BF16);
+}
+template <int DT>
+__device__ inline f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (DT == SSA_BF16)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
-                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Attention of 128 rows over an item's keys, a wave's 32 rows against all of them: tiles of 64 keys go
-// from memory to LDS, one ahead of the products, and serve the four waves. Scores are K Q^T: lane column
-// a row, so its statistics and its weights stay in its lanes and are the second product's operand as they
-// are; values are transposed by the LDS reads. A row's maximum is raised only where it grows by more
-// than kGrow, and nothing looks for infinite or NaN values: where a result is NaN, the item is done
-// again with care (values that are not finite taken out of the products, as paged_drafts_kernel does).
-template <int DT, int DP, int WPE>
+// Waits until at most N of this wave's loads are on their way and its LDS reads are done, then for the
+// other waves: what all but the last N loads wrote to LDS is there.
+template <int N>
+__device__ inline void ring_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 0 << 8 | (N >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Attention of a tile of rows over an item's keys, a wave's RW rows (16 or 32) against all of them:
+// tiles of KT keys go from memory to LDS, RING - 1 ahead of the products, and serve the four waves.
+// Scores are K Q^T: lane column a row, so its statistics and its weights stay in its lanes and are the
+// second product's operand as they are; values are transposed by the LDS reads. A lane's scores come in
+// quads: r of quad q is key 4 GR q + 4 grp + r, GR = 64 / RW lanes of a row. bf16 weights, whose
+// exponents suffice, go by the maximum of a row's first keys (fp16's maximum rises with the scores), and
+// nothing looks for infinite or NaN values: where a sum or a result is too large or not finite, the item is
+// done again with care (the maximum raised tile by tile, values that are not finite taken out of the
+// products as in paged_drafts_kernel).
+template <int DT, int DP, int RW, int KT, int RING, int WPE>
 __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams p) {
-  constexpr int M = 128, NW = 4, KD = DP / 16, DB = DP / 32, ROW = DP * 2, TILE = kKeys * ROW;
-  constexpr int CH = ROW / 16, RPI = 64 / CH, LPW = kKeys / RPI / NW;  // chunks, rows and loads a wave
+  typedef typename std::conditional<RW == 16, f32x4, f32x16>::type Acc;
+  constexpr int NW = 4, M = NW * RW, GR = 64 / RW, ROW = DP * 2, TILE = KT * ROW;
+  constexpr int KD = ROW / (16 * GR), DB = DP / RW, AR = RW * RW / 64;  // steps, blocks, results a lane
+  constexpr int NS = KT / RW, NQ = KT / (4 * GR), SUB = KT / 16;  // products, quads, subtiles of a tile
+  constexpr int CH = ROW / 16, RPI = 64 / CH, LPW = KT / RPI / NW;  // chunks, rows, loads of a wave
   constexpr float kShift = DT == SSA_F16 ? kF16Shift : 0.0f;
   constexpr float kGrow = DT == SSA_F16 ? 1.0f : 8.0f;  // fp16 weights end at 2^16
-  __shared__ __attribute__((aligned(1024))) unsigned char kst0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char vst0[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char kst1[TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char vst1[TILE];
+  static_assert(LPW >= 1 && RPI <= 16 && (RW == 16 || RW == 32) && RING >= 2 && RING <= 4, "");
+  // a stage is the keys' tile and the values'; objects of their own, so that the compiler's waits for
+  // one are not for the others
+  __shared__ __attribute__((aligned(1024))) unsigned char st0[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char st1[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) unsigned char st2[RING > 2 ? 2 * TILE : 16];
+  __shared__ __attribute__((aligned(1024))) unsigned char st3[RING > 3 ? 2 * TILE : 16];
   if (blockIdx.x >= p.blocks) {
     rest_rows<DT>(p, (int)(blockIdx.x - p.blocks));
     return;
@@ -846,19 +871,20 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   DraftItem found;
   if (!find_draft<M>(p, blockIdx.x, found)) return;
   const DraftItem it = uniform(found);
-  const int wv = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
+  const int wv = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane % RW, grp = lane / RW;
   const int ctx = it.s.ctx, n = it.s.n, first = it.s.span.first, len = it.s.span.len;
-  const int tiles = (it.end - it.begin + 3) / 4;
+  const int tiles = (it.end - it.begin + SUB - 1) / SUB;
 
-  const int64_t x = (int64_t)it.tile * M + wv * 32 + col;
+  const int64_t x = (int64_t)it.tile * M + wv * RW + col;
   const int t0 = (int)(x / p.G), tok = min(t0, n - 1), head = it.g * p.G + (int)(x - (int64_t)t0 * p.G);
   const bool real = t0 < n, any = __any(real);  // a wave without rows loads and waits with the others
   const int rpos = !p.masks ? ctx + tok : p.pos[(int64_t)it.c0 + tok];
   const int start = p.window > 0 && rpos >= p.window ? rpos - p.window + 1 : 0;
-  int late = start;
+  int late = start;  // the latest first key of the wave's rows
   if (p.window > 0) {
 #pragma unroll
-    for (int i = 1; i < 32; i <<= 1) late = max(late, lane_xor(late, i));
+    for (int i = 1; i < RW; i <<= 1) late = max(late, lane_xor(late, i));
   }
   late = uniform(late);
 
@@ -868,7 +894,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   u32x4 q[KD];
 #pragma unroll
   for (int c = 0; c < KD; ++c) {
-    const int at = c * 32 + hi * 16;
+    const int at = (c * GR + grp) * 16;
     q[c] = u32x4{};
     if (real && at < p.d * 2)
       q[c] = *(const u32x4*)(p.q + (((int64_t)it.c0 + tok) * p.qt + head * p.qh) * 2 + at) ^ sign;
@@ -893,143 +919,157 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     poff = (batch + lane) * 16 - page_of(batch + lane, p.div) * p.page;
   };
 
-  // load j of this wave: rows (j NW + wv) RPI.. of the tile, a lane a chunk; a row's place in its
-  // subtile of 16 and so its swizzle are the same for every j
-  const int lrow = (wv * RPI + lane / CH) & 15, lchunk = (lane % CH) ^ tile_swz<DP>(lrow);
-  const int koff = lrow * kps + lchunk * 16, voff = lrow * vps + lchunk * 16;
-  const bool inside = lchunk * 16 < row_bytes;
-  auto issue = [&](unsigned char* kdst, unsigned char* vdst, int i) __attribute__((always_inline)) {
-    const int s0 = it.begin + i * 4;
+  // load j of this wave: rows (j NW + wv) RPI.. of the tile, a lane a chunk. With up to 16 chunks a row
+  // a row's place in its subtile of 16, and so its swizzle, is the same for every j; with 32 it is for
+  // every other j, and the swizzle's other bit moves along.
+  const int lchunk = lane % CH;
+  auto load_row = [&](int j) { return ((j * NW + wv) * RPI + lane / CH) & 15; };
+  auto issue = [&](unsigned char* to, int i) __attribute__((always_inline)) {
+    const int s0 = it.begin + i * SUB;
     if (s0 >= batch + 64) {
       batch += 64;
       take_pages(pid_next);
       pid_next = pages_at(batch + 64);
     }
-    const bool full = DP == p.d && s0 * 16 >= first && s0 * 16 + kKeys <= len && s0 + 4 <= it.end;
+    const bool full = DP == p.d && s0 * 16 >= first && s0 * 16 + KT <= len && s0 + SUB <= it.end;
 #pragma unroll
     for (int j = 0; j < LPW; ++j) {
       const int u = j * NW + wv, s = s0 + u * RPI / 16, at = min(s, it.end - 1) - batch;
+      const int r = load_row(j), c = lchunk ^ tile_swz<DP>(r);
       const int64_t pg = __builtin_amdgcn_readlane(pid, at);
       const int64_t off = __builtin_amdgcn_readlane(poff, at);
-      const char* k = kbase + (pg * kpp + off * kps) + koff;
-      const char* v = vbase + (pg * vpp + off * vps) + voff;
+      const char* k = kbase + (pg * kpp + off * kps) + (r * kps + c * 16);
+      const char* v = vbase + (pg * vpp + off * vps) + (r * vps + c * 16);
       if (!full) {  // columns past d and rows that do not count are read as zero
-        const int key = s * 16 + lrow;
-        const char* const zero = (const char*)kZeroRow + (lane % CH) * 16;
-        if (!inside) k = zero;
-        if (!inside || s >= it.end || key < first || key >= len) v = zero;
+        const int key = s * 16 + r;
+        const char* const zero = (const char*)kZeroRow + lchunk * 16;
+        if (c * 16 >= row_bytes) k = zero;
+        if (c * 16 >= row_bytes || s >= it.end || key < first || key >= len) v = zero;
       }
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)k,
-                                       (LdsPtr)(kdst + u * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)v,
-                                       (LdsPtr)(vdst + u * 1024), 16, 0, 0);
+      if (it.stream) {
+        __builtin_amdgcn_global_load_lds((MemPtr)k, (LdsPtr)(to + u * 1024), 16, 0, kStream);
+        __builtin_amdgcn_global_load_lds((MemPtr)v, (LdsPtr)(to + TILE + u * 1024), 16, 0, kStream);
+      } else {
+        __builtin_amdgcn_global_load_lds((MemPtr)k, (LdsPtr)(to + u * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((MemPtr)v, (LdsPtr)(to + TILE + u * 1024), 16, 0, 0);
+      }
     }
   };
 
-  // LDS reads: keys row 32 t + col, chunk 2 c + hi; values (transposing) rows 16 s + 4 hi + (0..3, then
-  // 8 on), columns 32 db + 16 (lane / 16 % 2)..
-  const int kswz = (tile_swz<DP>(col & 15) ^ hi) * 16, krow = col * ROW;
-  const int vrow = 4 * hi + (lane & 15) / 4, vchunk = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-  const int vat0 = vrow * ROW + (lane & 1) * 8, vswz0 = (tile_swz<DP>(vrow) ^ vchunk) * 16;
-  const int vat1 = vat0 + 8 * ROW, vswz1 = (tile_swz<DP>(vrow + 8) ^ vchunk) * 16;
+  // LDS reads: keys row RW t + col, chunk GR c + grp; values (transposing) rows 4 GR q + 4 grp + (0..3)
+  // of quads q = 2 st and 2 st + 1, 16 columns of the block (RW 32: the upper lanes the other 16)
+  const int kswz = (tile_swz<DP>(col & 15) ^ grp) * 16, krow = col * ROW;
+  const int vrow = 4 * grp + (lane & 15) / 4;
+  const int vchunk = (RW == 32 ? 2 * (lane >> 4 & 1) : 0) + (lane >> 1 & 1);
+  const int vat0 = vrow * ROW + (lane & 1) * 8, vswz0 = (tile_swz<DP>(vrow & 15) ^ vchunk) * 16;
+  const int vat1 = vat0 + 4 * GR * ROW;
+  const int vswz1 = (tile_swz<DP>((vrow + 4 * GR) & 15) ^ vchunk) * 16;
 
   float m, l;
-  f32x16 acc[DB];
-  auto compute = [&](const unsigned char* ks, const unsigned char* vs, int i,
-                     auto careful) __attribute__((always_inline)) {
-    const int j0 = (it.begin + i * 4) * 16;
-    const bool edge = j0 < late || j0 + kKeys > ctx || it.begin + i * 4 + 4 > it.end;
-    f32x16 s[2] = {};
+  Acc acc[DB];
+  auto compute = [&](const unsigned char* ks, int i, auto careful) __attribute__((always_inline)) {
+    const unsigned char* const vs = ks + TILE;
+    const int s0 = it.begin + i * SUB, j0 = s0 * 16;
+    // up to the tile of the latest first key: past it every row has a maximum or no key of the context
+    const bool edge = j0 <= late || j0 + KT > ctx || s0 + SUB > it.end;
+    Acc sum_of[NS];
 #pragma unroll
-    for (int c = 0; c < KD; ++c)
+    for (int t = 0; t < NS; ++t) {
+      sum_of[t] = Acc{};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const u32x4 a = *(const u32x4*)(ks + t * 32 * ROW + krow + (kswz ^ c * 32));
-        s[t] = mfma32(a, q[c], s[t], DT == SSA_BF16);
+      for (int c = 0; c < KD; ++c) {
+        const u32x4 a = *(const u32x4*)(ks + t * RW * ROW + krow + (kswz ^ c * GR * 16));
+        sum_of[t] = mfma<DT>(a, q[c], sum_of[t]);
       }
-    // bit 8 g + r of word t: whether the row attends key 32 t + 8 g + 4 hi + r
-    unsigned int allow[2] = {0x0f0f0f0fu, 0x0f0f0f0fu};
+    }
+    float s[NQ][4];
+#pragma unroll
+    for (int t = 0; t < NS; ++t)
+#pragma unroll
+      for (int r = 0; r < AR; ++r) s[(t * AR + r) / 4][r % 4] = sum_of[t][r];
+    // bit 4 q + r: whether the row attends r of quad q
+    unsigned int allow = NQ == 8 ? ~0u : (1u << 4 * NQ % 32) - 1;
     float mx = -FLT_MAX;
     if (edge) {
       uint64_t keys = attended_keys(p, it, tok, start, j0);
-      const int own = (it.end - it.begin - i * 4) * 16;  // past the item's end the next item's keys lie
-      if (own < kKeys) keys &= (1ull << own) - 1;
-      keys = keys >> 4 * hi & 0x0f0f0f0f0f0f0f0full;
-      allow[0] = (unsigned)keys;
-      allow[1] = (unsigned)(keys >> 32);
-      if (keys == 0) mx = -INFINITY;
+      const int own = min(it.end - s0, SUB) * 16;  // past the item's end the next item's keys lie
+      if (own < 64) keys &= (1ull << own) - 1;
+      keys >>= 4 * grp;
+      allow = 0;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int y = 0; y < NQ; ++y) allow |= (unsigned)(keys >> 4 * GR * y & 15) << 4 * y;
+      if (allow == 0) mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] = allow[t] & 1u << (8 * (r >> 2) + (r & 3)) ? s[t][r] : -INFINITY;
+      for (int y = 0; y < NQ; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[y][r] = allow & 1u << (4 * y + r) ? s[y][r] : -INFINITY;
     }
-    float top = s[0][0];
+    if (DT != SSA_BF16 || edge || i == 0 || careful.value) {
+      float top = s[0][0];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int y = 0; y < NQ; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-    mx = fmaxf(mx, top * scale);
-    mx = fmaxf(mx, lane_xor(mx, 32));
-    if (__any(mx > m + kGrow)) {
-      const float up = fmaxf(m, mx);
-      const float a = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
-      m = up;
-      l *= a;
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[y][r]);
+      mx = fmaxf(mx, top * scale);
+      if constexpr (RW == 16) mx = fmaxf(mx, lane_xor(mx, 16));
+      mx = fmaxf(mx, lane_xor(mx, 32));
+      if (__any(mx > m + kGrow)) {
+        const float up = fmaxf(m, mx);
+        const float a = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
+        m = up;
+        l *= a;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[db][r] *= a;
+          for (int r = 0; r < AR; ++r) acc[db][r] *= a;
+      }
     }
     const float base = (m == -INFINITY ? 0.0f : m) - kShift;
     float sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int y = 0; y < NQ; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], scale, -base));
-        sum += s[t][r];
+      for (int r = 0; r < 4; ++r) {
+        s[y][r] = __builtin_amdgcn_exp2f(fmaf(s[y][r], scale, -base));
+        sum += s[y][r];
       }
     l += sum;
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      constexpr int PARTS = kParts<DT>;
-      u32x4 w[PARTS];
+    for (int st = 0; st < NQ / 2; ++st) {
+      u32x4 w[2];
 #pragma unroll
-      for (int i2 = 0; i2 < 4; ++i2) {
-        unsigned int y[PARTS];
-        const int r = 8 * (st & 1) + 2 * i2;
-        cut<DT>(s[st >> 1][r], s[st >> 1][r + 1], y);
-#pragma unroll
-        for (int k = 0; k < PARTS; ++k) w[k][i2] = y[k];
+      for (int y = 0; y < 4; ++y) {
+        const float* const of = &s[2 * st + y / 2][y % 2 * 2];
+        unsigned int parts[2];
+        parts_of<DT>(of[0], of[1], parts);
+        w[0][y] = parts[0];
+        w[1][y] = parts[1];
       }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const uint2 lo = lds_read_tr(vs + st * 16 * ROW + vat0 + (vswz0 ^ db * 64));
-        const uint2 up = lds_read_tr(vs + st * 16 * ROW + vat1 + (vswz1 ^ db * 64));
+        const unsigned char* const at = vs + st * 8 * GR * ROW;
+        const uint2 lo = lds_read_tr(at + vat0 + (vswz0 ^ db * RW * 2));
+        const uint2 up = lds_read_tr(at + vat1 + (vswz1 ^ db * RW * 2));
         u32x4 v = {lo.x, lo.y, up.x, up.y};
         if constexpr (careful.value) {
           u32x4 kinds, some, none;
 #pragma unroll
-          for (int i2 = 0; i2 < 4; ++i2) {
-            kinds[i2] = kind_of<DT>(v[i2]);
-            v[i2] = finite_part<DT>(v[i2]);
-            const int r = 8 * (st & 1) + 2 * i2;
-            const float w0 = s[st >> 1][r], w1 = s[st >> 1][r + 1];
-            const unsigned int yes = allow[st >> 1] >> (8 * (r >> 2) + (r & 3));
-            some[i2] = pack16<DT>(yes & 1 && !(w0 == 0.0f), yes & 2 && !(w1 == 0.0f));
-            none[i2] = pack16<DT>(yes & 1 && w0 == 0.0f, yes & 2 && w1 == 0.0f);
+          for (int y = 0; y < 4; ++y) {
+            kinds[y] = kind_of<DT>(v[y]);
+            v[y] = finite_part<DT>(v[y]);
+            const float* const of = &s[2 * st + y / 2][y % 2 * 2];
+            const unsigned int yes = allow >> (4 * (2 * st + y / 2) + y % 2 * 2);
+            some[y] = pack16<DT>(yes & 1 && !(of[0] == 0.0f), yes & 2 && !(of[1] == 0.0f));
+            none[y] = pack16<DT>(yes & 1 && of[0] == 0.0f, yes & 2 && of[1] == 0.0f);
           }
           if (__any((kinds[0] | kinds[1] | kinds[2] | kinds[3]) != 0)) {
-            f32x16 a{}, b{};
-            a = mfma32(kinds, some, a, DT == SSA_BF16);
-            b = mfma32(kinds, none, b, DT == SSA_BF16);
+            const Acc with = mfma<DT>(kinds, some, Acc{}), without = mfma<DT>(kinds, none, Acc{});
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[db][r] += not_finite_sum(a[r], b[r]);
+            for (int r = 0; r < AR; ++r) acc[db][r] += not_finite_sum(with[r], without[r]);
           }
         }
 #pragma unroll
-        for (int k = 0; k < PARTS; ++k) acc[db] = mfma32(v, w[k], acc[db], DT == SSA_BF16);
+        for (int k = 0; k < 2; ++k) acc[db] = mfma<DT>(v, w[k], acc[db]);
       }
     }
   };
@@ -1037,38 +1077,52 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     m = -INFINITY;
     l = 0.0f;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+    for (int db = 0; db < DB; ++db) acc[db] = Acc{};
     batch = it.begin;
     const int v = pages_at(batch);
     pid_next = pages_at(batch + 64);
     take_pages(v);
   };
   begin();
-  if (tiles > 0) issue(kst0, vst0, 0);
-  for (int i = 0; i < tiles; i += 2) {
-    dma_barrier();  // tile i is there for all waves; tile i - 1 is read no more
-    if (i + 1 < tiles) issue(kst1, vst1, i + 1);
-    if (any) compute(kst0, vst0, i, std::false_type{});
+  // Tile i is there for all waves, tile i - 1 is read no more: its stage takes the one RING - 1 on.
+  auto step = [&](const unsigned char* now, unsigned char* next, int i) __attribute__((always_inline)) {
+    if (RING > 2 && i + RING - 2 < tiles) ring_barrier<(RING - 2) * 2 * LPW>();
+    else ring_barrier<0>();
+    if (i + RING - 1 < tiles) issue(next, i + RING - 1);
+    if (any) compute(now, i, std::false_type{});
+  };
+  if (tiles > 0) issue(st0, 0);
+  if (RING > 2 && tiles > 1) issue(st1, 1);
+  if (RING > 3 && tiles > 2) issue(st2, 2);
+  for (int i = 0; i < tiles; i += RING) {
+    step(st0, RING > 3 ? st3 : RING > 2 ? st2 : st1, i);
     if (i + 1 >= tiles) break;
-    dma_barrier();
-    if (i + 2 < tiles) issue(kst0, vst0, i + 2);
-    if (any) compute(kst1, vst1, i + 1, std::false_type{});
+    step(st1, st0, i + 1);
+    if constexpr (RING > 2) {
+      if (i + 2 >= tiles) break;
+      step(st2, st1, i + 2);
+    }
+    if constexpr (RING > 3) {
+      if (i + 3 >= tiles) break;
+      step(st3, st2, i + 3);
+    }
   }
-  bool nan = false;
+  bool off = !(l < 0x1p100f);
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) nan |= acc[db][r] != acc[db][r];
-  if (__syncthreads_or(nan && real)) {
+    for (int r = 0; r < AR; ++r) off |= !(fabsf(acc[db][r]) < INFINITY);
+  if (__syncthreads_or(off && real)) {
     begin();
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
       __syncthreads();
-      issue(kst0, vst0, i);
+      issue(st0, i);
       dma_barrier();
-      if (any) compute(kst0, vst0, i, std::true_type{});
+      if (any) compute(st0, i, std::true_type{});
     }
   }
+  if constexpr (RW == 16) l += lane_xor(l, 16);
   l += lane_xor(l, 32);
   if (bad != 0 || !it.s.span.ok || rpos < ctx) l = NAN;
 
@@ -1080,12 +1134,12 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   const float inv = row_scale(m, l);
   const int64_t token = (int64_t)it.c0 + tok, to = token * p.ot + head * p.oh;
   const int64_t part = ((int64_t)it.first_part + ((int64_t)it.j * p.Hkv + it.g) * it.tiles + it.tile) * M +
-                       wv * 32 + col;
+                       wv * RW + col;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = 32 * db + 8 * g + 4 * hi;
+    for (int g = 0; g < AR / 4; ++g) {
+      const int c = RW * db + 4 * GR * g + 4 * grp;
       if (c >= p.d) continue;
       f32x4 y;
 #pragma unroll
@@ -1098,7 +1152,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
         store_row4<DT>(p.out, to + c, y);
       }
     }
-  if (hi != 0) return;
+  if (grp != 0) return;
   if (it.n > 1) {
     p.part_ml[part * 2] = m;
     p.part_ml[part * 2 + 1] = l;
@@ -1204,30 +1258,34 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   DraftLayout y{};
   const int64_t G = Hq / Hkv;
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
-  const bool many = N * G > 16 * B;
-  y.M = y.dp > 128 || !many ? 16 : dtype == SSA_F32 ? 32 : 128;
+  const int64_t rows = N * G;  // of a key head; of a request rows / B on average
+  if (dtype == SSA_F32) y.M = y.dp <= 128 && rows > 16 * B ? 32 : 16;
+  else y.M = y.dp == 512 || rows <= 16 * B ? 16 : y.dp == 256 || rows <= 64 * B ? 64 : 128;
   const int64_t tiles = draft_most_tiles(B, N, G, y.M) * Hkv;
   const int64_t cap = W * page;
   const int64_t units = paged_most_units(window > 0 ? std::min(cap, window + N + 15) : cap, 0);
   const auto rounded = [](int64_t x) { return (x + 7) / 8 * 8; };  // an XCD's run each
   y.blocks = rounded(tiles);
   if (units <= 4 || (units <= 16 && tiles >= 512)) return y;
-  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 || B == 1 || y.M == 128 ? 512 : 1024;
+  // workgroups aimed at: what the CUs hold at once (three a CU; two or one of the widest heads); twice
+  // as many even out uneven requests better (64 mixed requests 341 us for 768, 316 for 1536; 16 trees of
+  // 64 tokens 196 and 192), where one request is even by itself (16 tokens over 1M 165 and 178)
+  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 ? 512 : B == 1 ? 768 : y.M >= 64 ? 1536 : 1024;
   y.items = std::max<int64_t>(1, target / Hkv);
   y.blocks = rounded(std::min(tiles + y.items * Hkv, tiles * units));
   y.max_parts = std::min(2 * y.items * Hkv, y.blocks);
-  const size_t rows = (size_t)y.max_parts * y.M;
-  y.part_ml = rows * y.dp * 4;
-  y.info = y.part_ml + rows * 2 * 4;
+  const size_t held = (size_t)y.max_parts * y.M;
+  y.part_ml = held * y.dp * 4;
+  y.info = y.part_ml + held * 2 * 4;
   y.bytes = (y.info + (size_t)B * 8 + 15) / 16 * 16;
   return y;
 }
 
-template <int DT, int DP, int M, int WPE>
+template <int DT, int DP, int M, int KT, int RING, int WPE>
 int run_drafts(const DraftParams& p, hipStream_t st) {
   const unsigned blocks = (unsigned)(p.blocks + kRestBlocks);
-  if constexpr (M == 128)
-    paged_drafts_tile_kernel<DT, DP, WPE><<<blocks, 256, 0, st>>>(p);
+  if constexpr (KT != 0)
+    paged_drafts_tile_kernel<DT, DP, M / 4, KT, RING, WPE><<<blocks, 256, 0, st>>>(p);
   else
     paged_drafts_kernel<DT, DP, M / 16, WPE><<<blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_drafts_kernel"));
@@ -1239,17 +1297,21 @@ int run_drafts(const DraftParams& p, hipStream_t st) {
 
 template <int DT>
 int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
-  constexpr bool f32 = DT == SSA_F32;
-  constexpr int kMany = f32 ? 32 : 128;
+  if constexpr (DT != SSA_F32) {
+    if (y.M == 64 && y.dp == 64) return run_drafts<DT, 64, 64, 64, 3, 3>(p, st);
+    if (y.M == 64 && y.dp == 128) return run_drafts<DT, 128, 64, 32, 3, 3>(p, st);
+    if (y.M == 64 && y.dp == 256) return run_drafts<DT, 256, 64, 32, 2, 2>(p, st);
+    if (y.M == 128 && y.dp == 64) return run_drafts<DT, 64, 128, 64, 3, 3>(p, st);
+    if (y.M == 128 && y.dp == 128) return run_drafts<DT, 128, 128, 64, 2, 2>(p, st);
+  } else {
+    if (y.M == 32 && y.dp == 64) return run_drafts<DT, 64, 32, 0, 0, 2>(p, st);
+    if (y.M == 32 && y.dp == 128) return run_drafts<DT, 128, 32, 0, 0, 2>(p, st);
+  }
   switch (y.dp) {
-    case 64:
-      if (y.M == kMany) return run_drafts<DT, 64, kMany, f32 ? 2 : 3>(p, st);
-      return run_drafts<DT, 64, 16, 3>(p, st);
-    case 128:
-      if (y.M == kMany) return run_drafts<DT, 128, kMany, 2>(p, st);
-      return run_drafts<DT, 128, 16, 2>(p, st);
-    case 256: return run_drafts<DT, 256, 16, 1>(p, st);
-    default: return run_drafts<DT, 512, 16, 1>(p, st);
+    case 64: return run_drafts<DT, 64, 16, 0, 0, 3>(p, st);
+    case 128: return run_drafts<DT, 128, 16, 0, 0, 2>(p, st);
+    case 256: return run_drafts<DT, 256, 16, 0, 0, 1>(p, st);
+    default: return run_drafts<DT, 512, 16, 0, 0, 1>(p, st);
   }
 }
 

@@ -64,14 +64,15 @@ def attend(q, kpool, vpool, table, lens, cu, scale, window=0, masks=None, pos=No
       a score        |ds| <= (d + 3) u scale sum |q_i k_i|
       a weight       exp2 of (score - maximum): its own |ds| and the maximum's, 4 u for exp2 and u times
                      the exponent's size (at most 150)
-      its parts      bf16: three hold it exactly. fp16: two leave 2^-21 of it (the first, cut to 11 bits,
-                     leaves 2^-10, the second's rounding 2^-11 of that), or 2^-38 of the largest weight
-                     where the second falls below fp16's least number (weights are taken up to 2^14)
+      its parts      bf16: two, each rounded to 8 bits, leave 2^-9 of 2^-9 of it (three hold it exactly).
+                     fp16: two, cut to 11 bits, leave 2^-10 of 2^-10 of it, or 2^-38 of the largest
+                     weight where the second falls below fp16's least number (weights are taken up to
+                     2^14)
       the sums       the parts' products add up in any order: 3 n terms, the later parts' 2^-7 of the
                      first's or less, so 2 n u of the sum of sizes, the weights' own sum n u, and as much
                      again for the joins of partial sums
-    so an output is off by at most A (2 (2 ds + 160 u) + 2^-21 + 6 n u) + n 2^-37 max |v|, and by half a
-    step of its type."""
+    so an output is off by at most A (2 (2 ds + 160 u) + 2^-18 or 2^-20 + 6 n u) + n 2^-37 max |v|
+    (fp16), and by half a step of its type."""
     N, hq, d = q.shape
     hkv, G = kpool.shape[1], hq // kpool.shape[1]
     u = 2.0 ** -24
@@ -112,8 +113,8 @@ def attend(q, kpool, vpool, table, lens, cu, scale, window=0, masks=None, pos=No
             ds = ((x.abs() @ kz[h // G].abs().T).masked_fill(~see, 0.0).amax(1, keepdim=True)
                   * abs(scale) * (d + 3) * u)
             rel = 2 * (2 * ds + 160 * u) + 6 * count * u
-            part = 2.0 ** -21 if q.dtype == torch.float16 else 0.0
-            lost = count * 2.0 ** -37 * vz[h // G].abs().max() if part else 0.0
+            part = {torch.bfloat16: 2.0 ** -18, torch.float16: 2.0 ** -20}.get(q.dtype, 0.0)
+            lost = count * 2.0 ** -37 * vz[h // G].abs().max() if q.dtype == torch.float16 else 0.0
             out[rows, h] = torch.where(some[:, None], o, 0.0)
             lse[rows, h] = torch.where(some, torch.logsumexp(s, 1), -math.inf)
             t = ((w @ vz[h // G].abs()) * (rel + part) + lost) * (1 + fi.eps)
