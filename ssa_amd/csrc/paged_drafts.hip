@@ -1333,9 +1333,9 @@ struct KeepParams {
   PageDiv div;
 };
 
-constexpr int kKeepThreads = 256, kKeepBatch = 8;
+constexpr int kKeepThreads = 128, kKeepBatch = 32;
 
-// A workgroup for a request and 256 columns (a column: 16 bytes of a layer's keys or values of a head,
+// A workgroup for a request and 128 columns (a column: 16 bytes of a layer's keys or values of a head,
 // over all tokens), a thread a column. An accepted token never moves up and they move in order, so a
 // column's tokens are read kKeepBatch at a time before any of these is written, and none that is
 // written is read again. All or nothing: every workgroup of a request checks its whole path first.
@@ -1390,12 +1390,21 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
     for (int i = 0; i < m; i += kKeepBatch) {
       u32x4 x[kKeepBatch];
 #pragma unroll
-      for (int u = 0; u < kKeepBatch; ++u)
-        if (i + u < m)
-          x[u] = *(const u32x4*)(base + s_page[0][i + u] * pp + s_slot[0][i + u] * ps);
+      for (int g = 0; g < kKeepBatch; g += 8) {
+        if (i + g >= m) break;
 #pragma unroll
-      for (int u = 0; u < kKeepBatch; ++u)
-        if (i + u < m) *(u32x4*)(base + s_page[1][i + u] * pp + s_slot[1][i + u] * ps) = x[u];
+        for (int u = g; u < g + 8; ++u) {
+          const int at = min(i + u, m - 1);
+          x[u] = *(const u32x4*)(base + s_page[0][at] * pp + s_slot[0][at] * ps);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kKeepBatch; g += 8) {
+        if (i + g >= m) break;
+#pragma unroll
+        for (int u = g; u < g + 8; ++u)
+          if (i + u < m) *(u32x4*)(base + s_page[1][i + u] * pp + s_slot[1][i + u] * ps) = x[u];
+      }
     }
   }
 }

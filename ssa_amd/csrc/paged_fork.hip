@@ -36,7 +36,9 @@ struct ForkParams {
   int32_t* old_lens;  // (B)
   int32_t* given;     // (units): pages given back, then the sum of those before
   int32_t* bad;       // (units)
-  int32_t* taken;     // (B): whether a page is taken, then its place on the stack
+  int32_t* taken;     // (B): whether a page is taken, then the pages taken before it (-1: none)
+  int32_t* top;       // (B): the stack's top before, the first page on top
+  int32_t* nfree0;    // (1): free pages before
   int32_t* left;      // (1): free pages after, -1: nothing changes
   int64_t units;      // of at most kForkEntries entries of a row
   int chunks;         // of a row
@@ -97,7 +99,12 @@ __device__ inline void fork_clear(const ForkParams& p, int unit) {
   const bool any = __any(bad);
   if ((threadIdx.x & 63) == 0) {
     p.bad[unit] = any;
-    if (chunk == 0) p.old_lens[b] = p.lens[b];
+    if (chunk == 0) {
+      p.old_lens[b] = p.lens[b];
+      const int nfree = *p.nfree, at = nfree - 1 - b;
+      p.top[b] = at >= 0 && at < p.P ? p.free_pages[at] : -1;
+      if (b == 0) *p.nfree0 = nfree;
+    }
   }
 }
 
@@ -156,8 +163,15 @@ __device__ inline void fork_count(const ForkParams& p, int unit) {
 
 constexpr int kForkThreads = 1024, kForkWaves = kForkThreads / 64;
 
-// 4, by one workgroup: sums of the units and rows before each, the status (all or nothing), and the
-// pages taken off the stack.
+// All or nothing: -1 or the pages lacking, 0 where the call fits.
+__device__ inline int fork_status(const ForkParams& p, bool bad, int64_t taken, int64_t given) {
+  const int nfree = *p.nfree0;
+  const int64_t lack = taken - nfree;
+  if (bad || nfree < 0 || nfree > p.P || nfree - taken + given > p.P) return -1;
+  return lack > 0 ? (int)lack : 0;
+}
+
+// 4, by one workgroup: sums of the units and rows before each, and the free pages after.
 __device__ inline void fork_sum(const ForkParams& p) {
   __shared__ int64_t s_wave[kForkWaves];
   __shared__ int64_t s_all;
@@ -165,8 +179,8 @@ __device__ inline void fork_sum(const ForkParams& p) {
   bool bad = false;
   for (int64_t u = tid; u < p.units; u += kForkThreads) bad |= p.bad[u] != 0;
   bad = __syncthreads_or(bad);
-  // x becomes the sum before it, running on from `sum`
-  auto scan = [&](int32_t* x, int64_t n) {
+  // x becomes the sum before it; a row that takes no page keeps -1
+  auto scan = [&](int32_t* x, int64_t n, bool mark) {
     int64_t sum = 0;
     for (int64_t i0 = 0; i0 < n; i0 += kForkThreads) {
       const int64_t i = i0 + tid;
@@ -182,48 +196,42 @@ __device__ inline void fork_sum(const ForkParams& p) {
         if (lane == 0) s_all = t.all;
       }
       __syncthreads();
-      // a row that takes no page keeps -1
-      if (i < n) x[i] = x == p.taken && v == 0 ? -1 : (int)min(sum + s_wave[wv] + s.upto - v,
-                                                               (int64_t)0x7fffffff);
+      if (i < n)
+        x[i] = mark && v == 0 ? -1 : (int)min(sum + s_wave[wv] + s.upto - v, (int64_t)0x7fffffff);
       sum += s_all;
     }
     return sum;
   };
-  const int64_t taken = scan(p.taken, p.B), given = scan(p.given, p.units);
-  const int nfree = *p.nfree;
-  const int64_t lack = taken - nfree, left = nfree - taken + given;
-  const int status = bad || nfree < 0 || nfree > p.P || left > p.P ? -1 : lack > 0 ? (int)lack : 0;
-  __syncthreads();
-  for (int64_t b = tid; b < p.B; b += kForkThreads) {
-    const int nth = status == 0 ? p.taken[b] : -1;
-    int from = -1, to = -1, n = 0;
-    if (nth >= 0) {
-      const ForkRow r = fork_row(p, p.old_lens, (int)b);
-      from = p.old[(int64_t)r.from * p.W + r.whole];
-      to = p.free_pages[nfree - 1 - nth];
-      n = r.want - r.whole * p.page;
-    }
-    p.source[b] = from;
-    p.target[b] = to;
-    p.tokens[b] = n;
-  }
+  const int64_t taken = scan(p.taken, p.B, true), given = scan(p.given, p.units, false);
   if (tid == 0) {
+    const int status = fork_status(p, bad, taken, given);
     *p.status = status;
-    *p.left = status == 0 ? (int)left : -1;
-    if (status == 0) *p.nfree = (int)left;
+    *p.left = status == 0 ? (int)(*p.nfree0 - taken + given) : -1;
   }
 }
 
-// 5: pages onto the stack, the new rows, the new lengths.
-__device__ inline void fork_write(const ForkParams& p, int unit) {
-  const int left = *p.left;
-  if (left < 0) return;
+// What a unit of step 5 goes by: the free pages after (-1: nothing changes), its row's place among the
+// pages taken, the pages given back before it.
+struct ForkPlace {
+  int left, taken, given;
+};
+
+// 5: the pages taken, those given back onto the stack, the new rows and lengths.
+__device__ inline void fork_write(const ForkParams& p, int unit, const ForkPlace& at_) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks, lane = threadIdx.x & 63;
   const ForkRow r = fork_row(p, p.old_lens, b);
-  const int fresh = p.target[b];
+  const int fresh = at_.left >= 0 && at_.taken >= 0 ? p.top[at_.taken] : -1;
+  const bool takes = at_.left >= 0 && at_.taken >= 0;
+  if (chunk == 0 && lane == 0) {
+    p.source[b] = takes ? p.old[(int64_t)r.from * p.W + r.whole] : -1;
+    p.target[b] = fresh;
+    p.tokens[b] = takes ? r.want - r.whole * p.page : 0;
+    if (b == 0 && at_.left >= 0) *p.nfree = at_.left;
+  }
+  if (at_.left < 0) return;
   int32_t* const row = p.table + b * p.table_stride;
   if (!r.same) {
-    int at = left - 1 - p.given[unit];
+    int at = at_.left - 1 - at_.given;
     const int first = chunk * kForkEntries;
 #pragma unroll 1
     for (int e = first + lane; e - lane < min(r.have, first + kForkEntries); e += 64) {
@@ -234,12 +242,42 @@ __device__ inline void fork_write(const ForkParams& p, int unit) {
     }
     const int32_t* const theirs = p.old + (int64_t)max(r.from, 0) * p.W;
     each_entry(chunk, max(r.have, r.need), [&](int, int e) {
-      row[e] = e >= r.need ? -1 : e == r.whole && fresh >= 0 ? fresh : theirs[e];
+      row[e] = e >= r.need ? -1 : e == r.whole && takes ? fresh : theirs[e];
     });
     if (chunk == 0 && lane == 0) p.lens[b] = r.want;
-  } else if (fresh >= 0 && chunk == r.whole / kForkEntries && lane == 0) {
+  } else if (takes && chunk == r.whole / kForkEntries && lane == 0) {
     row[r.whole] = fresh;
   }
+}
+
+__device__ inline ForkPlace fork_place(const ForkParams& p, int unit) {  // after step 4
+  return ForkPlace{*p.left, p.taken[unit / p.chunks], p.given[unit]};
+}
+
+// 4 and 5 at once, each wave adding up the units and rows by itself: a launch fewer where these are few.
+__device__ inline void fork_sum_write(const ForkParams& p, int unit) {
+  const int lane = threadIdx.x & 63, b = unit / p.chunks;
+  int64_t given = 0, given_all = 0, taken = 0, taken_all = 0;
+  bool bad = false;
+  for (int u = lane; u < p.units; u += 64) {
+    const int n = p.given[u];
+    given_all += n;
+    given += u < unit ? n : 0;
+    bad |= p.bad[u] != 0;
+  }
+  for (int y = lane; y < p.B; y += 64) {
+    const int n = p.taken[y];
+    taken_all += n;
+    taken += y < b ? n : 0;
+  }
+  given = lane_sums(given).all;
+  given_all = lane_sums(given_all).all;
+  taken = lane_sums(taken).all;
+  taken_all = lane_sums(taken_all).all;
+  const int status = fork_status(p, __any(bad), taken_all, given_all);
+  if (unit == 0 && lane == 0) *p.status = status;
+  fork_write(p, unit, ForkPlace{status == 0 ? (int)(*p.nfree0 - taken_all + given_all) : -1,
+                                p.taken[b] ? (int)taken : -1, (int)given});
 }
 
 // Makes this workgroup's writes and atomics visible to its later reads.
@@ -260,7 +298,7 @@ __global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkParams p) 
   fork_step();
   fork_sum(p);
   fork_step();
-  for (int u = wv; u < p.units; u += kForkWaves) fork_write(p, u);
+  for (int u = wv; u < p.units; u += kForkWaves) fork_write(p, u, fork_place(p, u));
 }
 
 // The steps as launches of their own, four units a workgroup.
@@ -277,16 +315,19 @@ __global__ __launch_bounds__(256) void paged_fork_count_kernel(ForkParams p) {
   if (u < p.units) fork_count(p, (int)u);
 }
 __global__ __launch_bounds__(kForkThreads) void paged_fork_sum_kernel(ForkParams p) { fork_sum(p); }
+template <bool SUM>
 __global__ __launch_bounds__(256) void paged_fork_write_kernel(ForkParams p) {
   const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  if (u < p.units) fork_write(p, (int)u);
+  if (u >= p.units) return;
+  if constexpr (SUM) fork_sum_write(p, (int)u);
+  else fork_write(p, (int)u, fork_place(p, (int)u));
 }
 
-constexpr int64_t kForkInside = 64;
+constexpr int64_t kForkInside = 16, kForkSums = 2048;
 
 struct ForkLayout {
   int64_t chunks, units;
-  size_t old, old_lens, given, bad, taken, left, bytes;
+  size_t old, old_lens, given, bad, taken, top, nfree0, left, bytes;
 };
 
 ForkLayout fork_layout(int64_t B, int64_t W, int64_t pages) {
@@ -298,7 +339,9 @@ ForkLayout fork_layout(int64_t B, int64_t W, int64_t pages) {
   y.given = y.old_lens + (size_t)B * 4;
   y.bad = y.given + (size_t)y.units * 4;
   y.taken = y.bad + (size_t)y.units * 4;
-  y.left = y.taken + (size_t)B * 4;
+  y.top = y.taken + (size_t)B * 4;
+  y.nfree0 = y.top + (size_t)B * 4;
+  y.left = y.nfree0 + 4;
   y.bytes = (y.left + 4 + 15) / 16 * 16;
   return y;
 }
@@ -316,7 +359,24 @@ struct CopyParams {
   int64_t kpl, kpp, kph, kps, vpl, vpp, vph, vps;  // bytes
 };
 
-constexpr int kCopyBatch = 4;
+// Division by a number of the call: an estimate that is one or two short, and its correction.
+struct Quotient {
+  unsigned d, mul;
+  __device__ explicit Quotient(unsigned by) : d(by), mul(0xffffffffu / by) {}
+  __device__ unsigned operator()(unsigned x, unsigned& rest) const {
+    unsigned q = __umulhi(x, mul);
+    rest = x - q * d;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool more = rest >= d;
+      q += more;
+      rest -= more ? d : 0;
+    }
+    return q;
+  }
+};
+
+constexpr int kCopyBatch = 8;
 
 // A thread moves 16-byte pieces of the copied tokens' keys and values, kCopyBatch of them on their way
 // at a time; a workgroup row (y) a page, x over a page's pieces of all layers.
@@ -325,17 +385,18 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
   const int64_t from = p.source[i], to = p.target[i];
   const int n = p.tokens ? min(p.tokens[i], p.page) : p.page;
   if (from < 0 || from >= p.pages || to < 0 || to >= p.pages || from == to || n <= 0) return;
-  const int per = n * p.vecs;  // pieces of a layer's keys or values of a head
-  const int64_t all = (int64_t)2 * p.layers * p.Hkv * per, step = (int64_t)gridDim.x * 256;
-  for (int64_t x0 = (int64_t)blockIdx.x * 256 + threadIdx.x; x0 < all; x0 += step * kCopyBatch) {
+  const unsigned per = n * p.vecs;  // pieces of a layer's keys or values of a head
+  const unsigned all = 2u * p.layers * p.Hkv * per, step = gridDim.x * 256;
+  const Quotient block(per), slot_of(p.vecs), head(p.Hkv);
+  for (unsigned x0 = blockIdx.x * 256 + threadIdx.x; x0 < all; x0 += step * kCopyBatch) {
     u32x4 v[kCopyBatch];
     char* at[kCopyBatch];
 #pragma unroll
     for (int u = 0; u < kCopyBatch; ++u) {
-      const int64_t x = x0 + u * step;
-      if (x >= all) continue;
-      const int of = (int)(x / per), r = (int)(x - (int64_t)of * per), slot = r / p.vecs;
-      const int lv = of / p.Hkv, h = of - lv * p.Hkv, c = r - slot * p.vecs;
+      const unsigned x = x0 + u * step;
+      if (x >= all) break;
+      unsigned r, c, h;
+      const unsigned of = block(x, r), slot = slot_of(r, c), lv = head(of, h);
       const bool val = lv & 1;
       char* const base = (val ? p.vpool : p.kpool) + (lv >> 1) * (val ? p.vpl : p.kpl) +
                          h * (val ? p.vph : p.kph) + slot * (val ? p.vps : p.kps) + c * 16;
@@ -344,8 +405,10 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
       at[u] = base + to * pp;
     }
 #pragma unroll
-    for (int u = 0; u < kCopyBatch; ++u)
-      if (x0 + u * step < all) *(u32x4*)at[u] = v[u];
+    for (int u = 0; u < kCopyBatch; ++u) {
+      if (x0 + u * step >= all) break;
+      *(u32x4*)at[u] = v[u];
+    }
   }
 }
 
@@ -385,7 +448,8 @@ extern "C" int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32
                free_pages, pages, nfree, source, target, tokens, status,
                page_div((int)page / 16), (PageUse*)ws, (int32_t*)(ws + y.old),
                (int32_t*)(ws + y.old_lens), (int32_t*)(ws + y.given), (int32_t*)(ws + y.bad),
-               (int32_t*)(ws + y.taken), (int32_t*)(ws + y.left), y.units, (int)y.chunks};
+               (int32_t*)(ws + y.taken), (int32_t*)(ws + y.top), (int32_t*)(ws + y.nfree0),
+               (int32_t*)(ws + y.left), y.units, (int)y.chunks};
   hipStream_t st = (hipStream_t)stream;
   if (y.units <= kForkInside) {
     paged_fork_kernel<<<1, kForkThreads, 0, st>>>(p);
@@ -398,9 +462,13 @@ extern "C" int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32
   SSA_TRY(launch_status("paged_fork_mark_kernel"));
   paged_fork_count_kernel<<<grid, 256, 0, st>>>(p);
   SSA_TRY(launch_status("paged_fork_count_kernel"));
+  if (y.units <= kForkSums) {
+    paged_fork_write_kernel<true><<<grid, 256, 0, st>>>(p);
+    return launch_status("paged_fork_write_kernel");
+  }
   paged_fork_sum_kernel<<<1, kForkThreads, 0, st>>>(p);
   SSA_TRY(launch_status("paged_fork_sum_kernel"));
-  paged_fork_write_kernel<<<grid, 256, 0, st>>>(p);
+  paged_fork_write_kernel<false><<<grid, 256, 0, st>>>(p);
   return launch_status("paged_fork_write_kernel");
 }
 
@@ -419,10 +487,12 @@ extern "C" int ssa_paged_copy(void* kpool, void* vpool, int dtype, int64_t layer
   // strides: kpool(layer,page,head,slot), vpool(layer,page,head,slot)
   SSA_REQUIRE(rows16(kpool, strides, 4, es) && rows16(vpool, strides + 4, 4, es), SSA_ERR_INVALID,
               "%s: rows must start at multiples of 16 bytes", who);
-  SSA_REQUIRE(fits_int(2 * layers * Hkv), SSA_ERR_UNSUPPORTED, "%s: %lld layers", who,
-              (long long)layers);
+  const int64_t vecs = d * es / 16;
+  // counted in 32 bits, up to a step of all workgroups past the end
+  SSA_REQUIRE(layers <= (1 << 30) / (Hkv * page * vecs), SSA_ERR_UNSUPPORTED,
+              "%s: %lld layers (a page of at most 32 GiB over all of them)", who, (long long)layers);
   if (n == 0) return SSA_OK;
-  const int64_t vecs = d * es / 16, pieces = 2 * layers * Hkv * page * vecs;
+  const int64_t pieces = 2 * layers * Hkv * page * vecs;
   // at most eight workgroups a CU for all pages, each with kCopyBatch pieces a thread or more
   const int64_t blocks = std::max<int64_t>(
       1, std::min((pieces + 256 * kCopyBatch - 1) / (256 * kCopyBatch), (2048 + n - 1) / n));
