@@ -1333,14 +1333,14 @@ struct KeepParams {
   PageDiv div;
 };
 
-constexpr int kKeepThreads = 128, kKeepBatch = 32;
+constexpr int kKeepThreads = 64, kKeepBatch = 32;
 
-// A workgroup for a request and 128 columns (a column: 16 bytes of a layer's keys or values of a head,
+// A workgroup for a request and 64 columns (a column: 16 bytes of a layer's keys or values of a head,
 // over all tokens), a thread a column. An accepted token never moves up and they move in order, so a
 // column's tokens are read kKeepBatch at a time before any of these is written, and none that is
 // written is read again. All or nothing: every workgroup of a request checks its whole path first.
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
-  __shared__ int s_page[2][kKeepThreads], s_slot[2][kKeepThreads];
+  __shared__ int64_t s_from[2][kKeepThreads], s_to[2][kKeepThreads];  // of keys and values
   __shared__ int s_first;
   const int b = blockIdx.y, tid = threadIdx.x;
   const int len = p.lens[b], c0 = p.cu[b], c1 = p.cu[b + 1], count = p.counts[b];
@@ -1375,15 +1375,19 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
   const int first = s_first, column = blockIdx.x * kKeepThreads + tid;
   const int c = column % p.vecs, of = column / p.vecs, h = of % p.Hkv, lv = of / p.Hkv;
   const bool mine = column < p.columns, v = lv & 1;
-  const int64_t pp = v ? p.vpp : p.kpp, ps = v ? p.vps : p.kps;
   char* const base = (v ? p.vpool : p.kpool) + (lv >> 1) * (v ? p.vpl : p.kpl) +
                      h * (v ? p.vph : p.kph) + c * 16;
   for (int i0 = first; i0 < count; i0 += kKeepThreads) {
     const int m = min(count - i0, kKeepThreads);
     __syncthreads();
     if (tid < m) {
-      place(path[i0 + tid], s_page[0][tid], s_slot[0][tid]);
-      place(i0 + tid, s_page[1][tid], s_slot[1][tid]);
+      int page, slot;
+      place(path[i0 + tid], page, slot);
+      s_from[0][tid] = page * p.kpp + slot * p.kps;
+      s_from[1][tid] = page * p.vpp + slot * p.vps;
+      place(i0 + tid, page, slot);
+      s_to[0][tid] = page * p.kpp + slot * p.kps;
+      s_to[1][tid] = page * p.vpp + slot * p.vps;
     }
     __syncthreads();
     if (!mine) continue;
@@ -1394,8 +1398,7 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
         if (i + g >= m) break;
 #pragma unroll
         for (int u = g; u < g + 8; ++u) {
-          const int at = min(i + u, m - 1);
-          x[u] = *(const u32x4*)(base + s_page[0][at] * pp + s_slot[0][at] * ps);
+          x[u] = *(const u32x4*)(base + s_from[v][min(i + u, m - 1)]);
         }
       }
 #pragma unroll
@@ -1403,7 +1406,7 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
         if (i + g >= m) break;
 #pragma unroll
         for (int u = g; u < g + 8; ++u)
-          if (i + u < m) *(u32x4*)(base + s_page[1][i + u] * pp + s_slot[1][i + u] * ps) = x[u];
+          if (i + u < m) *(u32x4*)(base + s_to[v][i + u]) = x[u];
       }
     }
   }

@@ -9,6 +9,8 @@ namespace {
 
 // ---- rows of the table from other rows ---------------------------------------------------------
 
+struct ForkRow;
+
 // What the call's rows say of a page: the first row that listed it and changes, the first row that will
 // hold it as its last, partly filled page, whether a row will hold it whole.
 struct PageUse {
@@ -33,7 +35,7 @@ struct ForkParams {
   // workspace
   PageUse* use;       // (P)
   int32_t* old;       // (B, W): the held entries of the table before
-  int32_t* old_lens;  // (B)
+  ForkRow* rows;      // (B)
   int32_t* given;     // (units): pages given back, then the sum of those before
   int32_t* bad;       // (units)
   int32_t* taken;     // (B): whether a page is taken, then the pages taken before it (-1: none)
@@ -46,23 +48,24 @@ struct ForkParams {
 
 constexpr int kForkEntries = 1024, kForkLoads = kForkEntries / 64;
 
-// A row's change, from its lengths alone.
+// A row's change.
 struct ForkRow {
   int from, len, want, have, whole, need;  // pages held before, to hold whole and to hold
-  bool ok, same;
+  int ok, same;
 };
 
-__device__ inline ForkRow fork_row(const ForkParams& p, const int32_t* lens, int b) {
+__device__ inline ForkRow fork_row(const ForkParams& p, int b) {
   ForkRow r;
-  r.len = lens[b];
+  r.len = p.lens[b];
   r.want = p.new_lens[b];
   r.from = p.src ? p.src[b] : b;
   r.ok = r.len >= 0 && r.len <= p.cap && r.want >= 0;
   if (r.want > 0) {
     r.ok = r.ok && r.from >= 0 && r.from < p.B;
-    const int of = r.ok ? lens[r.from] : 0;
+    const int of = r.ok ? p.lens[r.from] : 0;
     r.ok = r.ok && of <= p.cap && r.want <= of;
   }
+  if (!r.ok || r.want == 0) r.from = b;  // no page is taken from there
   r.have = r.ok ? paged_pages(r.len, p.page, p.div) : 0;
   r.need = r.ok ? paged_pages(r.want, p.page, p.div) : 0;
   r.whole = r.need - (r.want > r.need * p.page - p.page && r.want < r.need * p.page ? 1 : 0);
@@ -86,7 +89,7 @@ __device__ inline void each_entry(int chunk, int end, F f) {
 // 1: the table's held entries are kept, the uses of their pages cleared.
 __device__ inline void fork_clear(const ForkParams& p, int unit) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks;
-  const ForkRow r = fork_row(p, p.lens, b);
+  const ForkRow r = fork_row(p, b);
   bool bad = !r.ok;
   const int32_t* const row = p.table + b * p.table_stride;
   int id[kForkLoads];
@@ -100,7 +103,7 @@ __device__ inline void fork_clear(const ForkParams& p, int unit) {
   if ((threadIdx.x & 63) == 0) {
     p.bad[unit] = any;
     if (chunk == 0) {
-      p.old_lens[b] = p.lens[b];
+      p.rows[b] = r;
       const int nfree = *p.nfree, at = nfree - 1 - b;
       p.top[b] = at >= 0 && at < p.P ? p.free_pages[at] : -1;
       if (b == 0) *p.nfree0 = nfree;
@@ -111,10 +114,9 @@ __device__ inline void fork_clear(const ForkParams& p, int unit) {
 // 2: the uses of the pages.
 __device__ inline void fork_mark(const ForkParams& p, int unit) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks;
-  const ForkRow r = fork_row(p, p.old_lens, b);
-  const bool here = r.from >= 0 && r.from < p.B;
+  const ForkRow r = p.rows[b];
   const int32_t* const mine = p.old + b * p.W;
-  const int32_t* const theirs = p.old + (here ? r.from : 0) * p.W;
+  const int32_t* const theirs = p.old + r.from * p.W;
   int id[kForkLoads];
   each_entry(chunk, r.need, [&](int k, int e) { id[k] = theirs[e]; });
   each_entry(chunk, r.need, [&](int k, int e) {
@@ -140,11 +142,11 @@ __device__ inline bool copies(const PageUse& u, int b) { return u.whole || u.fir
 // 3: pages given back by the unit, and whether its row takes one.
 __device__ inline void fork_count(const ForkParams& p, int unit) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks, lane = threadIdx.x & 63;
-  const ForkRow r = fork_row(p, p.old_lens, b);
+  const ForkRow r = p.rows[b];
   if (chunk == 0 && lane == 0) {
     bool take = false;
     if (r.whole < r.need) {
-      const int id = p.old[(int64_t)r.from * p.W + r.whole];
+      const int id = p.old[r.from * p.W + r.whole];
       take = id >= 0 && id < p.P && copies(p.use[id], b);
     }
     p.taken[b] = take;
@@ -219,11 +221,11 @@ struct ForkPlace {
 // 5: the pages taken, those given back onto the stack, the new rows and lengths.
 __device__ inline void fork_write(const ForkParams& p, int unit, const ForkPlace& at_) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks, lane = threadIdx.x & 63;
-  const ForkRow r = fork_row(p, p.old_lens, b);
+  const ForkRow r = p.rows[b];
   const int fresh = at_.left >= 0 && at_.taken >= 0 ? p.top[at_.taken] : -1;
   const bool takes = at_.left >= 0 && at_.taken >= 0;
   if (chunk == 0 && lane == 0) {
-    p.source[b] = takes ? p.old[(int64_t)r.from * p.W + r.whole] : -1;
+    p.source[b] = takes ? p.old[r.from * p.W + r.whole] : -1;
     p.target[b] = fresh;
     p.tokens[b] = takes ? r.want - r.whole * p.page : 0;
     if (b == 0 && at_.left >= 0) *p.nfree = at_.left;
@@ -231,16 +233,21 @@ __device__ inline void fork_write(const ForkParams& p, int unit, const ForkPlace
   if (at_.left < 0) return;
   int32_t* const row = p.table + b * p.table_stride;
   if (!r.same) {
+    int id[kForkLoads];
+    unsigned int give = 0;
+    each_entry(chunk, r.have, [&](int k, int e) { id[k] = p.old[b * p.W + e]; });
+    each_entry(chunk, r.have, [&](int k, int) {
+      give |= gives(p.use[id[k]], b) ? 1u << k : 0u;
+    });
     int at = at_.left - 1 - at_.given;
-    const int first = chunk * kForkEntries;
-#pragma unroll 1
-    for (int e = first + lane; e - lane < min(r.have, first + kForkEntries); e += 64) {
-      const int id = e < r.have ? p.old[b * p.W + e] : -1;
-      const unsigned long long all = __ballot(id >= 0 && gives(p.use[id], b));
-      if (all >> lane & 1) p.free_pages[at - __popcll(all & ((1ull << lane) - 1))] = id;
+#pragma unroll
+    for (int k = 0; k < kForkLoads; ++k) {
+      if (chunk * kForkEntries + k * 64 >= r.have) break;
+      const unsigned long long all = __ballot(give >> k & 1);
+      if (give >> k & 1) p.free_pages[at - __popcll(all & ((1ull << lane) - 1))] = id[k];
       at -= __popcll(all);
     }
-    const int32_t* const theirs = p.old + (int64_t)max(r.from, 0) * p.W;
+    const int32_t* const theirs = p.old + r.from * p.W;
     each_entry(chunk, max(r.have, r.need), [&](int, int e) {
       row[e] = e >= r.need ? -1 : e == r.whole && takes ? fresh : theirs[e];
     });
@@ -327,16 +334,16 @@ constexpr int64_t kForkInside = 16, kForkSums = 2048;
 
 struct ForkLayout {
   int64_t chunks, units;
-  size_t old, old_lens, given, bad, taken, top, nfree0, left, bytes;
+  size_t old, rows, given, bad, taken, top, nfree0, left, bytes;
 };
 
 ForkLayout fork_layout(int64_t B, int64_t W, int64_t pages) {
   ForkLayout y{};
   y.chunks = (W + kForkEntries - 1) / kForkEntries;
   y.units = B * y.chunks;
-  y.old = (size_t)pages * sizeof(PageUse);
-  y.old_lens = y.old + (size_t)B * W * 4;
-  y.given = y.old_lens + (size_t)B * 4;
+  y.rows = (size_t)pages * sizeof(PageUse);
+  y.old = y.rows + (size_t)B * sizeof(ForkRow);
+  y.given = y.old + (size_t)B * W * 4;
   y.bad = y.given + (size_t)y.units * 4;
   y.taken = y.bad + (size_t)y.units * 4;
   y.top = y.taken + (size_t)B * 4;
@@ -447,7 +454,7 @@ extern "C" int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32
   ForkParams p{src, new_lens, lens, table, table_stride, W, W * page, (int)B, (int)page,
                free_pages, pages, nfree, source, target, tokens, status,
                page_div((int)page / 16), (PageUse*)ws, (int32_t*)(ws + y.old),
-               (int32_t*)(ws + y.old_lens), (int32_t*)(ws + y.given), (int32_t*)(ws + y.bad),
+               (ForkRow*)(ws + y.rows), (int32_t*)(ws + y.given), (int32_t*)(ws + y.bad),
                (int32_t*)(ws + y.taken), (int32_t*)(ws + y.top), (int32_t*)(ws + y.nfree0),
                (int32_t*)(ws + y.left), y.units, (int)y.chunks};
   hipStream_t st = (hipStream_t)stream;
