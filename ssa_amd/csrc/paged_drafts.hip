@@ -828,18 +828,8 @@ __device__ inline f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Waits until at most N of this wave's loads are on their way and its LDS reads are done, then for the
-// other waves: what all but the last N loads wrote to LDS is there.
-template <int N>
-__device__ inline void ring_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 0 << 8 | (N >> 4) << 14);
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // Attention of a tile of rows over an item's keys, a wave's RW rows (16 or 32) against all of them:
-// tiles of KT keys go from memory to LDS, RING - 1 ahead of the products, and serve the four waves.
+// tiles of KT keys go from memory to LDS, one ahead of the products, and serve the four waves.
 // Scores are K Q^T: lane column a row, so its statistics and its weights stay in its lanes and are the
 // second product's operand as they are; values are transposed by the LDS reads. A lane's scores come in
 // quads: r of quad q is key 4 GR q + 4 grp + r, GR = 64 / RW lanes of a row. bf16 weights, whose
@@ -847,7 +837,7 @@ __device__ inline void ring_barrier() {
 // nothing looks for infinite or NaN values: where a sum or a result is too large or not finite, the item is
 // done again with care (the maximum raised tile by tile, values that are not finite taken out of the
 // products as in paged_drafts_kernel).
-template <int DT, int DP, int RW, int KT, int RING, int WPE>
+template <int DT, int DP, int RW, int KT, int WPE>
 __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams p) {
   typedef typename std::conditional<RW == 16, f32x4, f32x16>::type Acc;
   constexpr int NW = 4, M = NW * RW, GR = 64 / RW, ROW = DP * 2, TILE = KT * ROW;
@@ -856,13 +846,10 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   constexpr int CH = ROW / 16, RPI = 64 / CH, LPW = KT / RPI / NW;  // chunks, rows, loads of a wave
   constexpr float kShift = DT == SSA_F16 ? kF16Shift : 0.0f;
   constexpr float kGrow = DT == SSA_F16 ? 1.0f : 8.0f;  // fp16 weights end at 2^16
-  static_assert(LPW >= 1 && RPI <= 16 && (RW == 16 || RW == 32) && RING >= 2 && RING <= 4, "");
   // a stage is the keys' tile and the values'; objects of their own, so that the compiler's waits for
-  // one are not for the others
+  // one are not for the other
   __shared__ __attribute__((aligned(1024))) unsigned char st0[2 * TILE];
   __shared__ __attribute__((aligned(1024))) unsigned char st1[2 * TILE];
-  __shared__ __attribute__((aligned(1024))) unsigned char st2[RING > 2 ? 2 * TILE : 16];
-  __shared__ __attribute__((aligned(1024))) unsigned char st3[RING > 3 ? 2 * TILE : 16];
   if (blockIdx.x >= p.blocks) {
     rest_rows<DT>(p, (int)(blockIdx.x - p.blocks));
     return;
@@ -924,6 +911,10 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   // every other j, and the swizzle's other bit moves along.
   const int lchunk = lane % CH;
   auto load_row = [&](int j) { return ((j * NW + wv) * RPI + lane / CH) & 15; };
+  auto load = [&](const char* from, unsigned char* to) __attribute__((always_inline)) {
+    if (it.stream) __builtin_amdgcn_global_load_lds((MemPtr)from, (LdsPtr)to, 16, 0, kStream);
+    else __builtin_amdgcn_global_load_lds((MemPtr)from, (LdsPtr)to, 16, 0, 0);
+  };
   auto issue = [&](unsigned char* to, int i) __attribute__((always_inline)) {
     const int s0 = it.begin + i * SUB;
     if (s0 >= batch + 64) {
@@ -938,20 +929,18 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
       const int r = load_row(j), c = lchunk ^ tile_swz<DP>(r);
       const int64_t pg = __builtin_amdgcn_readlane(pid, at);
       const int64_t off = __builtin_amdgcn_readlane(poff, at);
-      const char* k = kbase + (pg * kpp + off * kps) + (r * kps + c * 16);
-      const char* v = vbase + (pg * vpp + off * vps) + (r * vps + c * 16);
-      if (!full) {  // columns past d and rows that do not count are read as zero
+      const char* const k = kbase + (pg * kpp + off * kps);
+      const char* const v = vbase + (pg * vpp + off * vps);
+      const unsigned int ko = r * kps + c * 16, vo = r * vps + c * 16;
+      if (full) {
+        load(k + ko, to + u * 1024);
+        load(v + vo, to + TILE + u * 1024);
+      } else {  // columns past d and rows that do not count are read as zero
         const int key = s * 16 + r;
+        const bool in = c * 16 < row_bytes;
         const char* const zero = (const char*)kZeroRow + lchunk * 16;
-        if (c * 16 >= row_bytes) k = zero;
-        if (c * 16 >= row_bytes || s >= it.end || key < first || key >= len) v = zero;
-      }
-      if (it.stream) {
-        __builtin_amdgcn_global_load_lds((MemPtr)k, (LdsPtr)(to + u * 1024), 16, 0, kStream);
-        __builtin_amdgcn_global_load_lds((MemPtr)v, (LdsPtr)(to + TILE + u * 1024), 16, 0, kStream);
-      } else {
-        __builtin_amdgcn_global_load_lds((MemPtr)k, (LdsPtr)(to + u * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((MemPtr)v, (LdsPtr)(to + TILE + u * 1024), 16, 0, 0);
+        load(in ? k + ko : zero, to + u * 1024);
+        load(in && s < it.end && key >= first && key < len ? v + vo : zero, to + TILE + u * 1024);
       }
     }
   };
@@ -1084,28 +1073,15 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     take_pages(v);
   };
   begin();
-  // Tile i is there for all waves, tile i - 1 is read no more: its stage takes the one RING - 1 on.
-  auto step = [&](const unsigned char* now, unsigned char* next, int i) __attribute__((always_inline)) {
-    if (RING > 2 && i + RING - 2 < tiles) ring_barrier<(RING - 2) * 2 * LPW>();
-    else ring_barrier<0>();
-    if (i + RING - 1 < tiles) issue(next, i + RING - 1);
-    if (any) compute(now, i, std::false_type{});
-  };
   if (tiles > 0) issue(st0, 0);
-  if (RING > 2 && tiles > 1) issue(st1, 1);
-  if (RING > 3 && tiles > 2) issue(st2, 2);
-  for (int i = 0; i < tiles; i += RING) {
-    step(st0, RING > 3 ? st3 : RING > 2 ? st2 : st1, i);
+  for (int i = 0; i < tiles; i += 2) {
+    dma_barrier();  // tile i is there for all waves; tile i - 1 is read no more
+    if (i + 1 < tiles) issue(st1, i + 1);
+    if (any) compute(st0, i, std::false_type{});
     if (i + 1 >= tiles) break;
-    step(st1, st0, i + 1);
-    if constexpr (RING > 2) {
-      if (i + 2 >= tiles) break;
-      step(st2, st1, i + 2);
-    }
-    if constexpr (RING > 3) {
-      if (i + 3 >= tiles) break;
-      step(st3, st2, i + 3);
-    }
+    dma_barrier();
+    if (i + 2 < tiles) issue(st0, i + 2);
+    if (any) compute(st1, i + 1, std::false_type{});
   }
   bool off = !(l < 0x1p100f);
 #pragma unroll
@@ -1281,11 +1257,11 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   return y;
 }
 
-template <int DT, int DP, int M, int KT, int RING, int WPE>
+template <int DT, int DP, int M, int KT, int WPE>
 int run_drafts(const DraftParams& p, hipStream_t st) {
   const unsigned blocks = (unsigned)(p.blocks + kRestBlocks);
   if constexpr (KT != 0)
-    paged_drafts_tile_kernel<DT, DP, M / 4, KT, RING, WPE><<<blocks, 256, 0, st>>>(p);
+    paged_drafts_tile_kernel<DT, DP, M / 4, KT, WPE><<<blocks, 256, 0, st>>>(p);
   else
     paged_drafts_kernel<DT, DP, M / 16, WPE><<<blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_drafts_kernel"));
@@ -1298,20 +1274,20 @@ int run_drafts(const DraftParams& p, hipStream_t st) {
 template <int DT>
 int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
   if constexpr (DT != SSA_F32) {
-    if (y.M == 64 && y.dp == 64) return run_drafts<DT, 64, 64, 64, 3, 3>(p, st);
-    if (y.M == 64 && y.dp == 128) return run_drafts<DT, 128, 64, 32, 3, 3>(p, st);
-    if (y.M == 64 && y.dp == 256) return run_drafts<DT, 256, 64, 32, 2, 2>(p, st);
-    if (y.M == 128 && y.dp == 64) return run_drafts<DT, 64, 128, 64, 3, 3>(p, st);
-    if (y.M == 128 && y.dp == 128) return run_drafts<DT, 128, 128, 64, 2, 2>(p, st);
+    if (y.M == 64 && y.dp == 64) return run_drafts<DT, 64, 64, 64, 4>(p, st);
+    if (y.M == 64 && y.dp == 128) return run_drafts<DT, 128, 64, 32, 4>(p, st);
+    if (y.M == 64 && y.dp == 256) return run_drafts<DT, 256, 64, 32, 2>(p, st);
+    if (y.M == 128 && y.dp == 64) return run_drafts<DT, 64, 128, 64, 3>(p, st);
+    if (y.M == 128 && y.dp == 128) return run_drafts<DT, 128, 128, 64, 2>(p, st);
   } else {
-    if (y.M == 32 && y.dp == 64) return run_drafts<DT, 64, 32, 0, 0, 2>(p, st);
-    if (y.M == 32 && y.dp == 128) return run_drafts<DT, 128, 32, 0, 0, 2>(p, st);
+    if (y.M == 32 && y.dp == 64) return run_drafts<DT, 64, 32, 0, 2>(p, st);
+    if (y.M == 32 && y.dp == 128) return run_drafts<DT, 128, 32, 0, 2>(p, st);
   }
   switch (y.dp) {
-    case 64: return run_drafts<DT, 64, 16, 0, 0, 3>(p, st);
-    case 128: return run_drafts<DT, 128, 16, 0, 0, 2>(p, st);
-    case 256: return run_drafts<DT, 256, 16, 0, 0, 1>(p, st);
-    default: return run_drafts<DT, 512, 16, 0, 0, 1>(p, st);
+    case 64: return run_drafts<DT, 64, 16, 0, 3>(p, st);
+    case 128: return run_drafts<DT, 128, 16, 0, 2>(p, st);
+    case 256: return run_drafts<DT, 256, 16, 0, 1>(p, st);
+    default: return run_drafts<DT, 512, 16, 0, 1>(p, st);
   }
 }
 
