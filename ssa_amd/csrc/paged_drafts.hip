@@ -127,33 +127,33 @@ __device__ inline DraftSpan draft_of(const DraftParams& p, int b) {
 
 // Finds workgroup `id`'s item from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. Of the call's row tiles an XCD takes a run, the tiles of the
-// same keys next to each other: its L2 serves them together. False past the last one.
+// same keys next to each other: its L2 serves them together. False past the last one. Sums of offsets
+// that do not ascend may wrap; the item's own numbers are checked.
 template <int M>
 __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   const int lane = threadIdx.x & 63;
   const int run = (p.B + 63) / 64, b0 = min(lane * run, p.B), b1 = min(b0 + run, p.B);
   DraftSpan own{};
-  int units = 0;
-  int64_t tiles = 0, work = 0;
+  int units = 0, tiles = 0;
+  float work = 0.0f;
   for (int b = b0; b < b1; ++b) {
     own = draft_of(p, b);
     units = draft_units(own);
     tiles = draft_tiles(own, p.G, M);
-    work += tiles * units;
+    work += (float)tiles * (float)units;
   }
   int chunk = 0x7fffffff;
   it.stream = p.stream_units == 0;
   if (p.items != 0) {
-    const int64_t all = lane_sums(work).all;
-    chunk = draft_chunk(all, p.items);
-    it.stream = all >= p.stream_units;
+    const float all = lane_sums(work).all;
+    chunk = draft_chunk(all, (float)p.items);
+    it.stream = all >= (float)p.stream_units;
   }
-  int64_t n = 0, parts = 0;
-  auto count = [&](int64_t of, int u) {
+  int n = 0, parts = 0;
+  auto count = [&](int of, int u) {
     const int splits = paged_items(u, chunk);
     n += of * splits;
     parts += splits > 1 ? of * splits : 0;
-    return splits;
   };
   if (run == 1) {
     count(tiles, units);
@@ -163,39 +163,39 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
       count(draft_tiles(s, p.G, M), draft_units(s));
     }
   }
-  const LaneSums<int64_t> sums = lane_sums(n);
-  const int64_t all = sums.all * p.Hkv, per = (all + 7) / 8, index = (id & 7) * per + (id >> 3);
+  const LaneSums<int> sums = lane_sums(n);
+  const int all = sums.all * p.Hkv, per = (int)(((unsigned)all + 7u) / 8u);
+  const int index = (id & 7) * per + (id >> 3);
   if ((id >> 3) >= per || index >= all) return false;
   const unsigned long long past = __ballot(sums.upto * p.Hkv > index);
   if (past == 0) return false;
   const int owner = __builtin_ctzll(past);
-  const LaneSums<int64_t> part_sums = lane_sums(parts);
-  auto pick = [&](int64_t x) {
-    const unsigned int lo = __builtin_amdgcn_readlane((unsigned int)x, owner);
-    const unsigned int hi = __builtin_amdgcn_readlane((unsigned int)(x >> 32), owner);
-    return (int64_t)((uint64_t)hi << 32 | lo);
-  };
-  int64_t first = pick(sums.upto - n), part = pick(part_sums.upto - parts);
+  const LaneSums<int> part_sums = lane_sums(parts);
+  int first = __builtin_amdgcn_readlane(sums.upto - n, owner);
+  int part = __builtin_amdgcn_readlane(part_sums.upto - parts, owner);
   it.b = owner * run;
   for (;; ++it.b) {
     it.s = draft_of(p, it.b);
     units = draft_units(it.s);
     tiles = draft_tiles(it.s, p.G, M);
     it.n = paged_items(units, chunk);
-    if (run == 1 || index < (first + tiles * it.n) * p.Hkv) break;
+    if (run == 1 || it.b + 1 >= min((owner + 1) * run, p.B) ||
+        index < (first + tiles * it.n) * p.Hkv) break;
     first += tiles * it.n;
     part += it.n > 1 ? tiles * it.n : 0;
   }
+  const unsigned int at = (unsigned)(index - first * p.Hkv);
+  if (tiles <= 0 || at / (unsigned)tiles >= (uint64_t)it.n * p.Hkv) return false;
   it.c0 = p.cu[it.b];
-  it.tiles = (int)tiles;
-  const int64_t at = index - first * p.Hkv, row = at / tiles;
+  it.tiles = tiles;
+  const unsigned int row = at / (unsigned)tiles;
   it.tile = (int)(at - row * tiles);
-  it.j = (int)(row / p.Hkv);
-  it.g = (int)(row - (int64_t)it.j * p.Hkv);
+  it.j = (int)(row / (unsigned)p.Hkv);
+  it.g = (int)(row - (unsigned)it.j * p.Hkv);
   it.stream = it.stream && it.tiles == 1;
   // parts that the workspace does not hold (offsets that do not ascend): the join answers
-  part *= p.Hkv;
-  it.first_part = it.n > 1 && part + tiles * it.n * p.Hkv > p.max_parts ? -1 : (int)part;
+  const int64_t part0 = (int64_t)part * p.Hkv, part_end = part0 + (int64_t)tiles * it.n * p.Hkv;
+  it.first_part = it.n > 1 && (part < 0 || part_end > p.max_parts) ? -1 : (int)part0;
   it.begin = it.end = 0;
   if (it.s.span.ok) {
     const PagedRange r = paged_item_range(it.s.span, units, it.j, it.n);
@@ -360,11 +360,11 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   int late = 0;  // the latest first key of the tile's rows
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int64_t x = (int64_t)it.tile * M + mt * 16 + col;
-    const int t = (int)(x / p.G);
+    const unsigned int x = it.tile * M + mt * 16 + col;
+    const int t = (int)(x / (unsigned)p.G);
     real[mt] = t < n;
     tok[mt] = min(t, n - 1);
-    head[mt] = it.g * p.G + (int)(x - (int64_t)t * p.G);
+    head[mt] = it.g * p.G + (int)(x - (unsigned)t * p.G);
     rpos[mt] = !p.masks ? ctx + tok[mt] : p.pos[(int64_t)it.c0 + tok[mt]];
     start[mt] = p.window > 0 && rpos[mt] >= p.window ? rpos[mt] - p.window + 1 : 0;
     late = max(late, start[mt]);
@@ -863,8 +863,9 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   const int ctx = it.s.ctx, n = it.s.n, first = it.s.span.first, len = it.s.span.len;
   const int tiles = (it.end - it.begin + SUB - 1) / SUB;
 
-  const int64_t x = (int64_t)it.tile * M + wv * RW + col;
-  const int t0 = (int)(x / p.G), tok = min(t0, n - 1), head = it.g * p.G + (int)(x - (int64_t)t0 * p.G);
+  const unsigned int x = it.tile * M + wv * RW + col;
+  const int t0 = (int)(x / (unsigned)p.G), tok = min(t0, n - 1);
+  const int head = it.g * p.G + (int)(x - (unsigned)t0 * p.G);
   const bool real = t0 < n, any = __any(real);  // a wave without rows loads and waits with the others
   const int rpos = !p.masks ? ctx + tok : p.pos[(int64_t)it.c0 + tok];
   const int start = p.window > 0 && rpos >= p.window ? rpos - p.window + 1 : 0;
@@ -1145,17 +1146,17 @@ template <int DT, int DP, int M>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;
   const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  const int64_t row = id / p.Hq;
+  const unsigned int id = blockIdx.x * 4 + uniform(threadIdx.x >> 6), token = id / (unsigned)p.Hq;
+  const int64_t row = token;
   if (row >= p.N || (p.status && *p.status != 0)) return;
-  const int h = (int)(id - row * p.Hq), g = h / p.G;
+  const int h = (int)(id - token * p.Hq), g = h / p.G;
   const int b = last_at_most(p.cu, p.B, (int)row), c0 = p.cu[b], c1 = p.cu[b + 1];
   const DraftSpan s = draft_of(p, b);
   if (row < c0 || row >= c1 || s.n == 0) return;
   const int first = p.info[2 * b], parts = p.info[2 * b + 1];
   if (parts <= 1) return;  // written by its one item
-  const int64_t x = (row - c0) * p.G + (h - g * p.G), tiles = draft_tiles(s, p.G, M);
-  const int64_t tile = x / M, step = tiles * p.Hkv;
+  const unsigned int x = (unsigned)(row - c0) * p.G + (h - g * p.G), tile = x / M;
+  const int64_t tiles = draft_tiles(s, p.G, M), step = tiles * p.Hkv;
   const bool held = first >= 0 && first + step * parts <= p.max_parts;
   const int64_t at = ((held ? first : 0) + g * tiles + tile) * M + x % M;
   const int split = lane / PER % NS, c = lane % PER * 4;
@@ -1465,7 +1466,7 @@ extern "C" int ssa_paged_attend_drafts(const void* q, const void* kpool, const v
   SSA_REQUIRE(workspace_bytes >= y.bytes && (y.bytes == 0 || (workspace && aligned16(workspace))),
               SSA_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who,
               y.bytes, workspace_bytes);
-  SSA_REQUIRE(fits_launch(y.blocks + kRestBlocks, kAttendWaves * 64) &&
+  SSA_REQUIRE(fits_launch(y.blocks + kRestBlocks, kAttendWaves * 64) && fits_int(N * Hq) &&
                   fits_launch((N * Hq + 3) / 4, 256), SSA_ERR_UNSUPPORTED,
               "%s: too many rows in one call", who);
   DraftParams p{};

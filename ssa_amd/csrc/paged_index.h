@@ -102,16 +102,17 @@ SSA_HD int draft_units(const DraftSpan& s) {
   return s.n == 0 ? 0 : s.span.ok ? paged_units(s.span) : 1;
 }
 
-// Tiles of M rows, a row a drafted token and one of the G query heads of a key head.
-SSA_HD int64_t draft_tiles(const DraftSpan& s, int64_t G, int M) {
-  return ((int64_t)s.n * G + M - 1) / M;
+// Tiles of M rows, a row a drafted token and one of the G query heads of a key head (a call's rows are
+// held below 2^31).
+SSA_HD int draft_tiles(const DraftSpan& s, int G, int M) {
+  return (int)(((unsigned)s.n * (unsigned)G + (unsigned)M - 1u) / (unsigned)M);
 }
 
-// Units per item so that `work` units (of every row tile) make at most `items` items besides one more
-// per row tile.
-SSA_HD int draft_chunk(int64_t work, int64_t items) {
-  const int64_t c = work <= items ? 1 : (work + items - 1) / items;
-  return c > (1 << 30) ? 1 << 30 : (int)c;
+// Units per item so that `work` units (of every row tile, a sum of floats that may be 10^-5 off) make
+// at most `items` items besides one more per row tile.
+SSA_HD int draft_chunk(float work, float items) {
+  const float c = work / items * 1.00002f;
+  return c >= 1e9f ? 1000000000 : (int)c + 1;
 }
 
 // The most row tiles that N tokens of B requests make, and the most items of requests that are cut

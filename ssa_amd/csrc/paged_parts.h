@@ -16,6 +16,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ inline int other_lane(int x, int j) { return lane_xor(x, j); }
+__device__ inline float other_lane(float x, int j) { return lane_xor(x, j); }
 __device__ inline int64_t other_lane(int64_t x, int j) {
   const unsigned int lo = lane_xor((unsigned int)x, j), hi = lane_xor((unsigned int)(x >> 32), j);
   return (int64_t)((uint64_t)hi << 32 | lo);
