@@ -792,8 +792,12 @@ __device__ inline int tile_swz(int r) {
   return (r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
 }
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
-typedef const __attribute__((address_space(1))) void* MemPtr;
+// 16 bytes of each lane from memory to LDS, the wave's one after the other from `to` on.
+template <int AUX>
+__device__ inline void load_lds(const char* from, unsigned char* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, AUX);
+}
 
 // Weights of two keys as 16-bit parts, two for either type: bf16's, rounded to nearest, leave 2^-18 of a
 // weight at most, fp16's, cut, 2^-20. The output keeps 8 and 11 bits. (bf16's third part, which holds
@@ -912,10 +916,6 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   // every other j, and the swizzle's other bit moves along.
   const int lchunk = lane % CH;
   auto load_row = [&](int j) { return ((j * NW + wv) * RPI + lane / CH) & 15; };
-  auto load = [&](const char* from, unsigned char* to) __attribute__((always_inline)) {
-    if (it.stream) __builtin_amdgcn_global_load_lds((MemPtr)from, (LdsPtr)to, 16, 0, kStream);
-    else __builtin_amdgcn_global_load_lds((MemPtr)from, (LdsPtr)to, 16, 0, 0);
-  };
   auto issue = [&](unsigned char* to, int i) __attribute__((always_inline)) {
     const int s0 = it.begin + i * SUB;
     if (s0 >= batch + 64) {
@@ -924,25 +924,35 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
       pid_next = pages_at(batch + 64);
     }
     const bool full = DP == p.d && s0 * 16 >= first && s0 * 16 + KT <= len && s0 + SUB <= it.end;
+    auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-      const int u = j * NW + wv, s = s0 + u * RPI / 16, at = min(s, it.end - 1) - batch;
-      const int r = load_row(j), c = lchunk ^ tile_swz<DP>(r);
-      const int64_t pg = __builtin_amdgcn_readlane(pid, at);
-      const int64_t off = __builtin_amdgcn_readlane(poff, at);
-      const char* const k = kbase + (pg * kpp + off * kps);
-      const char* const v = vbase + (pg * vpp + off * vps);
-      const unsigned int ko = r * kps + c * 16, vo = r * vps + c * 16;
-      if (full) {
-        load(k + ko, to + u * 1024);
-        load(v + vo, to + TILE + u * 1024);
-      } else {  // columns past d and rows that do not count are read as zero
-        const int key = s * 16 + r;
-        const bool in = c * 16 < row_bytes;
-        const char* const zero = (const char*)kZeroRow + lchunk * 16;
-        load(in ? k + ko : zero, to + u * 1024);
-        load(in && s < it.end && key >= first && key < len ? v + vo : zero, to + TILE + u * 1024);
+      for (int j = 0; j < LPW; ++j) {
+        const int u = j * NW + wv, s = s0 + u * RPI / 16, at = min(s, it.end - 1) - batch;
+        const int r = load_row(j), c = lchunk ^ tile_swz<DP>(r);
+        const int64_t pg = __builtin_amdgcn_readlane(pid, at);
+        const int64_t off = __builtin_amdgcn_readlane(poff, at);
+        f(kbase + (pg * kpp + off * kps) + (unsigned)(r * kps + c * 16),
+          vbase + (pg * vpp + off * vps) + (unsigned)(r * vps + c * 16), to + u * 1024, s * 16 + r,
+          c * 16 < row_bytes, s < it.end);
       }
+    };
+    if (full && it.stream) {
+      each([&](const char* k, const char* v, unsigned char* at, int, bool, bool) {
+        load_lds<kStream>(k, at);
+        load_lds<kStream>(v, at + TILE);
+      });
+    } else if (full) {
+      each([&](const char* k, const char* v, unsigned char* at, int, bool, bool) {
+        load_lds<0>(k, at);
+        load_lds<0>(v, at + TILE);
+      });
+    } else {  // columns past d and rows that do not count are read as zero
+      each([&](const char* k, const char* v, unsigned char* at, int key, bool in, bool own) {
+        const char* const zero = (const char*)kZeroRow + lchunk * 16;
+        const bool counts = in & own & (key >= first) & (key < len);
+        load_lds<0>(in ? k : zero, at);
+        load_lds<0>(counts ? v : zero, at + TILE);
+      });
     }
   };
 
