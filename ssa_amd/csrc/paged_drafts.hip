@@ -330,8 +330,9 @@ __device__ inline float not_finite_sum(float with, float without) {
 // paged_attend_kernel's, a row where that has a head. Tiles of keys that some row does not attend (the
 // drafted ones, the last, a window's first) take their masks from the rows' words; their lowest score
 // -FLT_MAX stands for attended keys, so that -INFINITY means a row without any. A value that is infinite
-// or NaN there would reach the rows that do not attend it as 0 x infinity: such values are taken out of
-// the product and added to the rows that attend them.
+// or NaN there reaches the rows that do not attend it as 0 x infinity: where a result is NaN, the wave
+// does its keys again with care, such values taken out of the product and added to the rows that attend
+// them.
 template <int DT, int DP, int MT, int WPE>
 __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(DraftParams p) {
   using T = Tile<DT, DP>;
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   }
   const int32_t* const row = p.table + it.b * p.table_stride;
   // page and offset of 64 subtiles at a time, one per lane; the next 64 are on their way
-  int pid = 0, poff = 0, pid_next = 0, batch = it.begin + i0 * NT;
+  int pid = 0, poff = 0, pid_next = 0, batch = 0;
   unsigned long long bad = 0;
   const int sub_end = min(it.begin + i1 * NT, it.end);
   auto pages_at = [&](int s) {
@@ -419,21 +420,8 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
     pid = x < 0 || x >= p.pages ? 0 : x;
     poff = (batch + lane) * 16 - page_of(batch + lane, p.div) * p.page;
   };
-  if (i0 < i1) {
-    const int x = pages_at(batch);
-    pid_next = pages_at(batch + 64);
-    take_pages(x);
-  }
-
   Rows<DT, DP> rows;
   Softmax<NA> st[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    st[mt].m = -INFINITY;
-    st[mt].l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NA; ++i) st[mt].acc[i] = f32x4{0, 0, 0, 0};
-  }
 
   // pages of tile i's subtiles (the last one again past the wave's end)
   int64_t pg[NT];
@@ -561,153 +549,175 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
         }
   };
 
-  if (i0 < i1) {
-    locate(i0);
-    load_k(0);
-    load_v(i0);
-  }
-  for (int i = i0; i < i1; ++i) {
-    const int j0 = (it.begin + i * NT) * 16;
-    const bool edge = j0 < late || j0 + NT * 16 > ctx;
-    if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
-    // scores: lane column a row, rows the keys 4 grp + r of each subtile; fp32 in kChains chains, as
-    // paged_attend_kernel
-    constexpr int kChains = DT != SSA_F32 ? 1 : DP == 64 ? 2 : 4;
-    f32x4 s[MT][NT], chain[MT][NT][kChains];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < kChains; ++e) chain[mt][t][e] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      constexpr int per = NC / T::KP;
-      if (c > 0 && c % per == 0) load_k(c / per);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        u32x4 qc;
-        if constexpr (T::kQInLds) qc = q_lds[mt][c][lane];
-        else qc = q[mt][c];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (DT == SSA_F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              f32x4& x = chain[mt][t][e % kChains];
-              const unsigned int a = rows.k[t][c % per][e], b = qc[e];
-              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), x,
-                                                       0, 0, 0);
-            }
-          } else {
-            chain[mt][t][0] = mfma16(rows.k[t][c % per], qc, chain[mt][t][0], DT == SSA_BF16);
-          }
-        }
-      }
-    }
-    const bool more = i + 1 < i1;
-    if (more) {
-      locate(i + 1);
-      load_k(0);
-    }
-    constexpr int PARTS = kParts<DT>;
-    u32x4 w[MT][PARTS];  // the weights in 16-bit parts
-    unsigned int allow[MT];
+  auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      Softmax<NA>& o = st[mt];
-      allow[mt] = edge ? attended(mt, j0) : 0xffu;
-      float mx = allow[mt] ? -FLT_MAX : -INFINITY;
+      st[mt].m = -INFINITY;
+      st[mt].l = 0.0f;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const auto& of = chain[mt][t];
-          float x = of[0][r];
-          if constexpr (kChains == 2) x += of[1][r];
-          if constexpr (kChains == 4) x = (x + of[1][r]) + (of[2][r] + of[3][r]);
-          x *= p.scale_log2;
-          if (edge && !(allow[mt] >> (t * 4 + r) & 1)) x = -INFINITY;
-          s[mt][t][r] = x;
-          mx = fmaxf(mx, x);
-        }
-      mx = fmaxf(mx, lane_xor(mx, 16));
-      mx = fmaxf(mx, lane_xor(mx, 32));
-      if (__any(mx > o.m)) {  // a row without a key so far stays at -inf, its sums at 0
-        const float m = fmaxf(o.m, mx);
-        const float a = __builtin_amdgcn_exp2f(o.m - (m == -INFINITY ? 0.0f : m));
-        o.m = m;
-        o.l *= a;
-#pragma unroll
-        for (int x = 0; x < NA; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o.acc[x][r] *= a;
-      }
-      const float base = (o.m == -INFINITY ? 0.0f : o.m) - T::kShift;
-      float sum = 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[mt][t][r] = __builtin_amdgcn_exp2f(s[mt][t][r] - base);
-          sum += s[mt][t][r];
-        }
-      o.l += sum;
-      if constexpr (DT != SSA_F32) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            unsigned int x[PARTS];
-            split<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], x);
-#pragma unroll
-            for (int y = 0; y < PARTS; ++y) w[mt][y][2 * t + h] = x[y];
-          }
-      }
+      for (int i = 0; i < NA; ++i) st[mt].acc[i] = f32x4{0, 0, 0, 0};
     }
-    if (edge) {
-      bool odd = false;
-      each_value([&](unsigned int& v) { odd |= not_finite<DT>(v); });
-      if (__any(odd)) {
-        add_not_finite(s, allow);
-        each_value([&](unsigned int& v) { v = finite_part<DT>(v); });
-      }
+    batch = it.begin + i0 * NT;
+    if (i0 < i1) {
+      const int x = pages_at(batch);
+      pid_next = pages_at(batch + 64);
+      take_pages(x);
+      locate(i0);
+      load_k(0);
+      load_v(i0);
     }
+    for (int i = i0; i < i1; ++i) {
+      const int j0 = (it.begin + i * NT) * 16;
+      const bool edge = j0 < late || j0 + NT * 16 > ctx;
+      if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
+      // scores: lane column a row, rows the keys 4 grp + r of each subtile; fp32 in kChains chains, as
+      // paged_attend_kernel
+      constexpr int kChains = DT != SSA_F32 ? 1 : DP == 64 ? 2 : 4;
+      f32x4 s[MT][NT], chain[MT][NT][kChains];
 #pragma unroll
-    for (int vb = 0; vb < VB; ++vb)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int e = 0; e < LC; ++e) {
-        if constexpr (DT == SSA_F32) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int e = 0; e < kChains; ++e) chain[mt][t][e] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+      for (int c = 0; c < NC; ++c) {
+        constexpr int per = NC / T::KP;
+        if (c > 0 && c % per == 0) load_k(c / per);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                f32x4& acc = st[mt].acc[vb * LC + e];
-                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                    __uint_as_float(rows.v[t][r][vb].w[e]), s[mt][t][r], acc, 0, 0, 0);
+        for (int mt = 0; mt < MT; ++mt) {
+          u32x4 qc;
+          if constexpr (T::kQInLds) qc = q_lds[mt][c][lane];
+          else qc = q[mt][c];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (DT == SSA_F32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                f32x4& x = chain[mt][t][e % kChains];
+                const unsigned int a = rows.k[t][c % per][e], b = qc[e];
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), x,
+                                                         0, 0, 0);
               }
-        } else {
-          // column e of the lane's values, key after key
-          u32x4 vt;
+            } else {
+              chain[mt][t][0] = mfma16(rows.k[t][c % per], qc, chain[mt][t][0], DT == SSA_BF16);
+            }
+          }
+        }
+      }
+      const bool more = i + 1 < i1;
+      if (more) {
+        locate(i + 1);
+        load_k(0);
+      }
+      constexpr int PARTS = kParts<DT>;
+      u32x4 w[MT][PARTS];  // the weights in 16-bit parts
+      unsigned int allow[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        Softmax<NA>& o = st[mt];
+        allow[mt] = edge ? attended(mt, j0) : 0xffu;
+        float mx = allow[mt] ? -FLT_MAX : -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const auto& of = chain[mt][t];
+            float x = of[0][r];
+            if constexpr (kChains == 2) x += of[1][r];
+            if constexpr (kChains == 4) x = (x + of[1][r]) + (of[2][r] + of[3][r]);
+            x *= p.scale_log2;
+            if (edge && !(allow[mt] >> (t * 4 + r) & 1)) x = -INFINITY;
+            s[mt][t][r] = x;
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, lane_xor(mx, 16));
+        mx = fmaxf(mx, lane_xor(mx, 32));
+        if (__any(mx > o.m)) {  // a row without a key so far stays at -inf, its sums at 0
+          const float m = fmaxf(o.m, mx);
+          const float a = __builtin_amdgcn_exp2f(o.m - (m == -INFINITY ? 0.0f : m));
+          o.m = m;
+          o.l *= a;
+#pragma unroll
+          for (int x = 0; x < NA; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o.acc[x][r] *= a;
+        }
+        const float base = (o.m == -INFINITY ? 0.0f : o.m) - T::kShift;
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[mt][t][r] = __builtin_amdgcn_exp2f(s[mt][t][r] - base);
+            sum += s[mt][t][r];
+          }
+        o.l += sum;
+        if constexpr (DT != SSA_F32) {
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              vt[2 * t + h] = __builtin_amdgcn_perm(
-                  rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
-                  e % 2 ? 0x07060302u : 0x05040100u);
+            for (int h = 0; h < 2; ++h) {
+              unsigned int x[PARTS];
+              split<DT>(s[mt][t][2 * h], s[mt][t][2 * h + 1], x);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            f32x4& acc = st[mt].acc[vb * LC + e];
-#pragma unroll
-            for (int y = 0; y < PARTS; ++y) acc = mfma16(vt, w[mt][y], acc, DT == SSA_BF16);
-          }
+              for (int y = 0; y < PARTS; ++y) w[mt][y][2 * t + h] = x[y];
+            }
         }
       }
-    if (more) load_v(i + 1);
-  }
+      if (careful.value && edge) {
+        bool odd = false;
+        each_value([&](unsigned int& v) { odd |= not_finite<DT>(v); });
+        if (__any(odd)) {
+          add_not_finite(s, allow);
+          each_value([&](unsigned int& v) { v = finite_part<DT>(v); });
+        }
+      }
+#pragma unroll
+      for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+        for (int e = 0; e < LC; ++e) {
+          if constexpr (DT == SSA_F32) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  f32x4& acc = st[mt].acc[vb * LC + e];
+                  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                      __uint_as_float(rows.v[t][r][vb].w[e]), s[mt][t][r], acc, 0, 0, 0);
+                }
+          } else {
+            // column e of the lane's values, key after key
+            u32x4 vt;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                vt[2 * t + h] = __builtin_amdgcn_perm(
+                    rows.v[t][2 * h + 1][vb].w[e / 2], rows.v[t][2 * h][vb].w[e / 2],
+                    e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              f32x4& acc = st[mt].acc[vb * LC + e];
+#pragma unroll
+              for (int y = 0; y < PARTS; ++y) acc = mfma16(vt, w[mt][y], acc, DT == SSA_BF16);
+            }
+          }
+        }
+      if (more) load_v(i + 1);
+    }
+  };
+  walk(std::false_type{});
+  bool nan = false;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) nan |= st[mt].acc[i][r] != st[mt].acc[i][r];
+  if (__any(nan)) walk(std::true_type{});
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     st[mt].l += lane_xor(st[mt].l, 16);
@@ -1254,10 +1264,12 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   const auto rounded = [](int64_t x) { return (x + 7) / 8 * 8; };  // an XCD's run each
   y.blocks = rounded(tiles);
   if (units <= 4 || (units <= 16 && tiles >= 512)) return y;
-  // workgroups aimed at: what the CUs hold at once (three a CU; two or one of the widest heads); twice
-  // as many even out uneven requests better (64 mixed requests 341 us for 768, 316 for 1536; 16 trees of
-  // 64 tokens 196 and 192), where one request is even by itself (16 tokens over 1M 165 and 178)
-  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 ? 512 : B == 1 ? 768 : y.M >= 64 ? 1536 : 1024;
+  // Workgroups aimed at: about what the CUs hold at once, or twice that where it evens out uneven
+  // requests (64 mixed requests 341 us for 768, 316 for 1536; 16 trees of 64 tokens 196 and 192); one
+  // request is even by itself (16 tokens over 1M 165 us for 768, 178 for 1536). Windows of 1024 at head
+  // dim 256 fit one round of 384 better than two of 512 (43 us and 46).
+  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 ? (y.M == 64 ? 384 : 512)
+                         : B == 1 ? 768 : y.M >= 64 ? 1536 : 1024;
   y.items = std::max<int64_t>(1, target / Hkv);
   y.blocks = rounded(std::min(tiles + y.items * Hkv, tiles * units));
   y.max_parts = std::min(2 * y.items * Hkv, y.blocks);
@@ -1284,7 +1296,8 @@ int run_drafts(const DraftParams& p, hipStream_t st) {
 
 template <int DT>
 int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
-  if constexpr (DT != SSA_F32) {
+  constexpr bool f32 = DT == SSA_F32;
+  if constexpr (!f32) {
     if (y.M == 64 && y.dp == 64) return run_drafts<DT, 64, 64, 64, 4>(p, st);
     if (y.M == 64 && y.dp == 128) return run_drafts<DT, 128, 64, 32, 4>(p, st);
     if (y.M == 64 && y.dp == 256) return run_drafts<DT, 256, 64, 32, 2>(p, st);
@@ -1295,9 +1308,9 @@ int run_drafts_dim(const DraftParams& p, const DraftLayout& y, hipStream_t st) {
     if (y.M == 32 && y.dp == 128) return run_drafts<DT, 128, 32, 0, 2>(p, st);
   }
   switch (y.dp) {
-    case 64: return run_drafts<DT, 64, 16, 0, 3>(p, st);
+    case 64: return run_drafts<DT, 64, 16, 0, f32 ? 3 : 4>(p, st);
     case 128: return run_drafts<DT, 128, 16, 0, 2>(p, st);
-    case 256: return run_drafts<DT, 256, 16, 0, 1>(p, st);
+    case 256: return run_drafts<DT, 256, 16, 0, 2>(p, st);
     default: return run_drafts<DT, 512, 16, 0, 1>(p, st);
   }
 }
