@@ -568,7 +568,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
     }
     for (int i = i0; i < i1; ++i) {
       const int j0 = (it.begin + i * NT) * 16;
-      const bool edge = j0 < late || j0 + NT * 16 > ctx;
+      const bool edge = j0 < late || ctx - j0 < NT * 16;
       if constexpr (T::kQInLds) asm volatile("" ::: "memory");  // read the queries here, every time
       // scores: lane column a row, rows the keys 4 grp + r of each subtile; fp32 in kChains chains, as
       // paged_attend_kernel
@@ -933,7 +933,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
       take_pages(pid_next);
       pid_next = pages_at(batch + 64);
     }
-    const bool full = DP == p.d && s0 * 16 >= first && s0 * 16 + KT <= len && s0 + SUB <= it.end;
+    const bool full = DP == p.d && s0 * 16 >= first && len - s0 * 16 >= KT && s0 + SUB <= it.end;
     auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < LPW; ++j) {
@@ -942,8 +942,8 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
         const int64_t pg = __builtin_amdgcn_readlane(pid, at);
         const int64_t off = __builtin_amdgcn_readlane(poff, at);
         f(kbase + (pg * kpp + off * kps) + (unsigned)(r * kps + c * 16),
-          vbase + (pg * vpp + off * vps) + (unsigned)(r * vps + c * 16), to + u * 1024, s * 16 + r,
-          c * 16 < row_bytes, s < it.end);
+          vbase + (pg * vpp + off * vps) + (unsigned)(r * vps + c * 16), to + u * 1024,
+          (int)(s * 16u + r), c * 16 < row_bytes, s < it.end);
       }
     };
     if (full && it.stream) {
@@ -981,7 +981,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     const unsigned char* const vs = ks + TILE;
     const int s0 = it.begin + i * SUB, j0 = s0 * 16;
     // up to the tile of the latest first key: past it every row has a maximum or no key of the context
-    const bool edge = j0 <= late || j0 + KT > ctx || s0 + SUB > it.end;
+    const bool edge = j0 <= late || ctx - j0 < KT || s0 + SUB > it.end;
     Acc sum_of[NS];
 #pragma unroll
     for (int t = 0; t < NS; ++t) {

@@ -299,6 +299,117 @@ def test_no_tokens_and_no_requests(cuda):
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq", [1, 20, 130])
+def test_attend_at_the_longest_lengths(cuda, dtype, hq):
+    """Positions up to 2^31 - 17, the last a table row can hold, through a window (every page but the last
+    is the same), for few, more and many rows."""
+    page, d, n = 16, 64, 3
+    cap = 2 ** 31 - 16
+    g = torch.Generator(device=cuda).manual_seed(1)
+    k, v = (torch.randn(2, 1, page, d, device=cuda, generator=g).to(dtype) for _ in range(2))
+    table = torch.zeros(1, cap // page, device=cuda, dtype=torch.int32)
+    q = torch.randn(n, hq, d, device=cuda, generator=g).to(dtype)
+    cu = int32([0, n], cuda)
+    parents = int32([-1, 0, 0], cuda)
+    for total, window in ((cap, 40), (cap - 1, 1), (cap - 15, 200), (cap - 16, 17), (cap - 13, 3000)):
+        table[0, (total - 1) // page] = 1
+        print(dtype, hq, total, window, flush=True)
+        lens = int32([total], cuda)
+        for tree in (None, P.draft_masks(parents, cu, lens, n)):
+            out, lse = P.attend_drafts(q, k, v, table, lens, cu, tree, window=window, return_lse=True)
+            torch.cuda.synchronize()
+            # the same keys at the start of a short row: a length that agrees modulo the page
+            m = window + 48 - (window - total) % page
+            assert (m - total) % page == 0
+            short = torch.zeros(1, m // page + 2, dtype=torch.int32)
+            short[0, (m - 1) // page] = 1
+            at = None if tree is None else tree.pos.cpu() - (total - m)
+            want, wlse, tol, ltol = D.attend(q, k, v, short, int32([m], "cpu"), cu, d ** -0.5, window,
+                                             None if tree is None else tree.masks, at)
+            U.close(out, want, tol)
+            U.close(lse, wlse, ltol)
+        table[0, (total - 1) // page] = 0
+
+
+@pytest.mark.parametrize("hq", [4, 16, 64])
+def test_pool_beyond_32_bit_offsets(cuda, hq):
+    """Pages whose elements lie past 2^32 bytes and 2^31 elements into the pool: attended, copied, kept."""
+    page, d, hkv = 256, 256, 2
+    pages = 2 ** 31 // (page * d * hkv) + 300
+    k = torch.empty(pages, hkv, page, d, device=cuda, dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    table, used = int32([[pages - 1, 3, pages - 5]], cuda), [pages - 1, 3, pages - 5]
+    for pid in used:
+        k[pid].normal_()
+        v[pid].normal_()
+    lens, cu = int32([600], cuda), int32([0, 4], cuda)
+    q = torch.randn(4, hq, d, device=cuda).to(torch.bfloat16)
+    print(hq, flush=True)
+    out = P.attend_drafts(q, k, v, table, lens, cu)
+    want, _, tol, _ = D.attend(q, k, v, table, lens, cu, 1 / math.sqrt(d))
+    U.close(out, want, tol)
+    P.copy_pages(k, v, int32([pages - 1, 3], cuda), int32([pages - 9, pages - 7], cuda))
+    assert torch.equal(k[pages - 9], k[pages - 1]) and torch.equal(v[pages - 7], v[3])
+    moved = k[pages - 5, :, 599 % page].clone()
+    got = P.keep_drafts(k, v, table, lens, cu, int32([[1, 3]], cuda), int32([2], cuda))
+    assert got.tolist() == [598] and torch.equal(k[pages - 5, :, 597 % page], moved)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,n", [(64, 4, 8), (64, 14, 24), (128, 8, 4), (128, 16, 5), (128, 32, 32),
+                                    (256, 8, 30)])
+def test_scores_that_climb_and_fall(cuda, dtype, d, hq, n):
+    """Rows whose scores rise by hundreds past those of their first keys (so that weights by an early maximum
+    would pass the type's range), fall by as much, or stay level, with small and large values."""
+    ctx = 1500
+    q, cache, cu = make(cuda, dtype, [ctx, 0], [n, 3], hq, 1, d, 64, seed=11, spread=1.0)
+    key = torch.zeros(d, device=cuda)
+    key[0] = 1.0
+    for shape, (a, b) in (("up", (-40.0, 40.0)), ("down", (40.0, -40.0)), ("late", (0.0, 0.0))):
+        for j in range(ctx + n):
+            size = a + (b - a) * j / (ctx + n)
+            if shape == "late":
+                size = 60.0 if j == ctx - 3 else -60.0
+            cache.k[0][int(cache.table[0, j // 64]), 0, j % 64] = (key * size).to(dtype)
+        q.zero_()
+        q[..., 0] = torch.linspace(0.0, 8.0 * math.sqrt(d), q.shape[0] * hq,
+                                   device=cuda).view(q.shape[:2]).to(dtype)
+        print(dtype, d, hq, n, shape, flush=True)
+        check(cache, q, cu, tree(cache, cu, [n, 3], 2))
+        check(cache, q, cu, None, scale=-0.11)
+        check(cache, q, cu, None, scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,n", [(64, 4, 4), (64, 8, 8), (64, 16, 16), (128, 16, 5), (128, 32, 8),
+                                    (256, 16, 8)])
+def test_weights_keep_their_bits(cuda, dtype, d, hq, n):
+    """Every key of equal weight and values of both signs: what is left of a mean shows bits that the
+    weights lose. Within the bound of the parts and sums, before the rounding."""
+    q, cache, cu = make(cuda, dtype, [4000], [n], hq, 1, d, 64, seed=12, spread=0.5)
+    check(cache, q, cu)
+    out, lse = cache.attend_drafts(0, q, cu, return_lse=True)
+    again, lse2 = cache.attend_drafts(0, q, cu, return_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)  # bit for bit
+
+
+def test_pools_of_other_layouts_and_shared_pages(cuda):
+    """Strided pools, a table that is a view, requests that share their first pages."""
+    q, cache, cu = make(cuda, torch.float16, [160, 160, 40], [5, 9, 2], 8, 2, 64, 16, seed=13)
+    big = torch.full((2, cache.k.shape[1], 3, 16, 128), math.nan, device=cuda, dtype=torch.float16)
+    k, v = big[0][:, :2, :, :64], big[1][:, 1:, :, 64:]
+    k.copy_(cache.k[0])
+    v.copy_(cache.v[0])
+    table = torch.full((3, 20), -1, device=cuda, dtype=torch.int32)[:, 3:14]
+    table[:, :11] = cache.table[:, :11]
+    table[1, :9] = table[0, :9]
+    out, lse = P.attend_drafts(q, k, v, table, cache.lens, cu, return_lse=True)
+    want, wlse, tol, ltol = D.attend(q, k, v, table, cache.lens, cu, 1 / 8)
+    U.close(out, want, tol)
+    U.close(lse, wlse, ltol)
+
+
 # ---- accepted tokens ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -497,3 +608,267 @@ def test_copy_equals_indexing(cuda, dtype, layers, hkv, d, page, token_major):
     P.copy_pages(cache.k[0], cache.v[0], int32([1], cuda), int32([2], cuda))
     assert torch.equal(cache.k[0, 2], cache.k[0, 1]) and torch.equal(cache.v[0, 2], cache.v[0, 1])
     P.copy_pages(cache.k, cache.v, int32([], cuda), int32([], cuda))
+
+
+# ---- the run of them ----------------------------------------------------------------------------
+
+class Told:
+    """What the requests of a cache hold, token by token and layer by layer, kept beside it."""
+
+    def __init__(self, cache):
+        self.cache, self.rows = cache, [[] for _ in range(cache.lens.numel())]
+
+    def check(self):
+        c = self.cache
+        c.check()
+        assert c.lens.tolist() == [len(x) for x in self.rows]
+        page, held = c.page, []
+        for b, row in enumerate(self.rows):
+            ids = c.table[b].tolist()
+            need = -(-len(row) // page)
+            assert all(x == -1 for x in ids[need:])
+            held.append(ids[:need])
+            if row:
+                at = torch.tensor([ids[j // page] for j in range(len(row))], device=c.k.device)
+                off = torch.arange(len(row), device=c.k.device) % page
+                want = torch.stack(row)  # (n, 2, layers, hkv, d)
+                for i, pool in enumerate((c.k, c.v)):
+                    got = pool.permute(1, 3, 0, 2, 4)[at, off]
+                    assert torch.equal(got, want[:, i])
+        free = c.free[:c.nfree.item()].tolist()
+        every = set(sum(held, []))
+        assert len(set(free)) == len(free) and not every & set(free)
+        assert len(every) + len(free) == c.k.shape[1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("token_major,hq,d", [(False, 4, 64), (True, 16, 128)])
+def test_drafts_verified_kept_and_forked(cuda, dtype, token_major, hq, d):
+    """Prompts, steps of drafted trees of which a part is accepted, requests forked and ended: after each
+    the cache holds what it should, attention is that of the plain form, pages are free or listed."""
+    rng = random.Random(d)
+    B, layers, hkv, page = 6, 2, 2, 16
+    cache = P.PagedCache(B, 400, 120, hkv, d, page=page, layers=layers, dtype=dtype, device=cuda,
+                         token_major=token_major)
+    told = Told(cache)
+    cache.k.fill_(math.nan)
+    cache.v.fill_(math.nan)
+    for step in range(14):
+        print(dtype, token_major, step, flush=True)
+        lens = cache.lens.tolist()
+        if step in (0, 7):  # prompts
+            grow = [rng.randrange(1, 60) if n == 0 else 0 for n in lens]
+            r = cache.resize(cache.lens + int32(grow, cuda), sum(grow))
+        elif step in (3, 9):  # a request's answers
+            src = [0, 0, 0, 3, 4, 3]
+            if step == 9:
+                src = [5, 4, 2, 2, 1, 1]
+            new = [rng.randrange(1, lens[a] + 1) if rng.random() < 0.5 else lens[a] for a in src]
+            cache.fork(int32(src, cuda), int32(new, cuda))
+            told.rows = [told.rows[a][:n] for a, n in zip(src, new)]
+            told.check()
+            continue
+        elif step in (6, 13):  # some end
+            new = [0 if step == 13 or b % 2 else n for b, n in enumerate(lens)]
+            cache.fork(None, int32(new, cuda))
+            told.rows = [row[:n] for row, n in zip(told.rows, new)]
+            told.check()
+            continue
+        else:
+            grow = [rng.choice([0, 1, rng.randrange(1, 20)]) if n else 0 for n in lens]
+            r = cache.resize(cache.lens + int32(grow, cuda), sum(grow) + 3)
+        N = r.slots.numel()
+        x = torch.randn(N, 2, layers, hkv, d, device=cuda).to(dtype)
+        for layer in range(layers):
+            cache.append(layer, x[:, 0, layer], x[:, 1, layer], r.slots)
+        at = offsets(grow)
+        for b in range(B):
+            told.rows[b] = told.rows[b] + list(x[at[b]:at[b + 1]])
+        told.check()
+        q = torch.randn(N, hq, d, device=cuda).to(dtype)
+        if step in (0, 7):
+            check(cache, q, r.cu)
+            continue
+        parents = sum((D.random_parents(rng, n) for n in grow), []) + [0] * 3
+        drafts = P.draft_masks(int32(parents, cuda), r.cu, cache.lens, 20)
+        check(cache, q, r.cu, drafts, window=rng.choice([0, 30]))
+        path = []
+        for b, n in enumerate(grow):  # a way down the tree, by the parents
+            way, t = [], rng.randrange(-1, n)
+            while t >= 0:
+                way.append(t)
+                t = parents[at[b] + t]
+            path.append(way[::-1])
+        K = max(map(len, path)) + 1
+        cache.accept(r.cu, int32([p + [-5] * (K - len(p)) for p in path], cuda),
+                     int32([len(p) for p in path], cuda))
+        for b, p in enumerate(path):
+            first = len(told.rows[b]) - grow[b]
+            told.rows[b] = told.rows[b][:first] + [told.rows[b][first + t] for t in p]
+        told.check()
+    assert cache.nfree.item() == 120
+
+
+def test_a_path_that_does_not_fit_refuses_the_resize(cuda):
+    cache = P.PagedCache(2, 64, 8, 1, 64, page=16, device=cuda)
+    r = cache.resize(int32([20, 9], cuda), 29)
+    cache.accept(r.cu, int32([[3, 2], [0, 1]], cuda), int32([2, 2], cuda))
+    assert cache.status.item() == -1 and cache.lens.tolist() == [20, 9]
+    with pytest.raises(RuntimeError, match="resize"):
+        cache.check()
+    cache.accept(r.cu, int32([[2, 3], [0, 1]], cuda), int32([2, 2], cuda))
+    cache.check()
+    assert cache.lens.tolist() == [2, 2]
+
+
+def test_a_refused_resize_leaves_no_drafts(cuda):
+    """After a resize that does not fit: no masks, NaN rows, nothing kept, until one fits."""
+    cache = P.PagedCache(2, 64, 4, 1, 64, page=16, device=cuda)
+    x = torch.randn(40, 1, 64, device=cuda).to(torch.bfloat16)
+    r = cache.resize(int32([20, 9], cuda), 40)
+    cache.append(0, x, x, r.slots)
+    held = cache.k.clone()
+    r = cache.resize(int32([60, 20], cuda), 60)
+    assert r.status.item() > 0
+    drafts = P.draft_masks(torch.zeros(60, device=cuda, dtype=torch.int32), r.cu, cache.lens, 60)
+    assert (drafts.masks == 0).all() and (drafts.pos == 0).all()
+    q = torch.randn(60, 2, 64, device=cuda).to(torch.bfloat16)
+    assert cache.attend_drafts(0, q, r.cu, drafts).isnan().all()
+    got = P.keep_drafts(cache.k, cache.v, cache.table, cache.lens, r.cu, int32([[0], [0]], cuda),
+                        int32([0, 0], cuda))
+    assert got.tolist() == [20, 9] and torch.equal(cache.k, held)
+    f = cache.fork(None, int32([20, 0], cuda))
+    assert f.status.item() == 0 and not cache.attend(0, q[:2]).isnan().any()
+
+
+def test_captured_run_replayed(cuda):
+    """A step of drafted tokens (room, masks, stored, attended, some kept) in a graph, replayed as requests
+    grow, with eager work between: equal to an eager cache beside it at every replay."""
+    B, hq, hkv, d, page = 5, 8, 2, 64, 16
+    a, b = (P.PagedCache(B, 500, 160, hkv, d, page=page, layers=2, dtype=torch.float16, device=cuda)
+            for _ in range(2))
+    start = int32([30, 1, 100, 64, 7], cuda)
+    x = torch.randn(202, hkv, d, device=cuda).to(torch.float16)
+    for c in (a, b):
+        r = c.resize(start, 202)
+        for layer in range(2):
+            c.append(layer, x, x, r.slots)
+    grow, N = int32([4, 1, 8, 2, 5], cuda), 23
+    parents = int32([0] * N, cuda)
+    path, counts = int32([[0, 1, 3]] * B, cuda), int32([0] * B, cuda)
+    q = torch.randn(N, hq, d, device=cuda).to(torch.float16)
+    k, v = (torch.randn(N, hkv, d, device=cuda).to(torch.float16) for _ in range(2))
+    src, give = torch.arange(B, device=cuda, dtype=torch.int32), int32([0] * B, cuda)
+
+    def step(c):
+        r = c.resize(c.lens + grow, N)
+        drafts = P.draft_masks(parents, r.cu, c.lens, 8)
+        outs = []
+        for layer in range(2):
+            c.append(layer, k, v, r.slots)
+            outs += c.attend_drafts(layer, q, r.cu, drafts, window=40 * layer, return_lse=True)
+        c.accept(r.cu, path, counts)
+        f = c.fork(src, c.lens - give)
+        return outs, drafts, f
+    parents.copy_(int32(sum((D.random_parents(random.Random(1), n) for n in grow.tolist()), [])
+                        + [0] * 3, cuda))
+    for c in (a, b):
+        step(c)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs, drafts, f = step(a)
+    for rep in range(20):
+        rng = random.Random(rep)
+        grow.copy_(int32([rng.randrange(5) for _ in range(B)], cuda))
+        n = grow.tolist()
+        ways = sum((D.random_parents(rng, m) for m in n), [])
+        parents.copy_(int32(ways + [0] * (N - len(ways)), cuda))
+        keep = [sorted(rng.sample(range(m), rng.randrange(min(m, 3) + 1))) for m in n]
+        path.copy_(int32([p + [0] * (3 - len(p)) for p in keep], cuda))
+        counts.copy_(int32([len(p) for p in keep], cuda))
+        src.copy_(int32([rng.choice([i, i, rng.randrange(B)]) for i in range(B)], cuda))
+        give.zero_()
+        low = torch.minimum(a.lens + counts, (a.lens + counts)[src.long()])
+        give.copy_(a.lens + counts - low)  # at most what the source holds
+        for t in (q, k, v):
+            t.normal_()
+        graph.replay()
+        torch.empty(1 << 20, device=cuda).normal_().sum().item()
+        torch.cuda.synchronize()
+        want, wdrafts, wf = step(b)
+        assert all(torch.equal(x, y) for x, y in zip(outs, want)), rep
+        assert all(torch.equal(x, y) for x, y in zip(drafts, wdrafts)), rep
+        assert all(torch.equal(x, y) for x, y in zip(f, wf)) and f.status.item() == 0, rep
+        for x, y in ((a.lens, b.lens), (a.table, b.table), (a.free, b.free), (a.nfree, b.nfree),
+                     (a.k, b.k), (a.v, b.v)):
+            assert torch.equal(x, y), rep
+
+
+def test_two_graphs_with_one_memory_pool(cuda):
+    """Two captured calls whose workspaces share a pool, replayed in turn with eager calls between."""
+    q, cache, cu = make(cuda, torch.bfloat16, [7000, 300], [9, 4], 8, 2, 64, 16, seed=14)
+    q2, other, cu2 = make(cuda, torch.bfloat16, [50, 9000], [3, 17], 8, 2, 64, 16, seed=15)
+    want, want2 = cache.attend_drafts(0, q, cu), other.attend_drafts(0, q2, cu2)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(a):
+        out = cache.attend_drafts(0, q, cu)
+    with torch.cuda.graph(b, pool=a.pool()):
+        out2 = other.attend_drafts(0, q2, cu2)
+    for _ in range(4):
+        a.replay()
+        assert torch.equal(out, want)
+        b.replay()
+        assert torch.equal(out2, want2)
+        torch.empty(1 << 20, device=cuda).normal_().sum().item()
+        assert torch.equal(cache.attend_drafts(0, q, cu), want)
+
+
+def test_other_streams(cuda):
+    q, cache, cu = make(cuda, torch.bfloat16, [7000, 50], [9, 30], 8, 2, 64, 16, seed=16)
+    drafts = tree(cache, cu, [9, 30])
+    want = cache.attend_drafts(0, q, cu, drafts)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(cache.attend_drafts(0, q, cu, tree(cache, cu, [9, 30])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_compiled_run_equals_eager(cuda):
+    caches = []
+    for _ in range(2):
+        c = P.PagedCache(3, 200, 40, 2, 64, page=16, layers=2, dtype=torch.float16, device=cuda)
+        torch.manual_seed(3)
+        x = torch.randn(90, 2, 64, device=cuda).to(torch.float16)
+        r = c.resize(int32([50, 7, 33], cuda), 90)
+        for layer in range(2):
+            c.append(layer, x, x, r.slots)
+        caches.append(c)
+    q, x = torch.randn(9, 4, 64, device=cuda).half(), torch.randn(9, 2, 64, device=cuda).half()
+    parents, grow = int32([-1, 0, 0, -1, 0, 1, 1, 9, 9], cuda), int32([3, 0, 4], cuda)
+    path, counts = int32([[0, 2], [0, 0], [0, 3]], cuda), int32([2, 0, 2], cuda)
+    src = int32([0, 0, 2], cuda)
+
+    def run(c, out):
+        r = c.resize(c.lens + grow, 9)
+        drafts = P.draft_masks(parents, r.cu, c.lens, 40)
+        c.append(0, x, x, r.slots)
+        a, lse = c.attend_drafts(0, q, r.cu, drafts, window=20, return_lse=True)
+        b = c.attend_drafts(0, q, r.cu, out=out)
+        c.accept(r.cu, path, counts)
+        f = c.fork(src, c.lens)
+        return a, lse, b, tuple(f), tuple(drafts)
+    outs = [torch.full((9, 4, 64), 7.0, device=cuda, dtype=torch.float16) for _ in range(2)]
+    want = run(caches[0], outs[0])
+    got = torch.compile(run, backend="aot_eager")(caches[1], outs[1])
+    flat = lambda t: [y for x in t for y in (flat(x) if isinstance(x, tuple) else [x])]  # noqa: E731
+    for x, y in zip(flat(want), flat(got)):
+        assert torch.equal(x, y)
+    assert (outs[0][7:] == 7).all() and torch.equal(outs[0], outs[1])
+    for x in ("lens", "table", "free", "nfree", "status", "k", "v"):
+        assert torch.equal(getattr(caches[0], x), getattr(caches[1], x)), x

@@ -178,6 +178,22 @@ def test_registered_operators_give_shapes():
     assert ops.paged_copy(pool, pool.clone(), i32(3), i32(3), None) is None
 
 
+def test_compiled_calls_refuse_what_eager_ones_refuse(monkeypatch):
+    monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    m = dict(device="meta")
+    i32 = lambda *n: torch.empty(n, dtype=torch.int32, **m)  # noqa: E731
+    q = torch.empty(5, 4, 64, dtype=torch.float16, **m)
+    pool = torch.empty(9, 2, 16, 64, dtype=torch.float16, **m)
+    call = lambda out: P.attend_drafts(q, pool, pool, i32(2, 4), i32(2), i32(3), out=out)  # noqa: E731
+    out = torch.empty_like(q)
+    assert call(out) is out and call(None).shape == q.shape
+    for bad in (q.float(), q[:4], torch.empty(3, 5, 4, 64, dtype=q.dtype, **m)):
+        with pytest.raises(ValueError, match="out must be"):
+            call(bad)
+    with pytest.raises(ValueError, match="most=0"):
+        P.draft_masks(i32(5), i32(3), i32(2), 0)
+
+
 def test_plain_fork_keeps_every_page_once():
     """After any run of resizes and forks a page is free or listed, the last partly filled ones by one
     row each."""
@@ -218,3 +234,20 @@ def test_plain_attention_is_the_softmax_of_the_attended_keys():
                 s = k @ q[row, h].double() * 0.3
                 torch.testing.assert_close(out[row, h], torch.softmax(s, 0) @ k)
                 torch.testing.assert_close(lse[row, h], torch.logsumexp(s, 0))
+
+
+def test_drafts_are_cut_to_fit(tmp_path):
+    """csrc/paged_index.h compiled for the host: requests that do not fit are answered there, row tiles
+    and items are no more than a call's launch and workspace hold, and every key lies in one item."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if cxx is None:
+        pytest.skip("no host compiler")
+    exe = tmp_path / "check"
+    subprocess.run([cxx, "-std=c++17", "-O1", f"-I{root / 'ssa_amd' / 'csrc'}",
+                    str(root / "tests/paged_drafts_check.cpp"), "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
