@@ -816,6 +816,7 @@ template <int DT>
 __device__ inline void parts_of(float p0, float p1, unsigned int (&w)[2]) {
   if constexpr (DT == SSA_BF16) {
     w[0] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
+    asm("" : "+v"(w[0]));  // the halves are taken from it, not rounded once more
     p0 -= __uint_as_float(w[0] << 16);
     p1 -= __uint_as_float(w[0] & 0xffff0000u);
     w[1] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
