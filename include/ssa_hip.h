@@ -559,7 +559,8 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the
  *   resize that gives back the pages behind; -1, and nothing moved, where a path, a count, the lengths
- *   or a page id do not fit. strides[8] = kpool(layer,page,head,slot), vpool(layer,page,head,slot).
+ *   or a page id do not fit. The pools do not overlap. strides[8] = kpool(layer,page,head,slot),
+ *   vpool(layer,page,head,slot).
  *
  * Requests that share pages:
  * ssa_paged_fork: row b of the table becomes the first new_lens[b] tokens of what row src[b] was (src,

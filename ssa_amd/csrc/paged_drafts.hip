@@ -1550,6 +1550,7 @@ extern "C" int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layer
                   path_stride >= 0, SSA_ERR_INVALID,
               "%s: B=%lld, layers=%lld, paths of %lld (at most 65535 requests)", who, (long long)B,
               (long long)layers, (long long)width);
+  SSA_REQUIRE(kpool != vpool, SSA_ERR_INVALID, "%s: keys and values in the same memory", who);
   SSA_TRY(check_table(who, W, table_stride, page));
   const int es = dtype_size(dtype);
   // strides: kpool(layer,page,head,slot), vpool(layer,page,head,slot)

@@ -68,7 +68,7 @@ __device__ inline ForkRow fork_row(const ForkParams& p, int b) {
   if (!r.ok || r.want == 0) r.from = b;  // no page is taken from there
   r.have = r.ok ? paged_pages(r.len, p.page, p.div) : 0;
   r.need = r.ok ? paged_pages(r.want, p.page, p.div) : 0;
-  r.whole = r.need - (r.want > r.need * p.page - p.page && r.want < r.need * p.page ? 1 : 0);
+  r.whole = r.need - (r.need > 0 && r.want < r.need * p.page ? 1 : 0);
   r.same = r.ok && r.want == r.len && (r.want == 0 || r.from == b);
   return r;
 }

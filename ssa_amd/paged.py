@@ -419,7 +419,7 @@ def _drafts_plan(q, kpool, vpool, table, lens, cu, masks, pos, out, window):
         if masks[2] != torch.int32:
             raise TypeError(f"masks is {masks[2]}, expected torch.int32")
         if len(masks[0]) != 2 or masks[0][0] != N or not 1 <= masks[0][1] <= 32 \
-                or N > 1 and masks[1] != (masks[0][1], 1):
+                or N > 1 and masks[1][0] != masks[0][1] or masks[0][1] > 1 and masks[1][1] != 1:
             raise ValueError(f"masks must be a contiguous ({N}, 1 to 32) tensor, got "
                              f"{tuple(masks[0])}")
         words = masks[0][1]
@@ -551,7 +551,7 @@ def keep_drafts(kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor, l
     path (B, K), counts (B,) int32, lens and cu as attend_drafts. Returns the lengths after (B,) int32,
     for the resize_pages that gives back the pages behind them; -1, and nothing is moved, for a request
     whose path, count, length or pages do not fit. The pages of the drafted tokens must be the request's
-    own."""
+    own, and keys and values lie in memory of their own."""
     if torch.compiler.is_compiling():
         from . import torch_ops as T
         return T.paged_keep(kpool, vpool, table, lens, cu, path, counts)

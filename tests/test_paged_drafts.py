@@ -69,8 +69,8 @@ S8 = _lib.i64_array([20480, 2048, 1024, 64] * 2)
 
 def test_keep_refuses():
     def f(kpool=FAKE, dtype=_lib.F16, layers=1, hkv=2, d=64, pages=10, page=16, st=S8, W=8, B=2,
-          path=FAKE, stride=3, width=3):
-        return status("ssa_paged_keep", kpool, FAKE, dtype, layers, hkv, d, pages, page, st, FAKE, 8,
+          path=FAKE, stride=3, width=3, vpool=ctypes.c_void_p(1 << 30)):
+        return status("ssa_paged_keep", kpool, vpool, dtype, layers, hkv, d, pages, page, st, FAKE, 8,
                       W, FAKE, FAKE, B, path, stride, width, FAKE, FAKE, None)
     assert f(kpool=NULL) == INVALID and f(path=NULL) == INVALID and f(B=0) == INVALID
     assert f(B=65536) == INVALID and f(layers=0) == INVALID and f(width=-1) == INVALID
@@ -78,6 +78,7 @@ def test_keep_refuses():
     assert f(dtype=5) == UNSUPPORTED and f(d=20) == UNSUPPORTED and f(page=20) == UNSUPPORTED
     assert f(layers=2 ** 30) == UNSUPPORTED and f(layers=2 ** 20, B=65535) == UNSUPPORTED
     assert f(st=_lib.i64_array([64, 64, 64, 60] * 2)) == INVALID
+    assert f(vpool=FAKE) == INVALID and b"same memory" in _lib.lib().ssa_last_error()
 
 
 def test_fork_and_copy_refuse():
@@ -116,6 +117,7 @@ def test_python_refuses(monkeypatch):
                dict(drafts=P.Drafts(i32(5, 1).long(), i32(5))),
                dict(drafts=P.Drafts(i32(1, 5).t(), i32(5))[:1] + (i32(5).long(),)),
                dict(drafts=P.Drafts(i32(2, 5).t(), i32(5))), dict(vpool=pool[:8]),
+               dict(q=q[:1], drafts=P.Drafts(i32(1, 8)[:, ::2], i32(1))),
                dict(out=q.half()), dict(out=q[:4]), dict(out=q[:1].expand(5, 4, 64))):
         with pytest.raises((ValueError, TypeError)):
             P.attend_drafts(**{**good, **kw})
