@@ -35,7 +35,8 @@ __device__ inline unsigned int way(int anc, int steps, bool bad) {
 
 // A workgroup for a request and four words of its masks, a thread a token. Every round joins a token's
 // way with that of the ancestor where it ends, so its length doubles: a chain of 1024 takes ten rounds.
-// The last workgroups clear the rows behind the last token. Bound by launch and barrier latency.
+// The last workgroups clear the rows behind the last token. Bound by launch and barrier latency: 64 trees
+// of up to 64 tokens 3.5 us, 8 of 1,024 10.8.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_draft_masks_kernel(MaskParams p) {
   __shared__ unsigned int ways[THREADS];
@@ -128,7 +129,9 @@ __device__ inline DraftSpan draft_of(const DraftParams& p, int b) {
 // Finds workgroup `id`'s item from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. Of the call's row tiles an XCD takes a run, the tiles of the
 // same keys next to each other: its L2 serves them together. False past the last one. Sums of offsets
-// that do not ascend may wrap; the item's own numbers are checked.
+// that do not ascend may wrap; the item's own numbers are checked. (Equal shares of all units instead,
+// a workgroup going on from one row tile to the next, cost a short call 8 us, and a mixed batch 550 us for
+// 313: a unit takes as long with few rows as with many.)
 template <int M>
 __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   const int lane = threadIdx.x & 63;
@@ -332,7 +335,8 @@ __device__ inline float not_finite_sum(float with, float without) {
 // -FLT_MAX stands for attended keys, so that -INFINITY means a row without any. A value that is infinite
 // or NaN there reaches the rows that do not attend it as 0 x infinity: where a result is NaN, the wave
 // does its keys again with care, such values taken out of the product and added to the rows that attend
-// them.
+// them. Bound by the reading of keys and values: 32 requests of 8,000 keys, 4 tokens of 4 heads a key head
+// (8 heads of 128, bf16) 185 us, 5.7 TB/s; one token a request 181, for which paged_attend_kernel takes 167.
 template <int DT, int DP, int MT, int WPE>
 __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(DraftParams p) {
   using T = Tile<DT, DP>;
@@ -852,6 +856,10 @@ __device__ inline f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
 // nothing looks for infinite or NaN values: where a sum or a result is too large or not finite, the item is
 // done again with care (the maximum raised tile by tile, values that are not finite taken out of the
 // products as in paged_drafts_kernel).
+// 16 tokens of 7 heads (of 64) over 1,048,561 keys, 537 MB: 143 us and 15 for the join; its loads alone take
+// 112, its products and weights alone 128, and the two overlap by half. 16 trees of 64 tokens over 2,000
+// to 9,000 keys (32 / 8 heads of 128): 176 us and 20, 129 and 147; matrix units busy 31 % of the time.
+// Rings of three and four tiles, with fewer workgroups a CU, took as long or longer.
 template <int DT, int DP, int RW, int KT, int WPE>
 __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams p) {
   typedef typename std::conditional<RW == 16, f32x4, f32x16>::type Acc;
@@ -1162,7 +1170,8 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
 constexpr int kJoinRows = 8;  // parts of a row on their way at a time
 
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
-// the columns, four waves a workgroup.
+// the columns, four waves a workgroup. Bound by memory: 32,768 rows of 3 to 11 parts of 128 columns (98 MB)
+// 20 us; by latency where rows are few, 4 us.
 template <int DT, int DP, int M>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;
@@ -1256,7 +1265,11 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   DraftLayout y{};
   const int64_t G = Hq / Hkv;
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
-  const int64_t rows = N * G;  // of a key head; of a request rows / B on average
+  // Rows of a key head; of a request rows / B on average. Tiles of 16 rows, whose waves take a run of keys
+  // each, win up to there; past them tiles that the waves share (bf16, 32 requests of 8,000 keys, 8 heads
+  // of 128): 16 rows a request 186 us for 210, 20 rows 212 for 232, 64 235 for 361. Past 64 rows tiles of
+  // 128: 128 rows 310 us for 341 (two of 64), 64 rows 249 for 235. fp32, 32 rows: 129 for 135 (two of 16).
+  const int64_t rows = N * G;
   if (dtype == SSA_F32) y.M = y.dp <= 128 && rows > 16 * B ? 32 : 16;
   else y.M = y.dp == 512 || rows <= 16 * B ? 16 : y.dp == 256 || rows <= 64 * B ? 64 : 128;
   const int64_t tiles = draft_most_tiles(B, N, G, y.M) * Hkv;
@@ -1339,7 +1352,9 @@ constexpr int kKeepThreads = 64, kKeepBatch = 32;
 // A workgroup for a request and 64 columns (a column: 16 bytes of a layer's keys or values of a head,
 // over all tokens), a thread a column. An accepted token never moves up and they move in order, so a
 // column's tokens are read kKeepBatch at a time before any of these is written, and none that is
-// written is read again. All or nothing: every workgroup of a request checks its whole path first.
+// written is read again. All or nothing: every workgroup of a request checks its whole path first. Bound
+// by the longest path's column: 24 requests with 200 of 600 tokens moved in 8 layers (5 heads of 80, fp32,
+// 93 MB in all) 37 us; 64 with 2 in 24 layers 4.1.
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
   __shared__ int64_t s_from[2][kKeepThreads], s_to[2][kKeepThreads];  // of keys and values
   __shared__ int s_first;

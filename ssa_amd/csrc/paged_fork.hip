@@ -85,7 +85,10 @@ __device__ inline void each_entry(int chunk, int end, F f) {
   }
 }
 
-// The steps, each a wave for a unit (a chunk of a row's entries). Between two of them all units are done.
+// A page is given back where no row lists it any more, and copied where two rows would write it; both are
+// known once every row has said what it will hold, so the call is steps between which all units (chunks of
+// a row's entries, a wave each) are done. Counts that are kept from call to call instead would have to be
+// right at every resize too.
 // 1: the table's held entries are kept, the uses of their pages cleared.
 __device__ inline void fork_clear(const ForkParams& p, int unit) {
   const int b = unit / p.chunks, chunk = unit - b * p.chunks;
@@ -287,28 +290,9 @@ __device__ inline void fork_sum_write(const ForkParams& p, int unit) {
                                 p.taken[b] ? (int)taken : -1, (int)given});
 }
 
-// Makes this workgroup's writes and atomics visible to its later reads.
-__device__ inline void fork_step() {
-  __threadfence();
-  __syncthreads();
-  __threadfence();
-}
-
-// The whole call by one workgroup, a wave a unit at a time.
-__global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkParams p) {
-  const int wv = uniform(threadIdx.x >> 6);
-  for (int u = wv; u < p.units; u += kForkWaves) fork_clear(p, u);
-  fork_step();
-  for (int u = wv; u < p.units; u += kForkWaves) fork_mark(p, u);
-  fork_step();
-  for (int u = wv; u < p.units; u += kForkWaves) fork_count(p, u);
-  fork_step();
-  fork_sum(p);
-  fork_step();
-  for (int u = wv; u < p.units; u += kForkWaves) fork_write(p, u, fork_place(p, u));
-}
-
-// The steps as launches of their own, four units a workgroup.
+// The steps as launches of their own, four units a workgroup. Bound by their launches and the chains of
+// memory latencies in each (row, page id, the page's use): 64 rows of up to 500 pages 15 us, forked or
+// ended.
 __global__ __launch_bounds__(256) void paged_fork_clear_kernel(ForkParams p) {
   const int64_t u = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   if (u < p.units) fork_clear(p, (int)u);
@@ -330,7 +314,10 @@ __global__ __launch_bounds__(256) void paged_fork_write_kernel(ForkParams p) {
   else fork_write(p, (int)u, fork_place(p, (int)u));
 }
 
-constexpr int64_t kForkInside = 16, kForkSums = 2048;
+// Up to so many units each wave adds them up by itself: 64 requests of 1,000 tokens 11.3 us a fork for
+// 13.7 with the sums in a launch of their own, 512 of 500 15.4 for 14.2, 4,096 of 300 47.5 for 25.6. (All
+// steps in one launch of one workgroup: 2 requests 33 us for 8.2, 64 56 for 11.3.)
+constexpr int64_t kForkSums = 256;
 
 struct ForkLayout {
   int64_t chunks, units;
@@ -386,7 +373,8 @@ struct Quotient {
 constexpr int kCopyBatch = 8;
 
 // A thread moves 16-byte pieces of the copied tokens' keys and values, kCopyBatch of them on their way
-// at a time; a workgroup row (y) a page, x over a page's pieces of all layers.
+// at a time; a workgroup row (y) a page, x over a page's pieces of all layers. Bound by memory: 96 pages
+// of up to 128 tokens, 8 heads of 128 in 4 layers (16-bit, 200 MB in all), 45 us, 4.4 TB/s.
 __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
   const int i = blockIdx.y;
   const int64_t from = p.source[i], to = p.target[i];
@@ -458,10 +446,6 @@ extern "C" int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32
                (int32_t*)(ws + y.taken), (int32_t*)(ws + y.top), (int32_t*)(ws + y.nfree0),
                (int32_t*)(ws + y.left), y.units, (int)y.chunks};
   hipStream_t st = (hipStream_t)stream;
-  if (y.units <= kForkInside) {
-    paged_fork_kernel<<<1, kForkThreads, 0, st>>>(p);
-    return launch_status("paged_fork_kernel");
-  }
   const unsigned grid = (unsigned)((y.units + 3) / 4);
   paged_fork_clear_kernel<<<grid, 256, 0, st>>>(p);
   SSA_TRY(launch_status("paged_fork_clear_kernel"));
