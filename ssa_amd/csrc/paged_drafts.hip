@@ -1167,12 +1167,12 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   }
 }
 
-constexpr int kJoinRows = 8;  // parts of a row on their way at a time
-
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
 // the columns, four waves a workgroup. Bound by memory: 32,768 rows of 3 to 11 parts of 128 columns (98 MB)
-// 20 us; by latency where rows are few, 4 us.
-template <int DT, int DP, int M>
+// 20 us; by latency where rows are few, 4 us. BATCH: parts of a row (and split of the wave) on their way at
+// a time: 16 where rows are few and long (4K keys, 112 rows of 33 parts 13.2 us the whole call, 13.5 with 4;
+// 1M 159 and 164), 4 where the rows fill the card (16 trees of 64 197, 208 with 16).
+template <int DT, int DP, int M, int BATCH>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;
   const int lane = threadIdx.x & 63;
@@ -1195,11 +1195,11 @@ __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   st.l = held ? 0.0f : NAN;
 #pragma unroll
   for (int v = 0; v < NV; ++v) st.acc[v] = f32x4{0, 0, 0, 0};
-  for (int i = split; held && i < parts; i += NS * kJoinRows) {
-    float m[kJoinRows], l[kJoinRows], mx = st.m;
-    f32x4 a[kJoinRows][NV];
+  for (int i = split; held && i < parts; i += NS * BATCH) {
+    float m[BATCH], l[BATCH], mx = st.m;
+    f32x4 a[BATCH][NV];
 #pragma unroll
-    for (int u = 0; u < kJoinRows; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
       const bool in = i + u * NS < parts;
       const int64_t from = at + (in ? i + u * NS : 0) * step * M;
       m[u] = in ? p.part_ml[from * 2] : -INFINITY;
@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
         a[u][v] = in ? *(const f32x4*)(p.part + from * DP + v * 256 + c) : f32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int u = 0; u < kJoinRows; ++u) mx = fmaxf(mx, m[u]);
+    for (int u = 0; u < BATCH; ++u) mx = fmaxf(mx, m[u]);
     const float base = mx == -INFINITY ? 0.0f : mx, y = __builtin_amdgcn_exp2f(st.m - base);
     st.m = mx;
     st.l *= y;
@@ -1218,7 +1218,7 @@ __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) st.acc[v][r] *= y;
 #pragma unroll
-    for (int u = 0; u < kJoinRows; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
       const float z = __builtin_amdgcn_exp2f(m[u] - base);
       st.l += l[u] * z;
 #pragma unroll
@@ -1294,6 +1294,9 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   return y;
 }
 
+// Rows up to which a join takes 16 parts at a time (its comment has both sides).
+constexpr int64_t kFewJoins = 1024;
+
 template <int DT, int DP, int M, int KT, int WPE>
 int run_drafts(const DraftParams& p, hipStream_t st) {
   const unsigned blocks = (unsigned)(p.blocks + kRestBlocks);
@@ -1303,8 +1306,9 @@ int run_drafts(const DraftParams& p, hipStream_t st) {
     paged_drafts_kernel<DT, DP, M / 16, WPE><<<blocks, kAttendWaves * 64, 0, st>>>(p);
   SSA_TRY(launch_status("paged_drafts_kernel"));
   if (p.items == 0) return SSA_OK;
-  paged_drafts_join_kernel<DT, DP, M>
-      <<<(unsigned)((p.N * p.Hq + 3) / 4), 256, 0, st>>>(p);
+  const int64_t rows = p.N * p.Hq, joins = (rows + 3) / 4;
+  if (rows <= kFewJoins) paged_drafts_join_kernel<DT, DP, M, 16><<<(unsigned)joins, 256, 0, st>>>(p);
+  else paged_drafts_join_kernel<DT, DP, M, 4><<<(unsigned)joins, 256, 0, st>>>(p);
   return launch_status("paged_drafts_join_kernel");
 }
 
