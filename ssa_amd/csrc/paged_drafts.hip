@@ -204,6 +204,11 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
     const PagedRange r = paged_item_range(it.s.span, units, it.j, it.n);
     it.begin = r.begin;
     it.end = r.end;
+    if (!p.masks) {  // a chain: none of the tile's tokens attends keys past its last one
+      const unsigned int last = ((unsigned)it.tile * M + M - 1) / (unsigned)p.G;
+      const int seen = (it.s.ctx + (int)min(last, (unsigned)it.s.n - 1)) / 16 + 1;
+      it.end = min(it.end, max(seen, it.begin));
+    }
   }
   return true;
 }

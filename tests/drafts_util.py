@@ -46,14 +46,16 @@ def bit(masks, row, i):
 
 def attended(n, ctx, window, masks=None, pos=None):
     """(n, ctx + n) booleans: which keys the drafted tokens of a request attend (masks, pos its rows)."""
-    at = [ctx + t for t in range(n)] if pos is None else pos
+    if masks is None:
+        t, j = ctx + torch.arange(n)[:, None], torch.arange(ctx + n)
+        return (j <= t) & (j > t - window) if window else j <= t
+    at = pos
     out = torch.zeros(n, ctx + n, dtype=torch.bool)
     for t in range(n):
         low = at[t] - window if window else -1
         out[t, max(0, min(ctx, low + 1)):ctx] = True
         for i in range(n):
-            seen = i <= t if masks is None else bit(masks, t, i)
-            out[t, ctx + i] = bool(seen) and (not window or at[i] > low)
+            out[t, ctx + i] = bool(bit(masks, t, i)) and (not window or at[i] > low)
     return out
 
 

@@ -151,6 +151,22 @@ def test_attend_long_and_uneven(cuda, dtype, ctx, n, hq, hkv, d, page):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 64), (1, 1, 128), (3, 1, 256), (1, 1, 512)])
+def test_attend_long_chains(cuda, dtype, hq, hkv, d):
+    """Prompts' pieces longer than masks can tell, from an empty cache on and behind a context: row tiles
+    that end among the drafted tokens."""
+    ctx, n = [0, 77, 0, 300], [1500, 1100, 1, 17]
+    q, cache, cu = make(cuda, dtype, ctx, n, hq, hkv, d, 16, seed=17, spread=2.0, pad=2)
+    for window in (0, 100):
+        print(dtype, hq, d, window, flush=True)
+        check(cache, q, cu, window=window)
+    cache.v[0][cache.table[0, 20].long(), :, 3:] = math.inf  # later tokens' values reach no earlier one
+    cache.k[0][cache.table[0, 30].long(), :, 3:] = math.nan
+    out, _ = check(cache, q, cu)
+    assert torch.isfinite(out[:323]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_many_requests(cuda, dtype):
     """More requests than a wave has lanes, most without drafted tokens."""
     rng = random.Random(2)
