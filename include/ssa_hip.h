@@ -547,14 +547,16 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  * ssa_paged_attend_drafts: q, out (N, Hq, d). Row t of request b attends the keys j < ctx and the
  *   drafted ones of its mask (masks (N, words), pos (N), or all NULL with words 0: the drafted tokens
  *   up to itself, one after the other from position ctx on); with a window only those at positions past
- *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, precision, head
- *   layout, lse (N, Hq), status, page ids and strides as ssa_paged_attend. A row that attends nothing:
+ *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, head layout,
+ *   lse (N, Hq), status, page ids and strides as ssa_paged_attend; scores, statistics and sums in fp32,
+ *   and a weight of the 16-bit types all but 2^-18 (bf16) or 2^-20 (fp16) of itself, fp16's down to 2^-38
+ *   of the row's largest. A row that attends nothing:
  *   out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request that does
  *   not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
  *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
  *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq and the
- *   workgroups that a call may need are held below 2^31 and 2^24. Workspace: ssa_paged_attend_drafts_workspace_size bytes, 16-byte aligned, nothing in it
- *   needs to be set.
+ *   workgroups that a call may need are held below 2^31 and 2^24. Workspace:
+ *   ssa_paged_attend_drafts_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
  * ssa_paged_keep: moves the accepted drafted tokens together: drafted token path[b][i] of request b to
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the
