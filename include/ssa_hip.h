@@ -549,9 +549,8 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   up to itself, one after the other from position ctx on); with a window only those at positions past
  *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, head layout,
  *   lse (N, Hq), status, page ids and strides as ssa_paged_attend; scores, statistics and sums in fp32,
- *   and a weight of the 16-bit types all but 2^-18 (bf16) or 2^-20 (fp16) of itself, fp16's down to 2^-38
- *   of the row's largest. A row that attends nothing:
- *   out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request that does
+ *   and a weight with all its bits (bf16) or all but 2^-20 of itself down to 2^-38 of the row's largest
+ *   (fp16). A row that attends nothing: out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request that does
  *   not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
  *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
  *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq and the

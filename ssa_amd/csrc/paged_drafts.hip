@@ -818,17 +818,20 @@ __device__ inline void load_lds(const char* from, unsigned char* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, AUX);
 }
 
-// Weights of two keys as 16-bit parts, two for either type: bf16's, rounded to nearest, leave 2^-18 of a
-// weight at most, fp16's, cut, 2^-20. The output keeps 8 and 11 bits. (bf16's third part, which holds
-// what is left, made trees of 64 tokens 17 % slower and 16 tokens over 1M 12 %.)
+// Weights of two keys as 16-bit parts: bf16's three, each rounded to 8 bits of what the ones before leave,
+// hold them exactly (two left up to 2^-17 of a weight, which put 0.4 % of the outputs on the other side of
+// their rounding); fp16's two, cut to 11 bits each, leave 2^-20, of which the output keeps 11 bits. A part
+// may be negative or zero: the walk that meets infinite values takes them out of the products first.
 template <int DT>
-__device__ inline void parts_of(float p0, float p1, unsigned int (&w)[2]) {
+__device__ inline void parts_of(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
   if constexpr (DT == SSA_BF16) {
-    w[0] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
-    asm("" : "+v"(w[0]));  // the halves are taken from it, not rounded once more
-    p0 -= __uint_as_float(w[0] << 16);
-    p1 -= __uint_as_float(w[0] & 0xffff0000u);
-    w[1] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      w[i] = __builtin_bit_cast(unsigned int, bf16x2{(__bf16)p0, (__bf16)p1});
+      asm("" : "+v"(w[i]));  // the halves are taken from it, not rounded once more
+      p0 -= __uint_as_float(w[i] << 16);
+      p1 -= __uint_as_float(w[i] & 0xffff0000u);
+    }
   } else {
     const auto h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
     w[0] = __builtin_bit_cast(unsigned int, h);
@@ -872,6 +875,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   constexpr int KD = ROW / (16 * GR), DB = DP / RW, AR = RW * RW / 64;  // steps, blocks, results a lane
   constexpr int NS = KT / RW, NQ = KT / (4 * GR), SUB = KT / 16;  // products, quads, subtiles of a tile
   constexpr int CH = ROW / 16, RPI = 64 / CH, LPW = KT / RPI / NW;  // chunks, rows, loads of a wave
+  constexpr int PARTS = kParts<DT>;  // of a weight
   constexpr float kShift = DT == SSA_F16 ? kF16Shift : 0.0f;
   constexpr float kGrow = DT == SSA_F16 ? 1.0f : 8.0f;  // fp16 weights end at 2^16
   // a stage is the keys' tile and the values'; objects of their own, so that the compiler's waits for
@@ -1060,14 +1064,14 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     l += sum;
 #pragma unroll
     for (int st = 0; st < NQ / 2; ++st) {
-      u32x4 w[2];
+      u32x4 w[PARTS];
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const float* const of = &s[2 * st + y / 2][y % 2 * 2];
-        unsigned int parts[2];
+        unsigned int parts[PARTS];
         parts_of<DT>(of[0], of[1], parts);
-        w[0][y] = parts[0];
-        w[1][y] = parts[1];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) w[k][y] = parts[k];
       }
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
@@ -1093,7 +1097,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
           }
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) acc[db] = mfma<DT>(v, w[k], acc[db]);
+        for (int k = 0; k < PARTS; ++k) acc[db] = mfma<DT>(v, w[k], acc[db]);
       }
     }
   };

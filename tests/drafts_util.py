@@ -162,3 +162,37 @@ class ForkState(U.PageState):
         self.table = [row + [-1] * (self.width - len(row)) for row in rows]
         self.lens = list(new)
         return source, target, tokens, 0
+
+
+# A key of score 0 and value 1 and three of score -3 WEIGHT_SCALE and values that add up to -1 / w, w their
+# weight: nothing is left of the sum but what the weights lack. w = 0.5051 loses 2^-17.2 of itself in two
+# bf16 parts and 2^-10.6 in one fp16 part. Every other key's score is so low that its weight is 0.
+WEIGHT_SCALE = 1865 / 8192
+WEIGHT_KEYS = {0: 0.0, 20: -3.0, 77: -3.0, 131: -3.0}
+
+
+def cancelling(dtype):
+    """Of each of WEIGHT_KEYS the value, the output's exact value and what it may be off by.
+
+    u = 2^-24: the weight's exp2 4 u, its exponent (scale, log2 e, their product and the score's) 3 u of
+    0.69; at most 10 products that are not zero, of sizes that add up to 2.01, added in fp32: 10 u of
+    that; fp16's two parts 2^-20 of the weight, whose products' sizes add up to 1.01."""
+    u = 2.0 ** -24
+    w = math.exp(-3.0 * WEIGHT_SCALE)
+    left, values = -1.0 / w, []
+    for _ in range(3):
+        values.append(torch.tensor(left, dtype=torch.float64).to(dtype).double().item())
+        left -= values[-1]
+    total = 1.0 + 3.0 * w
+    want = (1.0 + w * sum(values)) / total
+    off = 7 * u + 10 * u * 2.01 + (2.0 ** -20 * 1.01 if dtype == torch.float16 else 0.0)
+    return dict(zip(WEIGHT_KEYS, [1.0] + values)), want, off / total + torch.finfo(dtype).eps / 2 * abs(want)
+
+
+def in_parts(w, dtype, parts):
+    """A weight (fp32) as the sum of its first 16-bit parts, in float64."""
+    left, total = w.double(), torch.zeros_like(w.double())
+    for _ in range(parts):
+        x = left.float().to(dtype).double()
+        total, left = total + x, left - x
+    return total

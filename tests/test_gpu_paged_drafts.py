@@ -888,3 +888,26 @@ def test_compiled_run_equals_eager(cuda):
     assert (outs[0][7:] == 7).all() and torch.equal(outs[0], outs[1])
     for x in ("lens", "table", "free", "nfree", "status", "k", "v"):
         assert torch.equal(getattr(caches[0], x), getattr(caches[1], x)), x
+
+
+# ---- the bits of the weights ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,hq,n", [(64, 2, 3), (64, 8, 4), (64, 16, 16), (128, 2, 2), (128, 16, 4),
+                                    (128, 32, 8), (256, 1, 3), (256, 16, 4), (512, 2, 3)])
+def test_weights_hold_all_their_bits(cuda, dtype, d, hq, n):
+    """Values that cancel but for what a weight lacks (drafts_util.cancelling), at every tile size."""
+    q, cache, cu = make(cuda, dtype, [150], [n], hq, 1, d, 16)
+    values, want, off = D.cancelling(dtype)
+    q.zero_()
+    q[..., 0] = 1.0
+    for j in range(150 + n):
+        at = (int(cache.table[0, j // 16]), 0, j % 16)
+        cache.k[0][at].zero_()
+        cache.k[0][at][0] = D.WEIGHT_KEYS.get(j, -2000.0)
+        if j in values:
+            cache.v[0][at].fill_(values[j])
+    print(dtype, d, hq, n, flush=True)
+    out = cache.attend_drafts(0, q, cu, scale=D.WEIGHT_SCALE).double().cpu()
+    worst = (out - want).abs().max().item()
+    assert worst <= off, (worst, off, want)

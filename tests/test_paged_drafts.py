@@ -253,3 +253,15 @@ def test_drafts_are_cut_to_fit(tmp_path):
                     str(root / "tests/paged_drafts_check.cpp"), "-o", str(exe)], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
     assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
+
+
+def test_weights_that_lack_bits_are_seen():
+    """The bound that the GPU's outputs are held to tells weights of all their bits from those of fewer."""
+    for dtype, enough in ((torch.bfloat16, 3), (torch.float16, 2)):
+        values, want, off = D.cancelling(dtype)
+        w = torch.tensor([1.0] + [torch.tensor(-3.0 * D.WEIGHT_SCALE, dtype=torch.float64).exp()] * 3,
+                         dtype=torch.float64).float()
+        v = torch.tensor(list(values.values()), dtype=torch.float64)
+        for parts in range(1, 4):
+            got = (D.in_parts(w, dtype, parts) * v).sum() / w.double().sum()
+            assert (abs(got - want) <= off) == (parts >= enough), (dtype, parts, got, want, off)
