@@ -535,23 +535,25 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  * and some of the others (a tree that one step of the model verifies, a chain, the next piece of a
  * prompt). Request b's are rows [cu[b], cu[b + 1]) of N (cu (B + 1) int32, as ssa_paged_resize writes
  * it) and, stored by ssa_paged_append, the last n = cu[b + 1] - cu[b] of its lens[b] tokens in the
- * cache; ctx = lens[b] - n are before them. What does not fit is found on the device: offsets that
- * descend or pass N make a request none, 0 <= n <= lens[b] <= W * page and n <= 32 * words must hold.
+ * cache; ctx = lens[b] - n are before them. What does not fit is found on the device: 0 <= n <= lens[b]
+ * <= W * page and n <= 32 * words must hold. Offsets ascend: where they descend anywhere every row of the
+ * call is answered as one that does not fit. A request whose offsets lie outside 0 to N is none; of its rows
+ * those that are there, and the rows before the first request's, do not fit either.
  *
  * ssa_paged_draft_masks: parents (N) int32, of each drafted token the place of the one it continues
  *   among its request's (less than its own), or -1 for the context. masks (N, words) int32, words 1 to
  *   32: bit i % 32 of word i / 32 says that the token attends drafted token i: itself and its
  *   ancestors; pos (N) int32: its position, ctx + the ancestors. Of a token with a parent that does not
- *   fit, of those that continue it and of requests that do not fit: 0 and -1; of rows behind the last
- *   request's: 0 and 0.
+ *   fit, of those that continue it, of requests and rows that do not fit: 0 and -1; of rows behind the
+ *   last request's: 0 and 0.
  * ssa_paged_attend_drafts: q, out (N, Hq, d). Row t of request b attends the keys j < ctx and the
  *   drafted ones of its mask (masks (N, words), pos (N), or all NULL with words 0: the drafted tokens
  *   up to itself, one after the other from position ctx on); with a window only those at positions past
  *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, head layout,
  *   lse (N, Hq), status, page ids and strides as ssa_paged_attend; scores, statistics and sums in fp32,
  *   and a weight with all its bits (bf16) or all but 2^-20 of itself down to 2^-38 of the row's largest
- *   (fp16). A row that attends nothing: out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request that does
- *   not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
+ *   (fp16). A row that attends nothing: out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request or row that
+ *   does not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
  *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
  *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq and the
  *   workgroups that a call may need are held below 2^31 and 2^24. Workspace:

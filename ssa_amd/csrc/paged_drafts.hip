@@ -25,6 +25,8 @@ struct MaskParams {
   int32_t* pos;
   int64_t N;
   int B, words;
+  int first;  // the launch's first request
+  bool all;   // whether each of its workgroups looks at all offsets
 };
 
 // A token's way up so far: the next ancestor's place plus 1 (0: none), the tokens on the way, and
@@ -35,31 +37,40 @@ __device__ inline unsigned int way(int anc, int steps, bool bad) {
 
 // A workgroup for a request and four words of its masks, a thread a token. Every round joins a token's
 // way with that of the ancestor where it ends, so its length doubles: a chain of 1024 takes ten rounds.
-// The last workgroups clear the rows behind the last token. Bound by launch and barrier latency: 64 trees
-// of up to 64 tokens 3.5 us, 8 of 1,024 10.8.
+// The last workgroups answer the rows that no request's offsets hold, and all rows where the offsets
+// descend (they may be two requests' then). Bound by launch and barrier latency: 64 trees of up to 64 tokens
+// 3.5 us, 8 of 1,024 10.8.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_draft_masks_kernel(MaskParams p) {
   __shared__ unsigned int ways[THREADS];
   __shared__ u32x4 seen[THREADS];
-  const int b = blockIdx.x, t = threadIdx.x, w0 = blockIdx.y * 4;
+  const int b = p.first + blockIdx.x, t = threadIdx.x, w0 = blockIdx.y * 4;
   const int count = min(4, p.words - w0);
   auto store = [&](int64_t row, const u32x4& m, int pos) {
     for (int i = 0; i < count; ++i) p.masks[row * p.words + w0 + i] = m[i];
     if (w0 == 0) p.pos[row] = pos;
   };
+  bool falls = false;
+  if (p.all)
+    for (int i = t; i < p.B; i += THREADS) falls |= p.cu[i + 1] < p.cu[i];
   if (b == p.B) {
+    falls = __syncthreads_or(falls);
     const int end = p.cu[p.B];
-    for (int64_t row = max(end, 0) + t; row < p.N; row += THREADS) store(row, u32x4{}, 0);
+    const int64_t first = falls || end < 0 ? p.N : min((int64_t)max(p.cu[0], 0), p.N);
+    for (int64_t row = t; row < first; row += THREADS) store(row, u32x4{}, -1);
+    for (int64_t row = max((int64_t)end, first) + t; row < p.N; row += THREADS) store(row, u32x4{}, 0);
     return;
   }
-  const int c0 = p.cu[b];
-  const DraftSpan s = draft_span(p.lens[b], c0, p.cu[b + 1], p.N, 0, p.words, 0x7fffffff);
-  if (!s.span.ok) {
-    for (int i = t; i < s.n; i += THREADS) store((int64_t)c0 + i, u32x4{}, -1);
-    return;
-  }
-  const bool mine = t < s.n;
+  const int c0 = p.cu[b], c1 = p.cu[b + 1];
+  const DraftSpan s = draft_span(p.lens[b], c0, c1, p.N, 0, p.words, 0x7fffffff);
+  const bool mine = s.span.ok && t < s.n;
   const int parent = mine ? p.parents[(int64_t)c0 + t] : -1;
+  if (__syncthreads_or(falls)) return;
+  if (!s.span.ok) {  // of offsets that pass the rows, those that are there
+    const int64_t to = min((int64_t)c1, p.N);
+    for (int64_t row = max(c0, 0) + t; row < to; row += THREADS) store(row, u32x4{}, -1);
+    return;
+  }
   const bool bad = parent < -1 || parent >= t;
   unsigned int own = way(bad ? -1 : parent, 1, mine && bad);
   u32x4 m{};
@@ -82,6 +93,10 @@ __global__ __launch_bounds__(THREADS) void paged_draft_masks_kernel(MaskParams p
   const bool fits = own >> 31 == 0;
   store((int64_t)c0 + t, fits ? m : u32x4{}, fits ? s.ctx + (int)(own >> 16 & 0x7fff) - 1 : -1);
 }
+
+// Up to so many requests every workgroup looks at all offsets; past them the last ones do, in a launch of
+// their own that finds all rows written.
+constexpr int64_t kMaskScan = 1024;
 
 // ---- attention of drafted tokens ---------------------------------------------------------------
 
@@ -128,8 +143,8 @@ __device__ inline DraftSpan draft_of(const DraftParams& p, int b) {
 
 // Finds workgroup `id`'s item from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. Of the call's row tiles an XCD takes a run, the tiles of the
-// same keys next to each other: its L2 serves them together. False past the last one. Sums of offsets
-// that do not ascend may wrap; the item's own numbers are checked. (Equal shares of all units instead,
+// same keys next to each other: its L2 serves them together. False past the last one, and for all where
+// the offsets descend (rest_rows answers). (Equal shares of all units instead,
 // a workgroup going on from one row tile to the next, cost a short call 8 us, and a mixed batch 550 us for
 // 313: a unit takes as long with few rows as with many.)
 template <int M>
@@ -139,12 +154,15 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   DraftSpan own{};
   int units = 0, tiles = 0;
   float work = 0.0f;
+  bool falls = false;
   for (int b = b0; b < b1; ++b) {
     own = draft_of(p, b);
+    falls |= p.cu[b + 1] < p.cu[b];
     units = draft_units(own);
     tiles = draft_tiles(own, p.G, M);
     work += (float)tiles * (float)units;
   }
+  if (__any(falls)) return false;
   int chunk = 0x7fffffff;
   it.stream = p.stream_units == 0;
   if (p.items != 0) {
@@ -250,23 +268,47 @@ __device__ inline uint64_t attended_keys(const DraftParams& p, const DraftItem& 
   return context | (bits & ~below(-(int64_t)i0) & below((int64_t)it.s.n - i0));
 }
 
-// Rows that no request holds: zeros where the call wants them cleared; every row NaN after a refused
-// resize. Block `id` of kRestBlocks.
+// Rows that no request's items answer, by block `id` of kRestBlocks: those behind the last request's become
+// zeros where the call wants them cleared; NaN are those before the first, those of requests whose offsets
+// pass the rows, and all of them where the offsets descend or the resize was refused.
 template <int DT>
 __device__ inline void rest_rows(const DraftParams& p, int id) {
   constexpr int ES = DT == SSA_F32 ? 4 : 2;
-  const bool refused = p.status && *p.status != 0;
-  if (!refused && !p.clear) return;
+  __shared__ int s_lo, s_hi;  // the first and last offset among the rows
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    s_lo = 0x7fffffff;
+    s_hi = -1;
+  }
+  __syncthreads();
+  int lo = 0x7fffffff, hi = -1;
+  bool falls = false;
+  for (int b = tid; b <= p.B; b += 256) {
+    const int c = p.cu[b];
+    if (c >= 0) lo = min(lo, c);
+    if (c <= p.N) hi = max(hi, c);
+    falls |= b > 0 && c < p.cu[b - 1];
+  }
+  if (lo != 0x7fffffff) atomicMin(&s_lo, lo);
+  if (hi >= 0) atomicMax(&s_hi, hi);
+  falls = __syncthreads_or(falls);
+  if (falls && p.items != 0)  // nothing to join
+    for (int b = id * 256 + tid; b < p.B; b += kRestBlocks * 256) p.info[2 * b + 1] = 1;
+  const int end = p.cu[p.B];
+  const bool fits = end >= 0 && end <= p.N;
+  const int64_t first = falls || (p.status && *p.status != 0) ? p.N : min((int64_t)s_lo, p.N);
+  const int64_t last = fits && !p.clear ? p.N : max((int64_t)s_hi, first);
   const int per = p.d * ES / 16;
-  const float x = refused ? NAN : 0.0f;
-  const int64_t first = refused ? 0 : max(p.cu[p.B], 0), rows = (p.N - first) * p.Hq;
-  for (int64_t i = id * 256 + (int)threadIdx.x; i < rows * per; i += kRestBlocks * 256) {
-    const int64_t row = i / per, t = first + row / p.Hq, h = row % p.Hq;
+  const int64_t rows = (first + p.N - last) * p.Hq;
+  for (int64_t i = id * 256 + tid; i < rows * per; i += kRestBlocks * 256) {
+    const int64_t row = i / per, n = row / p.Hq, h = row - n * p.Hq, t = n < first ? n : last + n - first;
+    const bool bad = n < first || !fits;
     const int64_t to = t * p.ot + h * p.oh + (i - row * per) * (16 / ES);
+    const float x = bad ? NAN : 0.0f;
     const f32x4 v = {x, x, x, x};
     store_row4<DT>(p.out, to, v);
     if constexpr (ES == 2) store_row4<DT>(p.out, to + 4, v);
-    if (p.lse && i == row * per) p.lse[t * p.Hq + h] = refused ? NAN : -INFINITY;
+    if (p.lse && i == row * per) p.lse[t * p.Hq + h] = bad ? NAN : -INFINITY;
   }
 }
 
@@ -1191,7 +1233,7 @@ __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   const int h = (int)(id - token * p.Hq), g = h / p.G;
   const int b = last_at_most(p.cu, p.B, (int)row), c0 = p.cu[b], c1 = p.cu[b + 1];
   const DraftSpan s = draft_of(p, b);
-  if (row < c0 || row >= c1 || s.n == 0) return;
+  if (row < c0 || row >= c1 || s.n == 0) return;  // rest_rows answers
   const int first = p.info[2 * b], parts = p.info[2 * b + 1];
   if (parts <= 1) return;  // written by its one item
   const unsigned int x = (unsigned)(row - c0) * p.G + (h - g * p.G), tile = x / M;
@@ -1466,13 +1508,18 @@ extern "C" int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu,
   SSA_REQUIRE(fits_launch((B + 1) * ((words + 3) / 4), threads), SSA_ERR_UNSUPPORTED,
               "ssa_paged_draft_masks: %lld requests in one call", (long long)B);
   if (N == 0) return SSA_OK;
-  MaskParams p{parents, cu, lens, masks, pos, N, (int)B, (int)words};
-  const dim3 grid((unsigned)(B + 1), (unsigned)((words + 3) / 4));
   hipStream_t st = (hipStream_t)stream;
-  if (threads == 64) paged_draft_masks_kernel<64><<<grid, 64, 0, st>>>(p);
-  else if (threads == 256) paged_draft_masks_kernel<256><<<grid, 256, 0, st>>>(p);
-  else paged_draft_masks_kernel<1024><<<grid, 1024, 0, st>>>(p);
-  return launch_status("paged_draft_masks_kernel");
+  auto run = [&](int64_t first, int64_t blocks, bool all) {
+    MaskParams p{parents, cu, lens, masks, pos, N, (int)B, (int)words, (int)first, all};
+    const dim3 grid((unsigned)blocks, (unsigned)((words + 3) / 4));
+    if (threads == 64) paged_draft_masks_kernel<64><<<grid, 64, 0, st>>>(p);
+    else if (threads == 256) paged_draft_masks_kernel<256><<<grid, 256, 0, st>>>(p);
+    else paged_draft_masks_kernel<1024><<<grid, 1024, 0, st>>>(p);
+    return launch_status("paged_draft_masks_kernel");
+  };
+  if (B <= kMaskScan) return run(0, B + 1, true);
+  SSA_TRY(run(0, B, false));
+  return run(B, 1, true);
 }
 
 extern "C" size_t ssa_paged_attend_drafts_workspace_size(int dtype, int64_t B, int64_t N, int64_t Hq,

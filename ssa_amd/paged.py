@@ -382,8 +382,9 @@ def draft_masks(parents: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, mos
 
     A token attends itself and its ancestors; its position is the context's length + its ancestors. A
     parent that does not fit, and what continues it, gives no mask and position -1 (attend_drafts: NaN),
-    as does a request of more than `most` (rounded up to 32) or more than its length. Rows behind the
-    last request's: 0."""
+    as does a request of more than `most` (rounded up to 32) or more than its length, a row before the
+    first request's or of one whose offsets pass the rows, and every row where the offsets descend. Rows
+    behind the last request's: 0."""
     if not 1 <= most <= 1024:
         raise ValueError(f"most={most}: 1 to 1024 drafted tokens a request are served")
     if torch.compiler.is_compiling():
@@ -454,7 +455,8 @@ def attend_drafts(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tab
     are zeros and -inf; in a given `out` they are left as they were.
 
     status (1,) int32: a resize's; if that was refused, every row is NaN, as are the rows of a request
-    whose length or pages do not fit. For one token a request attend_pages is the faster call; prompts
+    whose length, offsets or pages do not fit, those before the first request's and, where the offsets
+    descend, all of them. For one token a request attend_pages is the faster call; prompts
     from their start are sparse_attention's and dense's (ssa_kernel)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])

@@ -196,3 +196,16 @@ def in_parts(w, dtype, parts):
         x = left.float().to(dtype).double()
         total, left = total + x, left - x
     return total
+
+
+def rows_of(cu, N):
+    """Of a call's rows: (first row, offsets, requests) of the requests whose offsets lie among them, and the
+    row from which they are behind the last request's (N: none are). Every other row does not fit."""
+    if any(b < a for a, b in zip(cu, cu[1:])):
+        return 0, [0], [], N
+    held = [b for b in range(len(cu) - 1) if cu[b] >= 0 and cu[b + 1] <= N]
+    behind = cu[-1] if 0 <= cu[-1] <= N else N
+    if not held:
+        return 0, [0], [], behind
+    first = cu[held[0]]
+    return first, [cu[b] - first for b in held] + [cu[held[-1] + 1] - first], held, behind

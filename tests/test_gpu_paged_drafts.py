@@ -911,3 +911,77 @@ def test_weights_hold_all_their_bits(cuda, dtype, d, hq, n):
     out = cache.attend_drafts(0, q, cu, scale=D.WEIGHT_SCALE).double().cpu()
     worst = (out - want).abs().max().item()
     assert worst <= off, (worst, off, want)
+
+
+# ---- rows that no request holds -----------------------------------------------------------------
+
+BAD_OFFSETS = [[0, 6, 25], [3, 6, 20], [3, 6, 17], [0, 0, 21], [0, 20, 2 ** 31 - 1], [-2, 5, 20], [-2, 5, 18],
+               [-2 ** 31, -1, 7], [20, 20, 20], [25, 30, 30], [-9, -5, -3], [-2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1],
+               [0, 12, 6], [5, 0, 20], [20, 4, 4], [2 ** 31 - 1, 0, 4]]
+
+
+def poison(dev, *shapes):
+    """Memory of these sizes that the next allocations of them get, full of sevens."""
+    held = [torch.full(shape, 7, device=dev, dtype=dtype) for shape, dtype in shapes]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("requests", [2, 70, 1500])
+def test_masks_of_rows_that_no_request_holds(cuda, requests):
+    """Written whatever the offsets: 0 and -1 where they do not fit, 0 and 0 behind the last request."""
+    N, most = 20, 40
+    rng = random.Random(1)
+    parents = D.random_parents(rng, N)
+    for bad in BAD_OFFSETS:
+        cu = bad[:1] * (requests - 2) + bad
+        lens = [2 ** 31 - 1 - b for b in range(requests)]
+        first, own, held, behind = D.rows_of(cu, N)
+        masks, pos = [[0, 0] for _ in range(N)], [-1] * behind + [0] * (N - behind)
+        ways = []  # parents of a request's tokens count from its first
+        for a, b in zip(own, own[1:]):
+            ways += D.random_parents(rng, b - a)
+        given = parents[:first] + ways + parents[first + len(ways):]
+        m, at = D.masks_and_pos(ways, [b - a for a, b in zip(own, own[1:])], [lens[b] for b in held], 2,
+                                len(ways))
+        masks[first:first + len(ways)], pos[first:first + len(ways)] = m, at
+        print(requests, bad, flush=True)
+        args = [int32(x, cuda) for x in (given, cu, lens)]
+        poison(cuda, ((N, 2), torch.int32), ((N,), torch.int32))
+        d = P.draft_masks(*args, most)
+        assert d.masks.tolist() == masks and d.pos.tolist() == pos, bad
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx,requests,hq,d", [(40, 2, 4, 64), (9000, 2, 2, 64), (9000, 2, 8, 128),
+                                               (5000, 2, 32, 64), (700, 70, 4, 256), (40, 70, 2, 512)])
+def test_attention_of_rows_that_no_request_holds(cuda, dtype, ctx, requests, hq, d):
+    """NaN where the offsets do not fit, whatever the memory held before, the other requests right; rows
+    behind the last request zeros, or as they were."""
+    N, page = 20, 64
+    q, cache, _ = make(cuda, dtype, [ctx], [N], hq, 2, d, page, seed=21)
+    table = cache.table.expand(requests, -1).contiguous()
+    lens = int32([ctx + N - b % 3 for b in range(requests)], cuda)
+    for bad in BAD_OFFSETS:
+        cu = bad[:1] * (requests - 2) + bad
+        first, own, held, behind = D.rows_of(cu, N)
+        rows = slice(first, first + own[-1])
+        print(dtype, ctx, requests, hq, d, bad, flush=True)
+        args = (q, cache.k[0], cache.v[0], table, lens, int32(cu, cuda))
+        poison(cuda, ((N, hq, d), dtype), ((N, hq), torch.float32))
+        out, lse = P.attend_drafts(*args, return_lse=True)
+        given = torch.full_like(q, 7.0)
+        got, glse = P.attend_drafts(*args, return_lse=True, out=given)
+        torch.cuda.synchronize()
+        if held:
+            want, wlse, tol, ltol = D.attend(q[rows], cache.k[0], cache.v[0], table[held], lens[held],
+                                             torch.tensor(own), 1 / math.sqrt(d))
+            U.close(out[rows], want, tol)
+            U.close(lse[rows], wlse, ltol)
+        misfit = torch.ones(N, dtype=torch.bool, device=cuda)
+        misfit[rows] = False
+        misfit[behind:] = False
+        assert out[misfit].isnan().all() and lse[misfit].isnan().all(), bad
+        assert (out[behind:] == 0).all() and (lse[behind:] == -math.inf).all(), bad
+        assert torch.equal(got[:behind].nan_to_num(5.0), out[:behind].nan_to_num(5.0)), bad
+        assert (got[behind:] == 7).all() and torch.equal(glse.nan_to_num(5.0), lse.nan_to_num(5.0)), bad

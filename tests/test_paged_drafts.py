@@ -265,3 +265,11 @@ def test_weights_that_lack_bits_are_seen():
         for parts in range(1, 4):
             got = (D.in_parts(w, dtype, parts) * v).sum() / w.double().sum()
             assert (abs(got - want) <= off) == (parts >= enough), (dtype, parts, got, want, off)
+
+
+def test_rows_of_offsets():
+    assert D.rows_of([0, 6, 25], 20) == (0, [0, 6], [0], 20)
+    assert D.rows_of([3, 6, 17], 20) == (3, [0, 3, 14], [0, 1], 17)
+    assert D.rows_of([-2, 5, 20], 20) == (5, [0, 15], [1], 20)
+    assert D.rows_of([0, 6, 4, 20], 20) == (0, [0], [], 20)
+    assert D.rows_of([25, 30], 20) == (0, [0], [], 20) and D.rows_of([-5, -3], 20)[3] == 20
