@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define SSA_ABI_VERSION 9
+#define SSA_ABI_VERSION 10
 
 typedef void* ssa_stream_t; /* hipStream_t */
 
@@ -562,7 +562,9 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the
  *   resize that gives back the pages behind; -1, and nothing moved, where a path, a count, the lengths
- *   or a page id do not fit. The pools do not overlap. strides[8] = kpool(layer,page,head,slot),
+ *   or a page id do not fit. A second call would move tokens that have moved. The pools do not overlap.
+ *   ssa_paged_keep_all: nothing is moved for any request unless all fit (so that the resize to new_lens,
+ *   which -1 refuses, and the moves are made together or not at all). strides[8] = kpool(layer,page,head,slot),
  *   vpool(layer,page,head,slot).
  *
  * Requests that share pages:
@@ -600,6 +602,11 @@ int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layers, int64_t 
                    int64_t table_stride, int64_t W, const int32_t* lens, const int32_t* cu,
                    int64_t B, const int32_t* path, int64_t path_stride, int64_t width,
                    const int32_t* counts, int32_t* new_lens, ssa_stream_t stream);
+int ssa_paged_keep_all(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv, int64_t d,
+                       int64_t pages, int64_t page, const int64_t* strides, const int32_t* table,
+                       int64_t table_stride, int64_t W, const int32_t* lens, const int32_t* cu,
+                       int64_t B, const int32_t* path, int64_t path_stride, int64_t width,
+                       const int32_t* counts, int32_t* new_lens, ssa_stream_t stream);
 size_t ssa_paged_fork_workspace_size(int64_t B, int64_t W, int64_t pages);
 int ssa_paged_fork(const int32_t* src, const int32_t* new_lens, int32_t* lens, int32_t* table,
                    int64_t table_stride, int64_t B, int64_t W, int64_t page, int32_t* free_pages,

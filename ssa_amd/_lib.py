@@ -14,7 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libssa_hip.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 SSA_OK, SSA_ERR_INVALID, SSA_ERR_UNSUPPORTED, SSA_ERR_HIP, SSA_ERR_WORKSPACE = 0, -1, -2, -3, -4
 F32, F16, BF16 = 0, 1, 2
@@ -110,6 +110,9 @@ _SIGNATURES = {
     "ssa_paged_keep": (_c_int, [_c_p] * 2 + [_c_int] + [_c_i64] * 5 +
                        [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64] +
                        [_c_p] * 3),
+    "ssa_paged_keep_all": (_c_int, [_c_p] * 2 + [_c_int] + [_c_i64] * 5 +
+                           [_c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_i64] +
+                           [_c_p] * 3),
     "ssa_paged_fork_workspace_size": (_c_sz, [_c_i64] * 3),
     "ssa_paged_fork": (_c_int, [_c_p] * 4 + [_c_i64] * 4 + [_c_p, _c_i64] + [_c_p] * 6 +
                        [_c_sz, _c_p]),

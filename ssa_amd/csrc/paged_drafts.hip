@@ -1404,12 +1404,17 @@ struct KeepParams {
 
 constexpr int kKeepThreads = 64, kKeepBatch = 32;
 
+// Whether a request's tokens move by its own check, or (all or none) by those of a launch before it.
+enum Keep { kKeepEach, kKeepCheck, kKeepAll };
+
 // A workgroup for a request and 64 columns (a column: 16 bytes of a layer's keys or values of a head,
 // over all tokens), a thread a column. An accepted token never moves up and they move in order, so a
 // column's tokens are read kKeepBatch at a time before any of these is written, and none that is
-// written is read again. All or nothing: every workgroup of a request checks its whole path first. Bound
+// written is read again. All or nothing: every workgroup of a request checks its whole path first, and
+// with kKeepAll looks at what the launch before it (kKeepCheck) found of every request. Bound
 // by the longest path's column: 24 requests with 200 of 600 tokens moved in 8 layers (5 heads of 80, fp32,
 // 93 MB in all) 37 us; 64 with 2 in 24 layers 4.1.
+template <Keep KEEP>
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
   __shared__ int64_t s_from[2][kKeepThreads], s_to[2][kKeepThreads];  // of keys and values
   __shared__ int s_first;
@@ -1441,8 +1446,13 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
     if (moved != 0x7fffffff) atomicMin(&s_first, moved);
     bad = __syncthreads_or(wrong);
   }
-  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = bad ? -1 : ctx + count;
-  if (bad || s_first >= count) return;
+  if (KEEP != kKeepAll && blockIdx.x == 0 && tid == 0) p.new_lens[b] = bad ? -1 : ctx + count;
+  if (KEEP == kKeepCheck || bad || s_first >= count) return;
+  if constexpr (KEEP == kKeepAll) {
+    bool none = false;
+    for (int i = tid; i < (int)gridDim.y; i += kKeepThreads) none |= p.new_lens[i] < 0;
+    if (__any(none)) return;
+  }
   const int first = s_first, column = blockIdx.x * kKeepThreads + tid;
   const int c = column % p.vecs, of = column / p.vecs, h = of % p.Hkv, lv = of / p.Hkv;
   const bool mine = column < p.columns, v = lv & 1;
@@ -1611,13 +1621,13 @@ extern "C" int ssa_paged_attend_drafts(const void* q, const void* kpool, const v
   return run_drafts_dim<SSA_BF16>(p, y, hs);
 }
 
-extern "C" int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
-                              int64_t d, int64_t pages, int64_t page, const int64_t* strides,
-                              const int32_t* table, int64_t table_stride, int64_t W,
-                              const int32_t* lens, const int32_t* cu, int64_t B,
-                              const int32_t* path, int64_t path_stride, int64_t width,
-                              const int32_t* counts, int32_t* new_lens, ssa_stream_t stream) {
-  const char* const who = "ssa_paged_keep";
+namespace {
+
+int keep(const char* who, bool all, void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
+         int64_t d, int64_t pages, int64_t page, const int64_t* strides, const int32_t* table,
+         int64_t table_stride, int64_t W, const int32_t* lens, const int32_t* cu, int64_t B,
+         const int32_t* path, int64_t path_stride, int64_t width, const int32_t* counts,
+         int32_t* new_lens, ssa_stream_t stream) {
   SSA_REQUIRE(kpool && vpool && strides && table && lens && cu && counts && new_lens &&
                   (path || width == 0), SSA_ERR_INVALID, "%s: NULL argument", who);
   SSA_TRY(check_pool(who, dtype, Hkv, d, pages, page));
@@ -1641,6 +1651,36 @@ extern "C" int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layer
                strides[0] * es, strides[1] * es, strides[2] * es, strides[3] * es,
                strides[4] * es, strides[5] * es, strides[6] * es, strides[7] * es,
                page_div((int)page / 16)};
-  paged_keep_kernel<<<dim3((unsigned)blocks, (unsigned)B), kKeepThreads, 0, (hipStream_t)stream>>>(p);
+  const dim3 grid((unsigned)blocks, (unsigned)B);
+  hipStream_t st = (hipStream_t)stream;
+  if (!all) {
+    paged_keep_kernel<kKeepEach><<<grid, kKeepThreads, 0, st>>>(p);
+  } else {
+    paged_keep_kernel<kKeepCheck><<<dim3(1, (unsigned)B), kKeepThreads, 0, st>>>(p);
+    SSA_TRY(launch_status("paged_keep_kernel"));
+    paged_keep_kernel<kKeepAll><<<grid, kKeepThreads, 0, st>>>(p);
+  }
   return launch_status("paged_keep_kernel");
+}
+
+}  // namespace
+
+extern "C" int ssa_paged_keep(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
+                              int64_t d, int64_t pages, int64_t page, const int64_t* strides,
+                              const int32_t* table, int64_t table_stride, int64_t W,
+                              const int32_t* lens, const int32_t* cu, int64_t B,
+                              const int32_t* path, int64_t path_stride, int64_t width,
+                              const int32_t* counts, int32_t* new_lens, ssa_stream_t stream) {
+  return keep("ssa_paged_keep", false, kpool, vpool, dtype, layers, Hkv, d, pages, page, strides, table,
+              table_stride, W, lens, cu, B, path, path_stride, width, counts, new_lens, stream);
+}
+
+extern "C" int ssa_paged_keep_all(void* kpool, void* vpool, int dtype, int64_t layers, int64_t Hkv,
+                                  int64_t d, int64_t pages, int64_t page, const int64_t* strides,
+                                  const int32_t* table, int64_t table_stride, int64_t W,
+                                  const int32_t* lens, const int32_t* cu, int64_t B,
+                                  const int32_t* path, int64_t path_stride, int64_t width,
+                                  const int32_t* counts, int32_t* new_lens, ssa_stream_t stream) {
+  return keep("ssa_paged_keep_all", true, kpool, vpool, dtype, layers, Hkv, d, pages, page, strides,
+              table, table_stride, W, lens, cu, B, path, path_stride, width, counts, new_lens, stream);
 }

@@ -17,8 +17,8 @@ The lengths live on the device: every call is asynchronous on the current stream
 device, works under graph capture and synchronises with nothing. What a call can only find out on
 the device (a length beyond the table, too few free pages, a page id outside the pool) is answered
 there: resize_pages and fork_pages change nothing and write a status, append_pages skips the row,
-attend_pages and attend_drafts return NaN for the row, keep_drafts moves nothing and gives a length of
--1; no call follows a bad length or page id.
+attend_pages and attend_drafts return NaN for the row, keep_drafts moves nothing of the request (or of
+any) and gives a length of -1; no call follows a bad length or page id.
 
 attend_pages is the dense counterpart of attend_rows and dense_decode (ivf_decode) for batches of
 requests: the decode of the layers that a routed model leaves dense or sliding. attend_drafts is that
@@ -545,25 +545,27 @@ def _keep_plan(table, lens, cu, path, counts):
 
 
 def keep_drafts(kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-                cu: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+                cu: torch.Tensor, path: torch.Tensor, counts: torch.Tensor,
+                all_or_none: bool = False) -> torch.Tensor:
     """Keeps the accepted ones of the drafted tokens: moves token path[b, i] of request b's (their
     places among them, ascending; a way down a tree is) to place i, for i < counts[b], in every layer
     of kpool, vpool (layers, pages, Hkv, page, d), or of one layer's (pages, Hkv, page, d).
 
     path (B, K), counts (B,) int32, lens and cu as attend_drafts. Returns the lengths after (B,) int32,
     for the resize_pages that gives back the pages behind them; -1, and nothing is moved, for a request
-    whose path, count, length or pages do not fit. The pages of the drafted tokens must be the request's
+    whose path, count, length or pages do not fit; with all_or_none nothing is moved for any then. (Kept
+    once: a second call would move tokens that have moved.) The pages of the drafted tokens must be the request's
     own, and keys and values lie in memory of their own."""
     if torch.compiler.is_compiling():
         from . import torch_ops as T
-        return T.paged_keep(kpool, vpool, table, lens, cu, path, counts)
+        return T.paged_keep(kpool, vpool, table, lens, cu, path, counts, bool(all_or_none))
     _one_device(kpool, vpool, table, lens, cu, path, counts)
     sizes = _layers_plan(_meta(kpool), _meta(vpool))
     row, W, B, prow, K = _keep_plan(_meta(table), _meta(lens), _meta(cu), _meta(path),
                                     _meta(counts))
     new_lens = torch.empty(B, device=lens.device, dtype=torch.int32)
     if B:
-        _launch("ssa_paged_keep", lens, kpool.data_ptr(), vpool.data_ptr(), *sizes,
+        _launch("ssa_paged_keep_all" if all_or_none else "ssa_paged_keep", lens, kpool.data_ptr(), vpool.data_ptr(), *sizes,
                 table.data_ptr(), row, W, lens.data_ptr(), cu.data_ptr(), B,
                 path.data_ptr() if K else None, prow, K, counts.data_ptr(), new_lens.data_ptr())
     return new_lens
@@ -666,7 +668,8 @@ class PagedCache:
     A request ends by a resize to length 0, or by a fork to it where requests share pages (`fork`); q,
     k_new and v_new have a row for every request, idle ones included. After a resize or fork that did
     not fit, append and step store nothing and attend, attend_drafts and step give NaN, until one fits;
-    `check` raises then (it synchronises; a caller that keeps count of the pages need not call it)."""
+    `check` raises then (it synchronises; a caller that keeps count of the pages need not call it). The same
+    holds after an `accept` of a path that does not fit; nothing is moved then."""
 
     def __init__(self, requests, max_len, pages, hkv, d, page=64, layers=1, dtype=torch.bfloat16,
                  device="cuda", token_major=False):
@@ -734,9 +737,11 @@ class PagedCache:
 
     @torch.no_grad()
     def accept(self, cu: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> Resized:
-        """keep_drafts in every layer, and the resize to the lengths it gives. A path or count that does
-        not fit refuses the resize (status -1); the other requests' tokens are moved then."""
-        return self.resize(keep_drafts(self.k, self.v, self.table, self.lens, cu, path, counts), 0)
+        """keep_drafts in every layer, and the resize to the lengths it gives. All or nothing: with a path
+        or count that does not fit no request's tokens are moved, the lengths stay and the status is -1;
+        the call can be made again."""
+        return self.resize(keep_drafts(self.k, self.v, self.table, self.lens, cu, path, counts,
+                                       all_or_none=True), 0)
 
     @torch.no_grad()
     def fork(self, src: torch.Tensor | None, new_lens: torch.Tensor) -> Forked:

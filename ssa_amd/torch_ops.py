@@ -29,7 +29,7 @@ dtypes. Run eagerly, the public functions call the library directly and skip the
     ssa_amd::paged_attend_drafts(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, status)
         -> (out, lse)
     ssa_amd::paged_attend_drafts_into(..., out!) -> lse
-    ssa_amd::paged_keep(kpool!, vpool!, table, lens, cu, path, counts) -> new_lens
+    ssa_amd::paged_keep(kpool!, vpool!, table, lens, cu, path, counts, all_or_none) -> new_lens
     ssa_amd::paged_fork(src, new_lens, lens!, table!, free!, nfree!, page)
         -> (source, target, tokens, status)
     ssa_amd::paged_copy(kpool!, vpool!, source, target, tokens)
@@ -267,13 +267,13 @@ def _(q, kpool, vpool, table, lens, cu, masks, pos, scale, window, status, out):
 
 @torch.library.custom_op("ssa_amd::paged_keep", mutates_args=("kpool", "vpool"))
 def paged_keep(kpool: Tensor, vpool: Tensor, table: Tensor, lens: Tensor, cu: Tensor, path: Tensor,
-               counts: Tensor) -> Tensor:
+               counts: Tensor, all_or_none: bool = False) -> Tensor:
     from .paged import keep_drafts
-    return keep_drafts(kpool, vpool, table, lens, cu, path, counts)
+    return keep_drafts(kpool, vpool, table, lens, cu, path, counts, all_or_none)
 
 
 @paged_keep.register_fake
-def _(kpool, vpool, table, lens, cu, path, counts):
+def _(kpool, vpool, table, lens, cu, path, counts, all_or_none=False):
     return lens.new_empty(lens.shape[0])
 
 

@@ -985,3 +985,56 @@ def test_attention_of_rows_that_no_request_holds(cuda, dtype, ctx, requests, hq,
         assert (out[behind:] == 0).all() and (lse[behind:] == -math.inf).all(), bad
         assert torch.equal(got[:behind].nan_to_num(5.0), out[:behind].nan_to_num(5.0)), bad
         assert (got[behind:] == 7).all() and torch.equal(glse.nan_to_num(5.0), lse.nan_to_num(5.0)), bad
+
+
+# ---- accepted for all requests or none ----------------------------------------------------------
+
+@pytest.mark.parametrize("requests", [2, 70])
+@pytest.mark.parametrize("wrong", ["order", "range", "count", "page"])
+def test_accept_is_all_or_nothing_and_can_be_made_again(cuda, requests, wrong):
+    """One path that does not fit: nothing is moved for any request; corrected and accepted again, every
+    request holds what its path says."""
+    page, layers, n = 16, 3, 9
+    ctx = [(7 * b) % 40 for b in range(requests)]
+    cache = P.PagedCache(requests, 80, 6 * requests, 2, 64, page=page, layers=layers, device=cuda)
+    cache.resize(int32(ctx, cuda), sum(ctx))
+    r = cache.resize(int32([c + n for c in ctx], cuda), n * requests)
+    cache.k.normal_()
+    cache.v.normal_()
+    held = cache.k.clone(), cache.v.clone()
+    paths = [sorted(random.Random(b).sample(range(n), 1 + b % 5)) for b in range(requests)]
+    paths[0], last = [1, 2, 4], requests - 1
+    paths[last] = [2, 5, 8]
+    width = max(map(len, paths))
+    path = int32([p + [-1] * (width - len(p)) for p in paths], cuda)
+    counts = int32([len(p) for p in paths], cuda)
+    bad_path, bad_counts, table = path.clone(), counts.clone(), cache.table.clone()
+    if wrong == "order":
+        bad_path[last, 2] = 3
+    elif wrong == "range":
+        bad_path[last, 2] = n
+    elif wrong == "count":
+        bad_counts[last] = -1
+    else:
+        cache.table[last, (ctx[last] + 8) // page] = 6 * requests
+    print(requests, wrong, flush=True)
+    cache.accept(r.cu, bad_path, bad_counts)
+    with pytest.raises(RuntimeError, match="resize"):
+        cache.check()
+    assert cache.lens.tolist() == [c + n for c in ctx]
+    assert torch.equal(cache.k, held[0]) and torch.equal(cache.v, held[1])
+    new = P.keep_drafts(cache.k, cache.v, cache.table, cache.lens, r.cu, bad_path, bad_counts,
+                        all_or_none=True).tolist()
+    assert new == [c + len(p) for c, p in zip(ctx[:-1], paths[:-1])] + [-1]
+    assert torch.equal(cache.k, held[0]) and torch.equal(cache.v, held[1])
+    cache.table.copy_(table)
+    want = held[0].clone(), held[1].clone()
+    for b, p in enumerate(paths):
+        for i, t in enumerate(p):
+            (a, s), (c, at) = (divmod(ctx[b] + x, page) for x in (t, i))
+            for x, y in zip(want, held):
+                x[:, table[b, c], :, at] = y[:, table[b, a], :, s]
+    cache.accept(r.cu, path, counts)
+    cache.check()
+    assert cache.lens.tolist() == [c + len(p) for c, p in zip(ctx, paths)]
+    assert torch.equal(cache.k, want[0]) and torch.equal(cache.v, want[1])

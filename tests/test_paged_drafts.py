@@ -273,3 +273,15 @@ def test_rows_of_offsets():
     assert D.rows_of([-2, 5, 20], 20) == (5, [0, 15], [1], 20)
     assert D.rows_of([0, 6, 4, 20], 20) == (0, [0], [], 20)
     assert D.rows_of([25, 30], 20) == (0, [0], [], 20) and D.rows_of([-5, -3], 20)[3] == 20
+
+
+def test_keep_all_refuses_what_keep_refuses():
+    def f(name, kpool=FAKE, vpool=ctypes.c_void_p(1 << 30), dtype=_lib.F16, d=64, W=8, B=2, path=FAKE):
+        return status(name, kpool, vpool, dtype, 1, 2, d, 10, 16, S8, FAKE, 8, W, FAKE, FAKE, B, path, 3, 3,
+                      FAKE, FAKE, None)
+    for kw in (dict(kpool=NULL), dict(vpool=FAKE), dict(dtype=5), dict(d=20), dict(W=9), dict(B=0),
+               dict(path=NULL)):
+        code = f("ssa_paged_keep_all", **kw)
+        assert code == f("ssa_paged_keep", **kw) and code in (INVALID, UNSUPPORTED)
+    f("ssa_paged_keep_all", W=9)
+    assert b"ssa_paged_keep_all" in _lib.lib().ssa_last_error()
