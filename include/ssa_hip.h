@@ -545,7 +545,7 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   32: bit i % 32 of word i / 32 says that the token attends drafted token i: itself and its
  *   ancestors; pos (N) int32: its position, ctx + the ancestors. Of a token with a parent that does not
  *   fit, of those that continue it, of requests and rows that do not fit: 0 and -1; of rows behind the
- *   last request's: 0 and 0.
+ *   last request's: 0 and 0. masks and pos overlap no input (SSA_ERR_INVALID).
  * ssa_paged_attend_drafts: q, out (N, Hq, d). Row t of request b attends the keys j < ctx and the
  *   drafted ones of its mask (masks (N, words), pos (N), or all NULL with words 0: the drafted tokens
  *   up to itself, one after the other from position ctx on); with a window only those at positions past
@@ -562,7 +562,8 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the
  *   resize that gives back the pages behind; -1, and nothing moved, where a path, a count, the lengths
- *   or a page id do not fit. A second call would move tokens that have moved. The pools do not overlap.
+ *   or a page id do not fit. A second call would move tokens that have moved. The pools do not overlap;
+ *   new_lens overlaps no input (SSA_ERR_INVALID).
  *   ssa_paged_keep_all: nothing is moved for any request unless all fit (so that the resize to new_lens,
  *   which -1 refuses, and the moves are made together or not at all). strides[8] = kpool(layer,page,head,slot),
  *   vpool(layer,page,head,slot).

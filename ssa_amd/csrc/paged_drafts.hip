@@ -1493,6 +1493,12 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) 
   }
 }
 
+// Whether the n ints from a on and the m from b on share any.
+bool overlap(const int32_t* a, int64_t n, const int32_t* b, int64_t m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && n > 0 && m > 0 && x < y + (uintptr_t)m * 4 && y < x + (uintptr_t)n * 4;
+}
+
 int check_table(const char* who, int64_t W, int64_t table_stride, int64_t page) {
   SSA_REQUIRE(W > 0 && table_stride >= W && W <= 0x7fffffff / page, SSA_ERR_INVALID,
               "%s: table of %lld pages a row, stride %lld (at most 2^31 - 1 tokens)", who,
@@ -1518,6 +1524,11 @@ extern "C" int ssa_paged_draft_masks(const int32_t* parents, const int32_t* cu,
   SSA_REQUIRE(fits_launch((B + 1) * ((words + 3) / 4), threads), SSA_ERR_UNSUPPORTED,
               "ssa_paged_draft_masks: %lld requests in one call", (long long)B);
   if (N == 0) return SSA_OK;
+  for (const int32_t* in : {parents, cu, lens}) {  // read by workgroups that others may be ahead of
+    const int64_t n = in == parents ? N : in == cu ? B + 1 : B;
+    SSA_REQUIRE(!overlap(masks, N * words, in, n) && !overlap(pos, N, in, n), SSA_ERR_INVALID,
+                "ssa_paged_draft_masks: an output lies over an input");
+  }
   hipStream_t st = (hipStream_t)stream;
   auto run = [&](int64_t first, int64_t blocks, bool all) {
     MaskParams p{parents, cu, lens, masks, pos, N, (int)B, (int)words, (int)first, all};
@@ -1645,6 +1656,12 @@ int keep(const char* who, bool all, void* kpool, void* vpool, int dtype, int64_t
   const int64_t blocks = (columns + kKeepThreads - 1) / kKeepThreads;
   SSA_REQUIRE(fits_int(columns) && fits_launch(blocks * B, kKeepThreads), SSA_ERR_UNSUPPORTED,
               "%s: %lld layers of %lld requests in one call", who, (long long)layers, (long long)B);
+  // a request's workgroups read its length while the first of them writes the new one
+  SSA_REQUIRE(!overlap(new_lens, B, lens, B) && !overlap(new_lens, B, counts, B) &&
+                  !overlap(new_lens, B, cu, B + 1) &&
+                  !overlap(new_lens, B, path, (B - 1) * path_stride + width) &&
+                  !overlap(new_lens, B, table, (B - 1) * table_stride + W),
+              SSA_ERR_INVALID, "%s: new_lens lies over an input", who);
   KeepParams p{(char*)kpool, (char*)vpool, table, lens, cu, path, counts, new_lens,
                table_stride, path_stride, W * page, pages, (int)width,
                (int)page, (int)Hkv, (int)vecs, (int)columns,

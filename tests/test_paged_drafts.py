@@ -285,3 +285,26 @@ def test_keep_all_refuses_what_keep_refuses():
         assert code == f("ssa_paged_keep", **kw) and code in (INVALID, UNSUPPORTED)
     f("ssa_paged_keep_all", W=9)
     assert b"ssa_paged_keep_all" in _lib.lib().ssa_last_error()
+
+
+def test_outputs_over_inputs_are_refused():
+    """Workgroups of a request read what the first of them would overwrite."""
+    at = lambda i: ctypes.c_void_p((1 << 32) + 4 * i)  # noqa: E731
+    lens, cu, path, counts, table = at(0), at(100), at(200), at(300), at(400)
+
+    def keep(name, new):
+        return status(name, FAKE, ctypes.c_void_p(1 << 40), _lib.F16, 1, 2, 64, 10, 16, S8, table, 8, 8, lens,
+                      cu, 5, path, 3, 3, counts, new, None)
+    for name in ("ssa_paged_keep", "ssa_paged_keep_all"):
+        for new in (0, 4, 96, 105, 196, 214, 300, 304, 439):  # 5 ints from there on
+            assert keep(name, at(new)) == INVALID, new
+            assert b"new_lens lies over an input" in _lib.lib().ssa_last_error()
+    parents = at(500)
+
+    def masks(out, pos, words=2):
+        return status("ssa_paged_draft_masks", parents, cu, lens, 5, 9, words, out, pos, None)
+    far = at(10000)
+    for x in (500, 508, 492, 105, 83, 4):
+        assert masks(at(x), far) == INVALID, x
+    for x in (500, 508, 492, 105, 92, 4):
+        assert masks(far, at(x)) == INVALID
