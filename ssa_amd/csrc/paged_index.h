@@ -108,10 +108,11 @@ SSA_HD int draft_tiles(const DraftSpan& s, int G, int M) {
   return (int)(((unsigned)s.n * (unsigned)G + (unsigned)M - 1u) / (unsigned)M);
 }
 
-// Units per item so that `work` units (of every row tile, a sum of floats that may be 10^-5 off) make
-// at most `items` items besides one more per row tile.
+// Units per item so that `work` units (of every row tile) make at most `items` items besides one more per
+// row tile. work is a sum in fp32 of up to 65,535 requests' by 64 lanes: 1,024 additions one after the
+// other, 6 across the lanes, 3 roundings of a term, 2 here, 2^-24 each, make it at most 6.2 10^-5 too small.
 SSA_HD int draft_chunk(float work, float items) {
-  const float c = work / items * 1.00002f;
+  const float c = work / items * 1.0001f;
   return c >= 1e9f ? 1000000000 : (int)c + 1;
 }
 

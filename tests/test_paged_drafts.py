@@ -308,3 +308,20 @@ def test_outputs_over_inputs_are_refused():
         assert masks(at(x), far) == INVALID, x
     for x in (500, 508, 492, 105, 92, 4):
         assert masks(far, at(x)) == INVALID
+
+
+def test_work_of_many_requests_is_covered(tmp_path):
+    """csrc/paged_index.h compiled for the host: the units per item cover the work of up to 65,535 requests
+    whatever the fp32 sum of it loses."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if cxx is None:
+        pytest.skip("no host compiler")
+    exe = tmp_path / "check"
+    subprocess.run([cxx, "-std=c++17", "-O1", f"-I{root / 'ssa_amd' / 'csrc'}",
+                    str(root / "tests/paged_drafts_work_check.cpp"), "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
