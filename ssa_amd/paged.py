@@ -628,6 +628,15 @@ def _copy_plan(source, target, tokens):
     return n
 
 
+def _copy_limits(n, pool):
+    """Refuses copies of n pages of a pool (layers, pages, Hkv, page, d) that ssa_paged_copy refuses."""
+    layers, _, hkv, page, d = pool.shape
+    if n > 65535:
+        raise ValueError(f"{n} pages in one copy: at most 65535 are served")
+    if layers * hkv * page * d * pool.element_size() > 1 << 34:
+        raise ValueError("a page over all layers passes 16 GiB of keys")
+
+
 def copy_pages(kpool: torch.Tensor, vpool: torch.Tensor, source: torch.Tensor,
                target: torch.Tensor, tokens: torch.Tensor | None = None) -> None:
     """Copies page source[i] to page target[i], its first tokens[i] tokens (None: all), keys and
@@ -746,7 +755,8 @@ class PagedCache:
     @torch.no_grad()
     def fork(self, src: torch.Tensor | None, new_lens: torch.Tensor) -> Forked:
         """fork_pages on this cache's state and copy_pages in every layer. attend, attend_drafts, step
-        and check go by its status as by a resize's."""
+        and check go by its status as by a resize's. At most 65535 requests."""
+        _copy_limits(self.lens.numel(), self.k)  # before the table changes
         f = fork_pages(src, new_lens, self.lens, self.table, self.free, self.nfree, self.page)
         torch.add(f.status, 0, out=self.status)
         copy_pages(self.k, self.v, f.source, f.target, f.tokens)

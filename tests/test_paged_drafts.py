@@ -325,3 +325,39 @@ def test_work_of_many_requests_is_covered(tmp_path):
                     str(root / "tests/paged_drafts_work_check.cpp"), "-o", str(exe)], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
     assert res.returncode == 0 and res.stdout.strip() == "ok", res.stdout + res.stderr
+
+
+@pytest.mark.parametrize("sizes,match", [((65536, 16, 4, 1, 8), "65536 pages"), ((2, 16, 4, 1, 8), None),
+                                         ((65535, 16, 4, 1, 8), None)])
+def test_a_fork_that_cannot_be_copied_changes_nothing(monkeypatch, sizes, match):
+    """The copy's limits are looked at before the table is written."""
+    steps = []
+    fork = P.Forked(*(torch.zeros(1, dtype=torch.int32) for _ in range(4)))
+    monkeypatch.setattr(P, "fork_pages", lambda *a: steps.append("fork") or fork)
+    monkeypatch.setattr(P, "copy_pages", lambda *a: steps.append("copy"))
+    cache = P.PagedCache(*sizes, page=16, device="cpu")
+    if match:
+        with pytest.raises(ValueError, match=match):
+            cache.fork(None, cache.lens)
+        assert steps == []
+    else:
+        cache.fork(None, cache.lens)
+        assert steps == ["fork", "copy"]
+
+
+@pytest.mark.parametrize("layers,hkv,page,d,dtype", [
+    (64, 8, 65536, 256, torch.bfloat16), (64, 8, 65536, 264, torch.bfloat16),
+    (65, 8, 65536, 128, torch.float32), (32, 8, 65536, 256, torch.float32), (1 << 13, 1, 65536, 16, torch.float16)])
+def test_the_limits_of_a_copy_are_the_entry_points(layers, hkv, page, d, dtype):
+    """_copy_limits refuses what ssa_paged_copy refuses, and nothing else (no page is copied)."""
+    pool = torch.empty(layers, 1, hkv, page, d, dtype=dtype, device="meta")
+    code = status("ssa_paged_copy", FAKE, FAKE, _lib.dtype_code(dtype), layers, hkv, d, 1, page,
+                  _lib.i64_array(list(pool.stride()[:4]) * 2), FAKE, FAKE, NULL, 0, None)
+    assert code in (_lib.SSA_OK, UNSUPPORTED)
+    if code == _lib.SSA_OK:
+        P._copy_limits(65535, pool)
+    else:
+        with pytest.raises(ValueError, match="over all layers"):
+            P._copy_limits(1, pool)
+    with pytest.raises(ValueError, match="65536 pages"):
+        P._copy_limits(65536, pool)
