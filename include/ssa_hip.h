@@ -576,7 +576,7 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   ssa_paged_resize: source[b], target[b], tokens[b] (B) say what ssa_paged_copy has to copy (-1, -1, 0
  *   where nothing); the lowest row keeps the page if no row lists it whole. With r such rows before it
  *   (rows in order) the page is free_pages[*nfree - 1 - r]. Pages that no row lists any more are given
- *   back as ssa_paged_resize does, each by the lowest row that listed it; forking and ending the forks
+ *   back as ssa_paged_resize does, each once, by the lowest row that listed it; forking and ending the forks
  *   restores the stack. *status: 0; or nothing was changed (source, target -1): the number of pages
  *   lacking, or -1 (a length, a row, a held page id or a count that does not fit). Workspace:
  *   ssa_paged_fork_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.

@@ -11,11 +11,19 @@ namespace {
 
 struct ForkRow;
 
-// What the call's rows say of a page: the first row that listed it and changes, the first row that will
-// hold it as its last, partly filled page, whether a row will hold it whole.
+// What the call's rows say of a page: the first row that listed it and changes with the first entry there
+// (a row may list a page twice), the first row that will hold it as its last, partly filled page, whether a
+// row will hold it whole.
 struct PageUse {
-  int holder, first_part, whole, unused;
+  unsigned long long holder;
+  int first_part, whole;
 };
+
+constexpr unsigned long long kNoHolder = ~0ull;
+
+__device__ inline unsigned long long holder_of(int b, int e) {
+  return (unsigned long long)b << 32 | (unsigned)e;
+}
 
 struct ForkParams {
   const int32_t* src;  // NULL: every row itself
@@ -100,7 +108,7 @@ __device__ inline void fork_clear(const ForkParams& p, int unit) {
   each_entry(chunk, r.have, [&](int k, int e) {
     p.old[b * p.W + e] = id[k];
     if (id[k] < 0 || id[k] >= p.P) bad = true;
-    else p.use[id[k]] = PageUse{0x7fffffff, 0x7fffffff, 0, 0};
+    else p.use[id[k]] = PageUse{kNoHolder, 0x7fffffff, 0};
   });
   const bool any = __any(bad);
   if ((threadIdx.x & 63) == 0) {
@@ -130,13 +138,13 @@ __device__ inline void fork_mark(const ForkParams& p, int unit) {
   if (r.same) return;
   each_entry(chunk, r.have, [&](int k, int e) { id[k] = mine[e]; });
   each_entry(chunk, r.have, [&](int k, int e) {
-    if (id[k] >= 0 && id[k] < p.P) atomicMin(&p.use[id[k]].holder, b);
+    if (id[k] >= 0 && id[k] < p.P) atomicMin(&p.use[id[k]].holder, holder_of(b, e));
   });
 }
 
-// Whether row b gives back a page of this use.
-__device__ inline bool gives(const PageUse& u, int b) {
-  return !u.whole && u.first_part == 0x7fffffff && u.holder == b;
+// Whether row b gives back a page of this use at entry e.
+__device__ inline bool gives(const PageUse& u, int b, int e) {
+  return !u.whole && u.first_part == 0x7fffffff && u.holder == holder_of(b, e);
 }
 
 // Whether row b needs a copy of its last page: another row holds it whole or was first.
@@ -159,7 +167,7 @@ __device__ inline void fork_count(const ForkParams& p, int unit) {
     int id[kForkLoads];
     each_entry(chunk, r.have, [&](int k, int e) { id[k] = p.old[b * p.W + e]; });
     each_entry(chunk, r.have, [&](int k, int e) {
-      if (id[k] >= 0 && id[k] < p.P) n += gives(p.use[id[k]], b);
+      if (id[k] >= 0 && id[k] < p.P) n += gives(p.use[id[k]], b, e);
     });
   }
   n = lane_sums(n).all;
@@ -239,8 +247,8 @@ __device__ inline void fork_write(const ForkParams& p, int unit, const ForkPlace
     int id[kForkLoads];
     unsigned int give = 0;
     each_entry(chunk, r.have, [&](int k, int e) { id[k] = p.old[b * p.W + e]; });
-    each_entry(chunk, r.have, [&](int k, int) {
-      give |= gives(p.use[id[k]], b) ? 1u << k : 0u;
+    each_entry(chunk, r.have, [&](int k, int e) {
+      give |= gives(p.use[id[k]], b, e) ? 1u << k : 0u;
     });
     int at = at_.left - 1 - at_.given;
 #pragma unroll

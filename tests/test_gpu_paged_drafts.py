@@ -1038,3 +1038,40 @@ def test_accept_is_all_or_nothing_and_can_be_made_again(cuda, requests, wrong):
     cache.check()
     assert cache.lens.tolist() == [c + len(p) for c, p in zip(ctx, paths)]
     assert torch.equal(cache.k, want[0]) and torch.equal(cache.v, want[1])
+
+
+# ---- rows that list a page more than once -------------------------------------------------------
+
+@pytest.mark.parametrize("page,width", [(16, 12), (16, 2600)])
+def test_pages_that_a_row_lists_twice_go_back_once(cuda, page, width):
+    """Rows set by the caller, a page at several places of a row and in several rows: forked, cut and ended as
+    in lists; every page is free once in the end."""
+    rng = random.Random(width)
+    B, pages = 4, 40
+    cache = P.PagedCache(B, width * page, pages, 1, 8, page=page, device=cuda)
+    ref = D.ForkState(B, width, pages, page)
+    for rep in range(6):
+        ref.table = [[-1] * width for _ in range(B)]
+        ref.lens = [rng.randrange(1, width * page + 1) if b else width * page for b in range(B)]
+        some = rng.sample(range(pages), 14)
+        for b, n in enumerate(ref.lens):
+            need = -(-n // page)
+            ref.table[b][:need] = [rng.choice(some[:11] if b else some[3:]) for _ in range(need)]
+        listed = set(sum(ref.table, [])) - {-1}
+        ref.free = [x for x in range(pages) if x not in listed]
+        rng.shuffle(ref.free)
+        cache.table.copy_(int32(ref.table, cuda))
+        cache.lens.copy_(int32(ref.lens, cuda))
+        cache.free[:len(ref.free)] = int32(ref.free, cuda)
+        cache.nfree.fill_(len(ref.free))
+        for kind in ("fork", "cut", "some end", "end"):
+            lens = ref.lens
+            src = [rng.randrange(B) for _ in range(B)] if kind == "fork" else list(range(B))
+            new = [0 if kind == "end" or kind == "some end" and b % 2 else
+                   lens[a] if kind == "some end" else rng.randrange(lens[a] + 1) for b, a in enumerate(src)]
+            print(page, width, rep, kind, flush=True)
+            want = ref.fork(src, new)
+            f = P.fork_pages(int32(src, cuda), int32(new, cuda), cache.lens, cache.table, cache.free,
+                             cache.nfree, page)
+            check_state(cache, ref, f, want)
+        assert sorted(cache.free.tolist()) == list(range(pages)) and cache.nfree.item() == pages
