@@ -240,17 +240,17 @@ __device__ inline DraftItem uniform(const DraftItem& x) {
                                        uniform((int)x.s.span.ok) != 0}}};
 }
 
-// Which of the 64 keys from j0 on a row attends: bit j - j0. tok, pos, start: the row's place among its
-// request's n drafted tokens, its position and its first key.
-__device__ inline uint64_t attended_keys(const DraftParams& p, const DraftItem& it, int tok, int start,
-                                         int j0) {
+// Which of the 64 keys from j0 on a row attends: bit j - j0. tok, pos: the row's place among its request's n
+// drafted tokens and its position.
+__device__ inline uint64_t attended_keys(const DraftParams& p, const DraftItem& it, int tok, int pos, int j0) {
   const int ctx = it.s.ctx, i0 = j0 - ctx;  // the first key's place among the drafted ones
+  const int64_t start = p.window > 0 ? (int64_t)pos - p.window + 1 : 0;  // below 0: keys' positions may be too
   auto below = [](int64_t x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; };
-  const uint64_t context = below(-(int64_t)i0) & ~below((int64_t)start - j0);
+  const uint64_t context = below(-(int64_t)i0) & ~below(start - j0);
   if (i0 + 64 <= 0) return context;
   uint64_t bits;
   if (!p.masks) {
-    bits = below((int64_t)tok - i0 + 1) & ~below((int64_t)start - j0);
+    bits = below((int64_t)tok - i0 + 1) & ~below(start - j0);
   } else {
     const int32_t* const words = p.masks + ((int64_t)it.c0 + tok) * p.words;
     auto word = [&](int w) { return w >= 0 && w < p.words ? (uint64_t)(unsigned)words[w] : 0ull; };
@@ -406,8 +406,8 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   const int i0 = uniform((int)((int64_t)tiles * wv / NW));
   const int i1 = uniform((int)((int64_t)tiles * (wv + 1) / NW));
 
-  // this lane's rows: drafted token, head, position and first key; past the last row the last again
-  int tok[MT], head[MT], rpos[MT], start[MT];
+  // this lane's rows: drafted token, head and position; past the last row the last again
+  int tok[MT], head[MT], rpos[MT];
   bool real[MT];
   int late = 0;  // the latest first key of the tile's rows
 #pragma unroll
@@ -418,8 +418,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
     tok[mt] = min(t, n - 1);
     head[mt] = it.g * p.G + (int)(x - (unsigned)t * p.G);
     rpos[mt] = !p.masks ? ctx + tok[mt] : p.pos[(int64_t)it.c0 + tok[mt]];
-    start[mt] = p.window > 0 && rpos[mt] >= p.window ? rpos[mt] - p.window + 1 : 0;
-    late = max(late, start[mt]);
+    if (p.window > 0 && rpos[mt] >= p.window) late = max(late, rpos[mt] - p.window + 1);
   }
   if (p.window > 0) {
     late = max(late, lane_xor(late, 1));
@@ -533,7 +532,7 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
   };
   // which of this lane's keys of the tile from j0 on its row attends: bit 4 t + r
   auto attended = [&](int mt, int j0) {
-    const uint64_t keys = attended_keys(p, it, tok[mt], start[mt], j0) >> grp * 4;
+    const uint64_t keys = attended_keys(p, it, tok[mt], rpos[mt], j0) >> grp * 4;
     unsigned int bits = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) bits |= (unsigned)(keys >> t * 16 & 15) << t * 4;
@@ -942,8 +941,8 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   const int head = it.g * p.G + (int)(x - (unsigned)t0 * p.G);
   const bool real = t0 < n, any = __any(real);  // a wave without rows loads and waits with the others
   const int rpos = !p.masks ? ctx + tok : p.pos[(int64_t)it.c0 + tok];
-  const int start = p.window > 0 && rpos >= p.window ? rpos - p.window + 1 : 0;
-  int late = start;  // the latest first key of the wave's rows
+  // the latest first key of the wave's rows
+  int late = p.window > 0 && rpos >= p.window ? rpos - p.window + 1 : 0;
   if (p.window > 0) {
 #pragma unroll
     for (int i = 1; i < RW; i <<= 1) late = max(late, lane_xor(late, i));
@@ -1061,7 +1060,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
     unsigned int allow = NQ == 8 ? ~0u : (1u << 4 * NQ % 32) - 1;
     float mx = -FLT_MAX;
     if (edge) {
-      uint64_t keys = attended_keys(p, it, tok, start, j0);
+      uint64_t keys = attended_keys(p, it, tok, rpos, j0);
       const int own = min(it.end - s0, SUB) * 16;  // past the item's end the next item's keys lie
       if (own < 64) keys &= (1ull << own) - 1;
       keys >>= 4 * grp;

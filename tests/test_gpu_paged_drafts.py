@@ -1075,3 +1075,34 @@ def test_pages_that_a_row_lists_twice_go_back_once(cuda, page, width):
                              cache.nfree, page)
             check_state(cache, ref, f, want)
         assert sorted(cache.free.tolist()) == list(range(pages)) and cache.nfree.item() == pages
+
+
+# ---- positions below 0 --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,hq", [(64, 2), (64, 16), (128, 8), (256, 2), (512, 2)])
+def test_windows_over_keys_at_positions_below_zero(cuda, dtype, d, hq):
+    """With any masks and positions a drafted key counts if it lies past its row's position less the window,
+    whatever its sign."""
+    ctx, n = [0, 5, 40], [9, 20, 33]
+    q, cache, cu = make(cuda, dtype, ctx, n, hq, 1, d, 16, seed=22)
+    rng = random.Random(d)
+    masks, pos = [], []
+    for c, count in zip(ctx, n):
+        for t in range(count):
+            low = t % 3 == 1  # a key only: its own row does not fit
+            bits = rng.getrandbits(count) | 1 << t
+            masks.append([bits >> 32 * w & 0xffffffff for w in range(2)])
+            pos.append(-rng.randrange(1, 12) if low else c + rng.randrange(count))
+    words = int32([[x - (1 << 32) if x >> 31 else x for x in m] for m in masks], cuda)
+    drafts = P.Drafts(words, int32(pos, cuda))
+    fits = torch.tensor([p >= 0 for p in pos])
+    for window in (1, 4, 10, 20, 70, 2 ** 31 - 1):
+        print(dtype, d, hq, window, flush=True)
+        out, lse = cache.attend_drafts(0, q, cu, drafts, window=window, return_lse=True)
+        torch.cuda.synchronize()
+        want, wlse, tol, ltol = D.attend(q, cache.k[0], cache.v[0], cache.table, cache.lens, cu, d ** -0.5,
+                                         window, *drafts)
+        U.close(out[fits], want[fits], tol[fits])
+        U.close(lse[fits], wlse[fits], ltol[fits])
+        assert out[~fits].isnan().all() and lse[~fits].isnan().all()
