@@ -132,7 +132,7 @@ constexpr int kRestBlocks = 8;
 
 // What one workgroup does: split j of n of a row tile of request b and key head g.
 struct DraftItem {
-  int b, g, tile, tiles, j, n, begin, end, first_part, c0;
+  int b, g, tile, tiles, j, n, begin, end, past, first_part, c0;  // past: the end of its share of the pages
   bool stream;
   DraftSpan s;
 };
@@ -217,11 +217,11 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   // parts that the workspace does not hold (offsets that do not ascend): the join answers
   const int64_t part0 = (int64_t)part * p.Hkv, part_end = part0 + (int64_t)tiles * it.n * p.Hkv;
   it.first_part = it.n > 1 && (part < 0 || part_end > p.max_parts) ? -1 : (int)part0;
-  it.begin = it.end = 0;
+  it.begin = it.end = it.past = 0;
   if (it.s.span.ok) {
     const PagedRange r = paged_item_range(it.s.span, units, it.j, it.n);
     it.begin = r.begin;
-    it.end = r.end;
+    it.end = it.past = r.end;
     if (!p.masks) {  // a chain: none of the tile's tokens attends keys past its last one
       const unsigned int last = ((unsigned)it.tile * M + M - 1) / (unsigned)p.G;
       const int seen = (it.s.ctx + (int)min(last, (unsigned)it.s.n - 1)) / 16 + 1;
@@ -234,7 +234,7 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
 __device__ inline DraftItem uniform(const DraftItem& x) {
   return DraftItem{uniform(x.b),     uniform(x.g),   uniform(x.tile), uniform(x.tiles),
                    uniform(x.j),     uniform(x.n),   uniform(x.begin), uniform(x.end),
-                   uniform(x.first_part), uniform(x.c0), uniform((int)x.stream) != 0,
+                   uniform(x.past),  uniform(x.first_part), uniform(x.c0), uniform((int)x.stream) != 0,
                    DraftSpan{uniform(x.s.ctx), uniform(x.s.n),
                              PagedSpan{uniform(x.s.span.first), uniform(x.s.span.len),
                                        uniform((int)x.s.span.ok) != 0}}};
@@ -266,6 +266,17 @@ __device__ inline uint64_t attended_keys(const DraftParams& p, const DraftItem& 
     }
   }
   return context | (bits & ~below(-(int64_t)i0) & below((int64_t)it.s.n - i0));
+}
+
+// Whether pages that an item's tile does not read, of tokens past all of its own, are in the table's row but
+// not in the pool: they make the request one that does not fit all the same.
+__device__ inline bool bad_past(const DraftParams& p, const DraftItem& it, const int32_t* row) {
+  bool bad = false;
+  for (int s = it.end + (int)(threadIdx.x & 63); s < it.past; s += 64) {
+    const int x = row[page_of(s, p.div)];
+    bad |= x < 0 || x >= p.pages;
+  }
+  return __any(bad);
 }
 
 // Rows that no request's items answer, by block `id` of kRestBlocks: those behind the last request's become
@@ -768,11 +779,12 @@ __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(Dr
 #pragma unroll
       for (int r = 0; r < 4; ++r) nan |= st[mt].acc[i][r] != st[mt].acc[i][r];
   if (__any(nan)) walk(std::true_type{});
+  const bool misfit = bad != 0 || !it.s.span.ok || (wv == 0 && bad_past(p, it, row));
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     st[mt].l += lane_xor(st[mt].l, 16);
     st[mt].l += lane_xor(st[mt].l, 32);
-    if (bad != 0 || !it.s.span.ok || rpos[mt] < ctx) st[mt].l = NAN;
+    if (misfit || rpos[mt] < ctx) st[mt].l = NAN;
   }
 
   // the waves' results, half of them into the other half at a time
@@ -1180,7 +1192,8 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
   }
   if constexpr (RW == 16) l += lane_xor(l, 16);
   l += lane_xor(l, 32);
-  if (bad != 0 || !it.s.span.ok || rpos < ctx) l = NAN;
+  const bool misfit = bad != 0 || !it.s.span.ok || bad_past(p, it, row);
+  if (misfit || rpos < ctx) l = NAN;
 
   if (p.items != 0 && it.j == 0 && it.g == 0 && it.tile == 0 && threadIdx.x == 0) {
     p.info[2 * it.b] = it.first_part;

@@ -1106,3 +1106,26 @@ def test_windows_over_keys_at_positions_below_zero(cuda, dtype, d, hq):
         U.close(out[fits], want[fits], tol[fits])
         U.close(lse[fits], wlse[fits], ltol[fits])
         assert out[~fits].isnan().all() and lse[~fits].isnan().all()
+
+
+# ---- pages that only a request's last tokens read -----------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,d,ctx", [(2, 64, 0), (2, 64, 9000), (1, 128, 77), (1, 256, 300), (1, 512, 0)])
+def test_a_bad_page_past_a_tile_makes_the_whole_request_nan(cuda, dtype, hq, d, ctx):
+    """A chain of many row tiles, of which the first do not read the last pages: NaN in every row all the
+    same, the request beside it right."""
+    page, n = 16, [900, 40]
+    q, cache, cu = make(cuda, dtype, [ctx, 20], n, hq, 1, d, page, seed=23)
+    good = cache.attend_drafts(0, q, cu)
+    assert good.isfinite().all()
+    held = cache.table.clone()
+    for at in (ctx + 899, ctx + 450, ctx + 16, ctx // 2):
+        for value in (-1, cache.k.shape[1], 2 ** 31 - 1):
+            cache.table[0, at // page] = value
+            print(dtype, hq, d, ctx, at, value, flush=True)
+            out, lse = cache.attend_drafts(0, q, cu, return_lse=True)
+            assert out[:900].isnan().all() and lse[:900].isnan().all()
+            assert torch.equal(out[900:], good[900:])
+        cache.table.copy_(held)
+    assert torch.equal(cache.attend_drafts(0, q, cu), good)
