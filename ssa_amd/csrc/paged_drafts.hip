@@ -1233,8 +1233,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
 // the columns, four waves a workgroup. Bound by memory: 32,768 rows of 3 to 11 parts of 128 columns (98 MB)
 // 20 us; by latency where rows are few, 4 us. BATCH: parts of a row (and split of the wave) on their way at
-// a time: 16 where rows are few and long (4K keys, 112 rows of 33 parts 13.2 us the whole call, 13.5 with 4;
-// 1M 159 and 164), 4 where the rows fill the card (16 trees of 64 197, 208 with 16).
+// a time: 16 where rows are few and long, 4 where the rows fill the card (kFewJoins has both sides).
 template <int DT, int DP, int M, int BATCH>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;
@@ -1341,12 +1340,14 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   const auto rounded = [](int64_t x) { return (x + 7) / 8 * 8; };  // an XCD's run each
   y.blocks = rounded(tiles);
   if (units <= 4 || (units <= 16 && tiles >= 512)) return y;
-  // Workgroups aimed at: about what the CUs hold at once, or twice that where it evens out uneven
-  // requests (64 mixed requests 341 us for 768, 316 for 1536; 16 trees of 64 tokens 196 and 192); one
-  // request is even by itself (16 tokens over 1M 165 us for 768, 178 for 1536). Windows of 1024 at head
-  // dim 256 fit one round of 384 better than two of 512 (43 us and 46).
-  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 ? (y.M == 64 ? 384 : 512)
-                         : B == 1 ? 768 : y.M >= 64 ? 1536 : 1024;
+  // Workgroups aimed at: what the CUs hold at once (one a CU at head dim 512, two at 256, three or four
+  // below), or twice that below 256 where it evens out uneven requests. Three a CU and twice as many: 64 mixed
+  // requests 280 us and 266, 16 trees of 64 tokens 229 and 218; one request is even by itself: 16 tokens over
+  // 1M 181 and 192, 8 over 1M 120 and 133, over 100K of 8 key heads 16 tokens 92 and 116, 4 tokens 84 and 92
+  // (so are two alike, which the host cannot know: 50,000 each 90 and 115). Head dim 256, two a CU and one and
+  // a half: 8 requests of 8,000 keys 71 and 79, one of 60,000 68 and 74, 64 of 2,000 68 and 78, windows of
+  // 2,048 of 48 requests 79 and 95, of 1,024 of 32 requests 48 and 43, 20 of 500 to 9,000 100 and 82.
+  const int64_t target = y.dp == 512 ? 256 : y.dp == 256 ? 512 : B == 1 ? 768 : y.M >= 64 ? 1536 : 1024;
   y.items = std::max<int64_t>(1, target / Hkv);
   y.blocks = rounded(std::min(tiles + y.items * Hkv, tiles * units));
   y.max_parts = std::min(2 * y.items * Hkv, y.blocks);
@@ -1357,7 +1358,9 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   return y;
 }
 
-// Rows up to which a join takes 16 parts at a time (its comment has both sides).
+// Rows up to which a join takes 16 parts at a time (the whole call with 4 and with 16: 32 rows of 100,000 keys
+// 31.7 and 28.8 us, 256 45.7 and 42.5, 1,024 in 8 requests of 8,000 23.8 and 23.5, 1,536 103.9 and 102.1,
+// 2,048 in one request 156.7 and 158.2, in 16 29.1 and 29.1, 4,096 in 32 28.9 and 29.6).
 constexpr int64_t kFewJoins = 1024;
 
 template <int DT, int DP, int M, int KT, int WPE>
