@@ -557,7 +557,8 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
  *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq and the
  *   workgroups that a call may need are held below 2^31 and 2^24. Workspace:
- *   ssa_paged_attend_drafts_workspace_size bytes, 16-byte aligned, nothing in it needs to be set.
+ *   ssa_paged_attend_drafts_workspace_size bytes (partial results, at most 205 MB), 16-byte aligned, nothing
+ *   in it needs to be set.
  * ssa_paged_keep: moves the accepted drafted tokens together: drafted token path[b][i] of request b to
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the

@@ -39,7 +39,7 @@ __device__ inline unsigned int way(int anc, int steps, bool bad) {
 // way with that of the ancestor where it ends, so its length doubles: a chain of 1024 takes ten rounds.
 // The last workgroups answer the rows that no request's offsets hold, and all rows where the offsets
 // descend (they may be two requests' then). Bound by launch and barrier latency: 64 trees of up to 64 tokens
-// 3.5 us, 8 of 1,024 10.8.
+// 3.7 us, 8 of 1,024 11.4.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_draft_masks_kernel(MaskParams p) {
   __shared__ unsigned int ways[THREADS];
@@ -394,7 +394,7 @@ __device__ inline float not_finite_sum(float with, float without) {
 // or NaN there reaches the rows that do not attend it as 0 x infinity: where a result is NaN, the wave
 // does its keys again with care, such values taken out of the product and added to the rows that attend
 // them. Bound by the reading of keys and values: 32 requests of 8,000 keys, 4 tokens of 4 heads a key head
-// (8 heads of 128, bf16) 185 us, 5.7 TB/s; one token a request 181, for which paged_attend_kernel takes 167.
+// (8 heads of 128, bf16) 184 us, 5.7 TB/s; one token a request 184, for which paged_attend_kernel takes 170.
 template <int DT, int DP, int MT, int WPE>
 __global__ __launch_bounds__(kAttendWaves * 64, WPE) void paged_drafts_kernel(DraftParams p) {
   using T = Tile<DT, DP>;
@@ -872,8 +872,8 @@ __device__ inline void load_lds(const char* from, unsigned char* to) {
 }
 
 // Weights of two keys as 16-bit parts: bf16's three, each rounded to 8 bits of what the ones before leave,
-// hold them exactly (two left up to 2^-17 of a weight, which put 0.4 % of the outputs on the other side of
-// their rounding); fp16's two, cut to 11 bits each, leave 2^-20, of which the output keeps 11 bits. A part
+// hold them exactly (two left up to 2^-17 of a weight; the third costs 16 tokens over 1M 149 -> 189 us, 16
+// trees of 64 182 -> 222); fp16's two, cut to 11 bits each, leave 2^-20, and the output keeps 11 bits. A part
 // may be negative or zero: the walk that meets infinite values takes them out of the products first.
 template <int DT>
 __device__ inline void parts_of(float p0, float p1, unsigned int (&w)[kParts<DT>]) {
@@ -917,9 +917,9 @@ __device__ inline f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
 // nothing looks for infinite or NaN values: where a sum or a result is too large or not finite, the item is
 // done again with care (the maximum raised tile by tile, values that are not finite taken out of the
 // products as in paged_drafts_kernel).
-// 16 tokens of 7 heads (of 64) over 1,048,561 keys, 537 MB: 143 us and 15 for the join; its loads alone take
-// 112, its products and weights alone 128, and the two overlap by half. 16 trees of 64 tokens over 2,000
-// to 9,000 keys (32 / 8 heads of 128): 176 us and 20, 129 and 147; matrix units busy 31 % of the time.
+// 16 tokens of 7 heads (of 64) over 1,048,561 keys, 537 MB: 178 us and 14 for the join after it; its products
+// and weights alone take 160, its loads alone 95. 16 trees of 64 tokens over 2,000 to 9,000 keys (32 / 8 heads
+// of 128): 198 us and 20, alone 174 and 110; matrix units busy 35 % of the time in both.
 // Rings of three and four tiles, with fewer workgroups a CU, took as long or longer.
 template <int DT, int DP, int RW, int KT, int WPE>
 __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams p) {
@@ -1232,7 +1232,7 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
 
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
 // the columns, four waves a workgroup. Bound by memory: 32,768 rows of 3 to 11 parts of 128 columns (98 MB)
-// 20 us; by latency where rows are few, 4 us. BATCH: parts of a row (and split of the wave) on their way at
+// 20 us; by latency where rows are few, 4 us, or 14 where each has many parts (224 rows over 1M keys). BATCH: parts of a row (and split of the wave) on their way at
 // a time: 16 where rows are few and long, 4 where the rows fill the card (kFewJoins has both sides).
 template <int DT, int DP, int M, int BATCH>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
@@ -1329,8 +1329,9 @@ DraftLayout draft_layout(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk
   y.dp = d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 512;
   // Rows of a key head; of a request rows / B on average. Tiles of 16 rows, whose waves take a run of keys
   // each, win up to there; past them tiles that the waves share (bf16, 32 requests of 8,000 keys, 8 heads
-  // of 128): 16 rows a request 186 us for 210, 20 rows 212 for 232, 64 235 for 361. Past 64 rows tiles of
-  // 128: 128 rows 310 us for 341 (two of 64), 64 rows 249 for 235. fp32, 32 rows: 129 for 135 (two of 16).
+  // of 128): 16 rows a request 176 us for 207, 20 rows 212 for 216, 64 231 for 353. Past 64 rows tiles of
+  // 128: 128 rows 330 us for 347 (two of 64), 96 299 for 313, 64 275 for 230. fp32, 32 rows: 121 for 125 (two
+  // of 16).
   const int64_t rows = N * G;
   if (dtype == SSA_F32) y.M = y.dp <= 128 && rows > 16 * B ? 32 : 16;
   else y.M = y.dp == 512 || rows <= 16 * B ? 16 : y.dp == 256 || rows <= 64 * B ? 64 : 128;
@@ -1428,7 +1429,7 @@ enum Keep { kKeepEach, kKeepCheck, kKeepAll };
 // written is read again. All or nothing: every workgroup of a request checks its whole path first, and
 // with kKeepAll looks at what the launch before it (kKeepCheck) found of every request. Bound
 // by the longest path's column: 24 requests with 200 of 600 tokens moved in 8 layers (5 heads of 80, fp32,
-// 93 MB in all) 37 us; 64 with 2 in 24 layers 4.1.
+// 93 MB in all) 38 us; 64 with 2 in 24 layers 4.1.
 template <Keep KEEP>
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
   __shared__ int64_t s_from[2][kKeepThreads], s_to[2][kKeepThreads];  // of keys and values
