@@ -552,13 +552,13 @@ int ssa_paged_attend(const void* q, void* kpool, void* vpool, void* out, float* 
  *   its own - window (drafted keys' positions are pos). softmax(scale * q.k), types, head layout,
  *   lse (N, Hq), status, page ids and strides as ssa_paged_attend; scores, statistics and sums in fp32,
  *   and a weight with all its bits (bf16) or all but 2^-20 of itself down to 2^-38 of the row's largest
- *   (fp16). A row that attends nothing: out 0, lse -inf, whatever the values it does not attend. A position before ctx, a request or row that
- *   does not fit: NaN. Rows behind the last request's are left as they were, or, with clear_rest != 0, out 0
- *   and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
+ *   (fp16). A row that attends nothing: out 0, lse -inf, whatever the values it does not attend. A position
+ *   before ctx, a request or row that does not fit: NaN. Rows behind the last request's are left as they
+ *   were, or, with clear_rest != 0, out 0 and lse -inf. Any masks are served, not those of trees only. strides[10] = q(t,h),
  *   kpool(page,head,slot), vpool(page,head,slot), out(t,h). N * Hq and the
  *   workgroups that a call may need are held below 2^31 and 2^24. Workspace:
- *   ssa_paged_attend_drafts_workspace_size bytes (partial results, at most 205 MB), 16-byte aligned, nothing
- *   in it needs to be set.
+ *   ssa_paged_attend_drafts_workspace_size bytes (partial results: with up to 1,536 key heads at most
+ *   205 MB and 8 bytes a request), 16-byte aligned, nothing in it needs to be set.
  * ssa_paged_keep: moves the accepted drafted tokens together: drafted token path[b][i] of request b to
  *   place i, i < counts[b], in every layer of pools (layers, pages, Hkv, page, d). path (B, width)
  *   int32, rows path_stride apart, ascending; counts (B). new_lens (B): ctx + counts[b], for the

@@ -144,9 +144,9 @@ __device__ inline DraftSpan draft_of(const DraftParams& p, int b) {
 // Finds workgroup `id`'s item from the lengths alone, each wave for itself: every lane sums a run of
 // requests, the wave adds the runs up. Of the call's row tiles an XCD takes a run, the tiles of the
 // same keys next to each other: its L2 serves them together. False past the last one, and for all where
-// the offsets descend (rest_rows answers). (Equal shares of all units instead,
-// a workgroup going on from one row tile to the next, cost a short call 8 us, and a mixed batch 550 us for
-// 313: a unit takes as long with few rows as with many.)
+// the offsets descend (rest_rows answers). (Equal shares of all units instead, a workgroup going on from one
+// row tile to the next, cost a short call 8 us, and a mixed batch 550 us for 313: a unit takes as long with
+// few rows as with many.)
 template <int M>
 __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   const int lane = threadIdx.x & 63;
@@ -214,7 +214,7 @@ __device__ inline bool find_draft(const DraftParams& p, int id, DraftItem& it) {
   it.j = (int)(row / (unsigned)p.Hkv);
   it.g = (int)(row - (unsigned)it.j * p.Hkv);
   it.stream = it.stream && it.tiles == 1;
-  // parts that the workspace does not hold (offsets that do not ascend): the join answers
+  // a bound on what is written: offsets that ascend make no more parts than the workspace holds
   const int64_t part0 = (int64_t)part * p.Hkv, part_end = part0 + (int64_t)tiles * it.n * p.Hkv;
   it.first_part = it.n > 1 && (part < 0 || part_end > p.max_parts) ? -1 : (int)part0;
   it.begin = it.end = it.past = 0;
@@ -1232,8 +1232,9 @@ __global__ __launch_bounds__(256, WPE) void paged_drafts_tile_kernel(DraftParams
 
 // Joins the parts of rows whose tiles were cut: a wave per row (a token's query head), its lanes over
 // the columns, four waves a workgroup. Bound by memory: 32,768 rows of 3 to 11 parts of 128 columns (98 MB)
-// 20 us; by latency where rows are few, 4 us, or 14 where each has many parts (224 rows over 1M keys). BATCH: parts of a row (and split of the wave) on their way at
-// a time: 16 where rows are few and long, 4 where the rows fill the card (kFewJoins has both sides).
+// 20 us; by latency where rows are few, 4 us, or 14 where each has many parts (224 rows over 1M keys). BATCH:
+// parts of a row (and split of the wave) on their way at a time: 16 where rows are few and long, 4 where the
+// rows fill the card (kFewJoins has both sides).
 template <int DT, int DP, int M, int BATCH>
 __global__ __launch_bounds__(256) void paged_drafts_join_kernel(DraftParams p) {
   constexpr int PER = DP / 4, NS = PER < 64 ? 64 / PER : 1, NV = PER > 64 ? PER / 64 : 1;

@@ -565,7 +565,8 @@ def keep_drafts(kpool: torch.Tensor, vpool: torch.Tensor, table: torch.Tensor, l
                                     _meta(counts))
     new_lens = torch.empty(B, device=lens.device, dtype=torch.int32)
     if B:
-        _launch("ssa_paged_keep_all" if all_or_none else "ssa_paged_keep", lens, kpool.data_ptr(), vpool.data_ptr(), *sizes,
+        _launch("ssa_paged_keep_all" if all_or_none else "ssa_paged_keep", lens, kpool.data_ptr(),
+                vpool.data_ptr(), *sizes,
                 table.data_ptr(), row, W, lens.data_ptr(), cu.data_ptr(), B,
                 path.data_ptr() if K else None, prow, K, counts.data_ptr(), new_lens.data_ptr())
     return new_lens
